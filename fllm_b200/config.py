@@ -80,6 +80,7 @@ class ModelConfig:
     attn_softcap: float = 0.0
     sliding_window: int = 0              # 0 = full attention
     window_pattern: Optional[List[int]] = None   # per layer: 1 = windowed, 0 = full
+    window_first: int = 0                # so many first tokens stay visible behind the window
     attn_sinks: bool = False             # learned per-head sink logit (gpt-oss)
     attn_scale: Optional[float] = None   # softmax scale when it is not head_dim ** -0.5 (Gemma-2: query_pre_attn_scalar ** -0.5)
     post_norms: bool = False             # Gemma-2: the attention and FFN outputs are normalised before the residual add

@@ -1,0 +1,93 @@
+// What a query row sees of a paged cache when a sliding window leaves the first tokens visible, and when rows are the nodes of a draft
+// tree; shared by the kernels of attention_span.cu and attention_span_tc.cu.
+//
+// Row r of a sequence stands at place P in its text and sees token j of the context (j < base) if j > P - window or j < first, and node n
+// of the tree (stored at base + n) if its bit is set in the row's mask (its ancestors and itself) and the same holds for the node's
+// place. Plain rows have base = P + 1 and no mask; tree rows P = base + (bits set) - 1, and the k-th bit set stands at base + k. So a
+// mask is trimmed once and every token is then two comparisons or one bit.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "fllm_ops.h"
+#include "ptx.cuh"
+
+namespace fllm {
+namespace {
+constexpr int kSpanWords = 4;              // 64-bit words of a tree mask: at most 256 nodes
+
+struct SpanRow {
+  int base;                                // context tokens are those in front of it
+  int beg;                                 // where the window begins
+};
+
+// Row `qi` of the qn rows of a sequence; `bits` (trees): its mask, trimmed, p.words of them.
+__device__ __forceinline__ SpanRow span_row(const SpanParams& p, int q0, int qn, int kv_len, int qi, unsigned long long* bits) {
+  SpanRow r;
+  int count = 0;
+  if (p.tree_mask) {
+    r.base = min(max(p.tree_base[q0 + qi], 0), kv_len);
+    const int nodes = kv_len - r.base;
+    for (int w = 0; w < p.words; ++w) {
+      unsigned long long m = p.tree_mask[(size_t)(q0 + qi) * p.words + w];
+      const int left = nodes - 64 * w;     // nodes that are stored
+      if (left < 64) m = left <= 0 ? 0ull : m & ((1ull << left) - 1);
+      bits[w] = m;
+      count += __popcll(m);
+    }
+  } else {
+    r.base = max(kv_len - qn + qi + 1, 0);
+  }
+  const int place = r.base + count - 1;
+  r.beg = p.window > 0 ? max(0, place - p.window + 1) : 0;
+  if (count && r.beg > r.base) {           // ancestors behind the window, those among the first tokens excepted
+    int k = 0;
+    for (int w = 0; w < p.words; ++w) {
+      unsigned long long m = bits[w], keep = 0;
+      while (m) {
+        const unsigned long long bit = m & (~m + 1);
+        if (r.base + k >= r.beg || r.base + k < p.first) keep |= bit;
+        m ^= bit;
+        ++k;
+      }
+      bits[w] = keep;
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ bool span_sees(const SpanParams& p, int tok, int base, int beg, const unsigned long long* bits) {
+  if (tok < base) return tok >= beg || tok < p.first;
+  const int n = tok - base;
+  return n < 64 * p.words && (bits[n >> 6] >> (n & 63) & 1);
+}
+
+// Tokens that the rows of a tile see between them, in pieces of `unit` tokens: the first `head` pieces of the text, then those from `lo` on.
+struct SpanRange {
+  int head, lo, count;
+  __device__ __forceinline__ int piece(int i) const { return i < head ? i : i - head + lo; }
+};
+__device__ __forceinline__ SpanRange span_range(const SpanParams& p, int unit, int min_beg, int end) {
+  SpanRange s;
+  s.lo = min_beg / unit;
+  s.head = p.first > 0 ? min((min(p.first, end) + unit - 1) / unit, s.lo) : 0;
+  s.count = end > 0 ? s.head + max((end + unit - 1) / unit - s.lo, 0) : 0;
+  return s;
+}
+
+// Block id of the 16 tokens from 16 * page on, or -1 where the table does not reach or the entry names no block of the pool.
+__device__ __forceinline__ int span_block(const SpanParams& p, const int* table, int page) {
+  const int at = page / p.block_pages;
+  const int b = at < p.max_blocks ? table[at] : -1;
+  return (unsigned)b < (unsigned)p.num_blocks ? b : -1;
+}
+// First row of a page of a key head in the pool seen as rows of head_dim values.
+__device__ __forceinline__ long long span_pool_row(const SpanParams& p, int block, int kvh, int page) {
+  return ((long long)block * p.hkv + kvh) * (16 * p.block_pages) + 16 * (page % p.block_pages);
+}
+
+__device__ __forceinline__ bool odd_bf16x2(uint32_t w) { return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u; }
+__device__ __forceinline__ bool odd_f16x2(uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
+}  // namespace
+}  // namespace fllm

@@ -289,6 +289,52 @@ void attention_prefill_tmem(const void* q, long long ldq, const void* k_cache, c
                             int mixed_rows = 0);   // > 0: shorter sequences are among them, and so many query rows in all
 size_t attention_tc_workspace_bytes(int tokens, int hq, int head_dim, int max_splits);
 
+// Attention under a window behind which the first tokens stay visible, and of the nodes of draft trees (attention_span.cu).
+struct SpanParams {
+  const void* q;               // bf16 [tokens, hq * head_dim], pitch ldq
+  long long ldq;
+  const void *k_cache, *v_cache;      // [num_blocks, hkv, 16 * block_pages, head_dim], bf16 or e4m3
+  const int* block_tables;     // [num_seqs, max_blocks]
+  int max_blocks, block_pages;
+  long long num_blocks;
+  const int* q_starts;         // [num_seqs + 1]
+  const int* kv_lens;          // [num_seqs]
+  const unsigned long long* tree_mask;      // [tokens, words] or null
+  const int* tree_base;        // [tokens]
+  int words;
+  void* out;                   // bf16 [tokens, hq * head_dim], pitch ldo
+  long long ldo;
+  const float* sinks;          // [hq] or null
+  int* status;
+  int tokens, num_seqs, hq, hkv, group, head_dim, kv_fp8;
+  int max_q_len, min_q_len, max_kv_len;
+  int window, first;           // window 0: no limit (first is 0 then)
+  float scale, scale_log2, softcap;
+  // set by the planner
+  int splits, min_pages;       // pieces of a sequence's visible tokens; fewest pages in one
+  int rows_from, rows_to;      // packed rows (query rows x group) of the sequences that a kernel takes: from < rows <= to
+  float* ws_o;                 // [tokens][hq][splits][head_dim]
+  float* ws_ml;                // [tokens][hq][splits][2]
+};
+size_t attention_span_workspace_bytes(SpanParams& p);      // plans the splits
+int attention_span(const SpanParams& p, cudaStream_t s);   // kernels launched
+
+// ---- rows of the cache pools (kv_moves.cu) ------------------------------------------
+struct KvPool {                // [planes][blocks][heads][block_size][row_bytes], a block's bytes contiguous
+  void* base;
+  long long plane_stride;      // bytes
+  int planes, heads, row_bytes;
+};
+constexpr int kMaxKvPools = 96;
+struct KvPools {
+  KvPool pool[kMaxKvPools];
+  int count, block_size, planes;      // planes: of all pools together
+  long long blocks;
+};
+int kv_copy_blocks(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s);
+int kv_compact(const KvPools& p, const int* block_tables, int max_blocks, const int* base, const int* path, int depth, const int* counts,
+               int seqs, int* status, cudaStream_t s);
+
 // ---- sampling -----------------------------------------------------------------------
 struct SampleRow {
   float temperature;         // <= 0: greedy

@@ -1,0 +1,165 @@
+// Rows and blocks of the cache pools that change places: copies of whole blocks (a fork that writes into a shared one) and the move of a
+// draft tree's accepted rows to the places behind the context that they would have had without the tree. Bytes are bytes here: the element
+// type only decides how wide an access may be.
+//
+// Both read and write what they move once and compute nothing; HBM bounds them where there is much to move and the launch where there is
+// little. Every pool and layer goes in one launch.
+#include <stdexcept>
+
+#include "fllm_ops.h"
+#include "ptx.cuh"
+#include "tma_host.h"
+
+namespace fllm {
+namespace {
+template <int V> struct Wide;
+template <> struct Wide<16> { using type = uint4; };
+template <> struct Wide<4> { using type = uint32_t; };
+template <> struct Wide<1> { using type = uint8_t; };
+
+__device__ __forceinline__ const KvPool& pool_of_plane(const KvPools& p, int& plane) {
+  int i = 0;
+  while (plane >= p.pool[i].planes) plane -= p.pool[i++].planes;
+  return p.pool[i];
+}
+
+constexpr int kCopyThreads = 256, kCopyEach = 4;       // accesses of a thread, all on their way at once
+
+template <int V>
+__global__ void __launch_bounds__(kCopyThreads) kv_copy_blocks_kernel(const __grid_constant__ KvPools p, const int* pairs, int n, int chunks, int* status) {
+  using T = typename Wide<V>::type;
+  int plane = blockIdx.x / chunks;
+  const int chunk = blockIdx.x - plane * chunks;
+  const KvPool& pool = pool_of_plane(p, plane);
+  const long long width = (long long)pool.heads * p.block_size * pool.row_bytes / V;       // of a block
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int i = blockIdx.y; i < n; i += gridDim.y) {
+    const int src = pairs[2 * i], dst = pairs[2 * i + 1];
+    if (src < 0 || dst < 0 || src >= p.blocks || dst >= p.blocks) {
+      if (threadIdx.x == 0 && status) atomicCAS(status, FLLM_OK, FLLM_ERR_BAD_ARGS);
+      continue;
+    }
+    T* base = reinterpret_cast<T*>(static_cast<uint8_t*>(pool.base) + plane * pool.plane_stride);
+    const T* from = base + src * width;
+    T* to = base + dst * width;
+    T v[kCopyEach];
+    const long long at = (long long)chunk * (kCopyThreads * kCopyEach) + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < kCopyEach; ++k)
+      if (at + k * kCopyThreads < width) v[k] = from[at + k * kCopyThreads];
+#pragma unroll
+    for (int k = 0; k < kCopyEach; ++k)
+      if (at + k * kCopyThreads < width) to[at + k * kCopyThreads] = v[k];
+  }
+}
+
+// A thread owns the same V bytes of every row of a sequence in one plane and head, and goes through the accepted path in its order: path[i] >= i
+// and rising, so no row is written before it has been read, whatever the rows of one path overwrite of each other.
+constexpr int kMoveThreads = 128, kMoveBatch = 8, kMoveSteps = 64;
+template <int V>
+__global__ void __launch_bounds__(kMoveThreads) kv_compact_kernel(const __grid_constant__ KvPools p, const int* tables, int max_blocks, const int* base,
+                                                                  const int* path, int depth, const int* counts, int chunks, int* status) {
+  using T = typename Wide<V>::type;
+  __shared__ long long from[kMoveSteps], to[kMoveSteps];       // rows of one head in front of the step's; to < 0: nothing moves
+  const int seq = blockIdx.y;
+  int plane = blockIdx.x / chunks;
+  const int chunk = blockIdx.x - plane * chunks;
+  const KvPool& pool = pool_of_plane(p, plane);
+  const int cols = pool.row_bytes / V;
+  const int at = chunk * kMoveThreads + threadIdx.x;           // (head, column)
+  const int head = at / cols, col = at - head * cols;
+  const bool mine = head < pool.heads;
+  T* rows = reinterpret_cast<T*>(static_cast<uint8_t*>(pool.base) + plane * pool.plane_stride);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int count = min(counts[seq], depth), b0 = base[seq];
+  const int* table = tables + (size_t)seq * max_blocks;
+  auto place = [&](int tok, long long& row) {                  // block and offset of a token; false: there is no such page
+    const int page = tok / p.block_size;
+    if (tok < 0 || page >= max_blocks) return false;
+    const int block = table[page];
+    if (block < 0 || block >= p.blocks) return false;
+    row = (long long)block * pool.heads * p.block_size + tok - page * p.block_size;
+    return true;
+  };
+  for (int s0 = 0; s0 < count; s0 += kMoveSteps) {
+    const int steps = min(kMoveSteps, count - s0);
+    if (threadIdx.x < steps) {
+      const int i = s0 + threadIdx.x, n = path[(size_t)seq * depth + i];
+      long long f = 0, t = -1;
+      if (n != i) {
+        if (n < i || b0 < 0 || !place(b0 + n, f) || !place(b0 + i, t)) {
+          t = -1;
+          if (status) atomicCAS(status, FLLM_OK, FLLM_ERR_BAD_ARGS);
+        }
+      }
+      from[threadIdx.x] = f;
+      to[threadIdx.x] = t;
+    }
+    __syncthreads();
+    if (mine) {
+      const long long shift = (long long)head * p.block_size;
+      for (int i0 = 0; i0 < steps; i0 += kMoveBatch) {
+        T v[kMoveBatch];
+#pragma unroll
+        for (int k = 0; k < kMoveBatch; ++k)
+          if (i0 + k < steps && to[i0 + k] >= 0) v[k] = rows[(from[i0 + k] + shift) * cols + col];
+#pragma unroll
+        for (int k = 0; k < kMoveBatch; ++k)
+          if (i0 + k < steps && to[i0 + k] >= 0) rows[(to[i0 + k] + shift) * cols + col] = v[k];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// widest access that all pools allow to whole blocks, or to rows
+int access_width(const KvPools& p, bool blocks) {
+  int v = 16;
+  for (int i = 0; i < p.count; ++i) {
+    const KvPool& q = p.pool[i];
+    const unsigned long long all = reinterpret_cast<uintptr_t>(q.base) | (unsigned long long)q.plane_stride |
+                                   (unsigned long long)q.row_bytes * (blocks ? q.heads * p.block_size : 1);
+    while (all & (v - 1)) v = v == 16 ? 4 : 1;
+  }
+  return v;
+}
+}  // namespace
+
+int kv_copy_blocks(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s) {
+  if (n <= 0 || p.planes <= 0) return 0;
+  const int v = access_width(p, true);
+  long long most = 0;
+  for (int i = 0; i < p.count; ++i) most = max(most, (long long)p.pool[i].heads * p.block_size * p.pool[i].row_bytes / v);
+  const long long chunks = (most + kCopyThreads * kCopyEach - 1) / (kCopyThreads * kCopyEach);
+  if (chunks * p.planes > 0x7fffffffLL) throw std::runtime_error("kv_copy_blocks: pools too large");
+  const dim3 grid((unsigned)(chunks * p.planes), (unsigned)min(n, 65535));
+  auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(kCopyThreads), 0, s, p, pairs, n, (int)chunks, status); };
+  if (v == 16) go(kv_copy_blocks_kernel<16>);
+  else if (v == 4) go(kv_copy_blocks_kernel<4>);
+  else go(kv_copy_blocks_kernel<1>);
+  cuda_check(cudaGetLastError(), "kv_copy_blocks launch");
+  return 1;
+}
+
+int kv_compact(const KvPools& p, const int* block_tables, int max_blocks, const int* base, const int* path, int depth, const int* counts,
+               int seqs, int* status, cudaStream_t s) {
+  if (seqs <= 0 || depth <= 0 || p.planes <= 0) return 0;
+  if (seqs > 65535) throw std::runtime_error("kv_compact: more than 65535 sequences");
+  const int v = access_width(p, false);
+  long long most = 0;
+  for (int i = 0; i < p.count; ++i) most = max(most, (long long)p.pool[i].heads * (p.pool[i].row_bytes / v));
+  const long long chunks = (most + kMoveThreads - 1) / kMoveThreads;
+  if (chunks * p.planes > 0x7fffffffLL || most > 0x3fffffffLL) throw std::runtime_error("kv_compact: pools too large");
+  const dim3 grid((unsigned)(chunks * p.planes), (unsigned)seqs);
+  auto go = [&](auto kernel) {
+    launch_pdl(kernel, grid, dim3(kMoveThreads), 0, s, p, block_tables, max_blocks, base, path, depth, counts, (int)chunks, status);
+  };
+  if (v == 16) go(kv_compact_kernel<16>);
+  else if (v == 4) go(kv_compact_kernel<4>);
+  else go(kv_compact_kernel<1>);
+  cuda_check(cudaGetLastError(), "kv_compact launch");
+  return 1;
+}
+}  // namespace fllm

@@ -67,6 +67,18 @@ class KVCache:
     def copy_block(self, src: int, dst: int) -> None:
         self.store[:, :, dst].copy_(self.store[:, :, src])
 
+    def pools(self) -> List[torch.Tensor]:
+        """The pool as [planes, blocks, heads, block_size, width], what the operators that move rows and blocks take."""
+        return [self.store.flatten(0, 1)]
+
+    def copy_blocks(self, pairs, ops) -> None:
+        """Blocks (source, destination) of all layers, as if one after the other."""
+        ops.kv_copy_blocks(self.pools(), pairs)
+
+    def compact(self, block_tables, base, path, counts, ops) -> None:
+        """The accepted rows of draft trees to the places behind their contexts (``ops.kv_compact``)."""
+        ops.kv_compact(self.pools(), block_tables, base, path, counts)
+
     @staticmethod
     def bytes_per_block(num_layers, kv_heads, block_size, head_dim, elem=2) -> int:
         return num_layers * 2 * kv_heads * block_size * head_dim * elem
@@ -76,6 +88,8 @@ class Decoder:
     def __init__(self, cfg: ModelConfig, weights: DecoderWeights, kv: KVCache, ops, spec: Optional[ShardSpec] = None,
                  tp_group=None, layer_range: Optional[range] = None, first_stage: bool = True,
                  last_stage: bool = True, rstate=None):
+        if cfg.window_first and (cfg.window_first < 0 or cfg.has_row_cache):
+            raise ValueError("window_first: first tokens that stay visible belong to layers that cache keys and values")
         self.cfg, self.w, self.kv, self.ops = cfg, weights, kv, ops
         self.rstate = rstate          # models.recurrent.RecurrentState when some layer is recurrent
         self.spec = spec or make_shard_spec(cfg)
@@ -201,7 +215,7 @@ class Decoder:
                               cfg.rms_eps, 1.0 if local_rope else self.attn_factor)
         a = ops.attention(q, kc, vc, b.block_tables, b.row_seq, b.positions, sp.hq_local, sp.hkv_local,
                           cfg.head_dim, self.scale, cfg.layer_window(li), lw.sinks, cfg.attn_softcap,
-                          meta=b)
+                          meta=b, first=cfg.window_first)
         if gated:                                # the attention output passes through a sigmoid gate of its own projection
             a = (a.float() * torch.sigmoid(ops.linear(h, lw.w_attn_gate).float())).to(a.dtype)
         return ops.linear(a, lw.wo, lw.bo, defer=defer_out and self._defer_out(lw.post_attn_norm))
@@ -458,7 +472,8 @@ class Decoder:
                                   sp.hq_local, sp.hkv_local, cfg.head_dim, cfg.rot_dim, self.rope_style,
                                   cfg.rms_eps, self.attn_factor)
             a = ops.attention(q, kc, vc, b.block_tables, b.row_seq, b.positions, sp.hq_local, sp.hkv_local,
-                              cfg.head_dim, self.scale, cfg.layer_window(li), lw.sinks, cfg.attn_softcap, meta=b)
+                              cfg.head_dim, self.scale, cfg.layer_window(li), lw.sinks, cfg.attn_softcap, meta=b,
+                              first=cfg.window_first)
             tp.linear_rs(a, lw.wo, lw.bo, bc)
             tp.norm(x, T, True, lw.ffn_norm, cfg.rms_eps, cfg.norm_weight_offset, bc)
             layout = getattr(lw, "glu_layout", 0)

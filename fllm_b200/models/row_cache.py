@@ -55,6 +55,19 @@ class RowCache:
         for t in self.rows + [f for f in self.factors + self.value_rows if f is not None]:
             t[dst].copy_(t[src])
 
+    def pools(self) -> List[torch.Tensor]:
+        """All tensors as [1, blocks, heads, block_size, width], what the operators that move rows and blocks take."""
+        rows = [t[:, None] if t.dim() == 3 else t for t in self.rows]
+        return [t[None] for t in rows + [f[..., None] for f in self.factors if f is not None] + [v for v in self.value_rows if v is not None]]
+
+    def copy_blocks(self, pairs, ops) -> None:
+        """Blocks (source, destination) of all layers, as if one after the other."""
+        ops.kv_copy_blocks(self.pools(), pairs)
+
+    def compact(self, block_tables, base, path, counts, ops) -> None:
+        """The accepted rows of draft trees to the places behind their contexts (``ops.kv_compact``)."""
+        ops.kv_compact(self.pools(), block_tables, base, path, counts)
+
     @staticmethod
     def specs(cfg: ModelConfig, layer_range) -> List[RowSpec]:
         out = []

@@ -16,6 +16,7 @@ from .latent import LatentNative
 from .maps import MapsNative
 from .prenorm import PreNormNative
 from .recurrent import RecurrentNative
+from .span import SpanNative, _check_span
 from .tied import TiedNative
 
 
@@ -34,7 +35,7 @@ class Deferred:
         return (self.rows, self.cols)
 
 
-class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNative):
+class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNative, SpanNative):
     name = "sm100a"
 
     def __init__(self, device: torch.device, workspace_bytes: int = 96 << 20, part: str = ""):
@@ -144,9 +145,14 @@ class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNa
 
     # ---------------------------------------------------------------- attention
     def attention(self, q, k_cache, v_cache, block_tables, row_seq, positions, hq, hkv, head_dim,
-                  scale, window=0, sinks=None, softcap=0.0, meta=None, bidirectional=False):
+                  scale, window=0, sinks=None, softcap=0.0, meta=None, bidirectional=False, first=0):
         """bidirectional: no causal mask (encoders); `positions` must then hold the last position of each row's
-        sequence (the generic kernel's visibility limit), the tensor-core kernels take the flag."""
+        sequence (the generic kernel's visibility limit), the tensor-core kernels take the flag. `first`: so many tokens
+        at the start of the text stay visible when the window has moved past them (causal, with `meta`; the rows of a
+        sequence are its last ones)."""
+        _check_span(window, first, bidirectional)
+        if first and window:
+            return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta)
         out = torch.empty(q.shape[0], hq * head_dim, dtype=q.dtype, device=q.device)
         kv8 = k_cache.element_size() == 1
         if (self.use_tc_attention and meta is not None and meta.q_starts is not None
@@ -195,10 +201,18 @@ class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNa
         return out
 
     def attention_tree(self, q, k_cache, v_cache, block_tables, row_seq, positions, tree_mask, tree_base, hq, hkv,
-                       head_dim, scale, window=0, sinks=None, softcap=0.0):
+                       head_dim, scale, window=0, sinks=None, softcap=0.0, first=0, meta=None):
         """Attention for the nodes of draft trees: row t sees the first tree_base[t] tokens of its sequence and the
         tree nodes whose bit is set in tree_mask[t] (int64, bit i = node i, stored at position tree_base[t] + i);
-        positions[t] = tree_base[t] + nodes - 1."""
+        positions[t] = tree_base[t] + nodes - 1. With `meta` (a sequence's rows are its nodes, seq_lens the positions
+        that are stored) the cache is read once for the rows and heads that share it, a mask may have several words
+        ([rows, words]), and `window` and `first` count places in the text: a node's is tree_base + its depth."""
+        _check_span(window, first)
+        if meta is not None:
+            return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta,
+                                        tree_mask, tree_base)
+        if first:
+            raise ValueError("attention_tree: first tokens need the step batch (meta)")
         out = torch.empty(q.shape[0], hq * head_dim, dtype=q.dtype, device=q.device)
         self.k.attention_generic(q, k_cache, v_cache, block_tables, row_seq, positions, out, hq, hkv, head_dim,
                                  float(scale), int(window), sinks, float(softcap), tree_mask, tree_base)

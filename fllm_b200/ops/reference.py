@@ -14,11 +14,12 @@ import torch.nn.functional as F
 from .latent import LatentRef
 from .maps import MapsRef
 from .prenorm import PreNormRef
+from .span import SpanRef, _check_span
 from .tied import TiedRef
 from .recurrent import RecurrentRef
 
 
-class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef):
+class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef, SpanRef):
     name = "reference"
 
     # ---------------------------------------------------------------- dense
@@ -120,9 +121,14 @@ class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef):
 
     # ---------------------------------------------------------------- attention
     def attention(self, q, k_cache, v_cache, block_tables, row_seq, positions, hq, hkv, head_dim,
-                  scale, window=0, sinks=None, softcap=0.0, meta=None, bidirectional=False):
+                  scale, window=0, sinks=None, softcap=0.0, meta=None, bidirectional=False, first=0):
         """`positions[t]` is the last visible token of row t: a causal decoder passes the row's own position, an
-        encoder (bidirectional) the last position of the row's sequence."""
+        encoder (bidirectional) the last position of the row's sequence. `first`: so many tokens at the start of the
+        text stay visible when the window has moved past them."""
+        _check_span(window, first, bidirectional)
+        if first and window:
+            return self.attention_first(q, k_cache, v_cache, block_tables, row_seq, positions, hq, hkv, head_dim, scale, window, first,
+                                        sinks, softcap)
         T = q.shape[0]
         bs = k_cache.shape[2]
         out = torch.empty(T, hq * head_dim, dtype=q.dtype, device=q.device)
@@ -173,8 +179,15 @@ class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef):
         return x
 
     def attention_tree(self, q, k_cache, v_cache, block_tables, row_seq, positions, tree_mask, tree_base, hq, hkv,
-                       head_dim, scale, window=0, sinks=None, softcap=0.0):
-        """Rows are nodes of draft trees: the context plus the ancestors named by a 64-bit mask per row."""
+                       head_dim, scale, window=0, sinks=None, softcap=0.0, first=0, meta=None):
+        """Rows are nodes of draft trees: the context plus the ancestors named by a 64-bit mask per row (with `meta`: by one
+        or more words, under a window and first tokens)."""
+        _check_span(window, first)
+        if meta is not None:
+            return self.attention_tree_span(q, k_cache, v_cache, block_tables, tree_mask, tree_base, hq, hkv, head_dim, scale, window,
+                                            sinks, softcap, first, meta)
+        if first:
+            raise ValueError("attention_tree: first tokens need the step batch (meta)")
         T = q.shape[0]
         bs = k_cache.shape[2]
         out = torch.empty(T, hq * head_dim, dtype=q.dtype, device=q.device)

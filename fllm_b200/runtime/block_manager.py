@@ -261,15 +261,15 @@ class BlockManager:
                 self.refs[b] += 1
         self.seqs[child_id] = SeqBlocks(list(p.table), p.num_tokens, list(p.hashes), p.first_live_block)
 
-    def prune_window(self, seq_id: int, window: int) -> int:
-        """Free blocks that lie entirely before the sliding window. Pruned entries stay in the
-        table as -1 so logical indices keep their meaning."""
+    def prune_window(self, seq_id: int, window: int, first: int = 0) -> int:
+        """Free blocks that lie entirely before the sliding window and hold none of the `first` tokens that stay
+        visible. Pruned entries stay in the table as -1 so logical indices keep their meaning."""
         sb = self.seqs[seq_id]
         if window <= 0:
             return 0
         first_needed = max(0, sb.num_tokens - window) // self.block_size
         freed = 0
-        for i in range(sb.first_live_block, min(first_needed, len(sb.table))):
+        for i in range(max(sb.first_live_block, self.blocks_needed(first)), min(first_needed, len(sb.table))):
             if sb.table[i] >= 0:
                 self._release(sb.table[i])
                 sb.table[i] = -1

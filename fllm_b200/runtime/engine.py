@@ -143,7 +143,7 @@ class LLMEngine:
         if self.rstate is not None:
             self.blocks.enable_state_slots(self.rstate.slots - 1)
         window = model_cfg.sliding_window if (model_cfg.sliding_window and model_cfg.window_pattern is None) else 0
-        self.scheduler = Scheduler(self.cfg, self.blocks, window)
+        self.scheduler = Scheduler(self.cfg, self.blocks, window, model_cfg.window_first)
         self.state_ckpt = None
         if self.rstate is not None and self.cfg.enable_prefix_caching:
             from .state_cache import StateCheckpoints
@@ -671,8 +671,8 @@ class LLMEngine:
     def _run_scheduled(self, step: ScheduledStep) -> List[TokenEvent]:
         """Forward + sample + commit of one scheduled step, waiting for its result."""
         events: List[TokenEvent] = []
-        for src, dst in step.cow:
-            self.kv.copy_block(src, dst)
+        if step.cow:
+            self.kv.copy_blocks(step.cow, self.ops)
         use_graph = self._graph_eligible(step)
         l0 = getattr(self.ops, "launches", 0)
         if use_graph:

@@ -52,11 +52,12 @@ class ScheduledStep:
 
 
 class Scheduler:
-    def __init__(self, cfg: EngineConfig, blocks: BlockManager, window: int = 0):
+    def __init__(self, cfg: EngineConfig, blocks: BlockManager, window: int = 0, window_first: int = 0):
         self.cfg, self.blocks = cfg, blocks
         self.waiting: Deque[Request] = deque()
         self.running: List[Request] = []
         self.window = window         # model-wide sliding window (0 when any layer attends fully)
+        self.window_first = window_first     # first tokens that stay visible behind it
         # swap preemption: the engine installs an object with swap_out(req) -> bool / swap_in(req) / drop(req)
         # that moves a request's KV blocks to host memory and back (rust/engine/src/kv_tier.rs)
         self.swapper = None
@@ -270,7 +271,7 @@ class Scheduler:
         if register:          # launch-ahead commits a placeholder first and registers once the id is known
             self.blocks.commit_tokens(r.seq_id, r.all_tokens, r.num_computed, self._salt(r))
         if self.window:
-            self.blocks.prune_window(r.seq_id, self.window)
+            self.blocks.prune_window(r.seq_id, self.window, self.window_first)
 
     def finish(self, r: Request, reason: str) -> None:
         if r in self.running:

@@ -1,0 +1,449 @@
+"""Attention under a window with first tokens that stay visible, draft trees over the cache, and moves inside the pools, on the kernels
+against fp64."""
+import math
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+import span_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from fllm_b200.ops.native import NativeOps
+    return NativeOps(torch.device("cuda:0"))
+
+
+def _window(ops, c, window, first, sinks=None, cap=0.0):
+    return ops.attention(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.hq, c.hkv, c.D, c.D ** -0.5, window, sinks, cap, meta=c.meta, first=first)
+
+
+def _tree(ops, c, window=0, first=0, sinks=None, cap=0.0):
+    return ops.attention_tree(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.masks, c.base, c.hq, c.hkv, c.D, c.D ** -0.5, window, sinks, cap,
+                              first=first, meta=c.meta)
+
+
+def _sinks(hq):
+    return torch.linspace(-3, 3, hq, device="cuda")
+
+
+HEADS = [(8, 2, 128), (16, 2, 64), (4, 4, 64), (5, 1, 128), (14, 2, 128), (32, 2, 64), (8, 4, 256)]
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,D", HEADS)
+@pytest.mark.parametrize("window,first,sink,cap", [(33, 4, False, 0.0), (128, 70, True, 0.0), (1, 1, False, 0.0), (250, 16, False, 20.0)])
+def test_window_rows(ops, hq, hkv, D, kv, window, first, sink, cap):
+    """Decode and short rows of sequences of many lengths, one of no row and ones shorter than the window or the first tokens."""
+    rows, ctx = [1, 2, 1, 0, 7, 1, 3], [0, 5, 300, 10, 129, 1777, 15]
+    c = so.setup(rows, ctx, hq, hkv, D, kv, seed=hq + D, fill=float("nan"))
+    s = _sinks(hq) if sink else None
+    y = _window(ops, c, window, first, s, cap)
+    so.check(y, *so.want(c, D ** -0.5, window, first, s, cap))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,D", HEADS)
+@pytest.mark.parametrize("window,first", [(64, 5), (500, 130), (17, 200)])
+def test_window_prompts(ops, hq, hkv, D, kv, window, first):
+    """Chunks of prompts beside decode rows, chunks from the first token on, tiles that end inside pages."""
+    rows, ctx = [130, 1, 257, 64], [0, 900, 411, 1]
+    c = so.setup(rows, ctx, hq, hkv, D, kv, seed=hq * D, fill=float("nan"))
+    y = _window(ops, c, window, first)
+    so.check(y, *so.want(c, D ** -0.5, window, first))
+    assert ops.check_status() == 0
+
+
+def test_window_long_prompt_with_sinks_and_cap(ops):
+    c = so.setup([700], [1300], 8, 2, 128, seed=3)
+    s = _sinks(8)
+    so.check(_window(ops, c, 600, 40, s, 15.0), *so.want(c, 128 ** -0.5, 600, 40, s, 15.0))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,D", HEADS)
+@pytest.mark.parametrize("window,first,sink", [(0, 0, False), (40, 3, True), (4, 2, False)])
+def test_tree(ops, hq, hkv, D, kv, window, first, sink):
+    """Trees of 1 to 200 nodes behind contexts of none to many tokens; windows that cut context and ancestors."""
+    nodes, ctx = [1, 13, 64, 3, 200, 65], [50, 0, 333, 1, 129, 1030]
+    c = so.setup(nodes, ctx, hq, hkv, D, kv, words=4, trees=[so.grow(n, n) for n in nodes], seed=D, fill=float("nan"))
+    s = _sinks(hq) if sink else None
+    y = _tree(ops, c, window, first, s)
+    so.check(y, *so.want(c, D ** -0.5, window, first, s))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("words", [1, 2, 3, 4])
+def test_tree_words_and_chains(ops, words):
+    """A chain is a plain causal chunk; masks of one to four words."""
+    n = 64 * words - 1
+    chain = list(range(-1, n - 1))
+    c = so.setup([n, 2], [77, 500], 8, 2, 128, words=words, trees=[chain, [-1, 0]], seed=words)
+    if words == 1:
+        c.masks = c.masks.view(-1)
+    y = _tree(ops, c)
+    so.check(y, *so.want(c, 128 ** -0.5, 0, 0))
+    plain = SimpleNamespace(**{**vars(c), "trees": None})
+    so.check(y, *so.want(plain, 128 ** -0.5, 0, 0))
+
+
+def test_tree_equals_the_kernel_without_a_step_batch(ops):
+    c = so.setup([30, 64], [100, 611], 8, 2, 128, words=1, trees=[so.grow(30, 1), so.grow(64, 2)], seed=11)
+    o, bound = so.want(c, 128 ** -0.5, 0, 0)
+    y = ops.attention_tree(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.masks.view(-1), c.base, 8, 2, 128, 128 ** -0.5)
+    so.check(y, o, bound)
+    so.check(_tree(ops, c), o, bound)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("hq", [2, 32])
+def test_rows_that_see_nothing(ops, D, hq):
+    """A mask of no bits behind an empty context: 0, with and without sinks; its neighbours are not disturbed."""
+    c = so.setup([20], [0], hq, 2, D, words=1, trees=[so.grow(20, 5)], seed=2)
+    c.masks[3] = 0
+    c.masks[11] = 0
+    for s in (None, _sinks(hq)):
+        o, bound = so.want(c, D ** -0.5, 0, 0, s)
+        y = _tree(ops, c, sinks=s)
+        keep = [i for i in range(20) if i not in (3, 11)]
+        so.check(y[keep], o[keep], bound[keep])
+        assert (y[[3, 11]] == 0).all()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,D", [(2, 2, 128), (8, 2, 128), (40, 2, 64), (4, 2, 256)])
+def test_infinities_and_nan_of_other_branches(ops, hq, hkv, D, kv):
+    """Keys and values of a node that only some rows see: the others are as if they were not there, the ones that see them get what the
+    formula gives."""
+    nodes = 40
+    par = [-1] + [max(0, i - 4) for i in range(1, nodes)]          # a root with four chains, one odd value in each
+    c = so.setup([nodes], [133], hq, hkv, D, kv, words=1, trees=[par], seed=5)
+    bad = {9: float("nan"), 22: float("inf"), 31: -float("inf")}
+    if kv == "e4m3":
+        bad = {9: float("nan"), 22: float("nan")}
+    for node, x in bad.items():
+        tok = 133 + node
+        blk, off = int(c.tables[0, tok // 16]), tok % 16
+        c.v[blk, :, off, 5] = x
+        c.values[0][tok, :, 5] = x
+    blk, off = int(c.tables[0, (133 + 16) // 16]), (133 + 16) % 16
+    c.k[blk, :, off, 3] = float("nan")
+    c.keys[0][133 + 16, :, 3] = float("nan")
+    seen = so.seen_rows(133, nodes, 0, 0, par)
+    y = _tree(ops, c).view(nodes, hq, D)
+    clean = [i for i in range(nodes) if not seen[i, [133 + n for n in list(bad) + [16]]].any()]
+    assert 0 < len(clean) < nodes
+    vals = torch.nan_to_num(c.values[0].float(), 0, 0, 0)
+    keys = torch.nan_to_num(c.keys[0].float(), 0, 0, 0)
+    o, bound = so.attend(c.q.view(nodes, hq, D), keys, vals, seen, D ** -0.5)
+    so.check(y[clean], o[clean], bound[clean])
+    for node, x in bad.items():
+        rows = [i for i in range(nodes) if seen[i, 133 + node] and not seen[i, 133 + 16] and not any(seen[i, 133 + n] for n in bad if n != node)]
+        assert rows
+        for i in rows:
+            assert (torch.isnan(y[i, :, 5]) if math.isnan(x) else y[i, :, 5] == x).all()
+            rest = [d for d in range(D) if d != 5]
+            so.check(y[i][:, rest], o[i][:, rest], bound[i][:, rest])
+    hit = [i for i in range(nodes) if seen[i, 133 + 16]]
+    assert torch.isnan(y[hit]).all()
+
+
+@pytest.mark.parametrize("hq,rows", [(2, 1), (8, 100)])
+def test_stale_values_behind_and_before_what_is_seen(ops, hq, rows):
+    """NaN in the rest of the last page, in pages that the window has passed and in tokens of its first page in front of it."""
+    ctx, window, first = 700, 90, 20
+    c = so.setup([rows], [ctx], hq, 2, 128, seed=8, fill=float("nan"))
+    o, bound = so.want(c, 128 ** -0.5, window, first)
+    for tok in range(first, ctx + 1 - window):
+        blk, off = int(c.tables[0, tok // 16]), tok % 16
+        c.v[blk, :, off] = float("nan")
+        c.k[blk, :, off] = float("inf")
+    for page in range(2, (ctx + 1 - window) // 16):
+        c.tables[0, page] = -1                        # freed
+    y = _window(ops, c, window, first)
+    so.check(y, o, bound)
+    assert ops.check_status() == 0
+
+
+def test_strided_queries_and_larger_blocks(ops):
+    c = so.setup([3, 150], [100, 200], 8, 2, 64, block=48, seed=4, q_pitch=8 * 64 + 264)
+    assert c.q.stride(0) == 8 * 64 + 264
+    y = _window(ops, c, 77, 9)
+    so.check(y, *so.want(c, 0.125, 77, 9))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_pools_of_more_than_32_bits(ops, kv, rows):
+    """Pages behind 2^32 bytes and 2^31 values of a pool."""
+    blocks = (1 << 31) // (8 * 16 * 128) + 500
+    c = so.setup([rows], [300], 16, 8, 128, kv, seed=6, pool_blocks=blocks)
+    assert int(c.tables.min()) * 8 * 16 * 128 > 1 << 31
+    y = _window(ops, c, 200, 30)
+    so.check(y, *so.want(c, 128 ** -0.5, 200, 30))
+    pools = [c.k[None], c.v[None]]
+    a = int(c.tables[0, 0])
+    ops.kv_copy_blocks(pools, [(a, 1), (a, blocks - 1)])
+    for t in (c.k, c.v):
+        assert torch.equal(t[1].view(torch.uint8), t[a].view(torch.uint8)) and torch.equal(t[blocks - 1].view(torch.uint8), t[a].view(torch.uint8))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 90])
+def test_pages_that_are_not_there(ops, rows):
+    """Entries of the block table that name no block are not followed; the status word says so."""
+    from fllm_b200.ops.native import NativeOps
+    mine = NativeOps(torch.device("cuda:0"), 1 << 20)
+    c = so.setup([rows], [300], 8, 2, 128, seed=9)
+    good = c.tables.clone()
+    for entry in (-1, c.k.shape[0], 1 << 30):
+        c.tables.copy_(good)
+        c.tables[0, 18] = entry
+        _window(mine, c, 200, 4)
+        assert mine.check_status() == 3
+    c.tables.copy_(good)
+    c.meta.seq_lens += 1 << 20                         # longer than its table
+    _window(mine, c, 100, 4)
+    assert mine.check_status() == 3
+
+
+def test_streams_graphs_and_many_calls(ops):
+    """On another stream, captured and replayed with other lengths and contents, two graphs replayed in turn, call after call."""
+    c = so.setup([1, 40, 3], [600, 100, 2000], 8, 2, 128, seed=12)
+    t = so.setup([30, 7], [500, 1500], 8, 2, 128, words=1, trees=[so.grow(30, 1), so.grow(7, 2)], seed=13)
+    w1, w2 = so.want(c, 128 ** -0.5, 300, 4), so.want(t, 128 ** -0.5, 0, 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = _window(ops, c, 300, 4)
+    side.synchronize()
+    so.check(y, *w1)
+    graphs, outs = [], []
+    for f in (lambda: _window(ops, c, 300, 4), lambda: _tree(ops, t)):
+        f()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(f())
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    so.check(outs[0], *w1)
+    so.check(outs[1], *w2)
+    # the same graph on shorter sequences: the lengths are read on the device
+    short = so.setup([1, 40, 3], [77, 0, 1999], 8, 2, 128, seed=14)
+    c.q.copy_(short.q)
+    c.tables.fill_(-1)
+    c.tables[:, :short.tables.shape[1]].copy_(short.tables)
+    c.meta.seq_lens.copy_(short.meta.seq_lens)
+    n = short.k.shape[0]
+    c.k[:n].copy_(short.k)
+    c.v[:n].copy_(short.v)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    so.check(outs[0], *so.want(short, 128 ** -0.5, 300, 4))
+    assert ops.check_status() == 0
+
+
+def test_same_call_same_bits(ops):
+    c = so.setup([33, 1, 256], [5000, 9000, 300], 16, 2, 128, seed=15)
+    first = _window(ops, c, 1000, 64)
+    for _ in range(5):
+        assert torch.equal(_window(ops, c, 1000, 64), first)
+
+
+def test_refusals(ops):
+    c = so.setup([2], [40], 4, 2, 64, words=1, trees=[[-1, 0]], seed=1)
+    call = lambda **kw: ops.attention(**{**dict(q=c.q, k_cache=c.k, v_cache=c.v, block_tables=c.tables, row_seq=c.row_seq, positions=c.positions, hq=4,
+                                                hkv=2, head_dim=64, scale=0.125, window=16, first=4, meta=c.meta), **kw})
+    bad = [dict(meta=None), dict(first=-1), dict(window=-3), dict(bidirectional=True), dict(q=c.q.float()), dict(q=c.q[:, 1:]), dict(scale=0.0),
+           dict(scale=float("nan")), dict(softcap=-1.0), dict(hkv=3), dict(head_dim=96), dict(k_cache=c.k[..., :32]), dict(v_cache=c.v.float()),
+           dict(k_cache=c.k.transpose(1, 2)), dict(block_tables=c.tables.long()), dict(sinks=torch.zeros(3, device="cuda")), dict(sinks=torch.zeros(4)),
+           dict(q=c.q.cpu())]
+    for kw in bad:
+        with pytest.raises((ValueError, RuntimeError)):
+            call(**kw)
+    tree = lambda **kw: ops.attention_tree(**{**dict(q=c.q, k_cache=c.k, v_cache=c.v, block_tables=c.tables, row_seq=c.row_seq, positions=c.positions,
+                                                     tree_mask=c.masks, tree_base=c.base, hq=4, hkv=2, head_dim=64, scale=0.125, meta=c.meta), **kw})
+    tree()
+    for kw in [dict(tree_mask=c.masks.int()), dict(tree_mask=c.masks[:1]), dict(tree_mask=c.masks.expand(2, 5).contiguous()), dict(tree_base=c.base.long()),
+               dict(meta=None, first=2, tree_mask=c.masks.view(-1)), dict(window=-1)]:
+        with pytest.raises((ValueError, RuntimeError)):
+            tree(**kw)
+    pool = torch.zeros(3, 6, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    for args in [([], [(0, 1)]), ([pool], [(0, 6)]), ([pool], [(-1, 2)]), ([pool], i32([0, 1])), ([pool], i32([[0, 1]]).long()), ([pool[0]], [(0, 1)]),
+                 ([pool.transpose(2, 3)], i32([[0, 1]])), ([pool, pool[:, :5]], i32([[0, 1]])), ([pool.cpu()], i32([[0, 1]]))]:
+        with pytest.raises((ValueError, RuntimeError, IndexError)):
+            ops.kv_copy_blocks(*args)
+    ok = (i32([[0, 1]]), i32([3]), i32([[0, 2]]), i32([2]))
+    ops.kv_compact([pool], *ok)
+    for k, x in [(0, i32([0, 1])), (0, i32([[0, 1]]).long()), (1, i32([])), (2, i32([0, 2])), (3, torch.tensor([2], dtype=torch.int32))]:
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.kv_compact([pool], *[x if k == j else a for j, a in enumerate(ok)])
+    assert ops.check_status() == 0
+
+
+# ------------------------------------------------------------------------------------------ moves
+def _pools(kind, blocks, bs=16):
+    g = torch.Generator(device="cuda").manual_seed(blocks)
+    bits = lambda *s: torch.randint(0, 256, s, generator=g, device="cuda", dtype=torch.uint8)
+    as_type = lambda x, t: x.view(t)
+    if kind == "kv":
+        return [as_type(bits(6, blocks, 3, bs, 256), torch.bfloat16)]
+    if kind == "e4m3":
+        return [as_type(bits(4, blocks, 2, bs, 64), torch.float8_e4m3fn)]
+    if kind == "planes":                     # every second plane of a larger tensor
+        return [as_type(bits(5, 2, blocks, 2, bs, 128), torch.bfloat16)[:, 1]]
+    if kind == "rows":                       # a latent row, heads with a factor each, value rows of another width
+        return [as_type(bits(1, blocks, 1, bs, 1152), torch.bfloat16), as_type(bits(1, blocks, 4, bs, 4), torch.float32), as_type(bits(1, blocks, 4, bs, 192), torch.bfloat16)]
+    if kind == "odd":                        # rows of 6 bytes
+        return [as_type(bits(2, blocks, 3, bs, 6), torch.bfloat16)]
+    return [as_type(bits(1, blocks, 1, bs, 16), torch.bfloat16) for _ in range(100)]
+
+
+def _same(a, b):
+    return all(torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8)) for x, y in zip(a, b))
+
+
+KINDS = ["kv", "e4m3", "planes", "rows", "odd", "many"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("bs", [16, 5])
+def test_copies_of_blocks(ops, kind, bs):
+    from fllm_b200.ops.reference import RefOps
+    pools = _pools(kind, 23, bs)
+    ref = [t.clone() for t in pools]
+    pairs = [(0, 22), (5, 6), (7, 8), (7, 9), (11, 11)]
+    RefOps().kv_copy_blocks(ref, pairs)
+    ops.kv_copy_blocks(pools, torch.tensor(pairs, dtype=torch.int32, device="cuda"))
+    assert _same(pools, ref)
+    chain = [(1, 2), (2, 3), (4, 2), (3, 1), (1, 4), (1, 5)]          # a list means one after the other
+    RefOps().kv_copy_blocks(ref, chain)
+    ops.kv_copy_blocks(pools, chain)
+    assert _same(pools, ref)
+    ops.kv_copy_blocks(pools, [])
+    ops.kv_copy_blocks(pools, torch.zeros(0, 2, dtype=torch.int32, device="cuda"))
+    assert _same(pools, ref) and ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("bs", [16, 5])
+def test_accepted_rows(ops, kind, bs):
+    """Paths whose sources and destinations overlap, longer than a batch and than a thread block's list, of no node and of one."""
+    from fllm_b200.ops.reference import RefOps
+    pools = _pools(kind, 120, bs)
+    ref = [t.clone() for t in pools]
+    paths = [[0, 1, 2], [0, 2, 3, 7, 8, 9, 10, 11, 12, 13, 14, 40], [], [1], list(range(3, 93)), [5, 6, 7]]
+    counts = [3, 12, 0, 1, 90, 2]
+    depth = 95
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    per = -(-140 // bs)
+    tables = torch.full((6, per), -1, dtype=torch.int32)
+    order = torch.randperm(120, generator=torch.Generator().manual_seed(3)).int()
+    used = [-(-n // bs) for n in (20, 60, 1, 9, 130, 16)]
+    for s, n in enumerate(used):
+        tables[s, :n] = order[sum(used[:s]):sum(used[:s]) + n]
+    args = (tables.cuda(), i32([3, 17, 0, 5, 30, 8]), i32([p + [-7] * (depth - len(p)) for p in paths]), i32(counts))
+    RefOps().kv_compact(ref, *args)
+    ops.kv_compact(pools, *args)
+    assert _same(pools, ref) and ops.check_status() == 0
+
+
+def test_moves_that_name_no_block(ops):
+    from fllm_b200.ops.native import NativeOps
+    mine = NativeOps(torch.device("cuda:0"), 1 << 20)
+    pools = _pools("kv", 20)
+    ref = [t.clone() for t in pools]
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    mine.kv_copy_blocks(pools, i32([[0, 20], [-1, 3], [1 << 30, 2]]))
+    assert mine.check_status() == 3 and _same(pools, ref)
+    for base, path in [(0, [0, 70]), (40, [0, 5]), (-9, [0, 2]), (4, [3, 0])]:
+        mine.kv_compact(pools, i32([[1, -1, 30]]), i32([base]), i32([path]), i32([2]))
+        assert mine.check_status() == 3
+        if path != [3, 0]:
+            assert _same(pools, ref)
+
+
+def test_moves_in_graphs_and_on_other_streams(ops):
+    from fllm_b200.ops.reference import RefOps
+    pools = _pools("kv", 30)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    pairs, path, counts = i32([[0, 1], [2, 3]]), i32([[0, 2, 5]]), i32([3])
+    tables, base = i32([[7, 8, 9]]), i32([14])
+    side = torch.cuda.Stream()
+    ref = [t.clone() for t in pools]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.kv_copy_blocks(pools, pairs)
+        ops.kv_compact(pools, tables, base, path, counts)
+    side.synchronize()
+    RefOps().kv_copy_blocks(ref, pairs)
+    RefOps().kv_compact(ref, tables, base, path, counts)
+    assert _same(pools, ref)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.kv_copy_blocks(pools, pairs)
+        ops.kv_compact(pools, tables, base, path, counts)
+    pairs.copy_(i32([[4, 5], [6, 10]]))
+    path.copy_(i32([[0, 1, 4]]))
+    g.replay()
+    torch.cuda.synchronize()
+    RefOps().kv_copy_blocks(ref, pairs)
+    RefOps().kv_compact(ref, tables, base, path, counts)
+    assert _same(pools, ref) and ops.check_status() == 0
+
+
+# ------------------------------------------------------------------------------------------ together
+@pytest.mark.parametrize("window,first", [(0, 0), (50, 4)])
+def test_tree_step_and_the_plain_step_after_it(ops, window, first):
+    """A forked sequence (its shared last block copied) runs a tree step; the accepted path's rows move to their places; a plain step on the
+    compacted cache sees exactly what a step after the accepted tokens alone would see."""
+    from fllm_b200.models.decoder import KVCache
+    from fllm_b200.runtime.speculative import DraftTree
+    hq, hkv, D, ctx = 8, 2, 128, 133
+    tree = DraftTree([5, 6, 7, 8, 9, 10, 11], [-1, 0, 0, 1, 2, 2, 5])
+    kv = KVCache(3, 40, hkv, 16, D, "cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    text = torch.randn(3, 2, ctx, hkv, D, generator=g, device="cuda").bfloat16()
+    node = torch.randn(3, 2, len(tree), hkv, D, generator=g, device="cuda").bfloat16()
+    table = list(range(10, 20))
+    for j in range(ctx):
+        kv.store[:, :, table[j // 16], :, j % 16] = text[:, :, j]
+    kv.copy_blocks([(table[8], 30)], ops)              # the block that is written next was shared
+    table[8] = 30
+    for i in range(len(tree)):
+        kv.store[:, :, table[(ctx + i) // 16], :, (ctx + i) % 16] = node[:, :, i]
+    assert torch.equal(kv.store[:, :, 18, :, 5], torch.zeros_like(kv.store[:, :, 18, :, 5]))           # the parent's copy has none of it
+    M = len(tree)
+    q = torch.randn(M, hq * D, generator=g, device="cuda").bfloat16()
+    meta = SimpleNamespace(q_starts=i32([0, M]), seq_lens=i32([ctx + M]), num_seqs=1, num_tokens=M, max_q_len=M, min_q_len=M, max_kv_len=ctx + M)
+    masks = torch.tensor(tree.masks_i64(), device="cuda")
+    for layer in range(3):
+        y = ops.attention_tree(q, kv.k(layer), kv.v(layer), i32([table]), i32([0] * M), i32([ctx + M - 1] * M), masks, i32([ctx] * M), hq, hkv, D,
+                               D ** -0.5, window, first=first, meta=meta)
+        o, b = so.attend(q.view(M, hq, D), torch.cat([text[layer, 0], node[layer, 0]]), torch.cat([text[layer, 1], node[layer, 1]]),
+                         so.seen_rows(ctx, M, window, first, tree.parents), D ** -0.5)
+        so.check(y.view(M, hq, D), o, b)
+    path, bonus = tree.verify_greedy(5, [7, 0, 10, 0, 0, 11, 3])
+    assert path == [0, 2, 5, 6] and bonus == 3
+    kv.compact(i32([table]), i32([ctx]), i32([path]), i32([len(path)]), ops)
+    n = ctx + len(path)
+    q1 = torch.randn(1, hq * D, generator=g, device="cuda").bfloat16()
+    meta = SimpleNamespace(q_starts=i32([0, 1]), seq_lens=i32([n]), num_seqs=1, num_tokens=1, max_q_len=1, min_q_len=1, max_kv_len=n)
+    for layer in range(3):
+        y = ops.attention(q1, kv.k(layer), kv.v(layer), i32([table]), i32([0]), i32([n - 1]), hq, hkv, D, D ** -0.5, window, meta=meta, first=first)
+        k, v = (torch.cat([text[layer, i], node[layer, i][path]]) for i in (0, 1))
+        o, b = so.attend(q1.view(1, hq, D), k, v, so.seen_rows(n - 1, 1, window, first), D ** -0.5)
+        so.check(y.view(1, hq, D), o, b)
+    assert ops.check_status() == 0
