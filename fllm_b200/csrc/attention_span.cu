@@ -79,7 +79,7 @@ struct RowsSmem {
 };
 
 template <int D, bool KV8>
-__global__ void __launch_bounds__(128) span_rows_kernel(const SpanParams p) {
+__global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ SpanParams p) {
   using S = RowsSmem<D, KV8>;
   extern __shared__ __align__(128) uint8_t smem[];
   bf16* qtile = reinterpret_cast<bf16*>(smem);
@@ -394,15 +394,25 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const SpanParams p) {
   }
 }
 
-// Joins the splits of a row: one warp per (token, head).
+// Joins the splits of a row: one warp per (token, head). `some`: only sequences of p.rows_from < packed rows <= p.rows_to were split.
 template <int D>
-__global__ void __launch_bounds__(128) span_merge_kernel(const SpanParams p) {
+__global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__ SpanParams p, int some) {
   pdl_launch_dependents();
   pdl_wait();
   const int pair = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (pair >= p.tokens * p.hq) return;
   const int tok = pair / p.hq, head = pair - tok * p.hq;
   if (tok < p.q_starts[0] || tok >= p.q_starts[p.num_seqs]) return;      // rows of no sequence stay as they are
+  if (some) {
+    int lo = 0, hi = p.num_seqs;                       // the last sequence that begins at or before tok
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (p.q_starts[mid] <= tok) lo = mid;
+      else hi = mid;
+    }
+    const int rows = (p.q_starts[lo + 1] - p.q_starts[lo]) * p.group;
+    if (rows <= p.rows_from || rows > p.rows_to) return;
+  }
   const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + (size_t)pair * p.splits;
   const float* part = p.ws_o + (size_t)pair * p.splits * D + lane;
   const float sk = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
@@ -452,37 +462,70 @@ void launch_rows(const SpanParams& p, cudaStream_t s) {
   launch_pdl(span_rows_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(128), RowsSmem<D, KV8>::kTotal, s, p);
 }
 template <int D>
-int launch(const SpanParams& p, cudaStream_t s) {
-  if (p.kv_fp8) launch_rows<D, true>(p, s);
-  else launch_rows<D, false>(p, s);
-  if (p.splits == 1) return 1;
-  launch_pdl(span_merge_kernel<D>, dim3((unsigned)(((long long)p.tokens * p.hq + 3) / 4)), dim3(128), 0, s, p);
-  return 2;
+void launch_merge(const SpanParams& p, bool some, cudaStream_t s) {
+  launch_pdl(span_merge_kernel<D>, dim3((unsigned)(((long long)p.tokens * p.hq + 3) / 4)), dim3(128), 0, s, p, some ? 1 : 0);
 }
+void merge(const SpanParams& p, bool some, cudaStream_t s) {
+  if (p.head_dim == 64) launch_merge<64>(p, some, s);
+  else if (p.head_dim == 128) launch_merge<128>(p, some, s);
+  else launch_merge<256>(p, some, s);
+}
+size_t partial_floats(const SpanParams& p, int splits) { return splits > 1 ? (size_t)p.tokens * p.hq * splits * (p.head_dim + 2) : 0; }
 }  // namespace
 
-size_t attention_span_workspace_bytes(SpanParams& p) {
-  const long long rows = (long long)p.max_q_len * p.group;
-  p.rows_from = 0;
-  p.rows_to = INT_MAX;
-  const long long ctas = (rows + kSpanRows - 1) / kSpanRows * p.num_seqs * p.hkv;
-  const long long span = p.window > 0 ? (long long)p.window + p.first + p.max_q_len : p.max_kv_len;
-  const long long pages = (std::min<long long>(span, p.max_kv_len) + kPage - 1) / kPage;
-  p.min_pages = 8;
-  long long splits = 1;
-  if (ctas < 4 * sm_count()) splits = std::min<long long>((4LL * sm_count() + ctas - 1) / ctas, (pages + p.min_pages - 1) / p.min_pages);
-  p.splits = (int)std::max<long long>(1, std::min<long long>(splits, 128));
-  return p.splits == 1 ? 0 : (size_t)p.tokens * p.hq * p.splits * (p.head_dim + 2) * sizeof(float);
+SpanPlan attention_span_plan(const SpanParams& p) {
+  SpanPlan plan{};
+  const bool tc = attention_span_tc_supported(p);
+  const long long most = (long long)p.max_q_len * p.group;
+  const long long span = std::min<long long>(p.window > 0 ? (long long)p.window + p.first + p.max_q_len : p.max_kv_len, p.max_kv_len);
+  if (!tc || (long long)p.min_q_len * p.group <= kSpanRows) {
+    const long long ctas = ((tc ? std::min<long long>(most, kSpanRows) : most) + kSpanRows - 1) / kSpanRows * p.num_seqs * p.hkv;
+    const long long pages = (span + kPage - 1) / kPage;
+    plan.min_pages = 8;
+    long long splits = 1;
+    if (ctas < 4 * sm_count()) splits = std::min<long long>((4LL * sm_count() + ctas - 1) / ctas, (pages + plan.min_pages - 1) / plan.min_pages);
+    plan.rows_splits = (int)std::max<long long>(1, std::min<long long>(splits, 128));
+  }
+  if (tc && most > kSpanRows) {
+    const long long ctas = (most + 255) / 256 * p.num_seqs * p.hkv, tiles = (span + 127) / 128 + (p.first > 0 ? 1 : 0);
+    plan.min_tiles = (int)std::max<long long>(1, ctas * tiles / (6LL * sm_count()));
+    plan.tile_splits = (int)std::max<long long>(1, std::min<long long>((tiles + plan.min_tiles - 1) / plan.min_tiles, 32));
+    if (ctas >= 2 * sm_count()) plan.tile_splits = 1;
+  }
+  plan.bytes = (partial_floats(p, plan.rows_splits) + partial_floats(p, plan.tile_splits)) * sizeof(float);
+  return plan;
 }
 
-int attention_span(const SpanParams& p, cudaStream_t s) {
-  if (p.tokens <= 0 || p.num_seqs <= 0) return 0;
-  int n;
-  switch (p.head_dim) {
-    case 64: n = launch<64>(p, s); break;
-    case 128: n = launch<128>(p, s); break;
-    case 256: n = launch<256>(p, s); break;
-    default: throw std::runtime_error("attention_span: head_dim must be 64, 128 or 256");
+int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStream_t s) {
+  int n = 0;
+  const bool both = plan.rows_splits > 0 && plan.tile_splits > 0;
+  p.min_pages = plan.min_pages;
+  p.min_tiles = plan.min_tiles;
+  auto take = [&](int splits) {
+    p.splits = splits;
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_ml = p.ws_o + (size_t)p.tokens * p.hq * splits * p.head_dim;
+    workspace = p.ws_o + partial_floats(p, splits);
+  };
+  if (plan.tile_splits > 0) {
+    take(plan.tile_splits);
+    p.rows_from = kSpanRows;
+    p.rows_to = INT_MAX;
+    attention_span_tc(p, s);
+    ++n;
+    if (p.splits > 1) { merge(p, both, s); ++n; }
+  }
+  if (plan.rows_splits > 0) {
+    take(plan.rows_splits);
+    p.rows_from = 0;
+    p.rows_to = attention_span_tc_supported(p) ? kSpanRows : INT_MAX;
+    switch (p.head_dim) {
+      case 64: p.kv_fp8 ? launch_rows<64, true>(p, s) : launch_rows<64, false>(p, s); break;
+      case 128: p.kv_fp8 ? launch_rows<128, true>(p, s) : launch_rows<128, false>(p, s); break;
+      default: p.kv_fp8 ? launch_rows<256, true>(p, s) : launch_rows<256, false>(p, s); break;
+    }
+    ++n;
+    if (p.splits > 1) { merge(p, both, s); ++n; }
   }
   cuda_check(cudaGetLastError(), "attention_span launch");
   return n;

@@ -1,0 +1,699 @@
+// Attention of attention_span.cuh on the fifth-generation tensor cores: sequences with more than 16 packed rows (query row x head of a key
+// head), that is draft trees and chunks of prompts.
+//
+// One CTA owns up to 256 packed rows of one sequence and key head and walks the tokens that they see between them, 128 at a time; a split of
+// the walk leaves partial sums for span_merge_kernel. S = Q K^T and O += P V are tcgen05.mma with their accumulators in tensor memory
+// (two of S, two of O: all 512 columns). Two softmax groups of four warps, a thread to a row, work on two items at a time, so that one's
+// exponentials run under the other's products:
+//
+//   more than 128 rows   items are (token tile, row tile): both row tiles read the same K and V
+//   up to 128 rows       items are token tiles: the groups take them in turn, for the same rows, and join (m, l, O) at the end
+//
+//   warps 0 - 7   softmax        warp 9   issuer
+//   bf16 cache    warps 8, 10 ask for K by TMA, warp 11 for V; it also looks through V where not every row sees the whole tile
+//   e4m3 cache    warp 8 asks for K and V as they are; warps 8, 10, 11 widen them to f16 operands in 128-byte swizzled rows
+//
+// What a row sees of a tile is four words of bits, from its bounds and its mask; tiles that all rows of a warp see whole have code
+// without them. Values of places that some row does not see may be infinite or NaN: they are taken out of the tile there, and rows that
+// do see them get them in the end from the cache (slow, and never taken otherwise). Every wait is bounded (ptx.cuh).
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <limits.h>
+
+#include <algorithm>
+
+#include "attention_span.cuh"
+#include "attention_util.cuh"
+#include "tma_host.h"
+
+namespace fllm {
+namespace {
+constexpr int kTcThreads = 384, kTcRows = 256;
+constexpr float kTcLift = 6.f;             // f16 weights: their reference lies so far below the row's (their largest is 2^14 then)
+constexpr int kTilePages = kTile / kPage;
+
+// Shared memory: two tiles of Q, two stages of K and of V, 16-bit values in rows of 128 bytes; e4m3: two slots of raw tiles (four where
+// there is one tile of Q).
+template <int D, bool KV8>
+struct TcSmem {
+  static constexpr int kT = tile_bytes<D>();           // a 128-row tile of 16-bit values
+  static constexpr int kRaw = KV8 ? kTile * D : 0;
+  static constexpr int kTiles = 6 * kT + 2 * kRaw;
+  static constexpr int kTotal = kTiles + 256 + kTcRows * 4 + 64 + 1024;
+};
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_16(float lo, float hi) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
+// bits [lo, hi) of 32
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 32);
+  return hi <= lo ? 0u : (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
+}
+
+// What a row sees of the 128 tokens from tok0 on.
+__device__ __forceinline__ void row_bits(const SpanParams& p, int tok0, int base, int beg, int q0, int qn, int kv_len, int qi, uint32_t (&vis)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int t = tok0 + 32 * c;
+    vis[c] = bits_between(beg - t, base - t) | bits_between(0, min(p.first, base) - t);
+  }
+  if (p.tree_mask && tok0 + kTile > base && qi >= 0) {
+    unsigned long long bits[kSpanWords + 1] = {0, 0, 0, 0, 0};
+    span_row(p, q0, qn, kv_len, qi, bits);
+    const unsigned long long* b = bits;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int n = tok0 + 32 * c - base;              // node of the word's first token
+      uint32_t w = 0;
+      if (n < 0) w = n > -32 ? (uint32_t)(b[0] << -n) : 0u;
+      else if (n < 64 * kSpanWords) w = (uint32_t)((b[n >> 6] >> (n & 63)) | ((n & 63) ? b[(n >> 6) + 1] << (64 - (n & 63)) : 0ull));
+      vis[c] |= w;
+    }
+  }
+}
+
+// A row's softmax over one tile of 128 tokens: scores in registers, weights as 16-bit values over the scores' first columns, the first 64 of them
+// handed over before the others are computed; O of the warp is rescaled when a row's maximum has moved by more than 2^8.
+template <int D, bool MASKED, bool CAPPED, bool F16>
+__device__ __forceinline__ void softmax_tile(const SpanParams& p, uint32_t t_s, uint32_t t_o, const uint32_t (&vis)[4], float factor, bool have_o,
+                                             uint64_t* p_half, float& m_used, float& l) {
+  const float cap_in = CAPPED ? factor / (p.softcap * kLog2e) : 0.f;
+  const float scale = CAPPED ? p.softcap * kLog2e : factor;
+  uint32_t s[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, s[c]);
+  tmem_ld_wait();
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 128; i += 2) {
+    float a[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      a[k] = __uint_as_float(s[i >> 5][(i & 31) + k]);
+      if (CAPPED) { a[k] = tanhf(a[k] * cap_in); s[i >> 5][(i & 31) + k] = __float_as_uint(a[k]); }
+      if (MASKED && !(vis[i >> 5] >> ((i & 31) + k) & 1)) a[k] = -INFINITY;
+    }
+    mx[(i >> 1) & 3] = fmaxf(fmaxf(mx[(i >> 1) & 3], a[0]), a[1]);
+  }
+  // the scale is positive, so it commutes with the maximum
+  const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+  const bool grow = m > m_used + kLazyRescale || (m_used == -INFINITY && m > -INFINITY);
+  if (__any_sync(0xffffffffu, grow)) {
+    const float m_new = fmaxf(m_used, m);
+    const float corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
+    m_used = m_new;
+    l *= corr;
+    if (have_o) {
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16];
+        tmem_ld_32x16(t_o + 16 * c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+        tmem_st_32x16(t_o + 16 * c, o);
+      }
+    }
+  }
+  const float m_ref = m_used == -INFINITY ? 0.f : m_used - (F16 ? kTcLift : 0.f);
+  uint64_t sum[2] = {0, 0};
+  const uint64_t scale2 = pack2(scale, scale), ref2 = pack2(-m_ref, -m_ref);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const uint64_t x = fma2(pack2(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])), scale2, ref2);
+      float2 e = unpack2(x);
+      e.x = ex2(e.x); e.y = ex2(e.y);
+      if (MASKED) {
+        if (!(vis[c] >> j & 1)) e.x = 0.f;
+        if (!(vis[c] >> (j + 1) & 1)) e.y = 0.f;
+      }
+      sum[j >> 1 & 1] = add2(sum[j >> 1 & 1], pack2(e.x, e.y));
+      w[j >> 1] = pack_16<F16>(e.x, e.y);
+    }
+    tmem_st_32x16(t_s + 16 * c, w);
+    if (c == 1) {
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(p_half);
+    }
+  }
+  const float2 l0 = unpack2(sum[0]), l1 = unpack2(sum[1]);
+  l += (l0.x + l0.y) + (l1.x + l1.y);
+  tmem_st_wait();
+}
+
+// Queries of rows [0, tiles x 128) to shared memory in swizzled rows, by the 256 threads of the softmax groups. f16 (beside an e4m3 cache): times a
+// power of two per row, which leaves the factor of its scores; bf16: asynchronous copies.
+template <int D, bool F16>
+__device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* factors, int tiles, int q0, int row0, int n_rows, int kvh) {
+  constexpr int C = D / 8;
+  const int G = p.group;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < tiles * kRows * C; i += 256) {
+    const int r = i / C, c = i % C, rr = r & (kRows - 1);
+    const bool valid = r < n_rows;
+    const int qi = valid ? (row0 + r) / G : 0, hg = valid ? (row0 + r) - qi * G : 0;
+    const bf16* src = static_cast<const bf16*>(p.q) + (size_t)(q0 + qi) * p.ldq + (size_t)(kvh * G + hg) * D + c * 8;
+    uint8_t* dst = sq + (r >> 7) * tile_bytes<D>() + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+    if constexpr (F16) {
+      uint4 v = valid ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+      uint32_t top = 0;                    // largest exponent field of the row, infinities and NaN aside
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t a = w[e] >> 7 & 0xFF, b = w[e] >> 23 & 0xFF;
+        if (a != 0xFF) top = max(top, a);
+        if (b != 0xFF) top = max(top, b);
+      }
+#pragma unroll
+      for (int o = C / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int up = top ? min(max(127 + 14 - (int)top, -100), 100) : 0;
+      const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = unpack_bf16x2(w[e]);
+        w[e] = pack_16<true>(x.x * f, x.y * f);
+      }
+      if (c == 0) factors[r] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+      *reinterpret_cast<uint4*>(dst) = v;
+    } else {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+      if (c == 0) factors[r] = p.scale_log2;
+    }
+  }
+  if constexpr (!F16) asm volatile("cp.async.wait_all;" ::: "memory");
+  fence_proxy_async_smem();
+}
+
+// First pool row of a page of a tile, or `none` (behind the pool: TMA fills it with zeros) for pages that nobody sees and pages that are not there.
+struct PageRows {
+  const SpanParams& p;
+  const int* table;
+  int kvh, head_end, lo, end, none;        // pages [0, head_end) and [lo, end) are seen
+  __device__ __forceinline__ int operator()(int page, bool& bad) const {
+    if (!(page < head_end || (page >= lo && page < end))) return none;
+    const int b = span_block(p, table, page);
+    bad |= b < 0;
+    return b < 0 ? none : (int)span_pool_row(p, b, kvh, page);
+  }
+};
+
+// Infinities and NaN of 16-bit values set to zero; true if there were any.
+__device__ __forceinline__ uint32_t without_odd_bf16(uint32_t w) {
+  return ((w & 0x7F80u) == 0x7F80u ? 0u : w & 0xFFFFu) | ((w & 0x7F800000u) == 0x7F800000u ? 0u : w & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint32_t without_odd_f16(uint32_t w) {
+  return ((w & 0x7C00u) == 0x7C00u ? 0u : w & 0xFFFFu) | ((w & 0x7C000000u) == 0x7C000000u ? 0u : w & 0xFFFF0000u);
+}
+
+template <int D, bool KV8>
+__global__ void __launch_bounds__(kTcThreads, 1)
+span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ SpanParams p, int row_tiles) {
+  using S = TcSmem<D, KV8>;
+  constexpr int TB = S::kT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sq = smem, *sk = smem + 2 * TB, *sv = smem + 4 * TB;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kTiles);
+  uint64_t *k_full = bars, *v_full = bars + 2, *k_empty = bars + 4, *v_empty = bars + 6;      // [2] by stage
+  uint64_t *s_full = bars + 8, *p_half = bars + 10, *p_ready = bars + 12;                     // [2] by softmax group
+  uint64_t* v_ready = bars + 14;                                                              // [2] by stage: looked through, or widened
+  uint64_t *o_done = bars + 16, *q_full = bars + 17;
+  uint64_t *raw_full = bars + 18, *raw_empty = bars + 22;                                     // [4] by slot
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* seen = reinterpret_cast<int*>(tmem_slot + 2);        // smallest and largest base, smallest and largest window begin, odd values met
+  float* factors = reinterpret_cast<float*>(smem + S::kTiles + 256);
+  static_assert(27 * 8 + 24 <= 256, "barriers and flags");
+
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  pdl_wait();
+  const int split = blockIdx.y;
+  int rest = blockIdx.x;
+  const int kvh = rest % p.hkv;
+  rest /= p.hkv;
+  const int seq = rest % p.num_seqs, tile = row_tiles - 1 - rest / p.num_seqs;      // the tiles that see the most first
+  const int q0 = p.q_starts[seq], qn = p.q_starts[seq + 1] - q0, G = p.group;
+  const int all_rows = qn > 0 && qn <= p.max_q_len ? qn * G : 0, row0 = tile * kTcRows;
+  if (all_rows <= p.rows_from || row0 >= all_rows) return;
+  if (q0 < 0 || q0 + qn > p.tokens) {
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
+    return;
+  }
+  const int n_rows = min(kTcRows, all_rows - row0), kv_len = max(p.kv_lens[seq], 0);
+  const bool two = n_rows > kRows;                     // two row tiles that share K and V, or two groups that share a row tile
+
+  const int group = warp >> 2;                         // of softmax warps
+  const int r = (two ? group * kRows : 0) + (warp & 3) * 32 + lane;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], KV8 ? 3 : D / 64); mbar_init(&v_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV8 ? 3 : 1);
+    }
+    for (int i = 0; i < 4; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 3); }
+    mbar_init(o_done, 1); mbar_init(q_full, 8);
+    *abort_flag = 0;
+    seen[0] = INT_MAX; seen[1] = 0; seen[2] = INT_MAX; seen[3] = 0; seen[4] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); tma_prefetch_desc(&tma_v); }
+  if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  SpanRow row{0, 0};
+  const int qi = warp < 8 && r < n_rows ? (row0 + r) / G : -1;
+  if (qi >= 0) {
+    unsigned long long bits[kSpanWords];
+    row = span_row(p, q0, qn, kv_len, qi, bits);
+  }
+  __syncthreads();
+  if (warp < 8) {
+    const int a = __reduce_min_sync(0xffffffffu, qi >= 0 ? row.base : INT_MAX), b = __reduce_max_sync(0xffffffffu, row.base);
+    const int c = __reduce_min_sync(0xffffffffu, qi >= 0 ? row.beg : INT_MAX), d = __reduce_max_sync(0xffffffffu, row.beg);
+    if (lane == 0 && a != INT_MAX) { atomicMin(&seen[0], a); atomicMax(&seen[1], b); atomicMin(&seen[2], c); atomicMax(&seen[3], d); }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_launch_dependents();                             // not before the allocation
+  const int end = p.tree_mask ? kv_len : seen[1], min_base = seen[0], max_beg = seen[3];
+  const SpanRange range = span_range(p, kTile, seen[2], end);
+  const int per_split = max(p.min_tiles, (range.count + p.splits - 1) / p.splits);
+  const int t0 = min(split * per_split, range.count), n_tiles = min(per_split, range.count - t0);
+  const int shift = two ? 1 : 0, n_items = n_tiles << shift;
+  // not every row of the CTA sees the whole tile
+  auto partial = [&](int tok0) { return !(tok0 + kTile <= min_base && (tok0 >= max_beg || tok0 + kTile <= p.first)); };
+  const PageRows page_rows{p, p.block_tables + (size_t)seq * p.max_blocks, kvh, (min(p.first, end) + kPage - 1) / kPage, seen[2] / kPage,
+                           (end + kPage - 1) / kPage, (int)(p.num_blocks * p.hkv * p.block_pages * kPage)};
+
+  // The block was launched with 168 registers a thread: 256 x 208 + 128 x 88 = 384 x 168.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    bool bad = false;
+    if (warp == 9) {
+      constexpr int fmt = KV8 ? 0 : 1;
+      constexpr uint32_t idesc_s = make_idesc(128, 128, fmt, fmt);
+      constexpr uint32_t idesc_pv = make_idesc(128, D, fmt, fmt) | (1u << 16);     // B is MN-major
+      const uint64_t dq = make_smem_desc_sw128(smem_u32(sq)), dk = make_smem_desc_sw128(smem_u32(sk));
+      // V: [page][D / 64][16][64]; at D = 128 the second 64-wide atom of a row lies half a page further
+      const uint64_t dv = (uint64_t)((smem_u32(sv) & 0x3FFFFu) >> 4) | (uint64_t)((D == 128 ? 2048 : 1024) >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+                          (uint64_t)1 << 46 | (uint64_t)2 << 61;
+      auto issue_s = [&](int n) {
+        const int g = n & 1, t = n >> shift;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+          tc_mma_bf16(tmem_base + 128 * g, dq + (uint64_t)((g & shift) * (TB >> 4)) + off, dk + (uint64_t)((t & 1) * (TB >> 4)) + off, idesc_s, k > 0);
+        }
+        tc_commit(&s_full[g]);
+        if (!two || g) tc_commit(&k_empty[t & 1]);
+      };
+      auto issue_pv = [&](int n, int part) {           // over tokens [64 part, 64 part + 64)
+        const int g = n & 1, t = n >> shift;
+        const uint32_t t_p = tmem_base + 128 * g, t_o = tmem_base + 256 + 128 * g;
+#pragma unroll
+        for (int k = 4 * part; k < 4 * part + 4; ++k)
+          tc_mma_bf16_ts(t_o, t_p + 8 * k, dv + (uint64_t)((t & 1) * (TB >> 4)) + k * (D / 64) * (2048 >> 4), idesc_pv, (n > 1 || k > 0) ? 1u : 0u);
+      };
+      if (n_items > 0 && elect_one()) {
+        bool ok = mbar_wait(q_full, 0, abort_flag);
+        for (int n = 0; ok && n < 2 && n < n_items; ++n) {
+          ok = mbar_wait(&k_full[(n >> shift) & 1], 0, abort_flag);
+          if (!ok) break;
+          tc_fence_after_sync();
+          issue_s(n);
+        }
+        for (int n = 0; ok && n < n_items; ++n) {
+          const int g = n & 1, t = n >> shift, k = n >> 1;
+          ok = mbar_wait(&v_ready[t & 1], (t >> 1) & 1, abort_flag) && mbar_wait(&p_half[g], k & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after_sync();
+          issue_pv(n, 0);
+          ok = mbar_wait(&p_ready[g], k & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after_sync();
+          issue_pv(n, 1);
+          if (!two || g) tc_commit(&v_empty[t & 1]);
+          if (n + 2 < n_items) {
+            const int t2 = (n + 2) >> shift;
+            ok = mbar_wait(&k_full[t2 & 1], (t2 >> 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after_sync();
+            issue_s(n + 2);
+          }
+          if (n == n_items - 1) tc_commit(o_done);
+        }
+      }
+      __syncwarp();
+    } else if constexpr (!KV8) {
+      const bool is_v = warp == 11;
+      const int half = warp == 10 ? 1 : 0;
+      int rows[kTilePages];
+      auto ask = [&](int it) {                         // all lanes; false: gave up
+        const int page0 = range.piece(t0 + it) * kTilePages, b = it & 1;
+#pragma unroll
+        for (int pg = 0; pg < kTilePages; ++pg) rows[pg] = page_rows(page0 + pg, bad);
+        if (it >= 2 && !mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag)) return false;
+        if (elect_one()) {
+          if (is_v) {
+            mbar_expect_tx(&v_full[b], TB);
+#pragma unroll
+            for (int pg = 0; pg < kTilePages; ++pg) tma_load_3d(sv + b * TB + pg * (D / 64) * 2048, &tma_v, &v_full[b], 0, rows[pg], 0);
+          } else {
+            mbar_expect_tx(&k_full[b], kHalf);
+#pragma unroll
+            for (int pg = 0; pg < kTilePages; ++pg) tma_load_2d(sk + b * TB + half * kHalf + pg * 2048, &tma_k, &k_full[b], 64 * half, rows[pg]);
+          }
+        }
+        __syncwarp();
+        return true;
+      };
+      if (!is_v) {
+        for (int it = 0; it < n_tiles && (half == 0 || D == 128); ++it)
+          if (!ask(it)) break;
+      } else if (n_tiles > 0) {
+        bool ok = ask(0);
+        for (int it = 0; ok && it < n_tiles; ++it) {
+          if (it == 0 && n_tiles > 1) ok = ask(1);
+          const int b = it & 1;
+          ok = ok && mbar_wait_warp(&v_full[b], (it >> 1) & 1, abort_flag);
+          if (!ok) break;
+          if (partial(range.piece(t0 + it) * kTile)) {
+            uint4* v = reinterpret_cast<uint4*>(sv + b * TB);
+            bool odd = false;
+#pragma unroll 8
+            for (int i = lane; i < TB / 16; i += 32) {
+              const uint4 w = v[i];
+              odd |= odd_bf16x2(w.x) || odd_bf16x2(w.y) || odd_bf16x2(w.z) || odd_bf16x2(w.w);
+            }
+            if (__any_sync(0xffffffffu, odd)) {
+              for (int i = lane; i < TB / 16; i += 32) {
+                uint4 w = v[i];
+                w.x = without_odd_bf16(w.x); w.y = without_odd_bf16(w.y); w.z = without_odd_bf16(w.z); w.w = without_odd_bf16(w.w);
+                v[i] = w;
+              }
+              fence_proxy_async_smem();
+              if (lane == 0) atomicOr(&seen[4], 1);
+              __syncwarp();
+            }
+          }
+          if (lane == 0) mbar_arrive(&v_ready[b]);
+          if (it >= 1 && it + 1 < n_tiles) ok = ask(it + 1);
+        }
+      }
+    } else {
+      // raw tiles K0 V0 K1 V1 ... through a ring of slots; each of the three warps widens a part of every one
+      const int part = warp == 8 ? 0 : warp - 9;
+      const int slots = two ? 2 : 4, pieces = 2 * n_tiles;
+      auto slot_at = [&](int s) { return s < 2 ? smem + 6 * TB + s * S::kRaw : sq + TB + (s - 2) * S::kRaw; };      // the unused tile of Q
+      auto ask = [&](int j) {                          // warp 8
+        const int page0 = range.piece(t0 + (j >> 1)) * kTilePages, s = j & (slots - 1);
+        int rows[kTilePages];
+#pragma unroll
+        for (int pg = 0; pg < kTilePages; ++pg) rows[pg] = page_rows(page0 + pg, bad);
+        if (j >= slots && !mbar_wait_warp(&raw_empty[s], (j / slots - 1) & 1, abort_flag)) return false;
+        if (elect_one()) {
+          uint8_t* dst = slot_at(s);
+          mbar_expect_tx(&raw_full[s], S::kRaw);
+#pragma unroll
+          for (int pg = 0; pg < kTilePages; ++pg) tma_load_2d(dst + pg * kPage * D, j & 1 ? &tma_v : &tma_k, &raw_full[s], 0, rows[pg]);
+        }
+        __syncwarp();
+        return true;
+      };
+      bool ok = true;
+      if (part == 0)
+        for (int j = 0; ok && j < slots - 1 && j < pieces; ++j) ok = ask(j);
+      for (int j = 0; ok && j < pieces; ++j) {
+        if (part == 0 && j + slots - 1 < pieces) ok = ask(j + slots - 1);
+        const int it = j >> 1, b = it & 1, s = j & (slots - 1);
+        const bool is_v = j & 1;
+        ok = ok && mbar_wait_warp(&raw_full[s], (j / slots) & 1, abort_flag) &&
+             (it < 2 || mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag));
+        if (!ok) break;
+        const uint8_t* src = slot_at(s);
+        uint8_t* dst = (is_v ? sv : sk) + b * TB;
+        const bool look = is_v && partial(range.piece(t0 + it) * kTile);
+        bool odd = false;
+        constexpr int CPR = D / 16;                    // 16-byte pieces of a raw row
+#pragma unroll 4
+        for (int i = part * 32 + lane; i < kTile * CPR; i += 96) {
+          const int rr = i / CPR, c = 2 * (i % CPR);
+          const uint4 raw = *reinterpret_cast<const uint4*>(src + i * 16);
+          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] & 0xFFFFu), __NV_E4M3);
+            const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] >> 16), __NV_E4M3);
+            h[2 * e] = (uint32_t)lo.x | ((uint32_t)lo.y << 16);
+            h[2 * e + 1] = (uint32_t)hi.x | ((uint32_t)hi.y << 16);
+          }
+          if (look) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (odd_f16x2(h[e])) { odd = true; h[e] = without_odd_f16(h[e]); }
+          }
+          // K: [half][128 rows][64]; V: [page][half][16][64]
+          uint8_t* line = is_v ? dst + (rr >> 4) * (D / 64) * 2048 + (c >> 3) * 2048 + (rr & 15) * 128 : dst + (c >> 3) * kHalf + rr * 128;
+          *reinterpret_cast<uint4*>(line + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(line + ((((c & 7) + 1) ^ (rr & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+        if (odd) atomicOr(&seen[4], 1);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(is_v ? &v_ready[b] : &k_full[b]); mbar_arrive(&raw_empty[s]); }
+      }
+    }
+    if (bad && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    load_q<D, KV8>(p, sq, factors, two ? 2 : 1, q0, row0, n_rows, kvh);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float factor = factors[r];
+    const uint32_t t_s = tmem_base + 128 * group + lane_off, t_o = tmem_base + 256 + 128 * group + lane_off;
+    // whole for the rows of this warp
+    const int w_base = __reduce_min_sync(0xffffffffu, qi >= 0 ? row.base : INT_MAX), w_beg = __reduce_max_sync(0xffffffffu, qi >= 0 ? row.beg : 0);
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int n = group; n < n_items; n += 2) {
+      const int k = n >> 1, tok0 = range.piece(t0 + (n >> shift)) * kTile;
+      if (!mbar_wait(&s_full[group], k & 1, abort_flag)) { ok = false; break; }
+      tc_fence_after_sync();
+      uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+      const bool whole = tok0 + kTile <= w_base && (tok0 >= w_beg || tok0 + kTile <= p.first);
+      if (!whole) row_bits(p, tok0, row.base, row.beg, q0, qn, kv_len, qi, vis);
+      if (p.softcap > 0.f) softmax_tile<D, true, true, KV8>(p, t_s, t_o, vis, factor, k > 0, &p_half[group], m_used, l);
+      else if (whole) softmax_tile<D, false, false, KV8>(p, t_s, t_o, vis, factor, k > 0, &p_half[group], m_used, l);
+      else softmax_tile<D, true, false, KV8>(p, t_s, t_o, vis, factor, k > 0, &p_half[group], m_used, l);
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[group]);
+    }
+    if (KV8) m_used -= kTcLift;
+    ok = ok && n_items > 0 && mbar_wait(o_done, 0, abort_flag);       // (a group without items too: what follows reuses K and V)
+    const bool have = ok && n_items > group;
+    tc_fence_after_sync();
+    float c_mine = 1.f, c_other = 0.f;
+    bool other = false;
+    float* swap = reinterpret_cast<float*>(sk);        // O of the second group, [column][row]; then its maxima and sums
+    if (!two) {
+      float2* swap_ml = reinterpret_cast<float2*>(sv);
+      const int at = (warp & 3) * 32 + lane;
+      if (group == 1) {
+        if (have) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(t_o + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) swap[(32 * c + i) * kRows + at] = __uint_as_float(o[i]);
+          }
+        }
+        swap_ml[at] = make_float2(have ? m_used : -INFINITY, have ? l : 0.f);
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (group == 0) {
+        other = n_items > 1;
+        const float2 ml = swap_ml[at];
+        const float mm = fmaxf(m_used, ml.x);
+        if (other) {
+          c_mine = m_used == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : ex2(m_used - mm);
+          c_other = ml.x == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : ex2(ml.x - mm);
+          l = l * c_mine + ml.y * c_other;
+          m_used = mm;
+        }
+      }
+    }
+    if (two || group == 0) {
+      // (m, l, O) of this warp's rows: to the workspace, or normalised with the head's sink to the output. Rows pass through shared memory of
+      // the warp's own (its part of Q, which has been read), 256 bytes of each at a time, so that a store writes whole lines.
+      const int G_row = qi >= 0 ? kvh * G + (row0 + r) - qi * G : 0;
+      const bool splits = p.splits > 1;
+      float scale = 1.f;
+      if (!splits) {
+        float ll = l, c = 1.f;
+        if (p.sinks && qi >= 0) {
+          const float sk2 = p.sinks[G_row] * kLog2e;
+          const float mn = fmaxf(m_used, sk2);
+          c = m_used == -INFINITY ? 0.f : ex2(m_used - mn);
+          ll = ll * c + ex2(sk2 - mn);
+        }
+        scale = ll == 0.f ? 0.f : c / ll;
+      } else if (qi >= 0) {
+        *reinterpret_cast<float2*>(p.ws_ml + (((size_t)(q0 + qi) * p.hq + G_row) * p.splits + split) * 2) = have ? make_float2(m_used, l) : make_float2(-INFINITY, 0.f);
+      }
+      c_mine *= scale;
+      c_other *= scale;
+      uint8_t* stage = sq + (size_t)(warp & 7) * (32 * 2 * 64);      // 32 rows of 128 bytes
+      const int row_first = (two ? group * kRows : 0) + (warp & 3) * 32;
+      const int at = (warp & 3) * 32 + lane;
+      const int cols = splits ? 32 : 64;               // of a pass: 128 bytes of a row
+      for (int c0 = 0; c0 < D; c0 += cols) {
+        __syncwarp();
+#pragma unroll 1
+        for (int h = 0; h < cols; h += 32) {
+          uint32_t o[32];
+          if (have) {
+            tmem_ld_32x32(t_o + c0 + h, o);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float x = have && scale != 0.f ? __uint_as_float(o[i]) * c_mine : 0.f;
+            if (c_mine == 0.f) x = 0.f;
+            if (other && c_other != 0.f) x += swap[(c0 + h + i) * kRows + at] * c_other;
+            o[i] = __float_as_uint(x);
+          }
+          if (splits) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 w;
+              w.x = pack_bf16x2(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
+              w.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
+              w.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
+              w.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((h / 8 + i) ^ (lane & 7)) << 4)) = w;
+            }
+          }
+        }
+        __syncwarp();
+#pragma unroll 2
+        for (int k = 0; k < 8; ++k) {
+          const int rr = k * 4 + lane / 8, piece = lane & 7, at_row = row0 + row_first + rr;
+          if (row_first + rr >= n_rows) continue;
+          const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((piece ^ (rr & 7)) << 4));
+          const int q = at_row / G, head = kvh * G + at_row - q * G;
+          if (splits) *reinterpret_cast<uint4*>(p.ws_o + (((size_t)(q0 + q) * p.hq + head) * p.splits + split) * D + c0 + piece * 4) = w;
+          else *reinterpret_cast<uint4*>(static_cast<bf16*>(p.out) + (size_t)(q0 + q) * p.ldo + (size_t)head * D + c0 + piece * 8) = w;
+        }
+      }
+      __syncwarp();
+      if (seen[4] && qi >= 0) {
+        // infinities and NaN that were taken out of tiles, added to the rows that see them
+        for (int it = 0; it < n_tiles; ++it) {
+          const int tok0 = range.piece(t0 + it) * kTile;
+          if (!partial(tok0)) continue;
+          uint32_t vis[4];
+          row_bits(p, tok0, row.base, row.beg, q0, qn, kv_len, qi, vis);
+          for (int i = 0; i < kTile; ++i) {
+            if (!(vis[i >> 5] >> (i & 31) & 1)) continue;
+            const int page = (tok0 + i) / kPage, b = span_block(p, page_rows.table, page);
+            if (b < 0) continue;
+            const size_t at = (size_t)(span_pool_row(p, b, kvh, page) + (i & 15)) * D;
+            for (int d = 0; d < D; ++d) {
+              float x;
+              if constexpr (KV8) {
+                x = (static_cast<const uint8_t*>(p.v_cache)[at + d] & 0x7F) == 0x7F ? __int_as_float(0x7FC00000) : 0.f;
+              } else {
+                x = __bfloat162float(static_cast<const bf16*>(p.v_cache)[at + d]);
+              }
+              if (isfinite(x)) continue;
+              if (splits) p.ws_o[(((size_t)(q0 + qi) * p.hq + G_row) * p.splits + split) * D + d] += x;
+              else {
+                bf16* y = static_cast<bf16*>(p.out) + (size_t)(q0 + qi) * p.ldo + (size_t)G_row * D + d;
+                *y = __float2bfloat16(__bfloat162float(*y) + x);
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 9) { tc_fence_after_sync(); tmem_dealloc(tmem_base, 512); }
+  if (threadIdx.x == 0 && *abort_flag && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_MBAR_TIMEOUT);
+}
+
+template <int D, bool KV8>
+void launch_tc(const SpanParams& p, cudaStream_t s) {
+  static bool configured[kMaxDevices] = {};
+  constexpr int smem = TcSmem<D, KV8>::kTotal;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  if (first_call_on_device(configured))
+    cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
+  const uint64_t rows = (uint64_t)p.num_blocks * p.hkv * p.block_pages * kPage;
+  // encoded for every call: they cost less than looking up by an address what another tensor may since have
+  CUtensorMap mk, mv;
+  if (KV8) {
+    mk = make_tmap_2d(p.k_cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, D, D, kPage, D, false);
+    mv = make_tmap_2d(p.v_cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, D, D, kPage, D, false);
+  } else {
+    mk = make_tmap_2d(p.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, D, D * 2, kPage, 64, true);
+    mv = make_tmap_parts(p.v_cache, rows, D, kPage, D / 64);
+  }
+  const long long tiles = ((long long)p.max_q_len * p.group + kTcRows - 1) / kTcRows;
+  const long long ctas = tiles * p.num_seqs * p.hkv;
+  if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
+  launch_pdl(span_tc_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(kTcThreads), smem, s, mk, mv, p, (int)tiles);
+}
+}  // namespace
+
+bool attention_span_tc_supported(const SpanParams& p) {
+  return (p.head_dim == 64 || p.head_dim == 128) && p.num_blocks * p.hkv * p.block_pages * kPage <= INT_MAX - kTile;
+}
+void attention_span_tc(const SpanParams& p, cudaStream_t s) {
+  if (p.head_dim == 64) p.kv_fp8 ? launch_tc<64, true>(p, s) : launch_tc<64, false>(p, s);
+  else p.kv_fp8 ? launch_tc<128, true>(p, s) : launch_tc<128, false>(p, s);
+}
+}  // namespace fllm

@@ -85,16 +85,11 @@ int64_t attention_span(const Tensor& q, const Tensor& k_cache, const Tensor& v_c
   p.scale = (float)scale; p.scale_log2 = (float)(scale * 1.4426950408889634); p.softcap = (float)softcap;
   if (p.tokens == 0 || num_seqs == 0 || p.max_q_len == 0) return 0;
   c10::cuda::CUDAGuard guard(q.device());
-  const size_t bytes = fllm::attention_span_workspace_bytes(p);
+  const fllm::SpanPlan plan = fllm::attention_span_plan(p);
   Tensor ws;                                  // of this call alone: two streams or two captured graphs do not share it
-  if (bytes) {
-    ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-    p.ws_o = reinterpret_cast<float*>(ws.data_ptr());
-    p.ws_ml = p.ws_o + (size_t)p.tokens * p.hq * p.splits * p.head_dim;
-  }
-  return fllm::attention_span(p, cur_stream());
+  if (plan.bytes) ws = at::empty({(int64_t)plan.bytes}, q.options().dtype(at::kByte));
+  return fllm::attention_span(p, plan, plan.bytes ? ws.data_ptr() : nullptr, cur_stream());
 }
-
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(fllm_b200, m) {

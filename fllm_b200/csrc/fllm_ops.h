@@ -310,14 +310,21 @@ struct SpanParams {
   int max_q_len, min_q_len, max_kv_len;
   int window, first;           // window 0: no limit (first is 0 then)
   float scale, scale_log2, softcap;
-  // set by the planner
-  int splits, min_pages;       // pieces of a sequence's visible tokens; fewest pages in one
-  int rows_from, rows_to;      // packed rows (query rows x group) of the sequences that a kernel takes: from < rows <= to
+  // set by the planner, for one kernel
+  int splits, min_pages, min_tiles;      // pieces of a sequence's visible tokens; fewest pages, or tiles of 128 tokens, in one
+  int rows_from, rows_to;      // packed rows (query rows x group) of the sequences that the kernel takes: from < rows <= to
   float* ws_o;                 // [tokens][hq][splits][head_dim]
   float* ws_ml;                // [tokens][hq][splits][2]
 };
-size_t attention_span_workspace_bytes(SpanParams& p);      // plans the splits
-int attention_span(const SpanParams& p, cudaStream_t s);   // kernels launched
+struct SpanPlan {
+  int rows_splits, tile_splits;          // of the kernel for few rows and of the tensor-memory kernel; 0: it has no rows
+  int min_pages, min_tiles;
+  size_t bytes;                          // of workspace
+};
+SpanPlan attention_span_plan(const SpanParams& p);
+int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStream_t s);   // kernels launched
+bool attention_span_tc_supported(const SpanParams& p);
+void attention_span_tc(const SpanParams& p, cudaStream_t s);
 
 // ---- rows of the cache pools (kv_moves.cu) ------------------------------------------
 struct KvPool {                // [planes][blocks][heads][block_size][row_bytes], a block's bytes contiguous
