@@ -21,6 +21,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_span.cuh"
 #include "attention_util.cuh"
@@ -31,15 +32,20 @@ namespace {
 constexpr int kTcThreads = 384, kTcRows = 256;
 constexpr float kTcLift = 6.f;             // f16 weights: their reference lies so far below the row's (their largest is 2^14 then)
 constexpr int kTilePages = kTile / kPage;
+template <int N> using Int = std::integral_constant<int, N>;
+template <bool B> using Bool = std::integral_constant<bool, B>;
 
-// Shared memory: two tiles of Q, two stages of K and of V, 16-bit values in rows of 128 bytes; e4m3: two slots of raw tiles (four where
+constexpr int kRawTokens = 64;             // of a piece of an e4m3 tile
+constexpr int kTcFlags = 320;              // bytes of barriers and flags
+
+// Shared memory: two tiles of Q, two stages of K and of V, 16-bit values in rows of 128 bytes; e4m3: four slots of raw pieces (eight where
 // there is one tile of Q).
 template <int D, bool KV8>
 struct TcSmem {
   static constexpr int kT = tile_bytes<D>();           // a 128-row tile of 16-bit values
-  static constexpr int kRaw = KV8 ? kTile * D : 0;
-  static constexpr int kTiles = 6 * kT + 2 * kRaw;
-  static constexpr int kTotal = kTiles + 256 + kTcRows * 4 + 64 + 1024;
+  static constexpr int kRaw = KV8 ? kRawTokens * D : 0;
+  static constexpr int kTiles = 6 * kT + 4 * kRaw;
+  static constexpr int kTotal = kTiles + kTcFlags + kTcRows * 4 + 1024;
 };
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -78,35 +84,35 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return hi <= lo ? 0u : (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
 }
 
-// What a row sees of the 128 tokens from tok0 on.
-__device__ __forceinline__ void row_bits(const SpanParams& p, int tok0, int base, int beg, int q0, int qn, int kv_len, int qi, uint32_t (&vis)[4]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int t = tok0 + 32 * c;
-    vis[c] = bits_between(beg - t, base - t) | bits_between(0, min(p.first, base) - t);
-  }
-  if (p.tree_mask && tok0 + kTile > base && qi >= 0) {
-    unsigned long long bits[kSpanWords + 1] = {0, 0, 0, 0, 0};
-    span_row(p, q0, qn, kv_len, qi, bits);
-    const unsigned long long* b = bits;
+// What row `qi` of a sequence (negative: none) sees of the 128 tokens from tok0 on. Out of line and from the beginning: few tiles need it, and what
+// it knows of the row would be held in registers beside the 128 scores of those that do not.
+__device__ __noinline__ uint4 row_bits(const SpanParams& p, int q0, int qn, int kv_len, int qi, int tok0) {
+  uint32_t vis[4] = {0, 0, 0, 0};
+  if (qi >= 0) {
+    unsigned long long b[kSpanWords + 1] = {0, 0, 0, 0, 0};
+    const SpanRow row = span_row(p, q0, qn, kv_len, qi, b);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int n = tok0 + 32 * c - base;              // node of the word's first token
-      uint32_t w = 0;
-      if (n < 0) w = n > -32 ? (uint32_t)(b[0] << -n) : 0u;
-      else if (n < 64 * kSpanWords) w = (uint32_t)((b[n >> 6] >> (n & 63)) | ((n & 63) ? b[(n >> 6) + 1] << (64 - (n & 63)) : 0ull));
-      vis[c] |= w;
+      const int t = tok0 + 32 * c, n = t - row.base;   // n: node of the word's first token
+      uint32_t w = bits_between(row.beg - t, row.base - t) | bits_between(0, min(p.first, row.base) - t);
+      if (p.tree_mask) {
+        if (n < 0) w |= n > -32 ? (uint32_t)(b[0] << -n) : 0u;
+        else if (n < 64 * kSpanWords) w |= (uint32_t)((b[n >> 6] >> (n & 63)) | ((n & 63) ? b[(n >> 6) + 1] << (64 - (n & 63)) : 0ull));
+      }
+      vis[c] = w;
     }
   }
+  return make_uint4(vis[0], vis[1], vis[2], vis[3]);
 }
 
 // A row's softmax over one tile of 128 tokens: scores in registers, weights as 16-bit values over the scores' first columns, the first 64 of them
 // handed over before the others are computed; O of the warp is rescaled when a row's maximum has moved by more than 2^8.
 template <int D, bool MASKED, bool CAPPED, bool F16>
-__device__ __forceinline__ void softmax_tile(const SpanParams& p, uint32_t t_s, uint32_t t_o, const uint32_t (&vis)[4], float factor, bool have_o,
-                                             uint64_t* p_half, float& m_used, float& l) {
-  const float cap_in = CAPPED ? factor / (p.softcap * kLog2e) : 0.f;
-  const float scale = CAPPED ? p.softcap * kLog2e : factor;
+__device__ __forceinline__ float2 softmax_tile(uint32_t t_s, uint32_t t_o, uint4 visible, float factor, float softcap, bool have_o, uint64_t* p_half,
+                                               float m_used, float l) {
+  const uint32_t vis[4] = {visible.x, visible.y, visible.z, visible.w};
+  const float cap_in = CAPPED ? factor / (softcap * kLog2e) : 0.f;
+  const float scale = CAPPED ? softcap * kLog2e : factor;
   uint32_t s[4][32];
 #pragma unroll
   for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, s[c]);
@@ -172,6 +178,16 @@ __device__ __forceinline__ void softmax_tile(const SpanParams& p, uint32_t t_s, 
   const float2 l0 = unpack2(sum[0]), l1 = unpack2(sum[1]);
   l += (l0.x + l0.y) + (l1.x + l1.y);
   tmem_st_wait();
+  return make_float2(m_used, l);
+}
+template <int D, bool F16>
+__device__ __noinline__ float2 softmax_masked(uint32_t t_s, uint32_t t_o, uint4 visible, float factor, bool have_o, uint64_t* p_half, float m_used, float l) {
+  return softmax_tile<D, true, false, F16>(t_s, t_o, visible, factor, 0.f, have_o, p_half, m_used, l);
+}
+template <int D, bool F16>
+__device__ __noinline__ float2 softmax_capped(uint32_t t_s, uint32_t t_o, uint4 visible, float factor, float softcap, bool have_o, uint64_t* p_half, float m_used,
+                                              float l) {
+  return softmax_tile<D, true, true, F16>(t_s, t_o, visible, factor, softcap, have_o, p_half, m_used, l);
 }
 
 // Queries of rows [0, tiles x 128) to shared memory in swizzled rows, by the 256 threads of the softmax groups. f16 (beside an e4m3 cache): times a
@@ -230,7 +246,33 @@ struct PageRows {
   }
 };
 
-// Infinities and NaN of 16-bit values set to zero; true if there were any.
+// The same for the tiles of a walk, by a whole warp: a lane looks up one page, so that of four tiles at a time, one round ahead. (Page after page by
+// all lanes, in front of every tile, the producers took longer than the products.)
+struct PagesAhead {
+  const PageRows& rows;
+  const SpanRange& range;
+  int t0, n_tiles, now, next;
+  bool bad;
+  __device__ __forceinline__ PagesAhead(const PageRows& r, const SpanRange& s, int first, int n) : rows(r), range(s), t0(first), n_tiles(n), now(0), next(0), bad(false) {
+    next = look(0);
+  }
+  __device__ __forceinline__ int look(int it) {
+    const int at = it + ((threadIdx.x & 31) >> 3);
+    return at < n_tiles ? rows(range.piece(t0 + at) * kTilePages + (threadIdx.x & 7), bad) : rows.none;
+  }
+  __device__ __forceinline__ void to(int it) {         // tile after tile
+    if ((it & 3) == 0) { now = next; next = look(it + 4); }
+  }
+  __device__ __forceinline__ int row(int it, int page) const { return __shfl_sync(0xffffffffu, now, (it & 3) * 8 + page); }
+};
+
+// Sum of 0 x value over 16-bit values, a NaN once there was an infinity or a NaN among them.
+template <bool F16>
+__device__ __forceinline__ void odd_sum(uint32_t& sum, uint32_t w) {
+  if constexpr (F16) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(w), "r"(0u));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(w), "r"(0u));
+}
+// Infinities and NaN of 16-bit values set to zero.
 __device__ __forceinline__ uint32_t without_odd_bf16(uint32_t w) {
   return ((w & 0x7F80u) == 0x7F80u ? 0u : w & 0xFFFFu) | ((w & 0x7F800000u) == 0x7F800000u ? 0u : w & 0xFFFF0000u);
 }
@@ -251,12 +293,12 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   uint64_t *s_full = bars + 8, *p_half = bars + 10, *p_ready = bars + 12;                     // [2] by softmax group
   uint64_t* v_ready = bars + 14;                                                              // [2] by stage: looked through, or widened
   uint64_t *o_done = bars + 16, *q_full = bars + 17;
-  uint64_t *raw_full = bars + 18, *raw_empty = bars + 22;                                     // [4] by slot
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  uint64_t *raw_full = bars + 18, *raw_empty = bars + 26;                                     // [8] by slot
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* seen = reinterpret_cast<int*>(tmem_slot + 2);        // smallest and largest base, smallest and largest window begin, odd values met
-  float* factors = reinterpret_cast<float*>(smem + S::kTiles + 256);
-  static_assert(27 * 8 + 24 <= 256, "barriers and flags");
+  float* factors = reinterpret_cast<float*>(smem + S::kTiles + kTcFlags);
+  static_assert(34 * 8 + 7 * 4 <= kTcFlags, "barriers and flags");
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   pdl_wait();
@@ -282,7 +324,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       mbar_init(&k_full[i], KV8 ? 3 : D / 64); mbar_init(&v_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV8 ? 3 : 1);
     }
-    for (int i = 0; i < 4; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 3); }
+    for (int i = 0; i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 3); }
     mbar_init(o_done, 1); mbar_init(q_full, 8);
     *abort_flag = 0;
     seen[0] = INT_MAX; seen[1] = 0; seen[2] = INT_MAX; seen[3] = 0; seen[4] = 0;
@@ -329,61 +371,76 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       // V: [page][D / 64][16][64]; at D = 128 the second 64-wide atom of a row lies half a page further
       const uint64_t dv = (uint64_t)((smem_u32(sv) & 0x3FFFFu) >> 4) | (uint64_t)((D == 128 ? 2048 : 1024) >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
                           (uint64_t)1 << 46 | (uint64_t)2 << 61;
-      auto issue_s = [&](int n) {
-        const int g = n & 1, t = n >> shift;
+      // The group of an item is known at compile time, and whether there are two row tiles: addresses and descriptors stay in uniform registers.
+      auto issue_s = [&](auto two_tiles, auto g, int n) {
+        constexpr bool kTwo = decltype(two_tiles)::value;
+        constexpr int kG = decltype(g)::value;
+        const int b = kTwo ? (n >> 1) & 1 : kG;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-          tc_mma_bf16(tmem_base + 128 * g, dq + (uint64_t)((g & shift) * (TB >> 4)) + off, dk + (uint64_t)((t & 1) * (TB >> 4)) + off, idesc_s, k > 0);
+          tc_mma_bf16(tmem_base + 128 * kG, dq + (uint64_t)(kTwo ? kG * (TB >> 4) : 0) + off, dk + (uint64_t)(b * (TB >> 4)) + off, idesc_s, k > 0);
         }
-        tc_commit(&s_full[g]);
-        if (!two || g) tc_commit(&k_empty[t & 1]);
+        tc_commit(&s_full[kG]);
+        if (!kTwo || kG) tc_commit(&k_empty[b]);
       };
-      auto issue_pv = [&](int n, int part) {           // over tokens [64 part, 64 part + 64)
-        const int g = n & 1, t = n >> shift;
-        const uint32_t t_p = tmem_base + 128 * g, t_o = tmem_base + 256 + 128 * g;
+      auto issue_pv = [&](auto g, int b, bool first, auto part) {            // over tokens [64 part, 64 part + 64)
+        constexpr int kG = decltype(g)::value, kPart = decltype(part)::value;
+        const uint32_t t_p = tmem_base + 128 * kG, t_o = tmem_base + 256 + 128 * kG;
 #pragma unroll
-        for (int k = 4 * part; k < 4 * part + 4; ++k)
-          tc_mma_bf16_ts(t_o, t_p + 8 * k, dv + (uint64_t)((t & 1) * (TB >> 4)) + k * (D / 64) * (2048 >> 4), idesc_pv, (n > 1 || k > 0) ? 1u : 0u);
+        for (int k = 4 * kPart; k < 4 * kPart + 4; ++k)
+          tc_mma_bf16_ts(t_o, t_p + 8 * k, dv + (uint64_t)(b * (TB >> 4)) + k * (D / 64) * (2048 >> 4), idesc_pv, (!first || k > 0) ? 1u : 0u);
+      };
+      auto step = [&](auto two_tiles, auto g, int n) {      // PV of item n, S of item n + 2
+        constexpr bool kTwo = decltype(two_tiles)::value;
+        constexpr int kG = decltype(g)::value;
+        const int t = kTwo ? n >> 1 : n, b = kTwo ? t & 1 : kG, k = n >> 1;
+        if (!mbar_wait(&v_ready[b], (t >> 1) & 1, abort_flag) || !mbar_wait(&p_half[kG], k & 1, abort_flag)) return false;
+        tc_fence_after_sync();
+        issue_pv(g, b, k == 0, Int<0>{});
+        if (!mbar_wait(&p_ready[kG], k & 1, abort_flag)) return false;
+        tc_fence_after_sync();
+        issue_pv(g, b, k == 0, Int<1>{});
+        if (!kTwo || kG) tc_commit(&v_empty[b]);
+        if (n + 2 < n_items) {
+          const int t2 = kTwo ? t + 1 : t + 2;
+          if (!mbar_wait(&k_full[kTwo ? t2 & 1 : kG], (t2 >> 1) & 1, abort_flag)) return false;
+          tc_fence_after_sync();
+          issue_s(two_tiles, g, n + 2);
+        }
+        return true;
+      };
+      auto walk = [&](auto two_tiles) {
+        constexpr bool kTwo = decltype(two_tiles)::value;
+        if (!mbar_wait(q_full, 0, abort_flag) || !mbar_wait(&k_full[0], 0, abort_flag)) return;
+        tc_fence_after_sync();
+        issue_s(two_tiles, Int<0>{}, 0);
+        if (n_items > 1) {
+          if (!kTwo && !mbar_wait(&k_full[1], 0, abort_flag)) return;
+          tc_fence_after_sync();
+          issue_s(two_tiles, Int<1>{}, 1);
+        }
+        for (int n = 0; n < n_items; n += 2) {
+          if (!step(two_tiles, Int<0>{}, n)) return;
+          if (n + 1 < n_items && !step(two_tiles, Int<1>{}, n + 1)) return;
+        }
+        tc_commit(o_done);
       };
       if (n_items > 0 && elect_one()) {
-        bool ok = mbar_wait(q_full, 0, abort_flag);
-        for (int n = 0; ok && n < 2 && n < n_items; ++n) {
-          ok = mbar_wait(&k_full[(n >> shift) & 1], 0, abort_flag);
-          if (!ok) break;
-          tc_fence_after_sync();
-          issue_s(n);
-        }
-        for (int n = 0; ok && n < n_items; ++n) {
-          const int g = n & 1, t = n >> shift, k = n >> 1;
-          ok = mbar_wait(&v_ready[t & 1], (t >> 1) & 1, abort_flag) && mbar_wait(&p_half[g], k & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after_sync();
-          issue_pv(n, 0);
-          ok = mbar_wait(&p_ready[g], k & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after_sync();
-          issue_pv(n, 1);
-          if (!two || g) tc_commit(&v_empty[t & 1]);
-          if (n + 2 < n_items) {
-            const int t2 = (n + 2) >> shift;
-            ok = mbar_wait(&k_full[t2 & 1], (t2 >> 1) & 1, abort_flag);
-            if (!ok) break;
-            tc_fence_after_sync();
-            issue_s(n + 2);
-          }
-          if (n == n_items - 1) tc_commit(o_done);
-        }
+        if (two) walk(Bool<true>{});
+        else walk(Bool<false>{});
       }
       __syncwarp();
     } else if constexpr (!KV8) {
       const bool is_v = warp == 11;
       const int half = warp == 10 ? 1 : 0;
-      int rows[kTilePages];
+      PagesAhead pages(page_rows, range, t0, n_tiles);
       auto ask = [&](int it) {                         // all lanes; false: gave up
-        const int page0 = range.piece(t0 + it) * kTilePages, b = it & 1;
+        const int b = it & 1;
+        int rows[kTilePages];
+        pages.to(it);
 #pragma unroll
-        for (int pg = 0; pg < kTilePages; ++pg) rows[pg] = page_rows(page0 + pg, bad);
+        for (int pg = 0; pg < kTilePages; ++pg) rows[pg] = pages.row(it, pg);
         if (it >= 2 && !mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag)) return false;
         if (elect_one()) {
           if (is_v) {
@@ -411,13 +468,13 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           if (!ok) break;
           if (partial(range.piece(t0 + it) * kTile)) {
             uint4* v = reinterpret_cast<uint4*>(sv + b * TB);
-            bool odd = false;
+            uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll 8
             for (int i = lane; i < TB / 16; i += 32) {
               const uint4 w = v[i];
-              odd |= odd_bf16x2(w.x) || odd_bf16x2(w.y) || odd_bf16x2(w.z) || odd_bf16x2(w.w);
+              odd_sum<false>(sum[0], w.x); odd_sum<false>(sum[1], w.y); odd_sum<false>(sum[2], w.z); odd_sum<false>(sum[3], w.w);
             }
-            if (__any_sync(0xffffffffu, odd)) {
+            if (__any_sync(0xffffffffu, odd_bf16x2(sum[0]) || odd_bf16x2(sum[1]) || odd_bf16x2(sum[2]) || odd_bf16x2(sum[3]))) {
               for (int i = lane; i < TB / 16; i += 32) {
                 uint4 w = v[i];
                 w.x = without_odd_bf16(w.x); w.y = without_odd_bf16(w.y); w.z = without_odd_bf16(w.z); w.w = without_odd_bf16(w.w);
@@ -432,22 +489,25 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           if (it >= 1 && it + 1 < n_tiles) ok = ask(it + 1);
         }
       }
+      bad = pages.bad;
     } else {
-      // raw tiles K0 V0 K1 V1 ... through a ring of slots; each of the three warps widens a part of every one
+      // raw half tiles K0 K0' V0 V0' K1 ... through a ring of slots; each of the three warps widens a part of every one
       const int part = warp == 8 ? 0 : warp - 9;
-      const int slots = two ? 2 : 4, pieces = 2 * n_tiles;
-      auto slot_at = [&](int s) { return s < 2 ? smem + 6 * TB + s * S::kRaw : sq + TB + (s - 2) * S::kRaw; };      // the unused tile of Q
+      const int slots = two ? 4 : 8, turn = two ? 2 : 3, pieces = 4 * n_tiles;
+      auto slot_at = [&](int s) { return s < 4 ? smem + 6 * TB + s * S::kRaw : sq + TB + (s - 4) * S::kRaw; };      // the unused tile of Q
+      PagesAhead pages(page_rows, range, t0, part == 0 ? n_tiles : 0);
       auto ask = [&](int j) {                          // warp 8
-        const int page0 = range.piece(t0 + (j >> 1)) * kTilePages, s = j & (slots - 1);
-        int rows[kTilePages];
+        const int it = j >> 2, s = j & (slots - 1);
+        if ((j & 3) == 0) pages.to(it);
+        int rows[kTilePages / 2];
 #pragma unroll
-        for (int pg = 0; pg < kTilePages; ++pg) rows[pg] = page_rows(page0 + pg, bad);
-        if (j >= slots && !mbar_wait_warp(&raw_empty[s], (j / slots - 1) & 1, abort_flag)) return false;
+        for (int pg = 0; pg < kTilePages / 2; ++pg) rows[pg] = pages.row(it, (j & 1) * (kTilePages / 2) + pg);
+        if (j >= slots && !mbar_wait_warp(&raw_empty[s], ((j >> turn) - 1) & 1, abort_flag)) return false;
         if (elect_one()) {
           uint8_t* dst = slot_at(s);
           mbar_expect_tx(&raw_full[s], S::kRaw);
 #pragma unroll
-          for (int pg = 0; pg < kTilePages; ++pg) tma_load_2d(dst + pg * kPage * D, j & 1 ? &tma_v : &tma_k, &raw_full[s], 0, rows[pg]);
+          for (int pg = 0; pg < kTilePages / 2; ++pg) tma_load_2d(dst + pg * kPage * D, j & 2 ? &tma_v : &tma_k, &raw_full[s], 0, rows[pg]);
         }
         __syncwarp();
         return true;
@@ -457,44 +517,55 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         for (int j = 0; ok && j < slots - 1 && j < pieces; ++j) ok = ask(j);
       for (int j = 0; ok && j < pieces; ++j) {
         if (part == 0 && j + slots - 1 < pieces) ok = ask(j + slots - 1);
-        const int it = j >> 1, b = it & 1, s = j & (slots - 1);
-        const bool is_v = j & 1;
-        ok = ok && mbar_wait_warp(&raw_full[s], (j / slots) & 1, abort_flag) &&
-             (it < 2 || mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag));
+        const int it = j >> 2, b = it & 1, s = j & (slots - 1);
+        const bool is_v = j & 2;
+        ok = ok && mbar_wait_warp(&raw_full[s], (j >> turn) & 1, abort_flag) &&
+             (it < 2 || (j & 1) || mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag));
         if (!ok) break;
         const uint8_t* src = slot_at(s);
         uint8_t* dst = (is_v ? sv : sk) + b * TB;
         const bool look = is_v && partial(range.piece(t0 + it) * kTile);
-        bool odd = false;
+        uint32_t sum[2] = {0, 0};
         constexpr int CPR = D / 16;                    // 16-byte pieces of a raw row
+        auto widen = [&](auto looking) {
 #pragma unroll 4
-        for (int i = part * 32 + lane; i < kTile * CPR; i += 96) {
-          const int rr = i / CPR, c = 2 * (i % CPR);
-          const uint4 raw = *reinterpret_cast<const uint4*>(src + i * 16);
-          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-          uint32_t h[8];
+          for (int i = part * 32 + lane; i < kRawTokens * CPR; i += 96) {
+            const int rr = (j & 1) * kRawTokens + i / CPR, c = 2 * (i % CPR);
+            const uint4 raw = *reinterpret_cast<const uint4*>(src + i * 16);
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            uint32_t h[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] & 0xFFFFu), __NV_E4M3);
-            const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] >> 16), __NV_E4M3);
-            h[2 * e] = (uint32_t)lo.x | ((uint32_t)lo.y << 16);
-            h[2 * e + 1] = (uint32_t)hi.x | ((uint32_t)hi.y << 16);
-          }
-          if (look) {
+            for (int e = 0; e < 4; ++e) {
+              const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] & 0xFFFFu), __NV_E4M3);
+              const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] >> 16), __NV_E4M3);
+              h[2 * e] = (uint32_t)lo.x | ((uint32_t)lo.y << 16);
+              h[2 * e + 1] = (uint32_t)hi.x | ((uint32_t)hi.y << 16);
+            }
+            if constexpr (decltype(looking)::value) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (odd_f16x2(h[e])) { odd = true; h[e] = without_odd_f16(h[e]); }
+              for (int e = 0; e < 8; ++e) {
+                odd_sum<true>(sum[e & 1], h[e]);
+                h[e] = without_odd_f16(h[e]);
+              }
+            }
+            // K: [half][128 rows][64]; V: [page][half][16][64]
+            uint8_t* line = is_v ? dst + (rr >> 4) * (D / 64) * 2048 + (c >> 3) * 2048 + (rr & 15) * 128 : dst + (c >> 3) * kHalf + rr * 128;
+            *reinterpret_cast<uint4*>(line + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(line + ((((c & 7) + 1) ^ (rr & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
           }
-          // K: [half][128 rows][64]; V: [page][half][16][64]
-          uint8_t* line = is_v ? dst + (rr >> 4) * (D / 64) * 2048 + (c >> 3) * 2048 + (rr & 15) * 128 : dst + (c >> 3) * kHalf + rr * 128;
-          *reinterpret_cast<uint4*>(line + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(line + ((((c & 7) + 1) ^ (rr & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-        }
-        if (odd) atomicOr(&seen[4], 1);
+        };
+        if (look) widen(Bool<true>{});
+        else widen(Bool<false>{});
+        if (odd_f16x2(sum[0]) || odd_f16x2(sum[1])) atomicOr(&seen[4], 1);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) { mbar_arrive(is_v ? &v_ready[b] : &k_full[b]); mbar_arrive(&raw_empty[s]); }
+        if (lane == 0) {
+          mbar_arrive(&raw_empty[s]);
+          if (j & 1) mbar_arrive(is_v ? &v_ready[b] : &k_full[b]);
+        }
+        __syncwarp();
       }
+      bad = pages.bad;
     }
     if (bad && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
   } else {
@@ -514,12 +585,14 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       const int k = n >> 1, tok0 = range.piece(t0 + (n >> shift)) * kTile;
       if (!mbar_wait(&s_full[group], k & 1, abort_flag)) { ok = false; break; }
       tc_fence_after_sync();
-      uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
       const bool whole = tok0 + kTile <= w_base && (tok0 >= w_beg || tok0 + kTile <= p.first);
-      if (!whole) row_bits(p, tok0, row.base, row.beg, q0, qn, kv_len, qi, vis);
-      if (p.softcap > 0.f) softmax_tile<D, true, true, KV8>(p, t_s, t_o, vis, factor, k > 0, &p_half[group], m_used, l);
-      else if (whole) softmax_tile<D, false, false, KV8>(p, t_s, t_o, vis, factor, k > 0, &p_half[group], m_used, l);
-      else softmax_tile<D, true, false, KV8>(p, t_s, t_o, vis, factor, k > 0, &p_half[group], m_used, l);
+      const uint4 vis = whole ? make_uint4(~0u, ~0u, ~0u, ~0u) : row_bits(p, q0, qn, kv_len, qi, tok0);
+      float2 ml;
+      if (p.softcap > 0.f) ml = softmax_capped<D, KV8>(t_s, t_o, vis, factor, p.softcap, k > 0, &p_half[group], m_used, l);
+      else if (whole) ml = softmax_tile<D, false, false, KV8>(t_s, t_o, vis, factor, 0.f, k > 0, &p_half[group], m_used, l);
+      else ml = softmax_masked<D, KV8>(t_s, t_o, vis, factor, k > 0, &p_half[group], m_used, l);
+      m_used = ml.x;
+      l = ml.y;
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[group]);
@@ -633,8 +706,8 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         for (int it = 0; it < n_tiles; ++it) {
           const int tok0 = range.piece(t0 + it) * kTile;
           if (!partial(tok0)) continue;
-          uint32_t vis[4];
-          row_bits(p, tok0, row.base, row.beg, q0, qn, kv_len, qi, vis);
+          const uint4 visible = row_bits(p, q0, qn, kv_len, qi, tok0);
+          const uint32_t vis[4] = {visible.x, visible.y, visible.z, visible.w};
           for (int i = 0; i < kTile; ++i) {
             if (!(vis[i >> 5] >> (i & 31) & 1)) continue;
             const int page = (tok0 + i) / kPage, b = span_block(p, page_rows.table, page);
