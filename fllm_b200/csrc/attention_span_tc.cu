@@ -11,7 +11,7 @@
 //
 //   warps 0 - 7   softmax        warp 9   issuer
 //   bf16 cache    warps 8, 10 ask for K by TMA, warp 11 for V; it also looks through V where not every row sees the whole tile
-//   e4m3 cache    warp 8 asks for K and V as they are; warps 8, 10, 11 widen them to f16 operands in 128-byte swizzled rows
+//   e4m3 cache    warp 8 asks for K and V as they are, page by page; warps 8, 10, 11 widen them to f16 operands in 128-byte swizzled rows
 //
 // What a row sees of a tile is four words of bits, from its bounds and its mask; tiles that all rows of a warp see whole have code
 // without them. Values of places that some row does not see may be infinite or NaN: they are taken out of the tile there, and rows that
@@ -84,51 +84,75 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return hi <= lo ? 0u : (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
 }
 
-// What row `qi` of a sequence (negative: none) sees of the 128 tokens from tok0 on. Out of line and from the beginning: few tiles need it, and what
-// it knows of the row would be held in registers beside the 128 scores of those that do not.
-__device__ __noinline__ uint4 row_bits(const SpanParams& p, int q0, int qn, int kv_len, int qi, int tok0) {
-  uint32_t vis[4] = {0, 0, 0, 0};
-  if (qi >= 0) {
-    unsigned long long b[kSpanWords + 1] = {0, 0, 0, 0, 0};
-    const SpanRow row = span_row(p, q0, qn, kv_len, qi, b);
+// What a row sees of the 128 tokens from tok0 on: its context, and (trees, out of line: few tiles hold nodes, and what a mask needs would be held in
+// registers beside the scores of those that do not) the nodes that row `qi` of the sequence sees.
+__device__ __forceinline__ uint4 context_bits(const SpanParams& p, int base, int beg, int tok0) {
+  uint32_t vis[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int t = tok0 + 32 * c, n = t - row.base;   // n: node of the word's first token
-      uint32_t w = bits_between(row.beg - t, row.base - t) | bits_between(0, min(p.first, row.base) - t);
-      if (p.tree_mask) {
-        if (n < 0) w |= n > -32 ? (uint32_t)(b[0] << -n) : 0u;
-        else if (n < 64 * kSpanWords) w |= (uint32_t)((b[n >> 6] >> (n & 63)) | ((n & 63) ? b[(n >> 6) + 1] << (64 - (n & 63)) : 0ull));
-      }
-      vis[c] = w;
-    }
+  for (int c = 0; c < 4; ++c) {
+    const int t = tok0 + 32 * c;
+    vis[c] = bits_between(beg - t, base - t) | bits_between(0, min(p.first, base) - t);
   }
   return make_uint4(vis[0], vis[1], vis[2], vis[3]);
 }
+__device__ __noinline__ uint4 tree_bits(const SpanParams& p, int q0, int qn, int kv_len, int qi, int tok0) {
+  unsigned long long b[kSpanWords + 1] = {0, 0, 0, 0, 0};
+  const SpanRow row = span_row(p, q0, qn, kv_len, qi, b);
+  const uint4 context = context_bits(p, row.base, row.beg, tok0);
+  uint32_t vis[4] = {context.x, context.y, context.z, context.w};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int n = tok0 + 32 * c - row.base;            // node of the word's first token
+    if (n < 0) vis[c] |= n > -32 ? (uint32_t)(b[0] << -n) : 0u;
+    else if (n < 64 * kSpanWords) vis[c] |= (uint32_t)((b[n >> 6] >> (n & 63)) | ((n & 63) ? b[(n >> 6) + 1] << (64 - (n & 63)) : 0ull));
+  }
+  return make_uint4(vis[0], vis[1], vis[2], vis[3]);
+}
+__device__ __forceinline__ uint4 row_bits(const SpanParams& p, int q0, int qn, int kv_len, int qi, int tok0) {
+  if (qi < 0) return make_uint4(0, 0, 0, 0);
+  if (p.tree_mask) return tree_bits(p, q0, qn, kv_len, qi, tok0);
+  const int base = max(kv_len - qn + qi + 1, 0);
+  return context_bits(p, base, p.window > 0 ? max(0, base - p.window) : 0, tok0);
+}
+
+// tanh of the scaled scores of a tile in place, for a soft-cap.
+__device__ __noinline__ void cap_scores(uint32_t t_s, float cap_in) {
+#pragma unroll 1
+  for (int c = 0; c < 8; ++c) {
+    uint32_t s[16];
+    tmem_ld_32x16(t_s + 16 * c, s);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __float_as_uint(tanhf(__uint_as_float(s[i]) * cap_in));
+    tmem_st_32x16(t_s + 16 * c, s);
+  }
+  tmem_st_wait();
+}
 
 // A row's softmax over one tile of 128 tokens: scores in registers, weights as 16-bit values over the scores' first columns, the first 64 of them
-// handed over before the others are computed; O of the warp is rescaled when a row's maximum has moved by more than 2^8.
-template <int D, bool MASKED, bool CAPPED, bool F16>
-__device__ __forceinline__ float2 softmax_tile(uint32_t t_s, uint32_t t_o, uint4 visible, float factor, float softcap, bool have_o, uint64_t* p_half,
-                                               float m_used, float l) {
-  const uint32_t vis[4] = {visible.x, visible.y, visible.z, visible.w};
-  const float cap_in = CAPPED ? factor / (softcap * kLog2e) : 0.f;
-  const float scale = CAPPED ? softcap * kLog2e : factor;
+// handed over before the others are computed; O of the warp is rescaled when a row's maximum has moved by more than 2^8. Scores that the row
+// does not see become -inf first, 32 columns at a time where some row of the warp does not see them all.
+template <int D, bool F16>
+__device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, bool whole, const uint4& visible, float scale, bool have_o, uint64_t* p_half,
+                                             float& m_used, float& l) {
   uint32_t s[4][32];
 #pragma unroll
   for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, s[c]);
   tmem_ld_wait();
+  if (!whole) {
+    const uint32_t vis[4] = {visible.x, visible.y, visible.z, visible.w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (__all_sync(0xffffffffu, vis[c] == 0xffffffffu)) continue;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (!(vis[c] & (1u << j))) s[c][j] = 0xFF800000u;
+    }
+  }
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int i = 0; i < 128; i += 2) {
-    float a[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      a[k] = __uint_as_float(s[i >> 5][(i & 31) + k]);
-      if (CAPPED) { a[k] = tanhf(a[k] * cap_in); s[i >> 5][(i & 31) + k] = __float_as_uint(a[k]); }
-      if (MASKED && !(vis[i >> 5] >> ((i & 31) + k) & 1)) a[k] = -INFINITY;
-    }
-    mx[(i >> 1) & 3] = fmaxf(fmaxf(mx[(i >> 1) & 3], a[0]), a[1]);
-  }
+  for (int i = 0; i < 128; i += 2)
+    mx[(i >> 1) & 3] = fmaxf(fmaxf(mx[(i >> 1) & 3], __uint_as_float(s[i >> 5][i & 31])), __uint_as_float(s[i >> 5][(i & 31) + 1]));
   // the scale is positive, so it commutes with the maximum
   const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
   const bool grow = m > m_used + kLazyRescale || (m_used == -INFINITY && m > -INFINITY);
@@ -160,10 +184,6 @@ __device__ __forceinline__ float2 softmax_tile(uint32_t t_s, uint32_t t_o, uint4
       const uint64_t x = fma2(pack2(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])), scale2, ref2);
       float2 e = unpack2(x);
       e.x = ex2(e.x); e.y = ex2(e.y);
-      if (MASKED) {
-        if (!(vis[c] >> j & 1)) e.x = 0.f;
-        if (!(vis[c] >> (j + 1) & 1)) e.y = 0.f;
-      }
       sum[j >> 1 & 1] = add2(sum[j >> 1 & 1], pack2(e.x, e.y));
       w[j >> 1] = pack_16<F16>(e.x, e.y);
     }
@@ -178,59 +198,78 @@ __device__ __forceinline__ float2 softmax_tile(uint32_t t_s, uint32_t t_o, uint4
   const float2 l0 = unpack2(sum[0]), l1 = unpack2(sum[1]);
   l += (l0.x + l0.y) + (l1.x + l1.y);
   tmem_st_wait();
-  return make_float2(m_used, l);
 }
-template <int D, bool F16>
-__device__ __noinline__ float2 softmax_masked(uint32_t t_s, uint32_t t_o, uint4 visible, float factor, bool have_o, uint64_t* p_half, float m_used, float l) {
-  return softmax_tile<D, true, false, F16>(t_s, t_o, visible, factor, 0.f, have_o, p_half, m_used, l);
-}
-template <int D, bool F16>
-__device__ __noinline__ float2 softmax_capped(uint32_t t_s, uint32_t t_o, uint4 visible, float factor, float softcap, bool have_o, uint64_t* p_half, float m_used,
-                                              float l) {
-  return softmax_tile<D, true, true, F16>(t_s, t_o, visible, factor, softcap, have_o, p_half, m_used, l);
-}
+
+// Rows of a tile that a thread goes through at a fixed distance, as (query row, head) pairs without a division for each.
+struct RowWalk {
+  int q, h, step_q, step_h, G;
+  __device__ __forceinline__ RowWalk(int row, int step, int group) : G(group) {
+    q = row / G; h = row - q * G;
+    step_q = step / G; step_h = step - step_q * G;
+  }
+  __device__ __forceinline__ void next() {
+    q += step_q; h += step_h;
+    if (h >= G) { h -= G; ++q; }
+  }
+};
 
 // Queries of rows [0, tiles x 128) to shared memory in swizzled rows, by the 256 threads of the softmax groups. f16 (beside an e4m3 cache): times a
 // power of two per row, which leaves the factor of its scores; bf16: asynchronous copies.
 template <int D, bool F16>
 __device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* factors, int tiles, int q0, int row0, int n_rows, int kvh) {
-  constexpr int C = D / 8;
-  const int G = p.group;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < tiles * kRows * C; i += 256) {
-    const int r = i / C, c = i % C, rr = r & (kRows - 1);
-    const bool valid = r < n_rows;
-    const int qi = valid ? (row0 + r) / G : 0, hg = valid ? (row0 + r) - qi * G : 0;
-    const bf16* src = static_cast<const bf16*>(p.q) + (size_t)(q0 + qi) * p.ldq + (size_t)(kvh * G + hg) * D + c * 8;
-    uint8_t* dst = sq + (r >> 7) * tile_bytes<D>() + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+  constexpr int C = D / 8, kStep = 256 / C, kBatch = 8;        // rows between those of a thread; loads on their way at once
+  const int c = threadIdx.x % C, r0 = threadIdx.x / C, G = p.group;
+  RowWalk at(row0 + r0, kStep, G);
+  const bf16* head = static_cast<const bf16*>(p.q) + (size_t)q0 * p.ldq + (size_t)kvh * G * D + c * 8;
+  for (int i0 = 0; i0 < tiles * kRows / kStep; i0 += kBatch) {
+    uint4 v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i, at.next()) {
+      const int r = r0 + (i0 + i) * kStep, rr = r & (kRows - 1);
+      const bool valid = r < n_rows;
+      const bf16* src = valid ? head + (size_t)at.q * p.ldq + (size_t)at.h * D : static_cast<const bf16*>(p.q);
+      if constexpr (F16) {
+        v[i] = valid ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+      } else {
+        uint8_t* dst = sq + (r >> 7) * tile_bytes<D>() + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+        if (c == 0) factors[r] = p.scale_log2;
+      }
+    }
     if constexpr (F16) {
-      uint4 v = valid ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-      uint32_t top = 0;                    // largest exponent field of the row, infinities and NaN aside
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t a = w[e] >> 7 & 0xFF, b = w[e] >> 23 & 0xFF;
-        if (a != 0xFF) top = max(top, a);
-        if (b != 0xFF) top = max(top, b);
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = r0 + (i0 + i) * kStep, rr = r & (kRows - 1);
+        uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t top = 0;                  // largest exponent field of the row, infinities and NaN aside
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a = w[e] >> 7 & 0xFF, b = w[e] >> 23 & 0xFF;
+          if (a != 0xFF) top = max(top, a);
+          if (b != 0xFF) top = max(top, b);
+        }
+#pragma unroll
+        for (int o = C / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int up = top ? min(max(127 + 14 - (int)top, -100), 100) : 0;
+        const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = unpack_bf16x2(w[e]);
+          w[e] = pack_16<true>(x.x * f, x.y * f);
+        }
+        if (c == 0) factors[r] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+        *reinterpret_cast<uint4*>(sq + (r >> 7) * tile_bytes<D>() + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
-#pragma unroll
-      for (int o = C / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int up = top ? min(max(127 + 14 - (int)top, -100), 100) : 0;
-      const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 x = unpack_bf16x2(w[e]);
-        w[e] = pack_16<true>(x.x * f, x.y * f);
-      }
-      if (c == 0) factors[r] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
-      *reinterpret_cast<uint4*>(dst) = v;
-    } else {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
-      if (c == 0) factors[r] = p.scale_log2;
     }
   }
   if constexpr (!F16) asm volatile("cp.async.wait_all;" ::: "memory");
   fence_proxy_async_smem();
+}
+
+// `bytes` (a multiple of 16) that lie in a row, to shared memory; both on 16-byte boundaries.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar)) : "memory");
 }
 
 // First pool row of a page of a tile, or `none` (behind the pool: TMA fills it with zeros) for pages that nobody sees and pages that are not there.
@@ -307,14 +346,14 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const int kvh = rest % p.hkv;
   rest /= p.hkv;
   const int seq = rest % p.num_seqs, tile = row_tiles - 1 - rest / p.num_seqs;      // the tiles that see the most first
-  const int q0 = p.q_starts[seq], qn = p.q_starts[seq + 1] - q0, G = p.group;
+  const int q0 = p.q_starts[seq], qn = p.q_starts[seq + 1] - q0, kv_len = max(p.kv_lens[seq], 0), G = p.group;
   const int all_rows = qn > 0 && qn <= p.max_q_len ? qn * G : 0, row0 = tile * kTcRows;
   if (all_rows <= p.rows_from || row0 >= all_rows) return;
   if (q0 < 0 || q0 + qn > p.tokens) {
     if (threadIdx.x == 0 && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
     return;
   }
-  const int n_rows = min(kTcRows, all_rows - row0), kv_len = max(p.kv_lens[seq], 0);
+  const int n_rows = min(kTcRows, all_rows - row0);
   const bool two = n_rows > kRows;                     // two row tiles that share K and V, or two groups that share a row tile
 
   const int group = warp >> 2;                         // of softmax warps
@@ -330,7 +369,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     seen[0] = INT_MAX; seen[1] = 0; seen[2] = INT_MAX; seen[3] = 0; seen[4] = 0;
     fence_barrier_init();
   }
-  if (warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); tma_prefetch_desc(&tma_v); }
+  if (!KV8 && warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); tma_prefetch_desc(&tma_v); }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   SpanRow row{0, 0};
   const int qi = warp < 8 && r < n_rows ? (row0 + r) / G : -1;
@@ -499,16 +538,20 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       auto ask = [&](int j) {                          // warp 8
         const int it = j >> 2, s = j & (slots - 1);
         if ((j & 3) == 0) pages.to(it);
-        int rows[kTilePages / 2];
-#pragma unroll
-        for (int pg = 0; pg < kTilePages / 2; ++pg) rows[pg] = pages.row(it, (j & 1) * (kTilePages / 2) + pg);
         if (j >= slots && !mbar_wait_warp(&raw_empty[s], ((j >> turn) - 1) & 1, abort_flag)) return false;
-        if (elect_one()) {
-          uint8_t* dst = slot_at(s);
-          mbar_expect_tx(&raw_full[s], S::kRaw);
-#pragma unroll
-          for (int pg = 0; pg < kTilePages / 2; ++pg) tma_load_2d(dst + pg * kPage * D, j & 2 ? &tma_v : &tma_k, &raw_full[s], 0, rows[pg]);
+        // A page is 16 D bytes in a row: the four lanes that looked the piece's pages up ask for one each. One that nobody sees, or that is not
+        // there, is zeros.
+        const int pg = lane - (it & 3) * kTilePages - (j & 1) * (kTilePages / 2);
+        const bool mine = pg >= 0 && pg < kTilePages / 2 && pages.now != page_rows.none;
+        const uint32_t asked = __ballot_sync(0xffffffffu, mine) >> ((it & 3) * kTilePages + (j & 1) * (kTilePages / 2));
+        if (asked != 15u) {
+          for (int i = lane; i < S::kRaw / 16; i += 32)
+            if (!(asked >> (i / D) & 1)) *reinterpret_cast<uint4*>(slot_at(s) + i * 16) = make_uint4(0, 0, 0, 0);
+          __syncwarp();
         }
+        if (lane == 0) mbar_expect_tx(&raw_full[s], __popc(asked) * kPage * D);
+        __syncwarp();
+        if (mine) bulk_load(slot_at(s) + pg * kPage * D, static_cast<const uint8_t*>(j & 2 ? p.v_cache : p.k_cache) + (size_t)pages.now * D, kPage * D, &raw_full[s]);
         __syncwarp();
         return true;
       };
@@ -522,17 +565,23 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         ok = ok && mbar_wait_warp(&raw_full[s], (j >> turn) & 1, abort_flag) &&
              (it < 2 || (j & 1) || mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag));
         if (!ok) break;
-        const uint8_t* src = slot_at(s);
-        uint8_t* dst = (is_v ? sv : sk) + b * TB;
-        const bool look = is_v && partial(range.piece(t0 + it) * kTile);
+        const uint8_t* src = slot_at(s) + lane * 16;
+        // A turn of the warp covers kTurnRows rows. The two 16-byte pieces that a lane makes of one lie in one half of the row; at D = 128
+        // neighbouring lanes of different halves store them in opposite order, so that eight lanes meet 32 banks.
+        constexpr int CPR = D / 16, kTurnRows = 32 / CPR, kTurns = kRawTokens / kTurnRows, kMost = (kTurns + 2) / 3;
+        const int rr = lane / CPR, c = 2 * (lane % CPR), flip = D == 128 ? (c >> 3) & 1 : 0;
+        uint8_t* dst = (is_v ? sv + b * TB + (j & 1) * (kRawTokens / kPage) * (D / 64) * 2048 + (c >> 3) * 2048
+                             : sk + b * TB + (j & 1) * kRawTokens * 128 + (c >> 3) * kHalf);
         uint32_t sum[2] = {0, 0};
-        constexpr int CPR = D / 16;                    // 16-byte pieces of a raw row
         auto widen = [&](auto looking) {
-#pragma unroll 4
-          for (int i = part * 32 + lane; i < kRawTokens * CPR; i += 96) {
-            const int rr = (j & 1) * kRawTokens + i / CPR, c = 2 * (i % CPR);
-            const uint4 raw = *reinterpret_cast<const uint4*>(src + i * 16);
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+          uint4 raw[kMost];
+#pragma unroll
+          for (int u = 0; u < kMost; ++u)
+            if (part + 3 * u < kTurns) raw[u] = *reinterpret_cast<const uint4*>(src + (part + 3 * u) * 512);
+#pragma unroll
+          for (int u = 0; u < kMost; ++u) {
+            if (part + 3 * u >= kTurns) continue;
+            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
             uint32_t h[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -549,15 +598,17 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
               }
             }
             // K: [half][128 rows][64]; V: [page][half][16][64]
-            uint8_t* line = is_v ? dst + (rr >> 4) * (D / 64) * 2048 + (c >> 3) * 2048 + (rr & 15) * 128 : dst + (c >> 3) * kHalf + rr * 128;
-            *reinterpret_cast<uint4*>(line + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(line + ((((c & 7) + 1) ^ (rr & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+            const int row = (part + 3 * u) * kTurnRows + rr;
+            uint8_t* line = dst + (is_v ? (row >> 4) * (D / 64) * 2048 + (row & 15) * 128 : row * 128);
+            const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), z = make_uint4(h[4], h[5], h[6], h[7]);
+            *reinterpret_cast<uint4*>(line + ((((c & 7) + flip) ^ (row & 7)) << 4)) = flip ? z : a;
+            *reinterpret_cast<uint4*>(line + ((((c & 7) + 1 - flip) ^ (row & 7)) << 4)) = flip ? a : z;
           }
         };
-        if (look) widen(Bool<true>{});
+        if (is_v && partial(range.piece(t0 + it) * kTile)) widen(Bool<true>{});
         else widen(Bool<false>{});
         if (odd_f16x2(sum[0]) || odd_f16x2(sum[1])) atomicOr(&seen[4], 1);
-        fence_proxy_async_smem();
+        if (j & 1) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&raw_empty[s]);
@@ -575,7 +626,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     __syncwarp();
     if (lane == 0) mbar_arrive(q_full);
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float factor = factors[r];
+    const float factor = factors[r], scale = p.softcap > 0.f ? p.softcap * kLog2e : factor;
     const uint32_t t_s = tmem_base + 128 * group + lane_off, t_o = tmem_base + 256 + 128 * group + lane_off;
     // whole for the rows of this warp
     const int w_base = __reduce_min_sync(0xffffffffu, qi >= 0 ? row.base : INT_MAX), w_beg = __reduce_max_sync(0xffffffffu, qi >= 0 ? row.beg : 0);
@@ -586,13 +637,10 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       if (!mbar_wait(&s_full[group], k & 1, abort_flag)) { ok = false; break; }
       tc_fence_after_sync();
       const bool whole = tok0 + kTile <= w_base && (tok0 >= w_beg || tok0 + kTile <= p.first);
-      const uint4 vis = whole ? make_uint4(~0u, ~0u, ~0u, ~0u) : row_bits(p, q0, qn, kv_len, qi, tok0);
-      float2 ml;
-      if (p.softcap > 0.f) ml = softmax_capped<D, KV8>(t_s, t_o, vis, factor, p.softcap, k > 0, &p_half[group], m_used, l);
-      else if (whole) ml = softmax_tile<D, false, false, KV8>(t_s, t_o, vis, factor, 0.f, k > 0, &p_half[group], m_used, l);
-      else ml = softmax_masked<D, KV8>(t_s, t_o, vis, factor, k > 0, &p_half[group], m_used, l);
-      m_used = ml.x;
-      l = ml.y;
+      uint4 vis = make_uint4(0, 0, 0, 0);
+      if (!whole) vis = row_bits(p, q0, qn, kv_len, qi, tok0);
+      if (p.softcap > 0.f) cap_scores(t_s, factor / (p.softcap * kLog2e));
+      softmax_tile<D, KV8>(t_s, t_o, whole, vis, scale, k > 0, &p_half[group], m_used, l);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[group]);
@@ -638,7 +686,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       // the warp's own (its part of Q, which has been read), 256 bytes of each at a time, so that a store writes whole lines.
       const int G_row = qi >= 0 ? kvh * G + (row0 + r) - qi * G : 0;
       const bool splits = p.splits > 1;
-      float scale = 1.f;
+      float norm = 1.f;
       if (!splits) {
         float ll = l, c = 1.f;
         if (p.sinks && qi >= 0) {
@@ -647,16 +695,26 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           c = m_used == -INFINITY ? 0.f : ex2(m_used - mn);
           ll = ll * c + ex2(sk2 - mn);
         }
-        scale = ll == 0.f ? 0.f : c / ll;
+        norm = ll == 0.f ? 0.f : c / ll;
       } else if (qi >= 0) {
         *reinterpret_cast<float2*>(p.ws_ml + (((size_t)(q0 + qi) * p.hq + G_row) * p.splits + split) * 2) = have ? make_float2(m_used, l) : make_float2(-INFINITY, 0.f);
       }
-      c_mine *= scale;
-      c_other *= scale;
+      c_mine *= norm;
+      c_other *= norm;
       uint8_t* stage = sq + (size_t)(warp & 7) * (32 * 2 * 64);      // 32 rows of 128 bytes
       const int row_first = (two ? group * kRows : 0) + (warp & 3) * 32;
-      const int at = (warp & 3) * 32 + lane;
+      const int at = (warp & 3) * 32 + lane, piece = lane & 7;
+      size_t line[8];                                  // where the rows that this lane stores begin, in elements
+      {
+        RowWalk w(row0 + row_first + lane / 8, 4, G);
+#pragma unroll
+        for (int k = 0; k < 8; ++k, w.next()) {
+          const size_t q = q0 + w.q, head = kvh * G + w.h;
+          line[k] = splits ? ((q * p.hq + head) * p.splits + split) * D + piece * 4 : q * p.ldo + head * D + piece * 8;
+        }
+      }
       const int cols = splits ? 32 : 64;               // of a pass: 128 bytes of a row
+#pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += cols) {
         __syncwarp();
 #pragma unroll 1
@@ -668,8 +726,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            float x = have && scale != 0.f ? __uint_as_float(o[i]) * c_mine : 0.f;
-            if (c_mine == 0.f) x = 0.f;
+            float x = have && c_mine != 0.f ? __uint_as_float(o[i]) * c_mine : 0.f;
             if (other && c_other != 0.f) x += swap[(c0 + h + i) * kRows + at] * c_other;
             o[i] = __float_as_uint(x);
           }
@@ -690,14 +747,14 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           }
         }
         __syncwarp();
-#pragma unroll 2
+        uint4 w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint4*>(stage + (k * 4 + lane / 8) * 128 + ((piece ^ ((k * 4 + lane / 8) & 7)) << 4));
+#pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int rr = k * 4 + lane / 8, piece = lane & 7, at_row = row0 + row_first + rr;
-          if (row_first + rr >= n_rows) continue;
-          const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((piece ^ (rr & 7)) << 4));
-          const int q = at_row / G, head = kvh * G + at_row - q * G;
-          if (splits) *reinterpret_cast<uint4*>(p.ws_o + (((size_t)(q0 + q) * p.hq + head) * p.splits + split) * D + c0 + piece * 4) = w;
-          else *reinterpret_cast<uint4*>(static_cast<bf16*>(p.out) + (size_t)(q0 + q) * p.ldo + (size_t)head * D + c0 + piece * 8) = w;
+          if (row_first + k * 4 + lane / 8 >= n_rows) continue;
+          if (splits) *reinterpret_cast<uint4*>(p.ws_o + line[k] + c0) = w[k];
+          else *reinterpret_cast<uint4*>(static_cast<bf16*>(p.out) + line[k] + c0) = w[k];
         }
       }
       __syncwarp();
@@ -747,11 +804,8 @@ void launch_tc(const SpanParams& p, cudaStream_t s) {
     cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
   const uint64_t rows = (uint64_t)p.num_blocks * p.hkv * p.block_pages * kPage;
   // encoded for every call: they cost less than looking up by an address what another tensor may since have
-  CUtensorMap mk, mv;
-  if (KV8) {
-    mk = make_tmap_2d(p.k_cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, D, D, kPage, D, false);
-    mv = make_tmap_2d(p.v_cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, D, D, kPage, D, false);
-  } else {
+  CUtensorMap mk{}, mv{};
+  if (!KV8) {
     mk = make_tmap_2d(p.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, D, D * 2, kPage, 64, true);
     mv = make_tmap_parts(p.v_cache, rows, D, kPage, D / 64);
   }
