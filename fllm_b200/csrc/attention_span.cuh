@@ -87,6 +87,13 @@ __device__ __forceinline__ long long span_pool_row(const SpanParams& p, int bloc
   return ((long long)block * p.hkv + kvh) * (16 * p.block_pages) + 16 * (page % p.block_pages);
 }
 
+// Four e4m3 bytes as f16, which holds all of their values.
+__device__ __forceinline__ uint2 e4m3x4_to_f16(uint32_t w) {
+  uint2 h;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(h.x), "=r"(h.y) : "r"(w));
+  return h;
+}
+
 __device__ __forceinline__ bool odd_bf16x2(uint32_t w) { return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u; }
 __device__ __forceinline__ bool odd_f16x2(uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
 }  // namespace

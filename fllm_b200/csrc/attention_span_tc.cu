@@ -11,7 +11,7 @@
 //
 //   warps 0 - 7   softmax        warp 9   issuer
 //   bf16 cache    warps 8, 10 ask for K by TMA, warp 11 for V; it also looks through V where not every row sees the whole tile
-//   e4m3 cache    warp 8 asks for K and V as they are, page by page; warps 8, 10, 11 widen them to f16 operands in 128-byte swizzled rows
+//   e4m3 cache    K is an operand as it is, with queries in two e4m3 pieces; V travels as f16: warp 8 asks for both, warps 10 - 15 widen V
 //
 // What a row sees of a tile is four words of bits, from its bounds and its mask; tiles that all rows of a warp see whole have code
 // without them. Values of places that some row does not see may be infinite or NaN: they are taken out of the tile there, and rows that
@@ -29,20 +29,22 @@
 
 namespace fllm {
 namespace {
-constexpr int kTcThreads = 384, kTcRows = 256;
+constexpr int kTcRows = 256, kWideners = 6;       // packed rows of a CTA; warps that widen V of an e4m3 cache
+template <bool KV8> constexpr int tc_threads() { return KV8 ? 512 : 384; }
 constexpr float kTcLift = 6.f;             // f16 weights: their reference lies so far below the row's (their largest is 2^14 then)
 constexpr int kTilePages = kTile / kPage;
 template <int N> using Int = std::integral_constant<int, N>;
 template <bool B> using Bool = std::integral_constant<bool, B>;
 
 constexpr int kRawTokens = 64;             // of a piece of an e4m3 tile
-constexpr int kTcFlags = 320;              // bytes of barriers and flags
+constexpr int kTcFlags = 384;              // bytes of barriers and flags
 
-// Shared memory: two tiles of Q, two stages of K and of V, 16-bit values in rows of 128 bytes; e4m3: four slots of raw pieces (eight where
-// there is one tile of Q).
+// Shared memory: two tiles of Q, two stages of K and of V, 16-bit values in rows of 128 bytes. e4m3: Q in two e4m3 pieces, four stages of K as it
+// is, V in 16 bits behind four slots of raw halves of tiles (eight where there is one tile of Q).
 template <int D, bool KV8>
 struct TcSmem {
   static constexpr int kT = tile_bytes<D>();           // a 128-row tile of 16-bit values
+  static constexpr int kStages = KV8 ? 4 : 2, kK = KV8 ? kTile * D : kT;      // of K
   static constexpr int kRaw = KV8 ? kRawTokens * D : 0;
   static constexpr int kTiles = 6 * kT + 4 * kRaw;
   static constexpr int kTotal = kTiles + kTcFlags + kTcRows * 4 + 1024;
@@ -213,11 +215,21 @@ struct RowWalk {
   }
 };
 
-// Queries of rows [0, tiles x 128) to shared memory in swizzled rows, by the 256 threads of the softmax groups. f16 (beside an e4m3 cache): times a
-// power of two per row, which leaves the factor of its scores; bf16: asynchronous copies.
+// K-major operand of 128 rows: 16-bit values in 128-byte swizzled rows, or rows of D bytes (128 or 64), swizzled over their length.
+template <int D, bool BYTES>
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t saddr) {
+  if constexpr (BYTES && D == 64)
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
+  else
+    return make_smem_desc_sw128(saddr);
+}
+
+// Queries of rows [0, tiles x 128) to shared memory in swizzled rows, by the 256 threads of the softmax groups. Beside an e4m3 cache: two e4m3
+// pieces, of the value times a power of two per row (its largest magnitude is between 2^7 and 2^8 then) and of what that leaves, four bits each of
+// a bf16's eight. Exact down to 2^-9 of the row's largest value, within 2^-17 of that value below. bf16: asynchronous copies.
 template <int D, bool F16>
 __device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* factors, int tiles, int q0, int row0, int n_rows, int kvh) {
-  constexpr int C = D / 8, kStep = 256 / C, kBatch = 8;        // rows between those of a thread; loads on their way at once
+  constexpr int C = D / 8, kStep = 256 / C, kBatch = kRows / kStep;      // rows between those of a thread; loads on their way at once: a tile's
   const int c = threadIdx.x % C, r0 = threadIdx.x / C, G = p.group;
   RowWalk at(row0 + r0, kStep, G);
   const bf16* head = static_cast<const bf16*>(p.q) + (size_t)q0 * p.ldq + (size_t)kvh * G * D + c * 8;
@@ -250,15 +262,25 @@ __device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* 
         }
 #pragma unroll
         for (int o = C / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int up = top ? min(max(127 + 14 - (int)top, -100), 100) : 0;
+        const int up = top ? min(max(127 + 7 - (int)top, -100), 100) : 0;
         const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+        uint32_t high[2] = {0, 0}, low[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 x = unpack_bf16x2(w[e]);
-          w[e] = pack_16<true>(x.x * f, x.y * f);
+          float2 x = unpack_bf16x2(w[e]);
+          x.x = isfinite(x.x) ? x.x * f : __int_as_float(0x7FC00000);
+          x.y = isfinite(x.y) ? x.y * f : __int_as_float(0x7FC00000);
+          const uint32_t a = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
+          const uint2 h = e4m3x4_to_f16(a);
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
+          const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(x.x - y.x, x.y - y.y), __NV_SATFINITE, __NV_E4M3);
+          high[e >> 1] |= a << (16 * (e & 1));
+          low[e >> 1] |= b << (16 * (e & 1));
         }
+        uint8_t* at8 = sq + (r >> 7) * tile_bytes<D>() + rr * D + (((c >> 1) ^ (D == 128 ? rr & 7 : (rr >> 1) & 3)) << 4) + (c & 1) * 8;
+        *reinterpret_cast<uint2*>(at8) = make_uint2(high[0], high[1]);
+        *reinterpret_cast<uint2*>(at8 + kRows * D) = make_uint2(low[0], low[1]);
         if (c == 0) factors[r] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
-        *reinterpret_cast<uint4*>(sq + (r >> 7) * tile_bytes<D>() + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   }
@@ -320,7 +342,7 @@ __device__ __forceinline__ uint32_t without_odd_f16(uint32_t w) {
 }
 
 template <int D, bool KV8>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(tc_threads<KV8>(), 1)
 span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ SpanParams p, int row_tiles) {
   using S = TcSmem<D, KV8>;
   constexpr int TB = S::kT;
@@ -328,16 +350,17 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sq = smem, *sk = smem + 2 * TB, *sv = smem + 4 * TB;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kTiles);
-  uint64_t *k_full = bars, *v_full = bars + 2, *k_empty = bars + 4, *v_empty = bars + 6;      // [2] by stage
-  uint64_t *s_full = bars + 8, *p_half = bars + 10, *p_ready = bars + 12;                     // [2] by softmax group
-  uint64_t* v_ready = bars + 14;                                                              // [2] by stage: looked through, or widened
-  uint64_t *o_done = bars + 16, *q_full = bars + 17;
-  uint64_t *raw_full = bars + 18, *raw_empty = bars + 26;                                     // [8] by slot
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
+  constexpr int KS = S::kStages;
+  uint64_t *k_full = bars, *k_empty = bars + 4;                                               // [KS] by stage
+  uint64_t *v_full = bars + 8, *v_empty = bars + 10, *v_ready = bars + 12;                    // [2] by stage; ready: looked through, or widened
+  uint64_t *s_full = bars + 14, *p_half = bars + 16, *p_ready = bars + 18;                    // [2] by softmax group
+  uint64_t *o_done = bars + 20, *q_full = bars + 21;
+  uint64_t *raw_full = bars + 22, *raw_empty = bars + 30;                                     // [8] by slot
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* seen = reinterpret_cast<int*>(tmem_slot + 2);        // smallest and largest base, smallest and largest window begin, odd values met
   float* factors = reinterpret_cast<float*>(smem + S::kTiles + kTcFlags);
-  static_assert(34 * 8 + 7 * 4 <= kTcFlags, "barriers and flags");
+  static_assert(38 * 8 + 7 * 4 <= kTcFlags, "barriers and flags");
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   pdl_wait();
@@ -360,16 +383,17 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const int r = (two ? group * kRows : 0) + (warp & 3) * 32 + lane;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], KV8 ? 3 : D / 64); mbar_init(&v_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV8 ? 3 : 1);
+      mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV8 ? kWideners : 1);
     }
-    for (int i = 0; i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 3); }
+    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], KV8 ? 1 : D / 64); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], kWideners); }
     mbar_init(o_done, 1); mbar_init(q_full, 8);
     *abort_flag = 0;
     seen[0] = INT_MAX; seen[1] = 0; seen[2] = INT_MAX; seen[3] = 0; seen[4] = 0;
     fence_barrier_init();
   }
-  if (!KV8 && warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); tma_prefetch_desc(&tma_v); }
+  if (warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); if (!KV8) tma_prefetch_desc(&tma_v); }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   SpanRow row{0, 0};
   const int qi = warp < 8 && r < n_rows ? (row0 + r) / G : -1;
@@ -398,15 +422,16 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const PageRows page_rows{p, p.block_tables + (size_t)seq * p.max_blocks, kvh, (min(p.first, end) + kPage - 1) / kPage, seen[2] / kPage,
                            (end + kPage - 1) / kPage, (int)(p.num_blocks * p.hkv * p.block_pages * kPage)};
 
-  // The block was launched with 168 registers a thread: 256 x 208 + 128 x 88 = 384 x 168.
+  // The block was launched with 168 registers a thread (e4m3: 128): 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if constexpr (KV8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     bool bad = false;
     if (warp == 9) {
       constexpr int fmt = KV8 ? 0 : 1;
-      constexpr uint32_t idesc_s = make_idesc(128, 128, fmt, fmt);
+      constexpr uint32_t idesc_s = make_idesc(128, 128, fmt, fmt);      // (e4m3 x e4m3 has the same bits as f16 x f16)
       constexpr uint32_t idesc_pv = make_idesc(128, D, fmt, fmt) | (1u << 16);     // B is MN-major
-      const uint64_t dq = make_smem_desc_sw128(smem_u32(sq)), dk = make_smem_desc_sw128(smem_u32(sk));
+      const uint64_t dq = desc_k_major<D, KV8>(smem_u32(sq)), dk = desc_k_major<D, KV8>(smem_u32(sk));
       // V: [page][D / 64][16][64]; at D = 128 the second 64-wide atom of a row lies half a page further
       const uint64_t dv = (uint64_t)((smem_u32(sv) & 0x3FFFFu) >> 4) | (uint64_t)((D == 128 ? 2048 : 1024) >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
                           (uint64_t)1 << 46 | (uint64_t)2 << 61;
@@ -414,11 +439,20 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       auto issue_s = [&](auto two_tiles, auto g, int n) {
         constexpr bool kTwo = decltype(two_tiles)::value;
         constexpr int kG = decltype(g)::value;
-        const int b = kTwo ? (n >> 1) & 1 : kG;
+        const int t = kTwo ? n >> 1 : n, b = kTwo || KV8 ? t & (KS - 1) : kG;
+        const uint64_t a0 = dq + (uint64_t)(kTwo ? kG * (TB >> 4) : 0), b0 = dk + (uint64_t)(b * (S::kK >> 4));
+        if constexpr (KV8) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-          tc_mma_bf16(tmem_base + 128 * kG, dq + (uint64_t)(kTwo ? kG * (TB >> 4) : 0) + off, dk + (uint64_t)(b * (TB >> 4)) + off, idesc_s, k > 0);
+          for (int k = 0; k < D / 16; ++k) {           // both pieces of Q on the same K
+            const int piece = k / (D / 32), off = (k % (D / 32)) * 2;
+            tc_mma_f8f6f4(tmem_base + 128 * kG, a0 + (uint64_t)(piece * (kRows * D >> 4) + off), b0 + (uint64_t)off, idesc_s, k > 0);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+            tc_mma_bf16(tmem_base + 128 * kG, a0 + off, b0 + off, idesc_s, k > 0);
+          }
         }
         tc_commit(&s_full[kG]);
         if (!kTwo || kG) tc_commit(&k_empty[b]);
@@ -443,7 +477,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         if (!kTwo || kG) tc_commit(&v_empty[b]);
         if (n + 2 < n_items) {
           const int t2 = kTwo ? t + 1 : t + 2;
-          if (!mbar_wait(&k_full[kTwo ? t2 & 1 : kG], (t2 >> 1) & 1, abort_flag)) return false;
+          if (!mbar_wait(&k_full[kTwo || KV8 ? t2 & (KS - 1) : kG], (t2 / KS) & 1, abort_flag)) return false;
           tc_fence_after_sync();
           issue_s(two_tiles, g, n + 2);
         }
@@ -530,14 +564,28 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       }
       bad = pages.bad;
     } else {
-      // raw half tiles K0 K0' V0 V0' K1 ... through a ring of slots; each of the three warps widens a part of every one
-      const int part = warp == 8 ? 0 : warp - 9;
-      const int slots = two ? 4 : 8, turn = two ? 2 : 3, pieces = 4 * n_tiles;
+      // Warp 8 asks for tiles of K, and for V in raw halves of tiles through a ring of slots; each of the other six warps widens a part of every half.
+      const int part = warp - 10;
+      const int slots = two ? 4 : 8, turn = two ? 2 : 3, pieces = 2 * n_tiles;
       auto slot_at = [&](int s) { return s < 4 ? smem + 6 * TB + s * S::kRaw : sq + TB + (s - 4) * S::kRaw; };      // the unused tile of Q
-      PagesAhead pages(page_rows, range, t0, part == 0 ? n_tiles : 0);
+      PagesAhead pages(page_rows, range, t0, warp == 8 ? n_tiles : 0);
+      auto ask_k = [&](int it) {                       // warp 8
+        const int b = it & (KS - 1);
+        int rows[kTilePages];
+        pages.to(it);
+#pragma unroll
+        for (int pg = 0; pg < kTilePages; ++pg) rows[pg] = pages.row(it, pg);
+        if (it >= KS && !mbar_wait_warp(&k_empty[b], (it / KS - 1) & 1, abort_flag)) return false;
+        if (elect_one()) {
+          mbar_expect_tx(&k_full[b], S::kK);
+#pragma unroll
+          for (int pg = 0; pg < kTilePages; ++pg) tma_load_2d(sk + b * S::kK + pg * kPage * D, &tma_k, &k_full[b], 0, rows[pg]);
+        }
+        __syncwarp();
+        return true;
+      };
       auto ask = [&](int j) {                          // warp 8
-        const int it = j >> 2, s = j & (slots - 1);
-        if ((j & 3) == 0) pages.to(it);
+        const int it = j >> 1, s = j & (slots - 1);
         if (j >= slots && !mbar_wait_warp(&raw_empty[s], ((j >> turn) - 1) & 1, abort_flag)) return false;
         // A page is 16 D bytes in a row: the four lanes that looked the piece's pages up ask for one each. One that nobody sees, or that is not
         // there, is zeros.
@@ -551,68 +599,53 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         }
         if (lane == 0) mbar_expect_tx(&raw_full[s], __popc(asked) * kPage * D);
         __syncwarp();
-        if (mine) bulk_load(slot_at(s) + pg * kPage * D, static_cast<const uint8_t*>(j & 2 ? p.v_cache : p.k_cache) + (size_t)pages.now * D, kPage * D, &raw_full[s]);
+        if (mine) bulk_load(slot_at(s) + pg * kPage * D, static_cast<const uint8_t*>(p.v_cache) + (size_t)pages.now * D, kPage * D, &raw_full[s]);
         __syncwarp();
         return true;
       };
       bool ok = true;
-      if (part == 0)
-        for (int j = 0; ok && j < slots - 1 && j < pieces; ++j) ok = ask(j);
-      for (int j = 0; ok && j < pieces; ++j) {
-        if (part == 0 && j + slots - 1 < pieces) ok = ask(j + slots - 1);
-        const int it = j >> 2, b = it & 1, s = j & (slots - 1);
-        const bool is_v = j & 2;
+      if (warp == 8)
+        for (int j = 0; ok && j < pieces; ++j) ok = ((j & 1) || ask_k(j >> 1)) && ask(j);
+      for (int j = 0; ok && warp != 8 && j < pieces; ++j) {
+        const int it = j >> 1, b = it & 1, s = j & (slots - 1);
         ok = ok && mbar_wait_warp(&raw_full[s], (j >> turn) & 1, abort_flag) &&
-             (it < 2 || (j & 1) || mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag));
+             (it < 2 || (j & 1) || mbar_wait_warp(&v_empty[b], ((it >> 1) - 1) & 1, abort_flag));
         if (!ok) break;
         const uint8_t* src = slot_at(s) + lane * 16;
         // A turn of the warp covers kTurnRows rows. The two 16-byte pieces that a lane makes of one lie in one half of the row; at D = 128
         // neighbouring lanes of different halves store them in opposite order, so that eight lanes meet 32 banks.
-        constexpr int CPR = D / 16, kTurnRows = 32 / CPR, kTurns = kRawTokens / kTurnRows, kMost = (kTurns + 2) / 3;
+        constexpr int CPR = D / 16, kTurnRows = 32 / CPR, kTurns = kRawTokens / kTurnRows, kMost = (kTurns + kWideners - 1) / kWideners;
         const int rr = lane / CPR, c = 2 * (lane % CPR), flip = D == 128 ? (c >> 3) & 1 : 0;
-        uint8_t* dst = (is_v ? sv + b * TB + (j & 1) * (kRawTokens / kPage) * (D / 64) * 2048 + (c >> 3) * 2048
-                             : sk + b * TB + (j & 1) * kRawTokens * 128 + (c >> 3) * kHalf);
+        uint8_t* dst = sv + b * TB + (j & 1) * (kRawTokens / kPage) * (D / 64) * 2048 + (c >> 3) * 2048;      // V: [page][half][16][64]
+        uint4 raw[kMost];
+#pragma unroll
+        for (int u = 0; u < kMost; ++u)
+          if (part + kWideners * u < kTurns) raw[u] = *reinterpret_cast<const uint4*>(src + (part + kWideners * u) * 512);
+        const bool look = partial(range.piece(t0 + it) * kTile);
         uint32_t sum[2] = {0, 0};
-        auto widen = [&](auto looking) {
-          uint4 raw[kMost];
 #pragma unroll
-          for (int u = 0; u < kMost; ++u)
-            if (part + 3 * u < kTurns) raw[u] = *reinterpret_cast<const uint4*>(src + (part + 3 * u) * 512);
-#pragma unroll
-          for (int u = 0; u < kMost; ++u) {
-            if (part + 3 * u >= kTurns) continue;
-            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-            uint32_t h[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] & 0xFFFFu), __NV_E4M3);
-              const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] >> 16), __NV_E4M3);
-              h[2 * e] = (uint32_t)lo.x | ((uint32_t)lo.y << 16);
-              h[2 * e + 1] = (uint32_t)hi.x | ((uint32_t)hi.y << 16);
-            }
-            if constexpr (decltype(looking)::value) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                odd_sum<true>(sum[e & 1], h[e]);
-                h[e] = without_odd_f16(h[e]);
-              }
-            }
-            // K: [half][128 rows][64]; V: [page][half][16][64]
-            const int row = (part + 3 * u) * kTurnRows + rr;
-            uint8_t* line = dst + (is_v ? (row >> 4) * (D / 64) * 2048 + (row & 15) * 128 : row * 128);
-            const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), z = make_uint4(h[4], h[5], h[6], h[7]);
-            *reinterpret_cast<uint4*>(line + ((((c & 7) + flip) ^ (row & 7)) << 4)) = flip ? z : a;
-            *reinterpret_cast<uint4*>(line + ((((c & 7) + 1 - flip) ^ (row & 7)) << 4)) = flip ? a : z;
+        for (int u = 0; u < kMost; ++u) {
+          if (part + kWideners * u >= kTurns) continue;
+          const uint2 h0 = e4m3x4_to_f16(flip ? raw[u].z : raw[u].x), h1 = e4m3x4_to_f16(flip ? raw[u].w : raw[u].y);
+          const uint2 h2 = e4m3x4_to_f16(flip ? raw[u].x : raw[u].z), h3 = e4m3x4_to_f16(flip ? raw[u].y : raw[u].w);
+          uint4 x = make_uint4(h0.x, h0.y, h1.x, h1.y), z = make_uint4(h2.x, h2.y, h3.x, h3.y);
+          if (look) {
+            odd_sum<true>(sum[0], x.x); odd_sum<true>(sum[1], x.y); odd_sum<true>(sum[0], x.z); odd_sum<true>(sum[1], x.w);
+            odd_sum<true>(sum[0], z.x); odd_sum<true>(sum[1], z.y); odd_sum<true>(sum[0], z.z); odd_sum<true>(sum[1], z.w);
+            x.x = without_odd_f16(x.x); x.y = without_odd_f16(x.y); x.z = without_odd_f16(x.z); x.w = without_odd_f16(x.w);
+            z.x = without_odd_f16(z.x); z.y = without_odd_f16(z.y); z.z = without_odd_f16(z.z); z.w = without_odd_f16(z.w);
           }
-        };
-        if (is_v && partial(range.piece(t0 + it) * kTile)) widen(Bool<true>{});
-        else widen(Bool<false>{});
+          const int row = (part + kWideners * u) * kTurnRows + rr;
+          uint8_t* line = dst + (row >> 4) * (D / 64) * 2048 + (row & 15) * 128;
+          *reinterpret_cast<uint4*>(line + ((((c & 7) + flip) ^ (row & 7)) << 4)) = x;
+          *reinterpret_cast<uint4*>(line + ((((c & 7) + 1 - flip) ^ (row & 7)) << 4)) = z;
+        }
         if (odd_f16x2(sum[0]) || odd_f16x2(sum[1])) atomicOr(&seen[4], 1);
         if (j & 1) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&raw_empty[s]);
-          if (j & 1) mbar_arrive(is_v ? &v_ready[b] : &k_full[b]);
+          if (j & 1) mbar_arrive(&v_ready[b]);
         }
         __syncwarp();
       }
@@ -620,7 +653,8 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     }
     if (bad && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if constexpr (KV8) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     load_q<D, KV8>(p, sq, factors, two ? 2 : 1, q0, row0, n_rows, kvh);
     __syncwarp();
@@ -805,14 +839,16 @@ void launch_tc(const SpanParams& p, cudaStream_t s) {
   const uint64_t rows = (uint64_t)p.num_blocks * p.hkv * p.block_pages * kPage;
   // encoded for every call: they cost less than looking up by an address what another tensor may since have
   CUtensorMap mk{}, mv{};
-  if (!KV8) {
+  if (KV8) {
+    mk = make_tmap_bytes(p.k_cache, rows, D, kPage);
+  } else {
     mk = make_tmap_2d(p.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, D, D * 2, kPage, 64, true);
     mv = make_tmap_parts(p.v_cache, rows, D, kPage, D / 64);
   }
   const long long tiles = ((long long)p.max_q_len * p.group + kTcRows - 1) / kTcRows;
   const long long ctas = tiles * p.num_seqs * p.hkv;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
-  launch_pdl(span_tc_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(kTcThreads), smem, s, mk, mv, p, (int)tiles);
+  launch_pdl(span_tc_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(tc_threads<KV8>()), smem, s, mk, mv, p, (int)tiles);
 }
 }  // namespace
 

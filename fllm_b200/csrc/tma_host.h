@@ -77,6 +77,21 @@ inline CUtensorMap make_tmap_parts(const void* base, uint64_t rows, uint64_t col
   return m;
 }
 
+// Rows of `cols` bytes (128 or 64) in boxes of `box_rows` whole rows, swizzled over their length. Rows beyond the tensor read as zero.
+inline CUtensorMap make_tmap_bytes(const void* base, uint64_t rows, uint32_t cols, uint32_t box_rows) {
+  CUtensorMap m;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {cols};
+  cuuint32_t box[2] = {cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (cols != 128 && cols != 64)) throw std::runtime_error("fllm_b200: TMA operand must be 16-byte aligned rows of 64 or 128 bytes");
+  CUresult r = get_encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                  cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("fllm_b200: cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return m;
+}
+
 // Programmatic dependent launch: the kernel may start while its predecessor in the stream is
 // still running; it must execute griddepcontrol.wait before it touches anything the predecessor
 // produces. FLLM_PDL=0 turns the attribute off (plain stream order).

@@ -3,7 +3,10 @@
 The bound of an output: its weights w_j are rounded to bf16 for the product with the values (relative 2^-8, f16: 2^-11), the output once more (2^-8 of
 it); a score is off by at most (D + 4) 2^-24 sum_d |q_d k_d| scale from its fp32 sum and by 2^-22 |s| from its factor, its exponent and a soft-cap (twice
 that of its magnitude), e^x and the sums over n keys add (n + 64) 2^-24. An error e of all scores moves an output by at most 2 e A,
-A = sum_j w_j |v_j|. So |o' - o| <= (2^-8 + 2 e_s) A + 2^-8 |o| + tiny, second-order terms covered by a factor of 1.1.
+A = sum_j w_j |v_j|. So |o' - o| <= (2^-8 + 2 e_s) A + 2^-8 |o| + tiny, second-order terms covered by a factor of 1.1. Beside an e4m3
+cache queries may lose 2^-17 of the row's largest magnitude in their small values, which moves a score by 2^-17 max|q| sum_d |k_d| scale; weights are f16
+there, and 2 x 2^-17 max|q| sum|k| scale <= 2^-8 - 2^-11 up to max|q| sum|k| scale = 223 (here: at most 6.75 x 256 x 0.8 / 16 = 87), so the bound is the
+same.
 """
 import math
 from types import SimpleNamespace
