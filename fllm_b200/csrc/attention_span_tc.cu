@@ -229,47 +229,45 @@ __device__ __forceinline__ uint64_t desc_k_major(uint32_t saddr) {
 // a bf16's eight. Exact down to 2^-9 of the row's largest value, within 2^-17 of that value below. bf16: asynchronous copies.
 template <int D, bool F16>
 __device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* factors, int tiles, int q0, int row0, int n_rows, int kvh) {
-  constexpr int C = D / 8, kStep = 256 / C, kBatch = kRows / kStep;      // rows between those of a thread; loads on their way at once: a tile's
-  const int c = threadIdx.x % C, r0 = threadIdx.x / C, G = p.group;
-  RowWalk at(row0 + r0, kStep, G);
-  const bf16* head = static_cast<const bf16*>(p.q) + (size_t)q0 * p.ldq + (size_t)kvh * G * D + c * 8;
-  for (int i0 = 0; i0 < tiles * kRows / kStep; i0 += kBatch) {
-    uint4 v[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i, at.next()) {
-      const int r = r0 + (i0 + i) * kStep, rr = r & (kRows - 1);
+  constexpr int C = D / 8, kStep = 256 / C;            // rows between those of a thread
+  const int c = threadIdx.x % C, r0 = threadIdx.x / C;
+  RowWalk at(row0 + r0, kStep, p.group);
+  const bf16* head = static_cast<const bf16*>(p.q) + (size_t)q0 * p.ldq + (size_t)kvh * p.group * D + c * 8;
+  if constexpr (!F16) {
+#pragma unroll 2
+    for (int r = r0; r < tiles * kRows; r += kStep, at.next()) {
       const bool valid = r < n_rows;
       const bf16* src = valid ? head + (size_t)at.q * p.ldq + (size_t)at.h * D : static_cast<const bf16*>(p.q);
-      if constexpr (F16) {
-        v[i] = valid ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
-      } else {
-        uint8_t* dst = sq + (r >> 7) * tile_bytes<D>() + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
-        if (c == 0) factors[r] = p.scale_log2;
-      }
+      uint8_t* dst = sq + (r >> 7) * tile_bytes<D>() + (c >> 3) * kHalf + (r & (kRows - 1)) * 128 + (((c & 7) ^ (r & 7)) << 4);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+      if (c == 0) factors[r] = p.scale_log2;
     }
-    if constexpr (F16) {
+  } else {
+    constexpr int kBatch = 4;                          // loads on their way at once
+#pragma unroll 1
+    for (int i0 = 0; i0 < tiles * kRows / kStep; i0 += kBatch) {
+      uint4 v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i, at.next()) {
+        const int r = r0 + (i0 + i) * kStep;
+        v[i] = r < n_rows ? __ldg(reinterpret_cast<const uint4*>(head + (size_t)at.q * p.ldq + (size_t)at.h * D)) : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int r = r0 + (i0 + i) * kStep, rr = r & (kRows - 1);
-        uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-        uint32_t top = 0;                  // largest exponent field of the row, infinities and NaN aside
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t most = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t a = w[e] >> 7 & 0xFF, b = w[e] >> 23 & 0xFF;
-          if (a != 0xFF) top = max(top, a);
-          if (b != 0xFF) top = max(top, b);
-        }
-#pragma unroll
-        for (int o = C / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int up = top ? min(max(127 + 7 - (int)top, -100), 100) : 0;
-        const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+        for (int o = C / 2; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const int top = (int)(max(most & 0xFFFFu, most >> 16) >> 7);      // largest exponent field of the row
+        const bool odd = top == 0xFF;                  // an infinity or a NaN: no score of the row is a number
+        const int up = top && !odd ? min(max(127 + 7 - top, -100), 100) : 0;
+        const float f = odd ? __int_as_float(0x7FC00000) : __uint_as_float((uint32_t)(127 + up) << 23);
         uint32_t high[2] = {0, 0}, low[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float2 x = unpack_bf16x2(w[e]);
-          x.x = isfinite(x.x) ? x.x * f : __int_as_float(0x7FC00000);
-          x.y = isfinite(x.y) ? x.y * f : __int_as_float(0x7FC00000);
+          x.x *= f; x.y *= f;
           const uint32_t a = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
           const uint2 h = e4m3x4_to_f16(a);
           const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
@@ -284,7 +282,9 @@ __device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* 
       }
     }
   }
-  if constexpr (!F16) asm volatile("cp.async.wait_all;" ::: "memory");
+}
+__device__ __forceinline__ void q_loaded() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
   fence_proxy_async_smem();
 }
 
@@ -395,6 +395,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   }
   if (warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); if (!KV8) tma_prefetch_desc(&tma_v); }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp < 8) load_q<D, KV8>(p, sq, factors, two ? 2 : 1, q0, row0, n_rows, kvh);
   SpanRow row{0, 0};
   const int qi = warp < 8 && r < n_rows ? (row0 + r) / G : -1;
   if (qi >= 0) {
@@ -656,7 +657,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     if constexpr (KV8) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    load_q<D, KV8>(p, sq, factors, two ? 2 : 1, q0, row0, n_rows, kvh);
+    q_loaded();
     __syncwarp();
     if (lane == 0) mbar_arrive(q_full);
     asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -680,15 +681,20 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       if (lane == 0) mbar_arrive(&p_ready[group]);
     }
     if (KV8) m_used -= kTcLift;
+    const bool splits = p.splits > 1;
+    const int G_row = qi >= 0 ? kvh * G + (row0 + r) - qi * G : 0;
+    const float sink = p.sinks && qi >= 0 ? p.sinks[G_row] * kLog2e : -INFINITY;
+    uint8_t* dst = splits ? reinterpret_cast<uint8_t*>(p.ws_o + (((size_t)(q0 + max(qi, 0)) * p.hq + G_row) * p.splits + split) * D)
+                          : reinterpret_cast<uint8_t*>(static_cast<bf16*>(p.out) + (size_t)(q0 + max(qi, 0)) * p.ldo + (size_t)G_row * D);
     ok = ok && n_items > 0 && mbar_wait(o_done, 0, abort_flag);       // (a group without items too: what follows reuses K and V)
     const bool have = ok && n_items > group;
     tc_fence_after_sync();
     float c_mine = 1.f, c_other = 0.f;
     bool other = false;
+    const int at = (warp & 3) * 32 + lane;
     float* swap = reinterpret_cast<float*>(sk);        // O of the second group, [column][row]; then its maxima and sums
     if (!two) {
       float2* swap_ml = reinterpret_cast<float2*>(sv);
-      const int at = (warp & 3) * 32 + lane;
       if (group == 1) {
         if (have) {
 #pragma unroll 1
@@ -716,83 +722,62 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       }
     }
     if (two || group == 0) {
-      // (m, l, O) of this warp's rows: to the workspace, or normalised with the head's sink to the output. Rows pass through shared memory of
-      // the warp's own (its part of Q, which has been read), 256 bytes of each at a time, so that a store writes whole lines.
-      const int G_row = qi >= 0 ? kvh * G + (row0 + r) - qi * G : 0;
-      const bool splits = p.splits > 1;
-      float norm = 1.f;
+      // (m, l, O) of the rows: to the workspace, or normalised with the head's sink to the output. A lane puts its row, kPass bytes of it at a time, into
+      // shared memory of the warp's own (Q and K have been read) and asks for it to be copied.
       if (!splits) {
-        float ll = l, c = 1.f;
+        float ll = l, less = 1.f;
         if (p.sinks && qi >= 0) {
-          const float sk2 = p.sinks[G_row] * kLog2e;
-          const float mn = fmaxf(m_used, sk2);
-          c = m_used == -INFINITY ? 0.f : ex2(m_used - mn);
-          ll = ll * c + ex2(sk2 - mn);
+          const float mn = fmaxf(m_used, sink);
+          less = m_used == -INFINITY ? 0.f : ex2(m_used - mn);
+          ll = ll * less + ex2(sink - mn);
         }
-        norm = ll == 0.f ? 0.f : c / ll;
+        const float norm = ll == 0.f || !have ? 0.f : less / ll;
+        c_mine *= norm;
+        c_other *= norm;
       } else if (qi >= 0) {
         *reinterpret_cast<float2*>(p.ws_ml + (((size_t)(q0 + qi) * p.hq + G_row) * p.splits + split) * 2) = have ? make_float2(m_used, l) : make_float2(-INFINITY, 0.f);
       }
-      c_mine *= norm;
-      c_other *= norm;
-      uint8_t* stage = sq + (size_t)(warp & 7) * (32 * 2 * 64);      // 32 rows of 128 bytes
-      const int row_first = (two ? group * kRows : 0) + (warp & 3) * 32;
-      const int at = (warp & 3) * 32 + lane, piece = lane & 7;
-      size_t line[8];                                  // where the rows that this lane stores begin, in elements
-      {
-        RowWalk w(row0 + row_first + lane / 8, 4, G);
-#pragma unroll
-        for (int k = 0; k < 8; ++k, w.next()) {
-          const size_t q = q0 + w.q, head = kvh * G + w.h;
-          line[k] = splits ? ((q * p.hq + head) * p.splits + split) * D + piece * 4 : q * p.ldo + head * D + piece * 8;
-        }
-      }
-      const int cols = splits ? 32 : 64;               // of a pass: 128 bytes of a row
+      constexpr int kPass = D == 128 ? 256 : 128, kPitch = kPass + 16;
+      static_assert(4 * 32 * kPitch <= 2 * TB && 8 * 32 * kPitch <= 4 * TB, "room of the rows");
+      uint8_t* stage = sq + (size_t)(warp * 32 + lane) * kPitch;
+      const int cols = splits ? kPass / 4 : kPass / 2;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += cols) {
-        __syncwarp();
+        if (c0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 #pragma unroll 1
         for (int h = 0; h < cols; h += 32) {
           uint32_t o[32];
           if (have) {
             tmem_ld_32x32(t_o + c0 + h, o);
             tmem_ld_wait();
-          }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float x = have && c_mine != 0.f ? __uint_as_float(o[i]) * c_mine : 0.f;
-            if (other && c_other != 0.f) x += swap[(c0 + h + i) * kRows + at] * c_other;
-            o[i] = __float_as_uint(x);
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c_mine);
+            if (other) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + swap[(c0 + h + i) * kRows + at] * c_other);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
           }
           if (splits) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(stage + (h + i) * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint4 w;
-              w.x = pack_bf16x2(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
-              w.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
-              w.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
-              w.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-              *reinterpret_cast<uint4*>(stage + lane * 128 + (((h / 8 + i) ^ (lane & 7)) << 4)) = w;
-            }
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4*>(stage + (h + i) * 2) =
+                  make_uint4(pack_bf16x2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), pack_bf16x2(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3])),
+                             pack_bf16x2(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5])), pack_bf16x2(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7])));
           }
         }
-        __syncwarp();
-        uint4 w[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint4*>(stage + (k * 4 + lane / 8) * 128 + ((piece ^ ((k * 4 + lane / 8) & 7)) << 4));
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (row_first + k * 4 + lane / 8 >= n_rows) continue;
-          if (splits) *reinterpret_cast<uint4*>(p.ws_o + line[k] + c0) = w[k];
-          else *reinterpret_cast<uint4*>(static_cast<bf16*>(p.out) + line[k] + c0) = w[k];
-        }
+        fence_proxy_async_smem();
+        if (qi >= 0)
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (size_t)c0 * (splits ? 4 : 2)), "r"(smem_u32(stage)), "r"(kPass) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
-      __syncwarp();
       if (seen[4] && qi >= 0) {
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         // infinities and NaN that were taken out of tiles, added to the rows that see them
         for (int it = 0; it < n_tiles; ++it) {
           const int tok0 = range.piece(t0 + it) * kTile;
@@ -812,17 +797,15 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
                 x = __bfloat162float(static_cast<const bf16*>(p.v_cache)[at + d]);
               }
               if (isfinite(x)) continue;
-              if (splits) p.ws_o[(((size_t)(q0 + qi) * p.hq + G_row) * p.splits + split) * D + d] += x;
-              else {
-                bf16* y = static_cast<bf16*>(p.out) + (size_t)(q0 + qi) * p.ldo + (size_t)G_row * D + d;
-                *y = __float2bfloat16(__bfloat162float(*y) + x);
-              }
+              if (splits) reinterpret_cast<float*>(dst)[d] += x;
+              else reinterpret_cast<bf16*>(dst)[d] = __float2bfloat16(__bfloat162float(reinterpret_cast<bf16*>(dst)[d]) + x);
             }
           }
         }
       }
     }
   }
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 9) { tc_fence_after_sync(); tmem_dealloc(tmem_base, 512); }
