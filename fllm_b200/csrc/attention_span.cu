@@ -415,30 +415,36 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
   }
   const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + (size_t)pair * p.splits;
   const float* part = p.ws_o + (size_t)pair * p.splits * D + lane;
+  float2 mine = lane < p.splits ? __ldcg(ml + lane) : make_float2(-INFINITY, 0.f);
+  if (__shfl_sync(0xffffffffu, mine.y, 0) < 0.f) return;      // the row was not split
   const float sk = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
-  float mm = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, __ldcg(ml + s).x);
+  float mm = mine.x;
+  for (int s = lane + 32; s < p.splits; s += 32) mm = fmaxf(mm, __ldcg(ml + s).x);
   mm = fmaxf(warp_max(mm), sk);
   float ll = 0.f, a[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) a[e] = 0.f;
   for (int s0 = 0; s0 < p.splits; s0 += 32) {
-    const float2 v = s0 + lane < p.splits ? __ldcg(ml + s0 + lane) : make_float2(-INFINITY, 0.f);
-    const float mine = v.x == -INFINITY ? (mm == -INFINITY && v.y != 0.f ? 1.f : 0.f) : ex2(v.x - mm);
-    ll += v.y * mine;
-    const int n = min(32, p.splits - s0);
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      float x[8][D / 32];
+    if (s0) mine = s0 + lane < p.splits ? __ldcg(ml + s0 + lane) : make_float2(-INFINITY, 0.f);
+    const float w = mine.x == -INFINITY ? (mm == -INFINITY && mine.y != 0.f ? 1.f : 0.f) : ex2(mine.x - mm);
+    ll += mine.y * w;
+    unsigned live = __ballot_sync(0xffffffffu, w != 0.f);     // (of the others there are no rows)
+    while (live) {
+      int at[4];
+      float x[4][D / 32];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < 4; ++k) {
+        at[k] = live ? __ffs(live) - 1 : -1;
+        live &= live - 1;
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) x[k][e] = k0 + k < n ? __ldcg(part + (size_t)(s0 + k0 + k) * D + 32 * e) : 0.f;
+        for (int e = 0; e < D / 32; ++e) x[k][e] = at[k] >= 0 ? __ldcg(part + (size_t)(s0 + at[k]) * D + 32 * e) : 0.f;
+      }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float w = __shfl_sync(0xffffffffu, mine, (k0 + k) & 31);
-        if (k0 + k < n && w != 0.f) {
+      for (int k = 0; k < 4; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, w, at[k] & 31);
+        if (at[k] >= 0) {
 #pragma unroll
-          for (int e = 0; e < D / 32; ++e) a[e] += x[k][e] * w;
+          for (int e = 0; e < D / 32; ++e) a[e] += x[k][e] * wk;
         }
       }
     }
@@ -487,10 +493,9 @@ SpanPlan attention_span_plan(const SpanParams& p) {
     plan.rows_splits = (int)std::max<long long>(1, std::min<long long>(splits, 128));
   }
   if (tc && most > kSpanRows) {
-    const long long ctas = (most + 255) / 256 * p.num_seqs * p.hkv, tiles = (span + 127) / 128 + (p.first > 0 ? 1 : 0);
-    plan.min_tiles = (int)std::max<long long>(1, ctas * tiles / (6LL * sm_count()));
-    plan.tile_splits = (int)std::max<long long>(1, std::min<long long>((tiles + plan.min_tiles - 1) / plan.min_tiles, 32));
-    if (ctas >= 2 * sm_count()) plan.tile_splits = 1;
+    // at most four places for a piece to each SM: those that the kernel finds no work for cost a start all the same
+    const long long ctas = (most + 255) / 256 * p.num_seqs * p.hkv, tiles = (span + 127) / 128 + 2;
+    plan.tile_splits = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(4LL * sm_count() / ctas, tiles), 32));
   }
   plan.bytes = (partial_floats(p, plan.rows_splits) + partial_floats(p, plan.tile_splits)) * sizeof(float);
   return plan;
@@ -500,7 +505,7 @@ int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStre
   int n = 0;
   const bool both = plan.rows_splits > 0 && plan.tile_splits > 0;
   p.min_pages = plan.min_pages;
-  p.min_tiles = plan.min_tiles;
+  p.sms = sm_count();
   auto take = [&](int splits) {
     p.splits = splits;
     p.ws_o = static_cast<float*>(workspace);

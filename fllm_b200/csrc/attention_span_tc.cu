@@ -341,6 +341,33 @@ __device__ __forceinline__ uint32_t without_odd_f16(uint32_t w) {
   return ((w & 0x7C00u) == 0x7C00u ? 0u : w & 0xFFFFu) | ((w & 0x7C000000u) == 0x7C000000u ? 0u : w & 0xFFFF0000u);
 }
 
+// Into how many pieces the walk of an item is cut. An item's share of all the work, counted in tiles of 128 rows from the lengths, times the number of
+// SMs is the number of SMs that it could keep; four tenths are rounded up. A piece costs a start, partial sums and their way through memory, so
+// pieces come to little more than one for each SM: 16 trees of 256 packed rows, 8 key heads, all behind 6000 tokens: 107 us in one piece each, 137 in two,
+// 161 in four; 4 trees of 128: 67 in one, 47 in two, 36 in four, 49 in six; 16 of 256 behind 1000 to 12,000: 201 in pieces of up to 13 tiles,
+// 182 in one each, 143 by this rule.
+__device__ __forceinline__ int tiles_of(const SpanParams& p, int qn, int kv_len) {
+  const int tiles = max((kv_len + kTile - 1) / kTile, 1);
+  return p.window > 0 ? (int)min((long long)tiles, ((long long)p.window + p.first + min(qn, kTcRows)) / kTile + 3) : tiles;
+}
+__device__ __forceinline__ float weight_of_rows(int rows) { return rows > kRows ? 2.f : 1.f; }
+__device__ __forceinline__ int pieces_of(const SpanParams& p, int n_rows, int tiles) {
+  float total = 0.f;
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 32) {
+    const int s = s0 + (threadIdx.x & 31);
+    float mine = 0.f;
+    if (s < p.num_seqs) {
+      const int qn = p.q_starts[s + 1] - p.q_starts[s], rows = qn > 0 && qn <= p.max_q_len ? qn * p.group : 0, whole = rows / kTcRows;
+      if (rows > p.rows_from) mine = (2.f * whole + (rows > whole * kTcRows ? weight_of_rows(rows - whole * kTcRows) : 0.f)) * tiles_of(p, qn, max(p.kv_lens[s], 0));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    total += mine;
+  }
+  const float sms = weight_of_rows(n_rows) * tiles * p.sms / (total * p.hkv);
+  return max(1, min(min((int)(sms + 0.4f), p.splits), tiles));
+}
+
 template <int D, bool KV8>
 __global__ void __launch_bounds__(tc_threads<KV8>(), 1)
 span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ SpanParams p, int row_tiles) {
@@ -377,6 +404,8 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     return;
   }
   const int n_rows = min(kTcRows, all_rows - row0);
+  const int pieces = p.splits > 1 ? pieces_of(p, n_rows, tiles_of(p, qn, kv_len)) : 1;
+  if (split >= pieces) return;
   const bool two = n_rows > kRows;                     // two row tiles that share K and V, or two groups that share a row tile
 
   const int group = warp >> 2;                         // of softmax warps
@@ -415,8 +444,8 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   pdl_launch_dependents();                             // not before the allocation
   const int end = p.tree_mask ? kv_len : seen[1], min_base = seen[0], max_beg = seen[3];
   const SpanRange range = span_range(p, kTile, seen[2], end);
-  const int per_split = max(p.min_tiles, (range.count + p.splits - 1) / p.splits);
-  const int t0 = min(split * per_split, range.count), n_tiles = min(per_split, range.count - t0);
+  const int per_piece = (tiles_of(p, qn, kv_len) + pieces - 1) / pieces;      // (the last one goes on to the end, should that be further)
+  const int t0 = min(split * per_piece, range.count), n_tiles = split == pieces - 1 ? range.count - t0 : min(per_piece, range.count - t0);
   const int shift = two ? 1 : 0, n_items = n_tiles << shift;
   // not every row of the CTA sees the whole tile
   auto partial = [&](int tok0) { return !(tok0 + kTile <= min_base && (tok0 >= max_beg || tok0 + kTile <= p.first)); };
@@ -681,7 +710,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       if (lane == 0) mbar_arrive(&p_ready[group]);
     }
     if (KV8) m_used -= kTcLift;
-    const bool splits = p.splits > 1;
+    const bool splits = pieces > 1;
     const int G_row = qi >= 0 ? kvh * G + (row0 + r) - qi * G : 0;
     const float sink = p.sinks && qi >= 0 ? p.sinks[G_row] * kLog2e : -INFINITY;
     uint8_t* dst = splits ? reinterpret_cast<uint8_t*>(p.ws_o + (((size_t)(q0 + max(qi, 0)) * p.hq + G_row) * p.splits + split) * D)
@@ -734,8 +763,12 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         const float norm = ll == 0.f || !have ? 0.f : less / ll;
         c_mine *= norm;
         c_other *= norm;
-      } else if (qi >= 0) {
-        *reinterpret_cast<float2*>(p.ws_ml + (((size_t)(q0 + qi) * p.hq + G_row) * p.splits + split) * 2) = have ? make_float2(m_used, l) : make_float2(-INFINITY, 0.f);
+      }
+      if (p.splits > 1 && qi >= 0) {                   // what span_merge_kernel reads: the row's maxima and sums, or that it is done
+        float2* ml = reinterpret_cast<float2*>(p.ws_ml) + ((size_t)(q0 + qi) * p.hq + G_row) * p.splits;
+        ml[split] = !splits ? make_float2(0.f, -1.f) : have ? make_float2(m_used, l) : make_float2(-INFINITY, 0.f);
+        if (splits && split == 0)
+          for (int i = pieces; i < p.splits; ++i) ml[i] = make_float2(-INFINITY, 0.f);
       }
       constexpr int kPass = D == 128 ? 256 : 128, kPitch = kPass + 16;
       static_assert(4 * 32 * kPitch <= 2 * TB && 8 * 32 * kPitch <= 4 * TB, "room of the rows");

@@ -311,14 +311,14 @@ struct SpanParams {
   int window, first;           // window 0: no limit (first is 0 then)
   float scale, scale_log2, softcap;
   // set by the planner, for one kernel
-  int splits, min_pages, min_tiles;      // pieces of a sequence's visible tokens; fewest pages, or tiles of 128 tokens, in one
+  int splits, min_pages, sms;  // pieces of what a sequence's rows see, at most; fewest pages in one; SMs
   int rows_from, rows_to;      // packed rows (query rows x group) of the sequences that the kernel takes: from < rows <= to
   float* ws_o;                 // [tokens][hq][splits][head_dim]
   float* ws_ml;                // [tokens][hq][splits][2]
 };
 struct SpanPlan {
   int rows_splits, tile_splits;          // of the kernel for few rows and of the tensor-memory kernel; 0: it has no rows
-  int min_pages, min_tiles;
+  int min_pages;
   size_t bytes;                          // of workspace
 };
 SpanPlan attention_span_plan(const SpanParams& p);
