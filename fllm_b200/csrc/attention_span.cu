@@ -6,7 +6,7 @@
 // (attention_span.cuh says what that is; a row that sees nothing is 0.) One CTA per (sequence, 16 packed rows, key head, split). Its four
 // warps take the 16-token pages that the rows see between them in turn: the first tokens' pages and the window's, nothing in between. Each
 // streams its pages through a private cp.async ring, so the main loop has no barrier; (m, l, O) of the warps are joined in shared memory,
-// those of the splits by span_merge_kernel. Sequences with more than 16 packed rows go to attention_span_tc.cu where that has a kernel.
+// those of up to eight splits in that of their cluster, of more by span_merge_kernel. Sequences with more than 16 packed rows go to attention_span_tc.cu where that has a kernel.
 //
 // Scores and sums are fp32. Weights are rounded to the operands' 16 bits for the product with the values (bf16, at most 2^-9 each and of
 // either sign; f16 beside an e4m3 cache). An e4m3 cache is widened to f16, which holds all of its values; queries are f16 there as well, times a
@@ -55,27 +55,51 @@ __device__ __forceinline__ float2 unpack_16(uint32_t w) {
   if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   else return unpack_bf16x2(w);
 }
-template <bool F16>
-__device__ __forceinline__ bool odd_16x2(uint32_t w) {
-  if constexpr (F16) return odd_f16x2(w);
-  else return odd_bf16x2(w);
-}
 __device__ __forceinline__ void cp_async16_or_zero(void* smem, const void* gmem, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(there ? 16 : 0) : "memory");
 }
 
+// Four values of a row, normalised with the head's sink.
+template <int D>
+__device__ __forceinline__ void store_row(const SpanParams& p, int q0, int row, int kvh, int d, float4 a, float mm, float ll) {
+  const int qi = row / p.group, head = kvh * p.group + row - qi * p.group;
+  float c = 1.f;
+  if (p.sinks) {
+    const float sk = p.sinks[head] * kLog2e, mn = fmaxf(mm, sk);
+    c = mm == -INFINITY ? 0.f : ex2(mm - mn);
+    ll = ll * c + ex2(sk - mn);
+  }
+  const float inv = ll == 0.f ? 0.f : c / ll;
+  *reinterpret_cast<uint2*>(static_cast<bf16*>(p.out) + (size_t)(q0 + qi) * p.ldo + (size_t)head * D + d) =
+      make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
+}
+
+// An e4m3 page stays as it is in shared memory and becomes operands in registers, which needs no order of columns that memory does not have: a lane
+// takes 16 bytes of a key row for four k-steps (queries lie in the same order), and 16 bytes of each of four value rows, two tokens of a dim to a
+// register. So of column block i of O, column n is dim i of the n-th piece of 16 (or 8, at D = 64) values. (Through f16 tiles in shared memory, ldmatrix
+// behind them, 48 sequences under a window of 1000 with 130 first tokens, 64 query and 8 key heads of 64, took 42 us, ROWS8_US so.)
+template <int D>
+__device__ __forceinline__ int dim_of(int i, int n) {
+  if constexpr (D == 64) return 8 * n + i;
+  return (i >> 4) * 128 + 16 * n + (i & 15);
+}
+// Pieces of 16 bytes of row r lie at piece ^ this: rows next to each other (keys), every second row (values) meet other banks.
+template <int D> __device__ __forceinline__ int turn_k(int r) { return D == 64 ? 0 : (r & 1) << 2; }
+template <int D> __device__ __forceinline__ int turn_v(int r) { return D == 64 ? (r >> 1) & 3 : r & 6; }
+
 template <int D, bool KV8>
 struct RowsSmem {
-  static constexpr int kStages = D == 256 && !KV8 ? 2 : 3;
+  static constexpr int kStages = KV8 ? 4 : D == 256 ? 2 : 3;
   static constexpr int kPageElems = kPage * D;
-  static constexpr int kPageBytes = kPageElems * (KV8 ? 1 : 2);          // a K or V page as it arrives
+  static constexpr int kPageBytes = kPageElems * (KV8 ? 1 : 2);          // a K or V page
   static constexpr int kWarpRing = kStages * 2 * kPageBytes;
-  static constexpr int kWarpTiles = KV8 ? 2 * kPageElems * 2 : 0;        // widened pages
-  static constexpr int kRing = 4 * (kWarpRing + kWarpTiles);
-  static constexpr int kMerge = 4 * kSpanRows * (D + 2) * 4;
-  static constexpr int kQ = kSpanRows * D * 2;
+  static constexpr int kRing = 4 * kWarpRing;
+  static constexpr int kMerge = 4 * kSpanRows * (D + 2) * 4, kPart = kSpanRows * (D + 4) * 4;
+  static constexpr int kQPitch = D + (KV8 ? 8 : 0);
+  static constexpr int kQ = kSpanRows * kQPitch * 2;
   static constexpr int kInfo = kSpanRows * (8 * kSpanWords + 4 * 3);
-  static constexpr int kTotal = kQ + kInfo + (kRing > kMerge ? kRing : kMerge) + 128;
+  static constexpr int kTotal = kQ + kInfo + kRing + 128;
+  static_assert(kMerge + kPart <= kRing && kQ % 16 == 0 && kInfo % 16 == 0, "shared memory");
 };
 
 template <int D, bool KV8>
@@ -88,21 +112,24 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
   int* begs = bases + kSpanRows;
   float* factors = reinterpret_cast<float*>(begs + kSpanRows);                         // of a row's scores, to base 2
   uint8_t* ring = smem + S::kQ + S::kInfo;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = p.group, split = blockIdx.y;
-  const int work = blockIdx.x / p.hkv, kvh = blockIdx.x - work * p.hkv;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = p.group;
+  int work = blockIdx.x / p.splits;
+  const int split = blockIdx.x - work * p.splits;
+  const int kvh = work % p.hkv;
+  work /= p.hkv;
   const int seq = work % p.num_seqs, tile = work / p.num_seqs;
   pdl_launch_dependents();
   pdl_wait();
-  const int q0 = p.q_starts[seq], qn = p.q_starts[seq + 1] - q0;
-  const int all_rows = qn * G, row0 = tile * kSpanRows;
-  if (qn <= 0 || all_rows <= p.rows_from || all_rows > p.rows_to || row0 >= all_rows) return;
+  // (what follows is the same for all splits, which are a cluster where they join in one: all of them leave, or none)
+  const int q0 = p.q_starts[seq], qn = p.q_starts[seq + 1] - q0, kv_len = max(p.kv_lens[seq], 0);
+  const int all_rows = qn > 0 && qn <= p.max_q_len ? qn * G : 0, row0 = tile * kSpanRows;
+  if (all_rows <= p.rows_from || all_rows > p.rows_to || row0 >= all_rows) return;
   if (q0 < 0 || q0 + qn > p.tokens) {
     if (threadIdx.x == 0 && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
     return;
   }
   const int n_rows = min(kSpanRows, all_rows - row0);
-  const int kv_len = max(p.kv_lens[seq], 0);
 
   if (threadIdx.x < kSpanRows) {
     SpanRow r{0, 0};
@@ -113,6 +140,7 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
     begs[threadIdx.x] = r.beg;
   }
   // queries; a row's 16-byte pieces lie with D / 8 neighbouring threads
+#pragma unroll
   for (int i = threadIdx.x; i < kSpanRows * (D / 8); i += 128) {
     const int r = i / (D / 8), c = i - r * (D / 8);
     uint4 v = make_uint4(0, 0, 0, 0);
@@ -140,34 +168,40 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
         const float2 x = unpack_bf16x2(w[e]);
         w[e] = pack_16<true>(x.x * f, x.y * f);
       }
+      *reinterpret_cast<uint4*>(qtile + r * S::kQPitch + c * 8) = v;
+    } else {
+      *reinterpret_cast<uint4*>(tile_ptr<D>(qtile, r, c)) = v;
     }
     if (c == 0) factors[r] = factor;
-    *reinterpret_cast<uint4*>(tile_ptr<D>(qtile, r, c)) = v;
   }
   __syncthreads();
   uint32_t qf[D / 16][4];
+  if constexpr (KV8) {
 #pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) ldsm_x4(qf[kk], tile_ptr<D>(qtile, lane & 15, 2 * kk + (lane >> 4)));
+    for (int k = 0; k < D / 16; ++k) {     // k-step k % 4 of 64 dims: a lane's two pairs of columns are its four bytes of that step
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint2 v = *reinterpret_cast<const uint2*>(qtile + (g + 8 * h) * S::kQPitch + (k >> 2) * 64 + 16 * t + 4 * (k & 3));
+        qf[k][h] = v.x;
+        qf[k][2 + h] = v.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) ldsm_x4(qf[kk], tile_ptr<D>(qtile, lane & 15, 2 * kk + (lane >> 4)));
+  }
 
   // what the tile's rows see between them, and what all of them see
   int min_base = INT_MAX, max_base = 0, min_beg = INT_MAX, max_beg = 0;
   if (lane < n_rows) { min_base = max_base = bases[lane]; min_beg = max_beg = begs[lane]; }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    min_base = min(min_base, __shfl_xor_sync(0xffffffffu, min_base, o));
-    max_base = max(max_base, __shfl_xor_sync(0xffffffffu, max_base, o));
-    min_beg = min(min_beg, __shfl_xor_sync(0xffffffffu, min_beg, o));
-    max_beg = max(max_beg, __shfl_xor_sync(0xffffffffu, max_beg, o));
-  }
-  min_base = __shfl_sync(0xffffffffu, min_base, 0);
-  max_base = __shfl_sync(0xffffffffu, max_base, 0);
-  min_beg = __shfl_sync(0xffffffffu, min_beg, 0);
-  max_beg = __shfl_sync(0xffffffffu, max_beg, 0);
+  min_base = __reduce_min_sync(0xffffffffu, min_base);
+  max_base = __reduce_max_sync(0xffffffffu, max_base);
+  min_beg = __reduce_min_sync(0xffffffffu, min_beg);
+  max_beg = __reduce_max_sync(0xffffffffu, max_beg);
   const SpanRange range = span_range(p, kPage, min_beg, p.tree_mask ? kv_len : max_base);
   const int per_split = max(p.min_pages, (range.count + p.splits - 1) / p.splits);
   const int pg0 = min(split * per_split, range.count), pg1 = min(pg0 + per_split, range.count);
 
-  const int g = lane >> 2;
   const int base0 = bases[g], base1 = bases[g + 8], beg0 = begs[g], beg1 = begs[g + 8];
   const float f0 = factors[g], f1 = factors[g + 8];
   const unsigned long long *bits0 = bits + g * kSpanWords, *bits1 = bits + (g + 8) * kSpanWords;
@@ -177,8 +211,7 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-  uint8_t* my_ring = ring + (size_t)warp * (S::kWarpRing + S::kWarpTiles);
-  bf16* my_tiles = reinterpret_cast<bf16*>(my_ring + S::kWarpRing);
+  uint8_t* my_ring = ring + (size_t)warp * S::kWarpRing;
   const int* table = p.block_tables + (size_t)seq * p.max_blocks;
   bool bad = false;
   auto issue = [&](int it) {
@@ -191,9 +224,11 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
       uint8_t* st = my_ring + (size_t)(it % S::kStages) * 2 * S::kPageBytes;
       if constexpr (KV8) {
         const uint8_t *kg = static_cast<const uint8_t*>(p.k_cache) + off, *vg = static_cast<const uint8_t*>(p.v_cache) + off;
+#pragma unroll
         for (int i = lane; i < S::kPageBytes / 16; i += 32) {
-          cp_async16_or_zero(st + i * 16, kg + i * 16, block >= 0);
-          cp_async16_or_zero(st + S::kPageBytes + i * 16, vg + i * 16, block >= 0);
+          const int r = i / (D / 16), c = i - r * (D / 16);
+          cp_async16_or_zero(st + r * D + ((c ^ turn_k<D>(r)) << 4), kg + i * 16, block >= 0);
+          cp_async16_or_zero(st + S::kPageBytes + r * D + ((c ^ turn_v<D>(r)) << 4), vg + i * 16, block >= 0);
         }
       } else {
         const bf16 *kg = static_cast<const bf16*>(p.k_cache) + off, *vg = static_cast<const bf16*>(p.v_cache) + off;
@@ -217,41 +252,36 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
     __syncwarp();
     uint8_t* st = my_ring + (size_t)(it % S::kStages) * 2 * S::kPageBytes;
     bf16 *ks = reinterpret_cast<bf16*>(st), *vs = ks + S::kPageElems;
-    if constexpr (KV8) {
-      ks = my_tiles;
-      vs = my_tiles + S::kPageElems;
-      constexpr int CPR = D / 16;
-      for (int i = lane; i < 2 * kPage * CPR; i += 32) {
-        const int which = i / (kPage * CPR), c16 = i - which * (kPage * CPR);
-        const int r = c16 / CPR, cc = c16 - r * CPR;
-        const uint4 raw = *reinterpret_cast<const uint4*>(st + which * S::kPageBytes + r * D + cc * 16);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        uint32_t h[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] & 0xFFFFu), __NV_E4M3);
-          const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[e] >> 16), __NV_E4M3);
-          h[2 * e] = (uint32_t)lo.x | ((uint32_t)lo.y << 16);
-          h[2 * e + 1] = (uint32_t)hi.x | ((uint32_t)hi.y << 16);
-        }
-        bf16* t = which ? vs : ks;
-        *reinterpret_cast<uint4*>(tile_ptr<D>(t, r, 2 * cc)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(tile_ptr<D>(t, r, 2 * cc + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
-      }
-      __syncwarp();
-    }
+    const uint8_t* v8 = st + S::kPageBytes;
     const int tok0 = range.piece(pg0 + warp + 4 * it) * kPage;
     const bool full = tok0 + kPage <= min_base && (tok0 >= max_beg || tok0 + kPage <= p.first);
     float s[2][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-    const int j = lane >> 3, t = lane & 3;
+    const int j = lane >> 3;
+    if constexpr (KV8) {
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      uint32_t b[4];
-      ldsm_x4(b, tile_ptr<D>(ks, (j >> 1) * 8 + (lane & 7), 2 * kk + (j & 1)));
-      mma_16<KV8>(s[0], qf[kk], b[0], b[1]);
-      mma_16<KV8>(s[1], qf[kk], b[2], b[3]);
+      for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+        for (int grp = 0; grp < D / 64; ++grp) {
+          const int r = nb * 8 + g;
+          const uint4 raw = *reinterpret_cast<const uint4*>(st + r * D + (((4 * grp + t) ^ turn_k<D>(r)) << 4));
+          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint2 h = e4m3x4_to_f16(w[k]);
+            mma_f16(s[nb], qf[4 * grp + k], h.x, h.y);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t b[4];
+        ldsm_x4(b, tile_ptr<D>(ks, (j >> 1) * 8 + (lane & 7), 2 * kk + (j & 1)));
+        mma_16<KV8>(s[0], qf[kk], b[0], b[1]);
+        mma_16<KV8>(s[1], qf[kk], b[2], b[3]);
+      }
     }
     float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
@@ -274,64 +304,115 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
     const float mn0 = fmaxf(m[0], mx0), mn1 = fmaxf(m[1], mx1);
-    const float c0 = mn0 == -INFINITY ? 1.f : ex2(m[0] - mn0), c1 = mn1 == -INFINITY ? 1.f : ex2(m[1] - mn1);
     constexpr float lift = KV8 ? kF16Lift : 0.f;
     const float r0 = mn0 == -INFINITY ? 0.f : mn0 - lift, r1 = mn1 == -INFINITY ? 0.f : mn1 - lift;
+    if (__any_sync(0xffffffffu, mn0 != m[0] || mn1 != m[1])) {
+      const float c0 = mn0 == -INFINITY ? 1.f : ex2(m[0] - mn0), c1 = mn1 == -INFINITY ? 1.f : ex2(m[1] - mn1);
+      l[0] *= c0;
+      l[1] *= c1;
+#pragma unroll
+      for (int db = 0; db < D / 8; ++db) {
+        o[db][0] *= c0; o[db][1] *= c0;
+        o[db][2] *= c1; o[db][3] *= c1;
+      }
+      m[0] = mn0;
+      m[1] = mn1;
+    }
     uint32_t pf[4];
-    float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
       const float p0 = ex2(s[nb][0] - r0), p1 = ex2(s[nb][1] - r0), p2 = ex2(s[nb][2] - r1), p3 = ex2(s[nb][3] - r1);
-      sum0 += p0 + p1;
-      sum1 += p2 + p3;
+      l[0] += p0 + p1;
+      l[1] += p2 + p3;
       pf[2 * nb] = pack_16<KV8>(p0, p1);
       pf[2 * nb + 1] = pack_16<KV8>(p2, p3);
     }
-    l[0] = l[0] * c0 + sum0;
-    l[1] = l[1] * c1 + sum1;
-    m[0] = mn0;
-    m[1] = mn1;
+    // infinities and NaN of V in a page that not every row sees whole: value(token, column block, which of the lane's two columns)
+    auto add_odd = [&](auto value) {
+      for (int tk = 0; tk < kPage; ++tk) {
+        const int src = (lane & ~3) | (tk & 7) >> 1;
+        const float2 a = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[0] : pf[2], src));
+        const float2 b = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[1] : pf[3], src));
+        const float w0 = tk & 1 ? a.y : a.x, w1 = tk & 1 ? b.y : b.x;
+        const bool sees0 = span_sees(p, tok0 + tk, base0, beg0, bits0), sees1 = span_sees(p, tok0 + tk, base1, beg1, bits1);
 #pragma unroll
-    for (int db = 0; db < D / 8; ++db) {
-      o[db][0] *= c0; o[db][1] *= c0;
-      o[db][2] *= c1; o[db][3] *= c1;
-    }
-    if (!full) {
-      uint32_t* vw = reinterpret_cast<uint32_t*>(vs);
-      bool odd = false;
-#pragma unroll 4
-      for (int i = lane; i < kPage * D / 2; i += 32) odd |= odd_16x2<KV8>(vw[i]);
-      if (__any_sync(0xffffffffu, odd)) {
-        for (int tk = 0; tk < kPage; ++tk) {
-          const int src = (lane & ~3) | (tk & 7) >> 1;
-          const float2 a = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[0] : pf[2], src));
-          const float2 b = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[1] : pf[3], src));
-          const float w0 = tk & 1 ? a.y : a.x, w1 = tk & 1 ? b.y : b.x;
-          const bool sees0 = span_sees(p, tok0 + tk, base0, beg0, bits0), sees1 = span_sees(p, tok0 + tk, base1, beg1, bits1);
+        for (int db = 0; db < D / 8; ++db) {
 #pragma unroll
-          for (int db = 0; db < D / 8; ++db) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(tile_ptr<D>(vs, tk, db) + 2 * t);
-            if (odd_16x2<KV8>(w)) {
-              const float2 v = unpack_16<KV8>(w);
-              if (!isfinite(v.x)) { if (sees0) o[db][0] += w0 * v.x; if (sees1) o[db][2] += w1 * v.x; }
-              if (!isfinite(v.y)) { if (sees0) o[db][1] += w0 * v.y; if (sees1) o[db][3] += w1 * v.y; }
-            }
+          for (int e = 0; e < 2; ++e) {
+            const float v = value(tk, db, e);
+            if (isfinite(v)) continue;
+            if (sees0) o[db][e] += w0 * v;
+            if (sees1) o[db][2 + e] += w1 * v;
           }
         }
-        __syncwarp();
-        for (int i = lane; i < kPage * D / 2; i += 32) {
-          const uint32_t w = vw[i];
-          if (odd_16x2<KV8>(w)) vw[i] = (odd_16x2<KV8>(w & 0xFFFFu) ? 0u : w & 0xFFFFu) | (odd_16x2<KV8>(w & 0xFFFF0000u) ? 0u : w & 0xFFFF0000u);
-        }
-        __syncwarp();
       }
-    }
+      __syncwarp();
+    };
+    if constexpr (KV8) {
+      constexpr int kWords = D == 64 ? 2 : 4, kParts = D == 256 ? 2 : 1;
+      uint32_t nan = 0;
 #pragma unroll
-    for (int db = 0; db < D / 8; db += 2) {
-      uint32_t b[4];
-      ldsm_x4_t(b, tile_ptr<D>(vs, (j & 1) * 8 + (lane & 7), db + (j >> 1)));
-      mma_16<KV8>(o[db], pf, b[0], b[1]);
-      mma_16<KV8>(o[db + 1], pf, b[2], b[3]);
+      for (int part = 0; part < kParts; ++part) {
+        uint32_t w[4][kWords];             // rows 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int r = 2 * t + (h & 1) + 8 * (h >> 1);
+          if constexpr (D == 64) {
+            const uint2 x = *reinterpret_cast<const uint2*>(v8 + r * D + (((g >> 1) ^ turn_v<D>(r)) << 4) + (g & 1) * 8);
+            w[h][0] = x.x; w[h][1] = x.y;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(v8 + r * D + (((8 * part + g) ^ turn_v<D>(r)) << 4));
+            w[h][0] = x.x; w[h][1] = x.y; w[h][2] = x.z; w[h][3] = x.w;
+          }
+        }
+        if (!full) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) {
+              const uint32_t n = e4m3_nan(w[h][k]);
+              nan |= n;
+              w[h][k] &= ~((n >> 7) * 0xFFu);
+            }
+          if (__any_sync(0xffffffffu, nan) && part == kParts - 1)
+            add_odd([&](int tk, int db, int e) {
+              const int d = dim_of<D>(db, 2 * t + e);
+              const uint8_t x = v8[tk * D + (((d >> 4) ^ turn_v<D>(tk)) << 4) + (d & 15)];
+              return (x & 0x7F) == 0x7F ? __int_as_float(0x7FC00000) : 0.f;
+            });
+        }
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+          const uint2 a = e4m3x4_to_f16(__byte_perm(w[0][k], w[1][k], 0x5140)), b = e4m3x4_to_f16(__byte_perm(w[0][k], w[1][k], 0x7362));
+          const uint2 c = e4m3x4_to_f16(__byte_perm(w[2][k], w[3][k], 0x5140)), d = e4m3x4_to_f16(__byte_perm(w[2][k], w[3][k], 0x7362));
+          mma_f16(o[16 * part + 4 * k], pf, a.x, c.x);
+          mma_f16(o[16 * part + 4 * k + 1], pf, a.y, c.y);
+          mma_f16(o[16 * part + 4 * k + 2], pf, b.x, d.x);
+          mma_f16(o[16 * part + 4 * k + 3], pf, b.y, d.y);
+        }
+      }
+    } else {
+      if (!full) {
+        uint32_t* vw = reinterpret_cast<uint32_t*>(vs);
+        bool odd = false;
+#pragma unroll 4
+        for (int i = lane; i < kPage * D / 2; i += 32) odd |= odd_bf16x2(vw[i]);
+        if (__any_sync(0xffffffffu, odd)) {
+          add_odd([&](int tk, int db, int e) { return __bfloat162float(tile_ptr<D>(vs, tk, db)[2 * t + e]); });
+          for (int i = lane; i < kPage * D / 2; i += 32) {
+            const uint32_t w = vw[i];
+            if (odd_bf16x2(w)) vw[i] = (odd_bf16x2(w & 0xFFFFu) ? 0u : w & 0xFFFFu) | (odd_bf16x2(w & 0xFFFF0000u) ? 0u : w & 0xFFFF0000u);
+          }
+          __syncwarp();
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < D / 8; db += 2) {
+        uint32_t b[4];
+        ldsm_x4_t(b, tile_ptr<D>(vs, (j & 1) * 8 + (lane & 7), db + (j >> 1)));
+        mma_16<KV8>(o[db], pf, b[0], b[1]);
+        mma_16<KV8>(o[db + 1], pf, b[2], b[3]);
+      }
     }
     __syncwarp();
   }
@@ -342,55 +423,76 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
   }
-
   if constexpr (KV8) { m[0] -= kF16Lift; m[1] -= kF16Lift; }
 
   __syncthreads();                                     // the ring is free
   float* mo = reinterpret_cast<float*>(ring);          // [4][16][D]
   float* mml = mo + 4 * kSpanRows * D;                 // [4][16][2]
-  const int t4 = lane & 3;
+  float* part_o = mml + 4 * kSpanRows * 2;             // [16][D]: the CTA's
+  float4* part_ml = reinterpret_cast<float4*>(part_o + kSpanRows * D);      // [16]
 #pragma unroll
-  for (int db = 0; db < D / 8; ++db) {
-    *reinterpret_cast<float2*>(mo + ((size_t)warp * 16 + g) * D + db * 8 + 2 * t4) = make_float2(o[db][0], o[db][1]);
-    *reinterpret_cast<float2*>(mo + ((size_t)warp * 16 + g + 8) * D + db * 8 + 2 * t4) = make_float2(o[db][2], o[db][3]);
-  }
-  if (t4 == 0) {
-    *reinterpret_cast<float2*>(mml + (warp * 16 + g) * 2) = make_float2(m[0], l[0]);
-    *reinterpret_cast<float2*>(mml + (warp * 16 + g + 8) * 2) = make_float2(m[1], l[1]);
+  for (int h = 0; h < 2; ++h) {
+    float* row = mo + ((size_t)warp * 16 + g + 8 * h) * D;
+    if constexpr (KV8) {                               // a lane has four neighbouring dims in four neighbouring column blocks
+#pragma unroll
+      for (int db = 0; db < D / 8; db += 4)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float4*>(row + dim_of<D>(db, 2 * t + e)) = make_float4(o[db][2 * h + e], o[db + 1][2 * h + e], o[db + 2][2 * h + e], o[db + 3][2 * h + e]);
+    } else {
+#pragma unroll
+      for (int db = 0; db < D / 8; ++db) *reinterpret_cast<float2*>(row + db * 8 + 2 * t) = make_float2(o[db][2 * h], o[db][2 * h + 1]);
+    }
+    if (t == 0) *reinterpret_cast<float2*>(mml + (warp * 16 + g + 8 * h) * 2) = make_float2(m[h], l[h]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n_rows * (D / 2); i += 128) {
-    const int r = i / (D / 2), d2 = (i - r * (D / 2)) * 2;
+  for (int i = threadIdx.x; i < n_rows * (D / 4); i += 128) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
     float mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mml[(w * 16 + r) * 2]);
-    float ll = 0.f, a0 = 0.f, a1 = 0.f;
+    float ll = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float mw = mml[(w * 16 + r) * 2];
-      const float c = mw == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : ex2(mw - mm);
-      const float2 v = *reinterpret_cast<const float2*>(mo + ((size_t)w * 16 + r) * D + d2);
-      ll += mml[(w * 16 + r) * 2 + 1] * c;
-      if (c != 0.f) { a0 += v.x * c; a1 += v.y * c; }
+      const float2 ml = *reinterpret_cast<const float2*>(mml + (w * 16 + r) * 2);
+      const float c = ml.x == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : ex2(ml.x - mm);
+      const float4 v = *reinterpret_cast<const float4*>(mo + ((size_t)w * 16 + r) * D + d);
+      ll += ml.y * c;
+      if (c != 0.f) { a.x += v.x * c; a.y += v.y * c; a.z += v.z * c; a.w += v.w * c; }
     }
-    const int qi = (row0 + r) / G, head = kvh * G + (row0 + r) - qi * G;
-    const size_t tok = (size_t)(q0 + qi);
     if (p.splits == 1) {
-      if (p.sinks) {
-        const float sk = p.sinks[head] * kLog2e;
-        const float mn = fmaxf(mm, sk);
-        const float c = mm == -INFINITY ? 0.f : ex2(mm - mn);
-        ll = ll * c + ex2(sk - mn);
-        a0 *= c;
-        a1 *= c;
-      }
-      const float inv = ll == 0.f ? 0.f : 1.f / ll;
-      *reinterpret_cast<uint32_t*>(static_cast<bf16*>(p.out) + tok * p.ldo + (size_t)head * D + d2) = pack_bf16x2(a0 * inv, a1 * inv);
+      store_row<D>(p, q0, row0 + r, kvh, d, a, mm, ll);
+    } else if (p.in_cluster) {
+      *reinterpret_cast<float4*>(part_o + r * D + d) = a;
+      if (d == 0) part_ml[r] = make_float4(mm, ll, 0.f, 0.f);
     } else {
-      const size_t at = (tok * p.hq + head) * p.splits + split;
-      *reinterpret_cast<float2*>(p.ws_o + at * D + d2) = make_float2(a0, a1);
-      if (d2 == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(mm, ll);
+      const int qi = (row0 + r) / G, head = kvh * G + (row0 + r) - qi * G;
+      const size_t at = ((size_t)(q0 + qi) * p.hq + head) * p.splits + split;
+      *reinterpret_cast<float4*>(p.ws_o + at * D + d) = a;
+      if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(mm, ll);
     }
+  }
+  if (p.in_cluster) {
+    // the splits are a cluster: each CTA takes a share of the row's values from all of them
+    cluster_sync();
+    for (int i = split * 128 + threadIdx.x; i < n_rows * (D / 4); i += 128 * p.splits) {
+      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+      float mm = -INFINITY, ll = 0.f;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int c = 0; c < p.splits; ++c) {
+        const float4 ml = ld_dsmem_f4(smem_u32(part_ml + r), c), v = ld_dsmem_f4(smem_u32(part_o + r * D + d), c);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        const float mn = fmaxf(mm, ml.x);
+        const float w0 = mm == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : ex2(mm - mn), w1 = ml.x == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : ex2(ml.x - mn);
+        mm = mn;
+        ll = ll * w0 + ml.y * w1;
+        a.x = a.x * w0 + v.x * w1; a.y = a.y * w0 + v.y * w1; a.z = a.z * w0 + v.z * w1; a.w = a.w * w0 + v.w * w1;
+      }
+      store_row<D>(p, q0, row0 + r, kvh, d, a, mm, ll);
+    }
+    cluster_sync();                                    // no CTA leaves while another reads its rows
   }
 }
 
@@ -463,9 +565,10 @@ void launch_rows(const SpanParams& p, cudaStream_t s) {
     cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D, KV8>::kTotal), "span_rows smem");
   const long long most = (long long)p.max_q_len * p.group < p.rows_to ? (long long)p.max_q_len * p.group : p.rows_to;
   const long long tiles = (most + kSpanRows - 1) / kSpanRows;
-  const long long ctas = tiles * p.num_seqs * p.hkv;
+  const long long ctas = tiles * p.num_seqs * p.hkv * p.splits;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
-  launch_pdl(span_rows_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(128), RowsSmem<D, KV8>::kTotal, s, p);
+  if (p.in_cluster) launch_cluster(true, span_rows_kernel<D, KV8>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, (unsigned)p.splits, p);
+  else launch_pdl(span_rows_kernel<D, KV8>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, p);
 }
 template <int D>
 void launch_merge(const SpanParams& p, bool some, cudaStream_t s) {
@@ -487,17 +590,21 @@ SpanPlan attention_span_plan(const SpanParams& p) {
   if (!tc || (long long)p.min_q_len * p.group <= kSpanRows) {
     const long long ctas = ((tc ? std::min<long long>(most, kSpanRows) : most) + kSpanRows - 1) / kSpanRows * p.num_seqs * p.hkv;
     const long long pages = (span + kPage - 1) / kPage;
-    plan.min_pages = 8;
+    // Splits up to eight are a cluster and join in it (a page for each of a CTA's warps at least); more, where few sequences are that long that it
+    // takes more SMs, leave their rows to a kernel behind.
+    plan.min_pages = 4;
     long long splits = 1;
     if (ctas < 4 * sm_count()) splits = std::min<long long>((4LL * sm_count() + ctas - 1) / ctas, (pages + plan.min_pages - 1) / plan.min_pages);
+    if (splits > 8 && pages < 8 * 64) splits = 8;
     plan.rows_splits = (int)std::max<long long>(1, std::min<long long>(splits, 128));
+    plan.in_cluster = plan.rows_splits > 1 && plan.rows_splits <= 8;
   }
   if (tc && most > kSpanRows) {
     // at most four places for a piece to each SM: those that the kernel finds no work for cost a start all the same
     const long long ctas = (most + 255) / 256 * p.num_seqs * p.hkv, tiles = (span + 127) / 128 + 2;
     plan.tile_splits = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(4LL * sm_count() / ctas, tiles), 32));
   }
-  plan.bytes = (partial_floats(p, plan.rows_splits) + partial_floats(p, plan.tile_splits)) * sizeof(float);
+  plan.bytes = (partial_floats(p, plan.in_cluster ? 1 : plan.rows_splits) + partial_floats(p, plan.tile_splits)) * sizeof(float);
   return plan;
 }
 
@@ -522,6 +629,7 @@ int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStre
   }
   if (plan.rows_splits > 0) {
     take(plan.rows_splits);
+    p.in_cluster = plan.in_cluster;
     p.rows_from = 0;
     p.rows_to = attention_span_tc_supported(p) ? kSpanRows : INT_MAX;
     switch (p.head_dim) {
@@ -530,7 +638,7 @@ int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStre
       default: p.kv_fp8 ? launch_rows<256, true>(p, s) : launch_rows<256, false>(p, s); break;
     }
     ++n;
-    if (p.splits > 1) { merge(p, both, s); ++n; }
+    if (p.splits > 1 && !p.in_cluster) { merge(p, both, s); ++n; }
   }
   cuda_check(cudaGetLastError(), "attention_span launch");
   return n;

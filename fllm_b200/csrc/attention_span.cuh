@@ -94,6 +94,9 @@ __device__ __forceinline__ uint2 e4m3x4_to_f16(uint32_t w) {
   return h;
 }
 
+// bit 7 of each byte that is a NaN
+__device__ __forceinline__ uint32_t e4m3_nan(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
 __device__ __forceinline__ bool odd_bf16x2(uint32_t w) { return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u; }
 __device__ __forceinline__ bool odd_f16x2(uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
 }  // namespace

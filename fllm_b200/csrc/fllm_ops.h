@@ -312,6 +312,7 @@ struct SpanParams {
   float scale, scale_log2, softcap;
   // set by the planner, for one kernel
   int splits, min_pages, sms;  // pieces of what a sequence's rows see, at most; fewest pages in one; SMs
+  bool in_cluster;             // the pieces join in a cluster
   int rows_from, rows_to;      // packed rows (query rows x group) of the sequences that the kernel takes: from < rows <= to
   float* ws_o;                 // [tokens][hq][splits][head_dim]
   float* ws_ml;                // [tokens][hq][splits][2]
@@ -319,6 +320,7 @@ struct SpanParams {
 struct SpanPlan {
   int rows_splits, tile_splits;          // of the kernel for few rows and of the tensor-memory kernel; 0: it has no rows
   int min_pages;
+  bool in_cluster;                       // the first one's splits join in a cluster
   size_t bytes;                          // of workspace
 };
 SpanPlan attention_span_plan(const SpanParams& p);
