@@ -214,12 +214,21 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
   uint8_t* my_ring = ring + (size_t)warp * S::kWarpRing;
   const int* table = p.block_tables + (size_t)seq * p.max_blocks;
   bool bad = false;
+  // Blocks of this warp's pages, one to a lane, 32 at a time and those ahead of their use: a table entry looked up where it is needed held every page
+  // back by a trip to memory.
+  auto look = [&](int it) {
+    const int pg = pg0 + warp + 4 * (it + lane);
+    const int block = pg < pg1 ? span_block(p, table, range.piece(pg)) : 0;
+    bad |= block < 0;
+    return block;
+  };
+  int blocks = 0, blocks_next = look(0);
   auto issue = [&](int it) {
     const int pg = pg0 + warp + 4 * it;
+    if ((it & 31) == 0) { blocks = blocks_next; blocks_next = look(it + 32); }
     if (pg < pg1) {
       const int page = range.piece(pg);
-      const int block = span_block(p, table, page);
-      bad |= block < 0;
+      const int block = __shfl_sync(0xffffffffu, blocks, it & 31);
       const long long off = block < 0 ? 0 : span_pool_row(p, block, kvh, page) * D;
       uint8_t* st = my_ring + (size_t)(it % S::kStages) * 2 * S::kPageBytes;
       if constexpr (KV8) {
