@@ -131,14 +131,75 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
   }
   const int n_rows = min(kSpanRows, all_rows - row0);
 
-  if (threadIdx.x < kSpanRows) {
+  // Every warp finds out what the rows see for itself (a lane to a row), so that its pages are on their way before the queries are.
+  int min_base = INT_MAX, max_base = 0, min_beg = INT_MAX, max_beg = 0;      // what they see between them, and what all of them see
+  if (lane < kSpanRows) {
     SpanRow r{0, 0};
-    unsigned long long* mine = bits + threadIdx.x * kSpanWords;
-    for (int w = 0; w < kSpanWords; ++w) mine[w] = 0;
-    if (threadIdx.x < n_rows) r = span_row(p, q0, qn, kv_len, (row0 + threadIdx.x) / G, mine);
-    bases[threadIdx.x] = r.base;
-    begs[threadIdx.x] = r.beg;
+    unsigned long long mine[kSpanWords] = {0, 0, 0, 0};
+    if (lane < n_rows) {
+      r = span_row(p, q0, qn, kv_len, (row0 + lane) / G, mine);
+      min_base = max_base = r.base;
+      min_beg = max_beg = r.beg;
+    }
+    if (warp == 0) {
+      bases[lane] = r.base;
+      begs[lane] = r.beg;
+#pragma unroll
+      for (int w = 0; w < kSpanWords; ++w) bits[lane * kSpanWords + w] = mine[w];
+    }
   }
+  min_base = __reduce_min_sync(0xffffffffu, min_base);
+  max_base = __reduce_max_sync(0xffffffffu, max_base);
+  min_beg = __reduce_min_sync(0xffffffffu, min_beg);
+  max_beg = __reduce_max_sync(0xffffffffu, max_beg);
+  const SpanRange range = span_range(p, kPage, min_beg, p.tree_mask ? kv_len : max_base);
+  const int per_split = max(p.min_pages, (range.count + p.splits - 1) / p.splits);
+  const int pg0 = min(split * per_split, range.count), pg1 = min(pg0 + per_split, range.count);
+
+  uint8_t* my_ring = ring + (size_t)warp * S::kWarpRing;
+  const int* table = p.block_tables + (size_t)seq * p.max_blocks;
+  bool bad = false;
+  // Blocks of this warp's pages, one to a lane, 32 at a time and those ahead of their use: a table entry looked up where it is needed held every page
+  // back by a trip to memory.
+  auto look = [&](int it) {
+    const int pg = pg0 + warp + 4 * (it + lane);
+    const int block = pg < pg1 ? span_block(p, table, range.piece(pg)) : 0;
+    bad |= block < 0;
+    return block;
+  };
+  int blocks = 0, blocks_next = look(0);
+  auto issue = [&](int it) {
+    const int pg = pg0 + warp + 4 * it;
+    if ((it & 31) == 0) { blocks = blocks_next; blocks_next = look(it + 32); }
+    if (pg < pg1) {
+      const int page = range.piece(pg);
+      const int block = __shfl_sync(0xffffffffu, blocks, it & 31);
+      const long long off = block < 0 ? 0 : span_pool_row(p, block, kvh, page) * D;
+      uint8_t* st = my_ring + (size_t)(it % S::kStages) * 2 * S::kPageBytes;
+      if constexpr (KV8) {
+        const uint8_t *kg = static_cast<const uint8_t*>(p.k_cache) + off, *vg = static_cast<const uint8_t*>(p.v_cache) + off;
+#pragma unroll
+        for (int i = lane; i < S::kPageBytes / 16; i += 32) {
+          const int r = i / (D / 16), c = i - r * (D / 16);
+          cp_async16_or_zero(st + r * D + ((c ^ turn_k<D>(r)) << 4), kg + i * 16, block >= 0);
+          cp_async16_or_zero(st + S::kPageBytes + r * D + ((c ^ turn_v<D>(r)) << 4), vg + i * 16, block >= 0);
+        }
+      } else {
+        const bf16 *kg = static_cast<const bf16*>(p.k_cache) + off, *vg = static_cast<const bf16*>(p.v_cache) + off;
+        bf16* ks = reinterpret_cast<bf16*>(st);
+#pragma unroll 8
+        for (int i = lane; i < kPage * (D / 8); i += 32) {
+          const int r = i / (D / 8), c = i - r * (D / 8);
+          cp_async16_or_zero(tile_ptr<D>(ks, r, c), kg + i * 8, block >= 0);
+          cp_async16_or_zero(tile_ptr<D>(ks + S::kPageElems, r, c), vg + i * 8, block >= 0);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  const int my_pages = pg1 > pg0 + warp ? (pg1 - pg0 - warp + 3) / 4 : 0;
+#pragma unroll
+  for (int s = 0; s < S::kStages - 1; ++s) issue(s);
   // queries; a row's 16-byte pieces lie with D / 8 neighbouring threads
 #pragma unroll
   for (int i = threadIdx.x; i < kSpanRows * (D / 8); i += 128) {
@@ -191,17 +252,6 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
     for (int kk = 0; kk < D / 16; ++kk) ldsm_x4(qf[kk], tile_ptr<D>(qtile, lane & 15, 2 * kk + (lane >> 4)));
   }
 
-  // what the tile's rows see between them, and what all of them see
-  int min_base = INT_MAX, max_base = 0, min_beg = INT_MAX, max_beg = 0;
-  if (lane < n_rows) { min_base = max_base = bases[lane]; min_beg = max_beg = begs[lane]; }
-  min_base = __reduce_min_sync(0xffffffffu, min_base);
-  max_base = __reduce_max_sync(0xffffffffu, max_base);
-  min_beg = __reduce_min_sync(0xffffffffu, min_beg);
-  max_beg = __reduce_max_sync(0xffffffffu, max_beg);
-  const SpanRange range = span_range(p, kPage, min_beg, p.tree_mask ? kv_len : max_base);
-  const int per_split = max(p.min_pages, (range.count + p.splits - 1) / p.splits);
-  const int pg0 = min(split * per_split, range.count), pg1 = min(pg0 + per_split, range.count);
-
   const int base0 = bases[g], base1 = bases[g + 8], beg0 = begs[g], beg1 = begs[g + 8];
   const float f0 = factors[g], f1 = factors[g + 8];
   const unsigned long long *bits0 = bits + g * kSpanWords, *bits1 = bits + (g + 8) * kSpanWords;
@@ -211,50 +261,6 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-  uint8_t* my_ring = ring + (size_t)warp * S::kWarpRing;
-  const int* table = p.block_tables + (size_t)seq * p.max_blocks;
-  bool bad = false;
-  // Blocks of this warp's pages, one to a lane, 32 at a time and those ahead of their use: a table entry looked up where it is needed held every page
-  // back by a trip to memory.
-  auto look = [&](int it) {
-    const int pg = pg0 + warp + 4 * (it + lane);
-    const int block = pg < pg1 ? span_block(p, table, range.piece(pg)) : 0;
-    bad |= block < 0;
-    return block;
-  };
-  int blocks = 0, blocks_next = look(0);
-  auto issue = [&](int it) {
-    const int pg = pg0 + warp + 4 * it;
-    if ((it & 31) == 0) { blocks = blocks_next; blocks_next = look(it + 32); }
-    if (pg < pg1) {
-      const int page = range.piece(pg);
-      const int block = __shfl_sync(0xffffffffu, blocks, it & 31);
-      const long long off = block < 0 ? 0 : span_pool_row(p, block, kvh, page) * D;
-      uint8_t* st = my_ring + (size_t)(it % S::kStages) * 2 * S::kPageBytes;
-      if constexpr (KV8) {
-        const uint8_t *kg = static_cast<const uint8_t*>(p.k_cache) + off, *vg = static_cast<const uint8_t*>(p.v_cache) + off;
-#pragma unroll
-        for (int i = lane; i < S::kPageBytes / 16; i += 32) {
-          const int r = i / (D / 16), c = i - r * (D / 16);
-          cp_async16_or_zero(st + r * D + ((c ^ turn_k<D>(r)) << 4), kg + i * 16, block >= 0);
-          cp_async16_or_zero(st + S::kPageBytes + r * D + ((c ^ turn_v<D>(r)) << 4), vg + i * 16, block >= 0);
-        }
-      } else {
-        const bf16 *kg = static_cast<const bf16*>(p.k_cache) + off, *vg = static_cast<const bf16*>(p.v_cache) + off;
-        bf16* ks = reinterpret_cast<bf16*>(st);
-#pragma unroll 8
-        for (int i = lane; i < kPage * (D / 8); i += 32) {
-          const int r = i / (D / 8), c = i - r * (D / 8);
-          cp_async16_or_zero(tile_ptr<D>(ks, r, c), kg + i * 8, block >= 0);
-          cp_async16_or_zero(tile_ptr<D>(ks + S::kPageElems, r, c), vg + i * 8, block >= 0);
-        }
-      }
-    }
-    cp_async_commit();
-  };
-  const int my_pages = pg1 > pg0 + warp ? (pg1 - pg0 - warp + 3) / 4 : 0;
-#pragma unroll
-  for (int s = 0; s < S::kStages - 1; ++s) issue(s);
   for (int it = 0; it < my_pages; ++it) {
     issue(it + S::kStages - 1);
     cp_async_wait<S::kStages - 1>();
@@ -599,11 +605,12 @@ SpanPlan attention_span_plan(const SpanParams& p) {
   if (!tc || (long long)p.min_q_len * p.group <= kSpanRows) {
     const long long ctas = ((tc ? std::min<long long>(most, kSpanRows) : most) + kSpanRows - 1) / kSpanRows * p.num_seqs * p.hkv;
     const long long pages = (span + kPage - 1) / kPage;
-    // Splits up to eight are a cluster and join in it (a page for each of a CTA's warps at least); more, where few sequences are that long that it
-    // takes more SMs, leave their rows to a kernel behind.
+    // As many splits as leave all CTAs on the SMs at once, a page for each of a CTA's warps at least: a CTA's way in and out is some 5 us (64 sequences
+    // under a window of 4096, 8 key heads of 128: 170 us whole, 182 in two, 202 in four; 16 under one of 1024: 24, 17, 24). Up to eight are a
+    // cluster and join in it; more, where few sequences are long, leave their rows to a kernel behind.
+    const int resident = p.head_dim == 256 ? 1 : p.head_dim == 64 ? 4 : p.kv_fp8 ? 3 : 2;      // CTAs of an SM, by registers and shared memory
     plan.min_pages = 4;
-    long long splits = 1;
-    if (ctas < 4 * sm_count()) splits = std::min<long long>((4LL * sm_count() + ctas - 1) / ctas, (pages + plan.min_pages - 1) / plan.min_pages);
+    long long splits = std::min<long long>((long long)resident * sm_count() / ctas, (pages + plan.min_pages - 1) / plan.min_pages);
     if (splits > 8 && pages < 8 * 64) splits = 8;
     plan.rows_splits = (int)std::max<long long>(1, std::min<long long>(splits, 128));
     plan.in_cluster = plan.rows_splits > 1 && plan.rows_splits <= 8;
