@@ -599,9 +599,13 @@ size_t partial_floats(const SpanParams& p, int splits) { return splits > 1 ? (si
 
 SpanPlan attention_span_plan(const SpanParams& p) {
   SpanPlan plan{};
-  const bool tc = attention_span_tc_supported(p);
   const long long most = (long long)p.max_q_len * p.group;
   const long long span = std::min<long long>(p.window > 0 ? (long long)p.window + p.first + p.max_q_len : p.max_kv_len, p.max_kv_len);
+  // Sequences of more than 16 packed rows go to the tensor-memory kernel, unless all there is to do is less than 28 pages of 16 rows for each SM: its way
+  // in and out is longer (one tree of 8, 12, 32 and 64 nodes behind 900 tokens, 32 query and 8 key heads of 128: 10.6, 11.0, 13.9, 20.4 us here, 15.5, 15.6,
+  // 16.1, 18.6 there; 12 nodes behind 4000: 19.2 and 18.6).
+  const long long all_tiles = (most + kSpanRows - 1) / kSpanRows * p.num_seqs * p.hkv;
+  const bool tc = attention_span_tc_supported(p) && all_tiles * ((span + kPage - 1) / kPage) > 28LL * sm_count();
   if (!tc || (long long)p.min_q_len * p.group <= kSpanRows) {
     const long long ctas = ((tc ? std::min<long long>(most, kSpanRows) : most) + kSpanRows - 1) / kSpanRows * p.num_seqs * p.hkv;
     const long long pages = (span + kPage - 1) / kPage;
@@ -647,7 +651,7 @@ int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStre
     take(plan.rows_splits);
     p.in_cluster = plan.in_cluster;
     p.rows_from = 0;
-    p.rows_to = attention_span_tc_supported(p) ? kSpanRows : INT_MAX;
+    p.rows_to = plan.tile_splits > 0 ? kSpanRows : INT_MAX;
     switch (p.head_dim) {
       case 64: p.kv_fp8 ? launch_rows<64, true>(p, s) : launch_rows<64, false>(p, s); break;
       case 128: p.kv_fp8 ? launch_rows<128, true>(p, s) : launch_rows<128, false>(p, s); break;

@@ -20,7 +20,8 @@ inline void check_ints(const Tensor& t, const Tensor& like, int64_t at_least, co
 
 // Pools [planes, blocks, heads, block_size, width], a block's values contiguous; up to kMaxKvPools of them from `from` on
 fllm::KvPools make_pools(const std::vector<Tensor>& pools, size_t from) {
-  fllm::KvPools p{};
+  fllm::KvPools p;
+  p.count = p.planes = 0;
   for (size_t i = from; i < pools.size() && p.count < fllm::kMaxKvPools; ++i) {
     const Tensor& t = pools[i];
     fllm::KvPool& q = p.pool[p.count++];
@@ -41,7 +42,7 @@ void check_pools(const std::vector<Tensor>& pools) {
   for (const Tensor& t : pools) {
     TORCH_CHECK(t.is_cuda() && t.device() == pools[0].device() && t.dim() == 5 && t.numel() > 0, "cache pools must be CUDA tensors [planes, blocks, heads, block_size, width] of one device");
     TORCH_CHECK(t.size(1) == pools[0].size(1) && t.size(3) == pools[0].size(3) && t.size(1) < INT32_MAX, "cache pools must agree in blocks and block size");
-    TORCH_CHECK(t[0].is_contiguous() && t.size(4) * (int64_t)t.element_size() < (1 << 24) && t.size(0) < (1 << 24), "the blocks of a cache pool must be contiguous");
+    TORCH_CHECK(t.stride(4) == 1 && t.stride(3) == t.size(4) && t.stride(2) == t.size(3) * t.size(4) && t.stride(1) == t.size(2) * t.stride(2) && t.size(4) * (int64_t)t.element_size() < (1 << 24) && t.size(0) < (1 << 24), "the blocks of a cache pool must be contiguous");
   }
 }
 

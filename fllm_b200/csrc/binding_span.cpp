@@ -21,20 +21,17 @@ inline void check_ints(const Tensor& t, const Tensor& like, int64_t at_least, co
 }
 inline bool is_e4m3(const Tensor& t) { return t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kByte; }
 
-int64_t attention_span(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_tables, const Tensor& q_starts,
-                       const Tensor& kv_lens, Tensor out, int64_t num_seqs, int64_t max_q_len, int64_t min_q_len, int64_t max_kv_len, int64_t hq,
+// -> (output rows, kernels launched)
+std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_tables, const Tensor& q_starts,
+                       const Tensor& kv_lens, int64_t num_seqs, int64_t max_q_len, int64_t min_q_len, int64_t max_kv_len, int64_t hq,
                        int64_t hkv, int64_t head_dim, double scale, int64_t window, int64_t first, const optional<Tensor>& sinks, double softcap,
                        const optional<Tensor>& tree_mask, const optional<Tensor>& tree_base, const optional<Tensor>& status) {
   fllm::SpanParams p{};
   TORCH_CHECK(hq > 0 && hkv > 0 && hq % hkv == 0 && hq <= 65536, "attention: query heads must be a multiple of the key heads");
   TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "attention: head_dim must be 64, 128 or 256");
-  auto rows = [&](const Tensor& t, const char* name) {
-    TORCH_CHECK(t.is_cuda() && t.device() == q.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.stride(1) == 1 && t.size(0) == q.size(0) &&
-                    t.size(1) == hq * head_dim && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
-                name, " must be bf16 rows of hq * head_dim values on 16-byte boundaries");
-  };
-  rows(q, "q");
-  rows(out, "out");
+  TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 2 && q.stride(1) == 1 && q.size(1) == hq * head_dim && q.stride(0) % 8 == 0 &&
+                  (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) == 0,
+              "q must be bf16 rows of hq * head_dim values on 16-byte boundaries");
   auto pool = [&](const Tensor& t, const char* name) {
     TORCH_CHECK(t.is_cuda() && t.device() == q.device() && t.dim() == 4 && t.is_contiguous() && t.sizes() == k_cache.sizes() &&
                     t.scalar_type() == k_cache.scalar_type() && (t.scalar_type() == at::kBFloat16 || is_e4m3(t)) && t.size(1) == hkv &&
@@ -76,24 +73,26 @@ int64_t attention_span(const Tensor& q, const Tensor& k_cache, const Tensor& v_c
   p.block_tables = block_tables.data_ptr<int>(); p.max_blocks = (int)block_tables.size(1);
   p.block_pages = (int)(k_cache.size(2) / 16); p.num_blocks = k_cache.size(0);
   p.q_starts = q_starts.data_ptr<int>(); p.kv_lens = kv_lens.data_ptr<int>();
-  p.out = out.data_ptr(); p.ldo = out.stride(0);
   p.tokens = (int)q.size(0); p.num_seqs = (int)num_seqs;
   p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv); p.head_dim = (int)head_dim;
   p.kv_fp8 = is_e4m3(k_cache);
   p.max_q_len = (int)std::min<int64_t>(max_q_len, q.size(0)); p.min_q_len = (int)min_q_len; p.max_kv_len = (int)max_kv_len;
   p.window = (int)window; p.first = window > 0 ? (int)first : 0;
   p.scale = (float)scale; p.scale_log2 = (float)(scale * 1.4426950408889634); p.softcap = (float)softcap;
-  if (p.tokens == 0 || num_seqs == 0 || p.max_q_len == 0) return 0;
   c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({q.size(0), q.size(1)}, q.options());
+  if (p.tokens == 0 || num_seqs == 0 || p.max_q_len == 0) return {out, 0};
+  p.out = out.data_ptr(); p.ldo = out.stride(0);
   const fllm::SpanPlan plan = fllm::attention_span_plan(p);
   Tensor ws;                                  // of this call alone: two streams or two captured graphs do not share it
   if (plan.bytes) ws = at::empty({(int64_t)plan.bytes}, q.options().dtype(at::kByte));
-  return fllm::attention_span(p, plan, plan.bytes ? ws.data_ptr() : nullptr, cur_stream());
+  const int n = fllm::attention_span(p, plan, plan.bytes ? ws.data_ptr() : nullptr, cur_stream());
+  return {out, n};
 }
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(fllm_b200, m) {
-  m.def("attention_span(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor q_starts, Tensor kv_lens, Tensor(a!) out, int num_seqs, "
+  m.def("attention_span(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor q_starts, Tensor kv_lens, int num_seqs, "
         "int max_q_len, int min_q_len, int max_kv_len, int hq, int hkv, int head_dim, float scale, int window, int first, Tensor? sinks, float softcap, "
-        "Tensor? tree_mask=None, Tensor? tree_base=None, Tensor? status=None) -> int", &attention_span);
+        "Tensor? tree_mask=None, Tensor? tree_base=None, Tensor? status=None) -> (Tensor, int)", &attention_span);
 }

@@ -150,7 +150,8 @@ class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNa
         sequence (the generic kernel's visibility limit), the tensor-core kernels take the flag. `first`: so many tokens
         at the start of the text stay visible when the window has moved past them (causal, with `meta`; the rows of a
         sequence are its last ones)."""
-        _check_span(window, first, bidirectional)
+        if first or window < 0:
+            _check_span(window, first, bidirectional)
         if first and window:
             return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta)
         out = torch.empty(q.shape[0], hq * head_dim, dtype=q.dtype, device=q.device)
@@ -207,10 +208,10 @@ class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNa
         positions[t] = tree_base[t] + nodes - 1. With `meta` (a sequence's rows are its nodes, seq_lens the positions
         that are stored) the cache is read once for the rows and heads that share it, a mask may have several words
         ([rows, words]), and `window` and `first` count places in the text: a node's is tree_base + its depth."""
-        _check_span(window, first)
         if meta is not None:
             return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta,
                                         tree_mask, tree_base)
+        _check_span(window, first)
         if first:
             raise ValueError("attention_tree: first tokens need the step batch (meta)")
         out = torch.empty(q.shape[0], hq * head_dim, dtype=q.dtype, device=q.device)

@@ -110,10 +110,9 @@ class SpanNative:
     def _attention_span(self, q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta, tree_mask=None, tree_base=None):
         if meta is None or meta.q_starts is None or meta.seq_lens is None:
             raise ValueError("this attention takes its rows from the step batch: q_starts, seq_lens and their bounds")
-        out = torch.empty(q.shape[0], hq * head_dim, dtype=q.dtype, device=q.device)
-        self.launches += self.k.attention_span(q, k_cache, v_cache, block_tables, meta.q_starts, meta.seq_lens, out, meta.num_seqs, meta.max_q_len,
-                                               meta.min_q_len, meta.max_kv_len, hq, hkv, head_dim, float(scale), int(window), int(first), sinks,
-                                               float(softcap), tree_mask, tree_base, self.status)
+        out, n = self.k.attention_span(q, k_cache, v_cache, block_tables, meta.q_starts, meta.seq_lens, meta.num_seqs, meta.max_q_len, meta.min_q_len,
+                                       meta.max_kv_len, hq, hkv, head_dim, scale, window, first, sinks, softcap, tree_mask, tree_base, self.status)
+        self.launches += n
         return out
 
     def kv_copy_blocks(self, pools, pairs):
@@ -121,11 +120,10 @@ class SpanNative:
         device in one launch: it names no block as a destination twice, or as a source and a destination (pairs out of range are skipped and
         reported in ``status``)."""
         if isinstance(pairs, torch.Tensor):
-            groups = [pairs] if pairs.shape[0] else []
-        else:
-            groups = [torch.tensor(g, dtype=torch.int32).to(pools[0].device) for g in ordered_copies(pairs, pools[0].shape[1])]
-        for g in groups:
-            self.launches += self.k.kv_copy_blocks(pools, g, self.status)
+            self.launches += self.k.kv_copy_blocks(pools, pairs, self.status)
+            return
+        for g in ordered_copies(pairs, pools[0].shape[1] if pools else 0):
+            self.launches += self.k.kv_copy_blocks(pools, torch.tensor(g, dtype=torch.int32).to(pools[0].device), self.status)
 
     def kv_compact(self, pools, block_tables, base, path, counts):
         """For every sequence b the row of position ``base[b] + path[b, i]`` to position ``base[b] + i``, for i < counts[b], in this order: what is
