@@ -31,6 +31,7 @@ namespace fllm {
 namespace {
 constexpr int kTcRows = 256, kWideners = 6;       // packed rows of a CTA; warps that widen V of an e4m3 cache
 template <bool KV8> constexpr int tc_threads() { return KV8 ? 512 : 384; }
+template <bool KV8> constexpr int kQThreads = KV8 ? 384 : 256;      // that load queries
 constexpr float kTcLift = 6.f;             // f16 weights: their reference lies so far below the row's (their largest is 2^14 then)
 constexpr int kTilePages = kTile / kPage;
 template <int N> using Int = std::integral_constant<int, N>;
@@ -224,13 +225,13 @@ __device__ __forceinline__ uint64_t desc_k_major(uint32_t saddr) {
     return make_smem_desc_sw128(saddr);
 }
 
-// Queries of rows [0, tiles x 128) to shared memory in swizzled rows, by the 256 threads of the softmax groups. Beside an e4m3 cache: two e4m3
+// Queries of rows [0, tiles x 128) to shared memory in swizzled rows, by THREADS threads, `tid` of them this one. Beside an e4m3 cache: two e4m3
 // pieces, of the value times a power of two per row (its largest magnitude is between 2^7 and 2^8 then) and of what that leaves, four bits each of
 // a bf16's eight. Exact down to 2^-9 of the row's largest value, within 2^-17 of that value below. bf16: asynchronous copies.
-template <int D, bool F16>
-__device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* factors, int tiles, int q0, int row0, int n_rows, int kvh) {
-  constexpr int C = D / 8, kStep = 256 / C;            // rows between those of a thread
-  const int c = threadIdx.x % C, r0 = threadIdx.x / C;
+template <int D, bool F16, int THREADS>
+__device__ __forceinline__ void load_q(const SpanParams& p, int tid, uint8_t* sq, float* factors, int tiles, int q0, int row0, int n_rows, int kvh) {
+  constexpr int C = D / 8, kStep = THREADS / C;        // rows between those of a thread
+  const int c = tid % C, r0 = tid / C;
   RowWalk at(row0 + r0, kStep, p.group);
   const bf16* head = static_cast<const bf16*>(p.q) + (size_t)q0 * p.ldq + (size_t)kvh * p.group * D + c * 8;
   if constexpr (!F16) {
@@ -245,7 +246,7 @@ __device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* 
   } else {
     constexpr int kBatch = 4;                          // loads on their way at once
 #pragma unroll 1
-    for (int i0 = 0; i0 < tiles * kRows / kStep; i0 += kBatch) {
+    for (int i0 = 0; i0 * kStep < tiles * kRows; i0 += kBatch) {
       uint4 v[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i, at.next()) {
@@ -275,6 +276,7 @@ __device__ __forceinline__ void load_q(const SpanParams& p, uint8_t* sq, float* 
           high[e >> 1] |= a << (16 * (e & 1));
           low[e >> 1] |= b << (16 * (e & 1));
         }
+        if (r >= tiles * kRows) continue;
         uint8_t* at8 = sq + (r >> 7) * tile_bytes<D>() + rr * D + (((c >> 1) ^ (D == 128 ? rr & 7 : (rr >> 1) & 3)) << 4) + (c & 1) * 8;
         *reinterpret_cast<uint2*>(at8) = make_uint2(high[0], high[1]);
         *reinterpret_cast<uint2*>(at8 + kRows * D) = make_uint2(low[0], low[1]);
@@ -368,6 +370,34 @@ __device__ __forceinline__ int pieces_of(const SpanParams& p, int n_rows, int ti
   return max(1, min(min((int)(sms + 0.4f), p.splits), tiles));
 }
 
+// What the rows of a tile see between them and what all of them see, by a warp for itself: the end of the context that all see, where windows begin
+// first and last, the end of what any sees.
+struct TileSees {
+  int min_base, min_beg, max_beg, end;
+};
+__device__ __forceinline__ TileSees tile_sees(const SpanParams& p, int q0, int qn, int kv_len, int row0, int n_rows) {
+  TileSees t;
+  const int first = row0 / p.group, last = (row0 + n_rows - 1) / p.group;      // query rows
+  if (p.tree_mask) {
+    int a = INT_MAX, b = INT_MAX, d = 0;
+    for (int qi = first + (threadIdx.x & 31); qi <= last; qi += 32) {
+      unsigned long long bits[kSpanWords];
+      const SpanRow r = span_row(p, q0, qn, kv_len, qi, bits);
+      a = min(a, r.base); b = min(b, r.beg); d = max(d, r.beg);
+    }
+    t.min_base = __reduce_min_sync(0xffffffffu, a);
+    t.min_beg = __reduce_min_sync(0xffffffffu, b);
+    t.max_beg = __reduce_max_sync(0xffffffffu, d);
+    t.end = kv_len;
+  } else {
+    t.min_base = max(kv_len - qn + first + 1, 0);
+    t.end = max(kv_len - qn + last + 1, 0);
+    t.min_beg = p.window > 0 ? max(t.min_base - p.window, 0) : 0;
+    t.max_beg = p.window > 0 ? max(t.end - p.window, 0) : 0;
+  }
+  return t;
+}
+
 template <int D, bool KV8>
 __global__ void __launch_bounds__(tc_threads<KV8>(), 1)
 span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ SpanParams p, int row_tiles) {
@@ -385,11 +415,24 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   uint64_t *raw_full = bars + 22, *raw_empty = bars + 30;                                     // [8] by slot
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* seen = reinterpret_cast<int*>(tmem_slot + 2);        // smallest and largest base, smallest and largest window begin, odd values met
+  int* odd_met = reinterpret_cast<int*>(tmem_slot + 2);     // values were taken out of tiles of V
   float* factors = reinterpret_cast<float*>(smem + S::kTiles + kTcFlags);
-  static_assert(38 * 8 + 7 * 4 <= kTcFlags, "barriers and flags");
+  static_assert(38 * 8 + 3 * 4 <= kTcFlags, "barriers and flags");
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV8 ? kWideners : 1);
+    }
+    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], KV8 ? 1 : D / 64); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], kWideners); }
+    mbar_init(o_done, 1); mbar_init(q_full, kQThreads<KV8> / 32);
+    *abort_flag = 0;
+    *odd_met = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); if (!KV8) tma_prefetch_desc(&tma_v); }
   pdl_wait();
   const int split = blockIdx.y;
   int rest = blockIdx.x;
@@ -407,49 +450,29 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const int pieces = p.splits > 1 ? pieces_of(p, n_rows, tiles_of(p, qn, kv_len)) : 1;
   if (split >= pieces) return;
   const bool two = n_rows > kRows;                     // two row tiles that share K and V, or two groups that share a row tile
-
-  const int group = warp >> 2;                         // of softmax warps
-  const int r = (two ? group * kRows : 0) + (warp & 3) * 32 + lane;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV8 ? kWideners : 1);
-    }
-    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], KV8 ? 1 : D / 64); mbar_init(&k_empty[i], 1); }
-    for (int i = 0; i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], kWideners); }
-    mbar_init(o_done, 1); mbar_init(q_full, 8);
-    *abort_flag = 0;
-    seen[0] = INT_MAX; seen[1] = 0; seen[2] = INT_MAX; seen[3] = 0; seen[4] = 0;
-    fence_barrier_init();
-  }
-  if (warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); if (!KV8) tma_prefetch_desc(&tma_v); }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-  if (warp < 8) load_q<D, KV8>(p, sq, factors, two ? 2 : 1, q0, row0, n_rows, kvh);
-  SpanRow row{0, 0};
-  const int qi = warp < 8 && r < n_rows ? (row0 + r) / G : -1;
-  if (qi >= 0) {
-    unsigned long long bits[kSpanWords];
-    row = span_row(p, q0, qn, kv_len, qi, bits);
-  }
-  __syncthreads();
-  if (warp < 8) {
-    const int a = __reduce_min_sync(0xffffffffu, qi >= 0 ? row.base : INT_MAX), b = __reduce_max_sync(0xffffffffu, row.base);
-    const int c = __reduce_min_sync(0xffffffffu, qi >= 0 ? row.beg : INT_MAX), d = __reduce_max_sync(0xffffffffu, row.beg);
-    if (lane == 0 && a != INT_MAX) { atomicMin(&seen[0], a); atomicMax(&seen[1], b); atomicMin(&seen[2], c); atomicMax(&seen[3], d); }
-  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   pdl_launch_dependents();                             // not before the allocation
-  const int end = p.tree_mask ? kv_len : seen[1], min_base = seen[0], max_beg = seen[3];
-  const SpanRange range = span_range(p, kTile, seen[2], end);
+  // Queries: the softmax groups, and beside an e4m3 cache, where there is more to it than to copy them, four of the warps that wait for V. (Whoever
+  // asks for K and V is not among them.)
+  const bool q_too = KV8 && warp >= 12;
+  if (warp < 8 || q_too) load_q<D, KV8, kQThreads<KV8>>(p, warp < 8 ? (int)threadIdx.x : (int)threadIdx.x - 128, sq, factors, two ? 2 : 1, q0, row0, n_rows, kvh);
+
+  const int group = warp >> 2;                         // of softmax warps
+  const int r_first = (two ? group * kRows : 0) + (warp & 3) * 32, r = r_first + lane;
+  const int qi = warp < 8 && r < n_rows ? (row0 + r) / G : -1;
+  const TileSees sees = tile_sees(p, q0, qn, kv_len, row0, n_rows);
+  const int min_base = sees.min_base, max_beg = sees.max_beg, end = sees.end;
+  const SpanRange range = span_range(p, kTile, sees.min_beg, end);
   const int per_piece = (tiles_of(p, qn, kv_len) + pieces - 1) / pieces;      // (the last one goes on to the end, should that be further)
   const int t0 = min(split * per_piece, range.count), n_tiles = split == pieces - 1 ? range.count - t0 : min(per_piece, range.count - t0);
   const int shift = two ? 1 : 0, n_items = n_tiles << shift;
   // not every row of the CTA sees the whole tile
   auto partial = [&](int tok0) { return !(tok0 + kTile <= min_base && (tok0 >= max_beg || tok0 + kTile <= p.first)); };
-  const PageRows page_rows{p, p.block_tables + (size_t)seq * p.max_blocks, kvh, (min(p.first, end) + kPage - 1) / kPage, seen[2] / kPage,
+  const PageRows page_rows{p, p.block_tables + (size_t)seq * p.max_blocks, kvh, (min(p.first, end) + kPage - 1) / kPage, sees.min_beg / kPage,
                            (end + kPage - 1) / kPage, (int)(p.num_blocks * p.hkv * p.block_pages * kPage)};
 
   // The block was launched with 168 registers a thread (e4m3: 128): 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128.
@@ -457,6 +480,12 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     if constexpr (KV8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     bool bad = false;
+    if (q_too) {
+      q_loaded();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      asm volatile("bar.arrive 2, 384;" ::: "memory");
+    }
     if (warp == 9) {
       constexpr int fmt = KV8 ? 0 : 1;
       constexpr uint32_t idesc_s = make_idesc(128, 128, fmt, fmt);      // (e4m3 x e4m3 has the same bits as f16 x f16)
@@ -584,7 +613,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
                 v[i] = w;
               }
               fence_proxy_async_smem();
-              if (lane == 0) atomicOr(&seen[4], 1);
+              if (lane == 0) atomicOr(odd_met, 1);
               __syncwarp();
             }
           }
@@ -670,7 +699,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           *reinterpret_cast<uint4*>(line + ((((c & 7) + flip) ^ (row & 7)) << 4)) = x;
           *reinterpret_cast<uint4*>(line + ((((c & 7) + 1 - flip) ^ (row & 7)) << 4)) = z;
         }
-        if (odd_f16x2(sum[0]) || odd_f16x2(sum[1])) atomicOr(&seen[4], 1);
+        if (odd_f16x2(sum[0]) || odd_f16x2(sum[1])) atomicOr(odd_met, 1);
         if (j & 1) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -689,11 +718,17 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     q_loaded();
     __syncwarp();
     if (lane == 0) mbar_arrive(q_full);
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if constexpr (KV8) asm volatile("bar.sync 2, 384;" ::: "memory");
+    else asm volatile("bar.sync 1, 256;" ::: "memory");
     const float factor = factors[r], scale = p.softcap > 0.f ? p.softcap * kLog2e : factor;
     const uint32_t t_s = tmem_base + 128 * group + lane_off, t_o = tmem_base + 256 + 128 * group + lane_off;
-    // whole for the rows of this warp
-    const int w_base = __reduce_min_sync(0xffffffffu, qi >= 0 ? row.base : INT_MAX), w_beg = __reduce_max_sync(0xffffffffu, qi >= 0 ? row.beg : 0);
+    // tokens [w_beg, w_base) are seen by all rows of this warp
+    int w_base = min_base, w_beg = max_beg;
+    if (!p.tree_mask) {
+      const int ctx = kv_len - qn + 1;
+      w_base = max(ctx + (row0 + r_first) / G, 0);
+      w_beg = p.window > 0 ? max(ctx + (row0 + min(r_first + 31, n_rows - 1)) / G - p.window, 0) : 0;
+    }
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int n = group; n < n_items; n += 2) {
@@ -809,7 +844,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (size_t)c0 * (splits ? 4 : 2)), "r"(smem_u32(stage)), "r"(kPass) : "memory");
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
-      if (seen[4] && qi >= 0) {
+      if (*odd_met && qi >= 0) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         // infinities and NaN that were taken out of tiles, added to the rows that see them
         for (int it = 0; it < n_tiles; ++it) {
