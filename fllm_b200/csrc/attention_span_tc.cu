@@ -344,10 +344,10 @@ __device__ __forceinline__ uint32_t without_odd_f16(uint32_t w) {
 }
 
 // Into how many pieces the walk of an item is cut. An item's share of all the work, counted in tiles of 128 rows from the lengths, times the number of
-// SMs is the number of SMs that it could keep; four tenths are rounded up. A piece costs a start, partial sums and their way through memory, so
-// pieces come to little more than one for each SM: 16 trees of 256 packed rows, 8 key heads, all behind 6000 tokens: 107 us in one piece each, 137 in two,
-// 161 in four; 4 trees of 128: 67 in one, 47 in two, 36 in four, 49 in six; 16 of 256 behind 1000 to 12,000: 201 in pieces of up to 13 tiles,
-// 182 in one each, 143 by this rule.
+// SMs is the number of SMs that it could keep; a piece costs a start, partial sums and their way through memory, so that is rounded down, but for
+// items that would hold two SMs almost. us of 32 query and 8 key heads of 128: 16 trees of 64 nodes behind 6000 tokens: 107 in one piece each,
+// 137 in two, 161 in four; 4 of 32: 67 in one, 36 in four, 49 in six; 16 of 64 behind 1000 to 12,000: 182 in one each, 201 in pieces of up to 13 tiles,
+// 157 by this rule, 172 where two pieces begin at 1.35 SMs.
 __device__ __forceinline__ int tiles_of(const SpanParams& p, int qn, int kv_len) {
   const int tiles = max((kv_len + kTile - 1) / kTile, 1);
   return p.window > 0 ? (int)min((long long)tiles, ((long long)p.window + p.first + min(qn, kTcRows)) / kTile + 3) : tiles;
@@ -367,7 +367,7 @@ __device__ __forceinline__ int pieces_of(const SpanParams& p, int n_rows, int ti
     total += mine;
   }
   const float sms = weight_of_rows(n_rows) * tiles * p.sms / (total * p.hkv);
-  return max(1, min(min((int)(sms + 0.4f), p.splits), tiles));
+  return max(1, min(min(sms < 2.f ? (sms >= 1.7f ? 2 : 1) : (int)sms, p.splits), tiles));
 }
 
 // What the rows of a tile see between them and what all of them see, by a warp for itself: the end of the context that all see, where windows begin
