@@ -37,11 +37,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <bool F16>
-__device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (F16) mma_f16(d, a, b0, b1);
-  else mma_bf16(d, a, b0, b1);
-}
-template <bool F16>
 __device__ __forceinline__ uint32_t pack_16(float lo, float hi) {
   if constexpr (F16) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -89,7 +84,8 @@ template <int D> __device__ __forceinline__ int turn_v(int r) { return D == 64 ?
 
 template <int D, bool KV8>
 struct RowsSmem {
-  static constexpr int kStages = KV8 ? 4 : D == 256 ? 2 : 3;
+  static constexpr int kPages = KV8 && D <= 128 ? 2 : 1;                 // of a turn of a warp
+  static constexpr int kStages = KV8 ? (D == 64 ? 6 : 4) : D == 256 ? 2 : 3;
   static constexpr int kPageElems = kPage * D;
   static constexpr int kPageBytes = kPageElems * (KV8 ? 1 : 2);          // a K or V page
   static constexpr int kWarpRing = kStages * 2 * kPageBytes;
@@ -102,8 +98,11 @@ struct RowsSmem {
   static_assert(kMerge + kPart <= kRing && kQ % 16 == 0 && kInfo % 16 == 0, "shared memory");
 };
 
+// CTAs of an SM, by registers and shared memory.
+template <int D, bool KV8> constexpr int rows_resident() { return D == 256 ? 1 : D == 64 ? 4 : KV8 ? 3 : 2; }
+
 template <int D, bool KV8>
-__global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ SpanParams p) {
+__global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel(const __grid_constant__ SpanParams p) {
   using S = RowsSmem<D, KV8>;
   extern __shared__ __align__(128) uint8_t smem[];
   bf16* qtile = reinterpret_cast<bf16*>(smem);
@@ -198,8 +197,9 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
     cp_async_commit();
   };
   const int my_pages = pg1 > pg0 + warp ? (pg1 - pg0 - warp + 3) / 4 : 0;
+  constexpr int kPages = S::kPages;
 #pragma unroll
-  for (int s = 0; s < S::kStages - 1; ++s) issue(s);
+  for (int s = 0; s < S::kStages - kPages; ++s) issue(s);
   // queries; a row's 16-byte pieces lie with D / 8 neighbouring threads
 #pragma unroll
   for (int i = threadIdx.x; i < kSpanRows * (D / 8); i += 128) {
@@ -261,26 +261,34 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-  for (int it = 0; it < my_pages; ++it) {
-    issue(it + S::kStages - 1);
-    cp_async_wait<S::kStages - 1>();
-    __syncwarp();
-    uint8_t* st = my_ring + (size_t)(it % S::kStages) * 2 * S::kPageBytes;
-    bf16 *ks = reinterpret_cast<bf16*>(st), *vs = ks + S::kPageElems;
-    const uint8_t* v8 = st + S::kPageBytes;
-    const int tok0 = range.piece(pg0 + warp + 4 * it) * kPage;
-    const bool full = tok0 + kPage <= min_base && (tok0 >= max_beg || tok0 + kPage <= p.first);
-    float s[2][4];
+  // kPages pages at a time: with two there are two chains of products and one maximum for both. (One that is not there any more has no token that
+  // a row sees.)
+  for (int it = 0; it < my_pages; it += kPages) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int h = 0; h < kPages; ++h) issue(it + h + S::kStages - kPages);
+    cp_async_wait<S::kStages - kPages>();
+    __syncwarp();
+    const uint8_t* page_at[kPages];
+    int tok0[kPages];
+    bool full[kPages];
+#pragma unroll
+    for (int h = 0; h < kPages; ++h) {
+      page_at[h] = my_ring + (size_t)((it + h) % S::kStages) * 2 * S::kPageBytes;
+      const bool there = h == 0 || it + h < my_pages;
+      tok0[h] = there ? range.piece(pg0 + warp + 4 * (it + h)) * kPage : INT_MAX / 2;
+      full[h] = tok0[h] + kPage <= min_base && (tok0[h] >= max_beg || tok0[h] + kPage <= p.first);
+    }
+    float s[2 * kPages][4];
+#pragma unroll
+    for (int i = 0; i < 2 * kPages; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
     const int j = lane >> 3;
     if constexpr (KV8) {
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
+      for (int grp = 0; grp < D / 64; ++grp) {
 #pragma unroll
-        for (int grp = 0; grp < D / 64; ++grp) {
-          const int r = nb * 8 + g;
-          const uint4 raw = *reinterpret_cast<const uint4*>(st + r * D + (((4 * grp + t) ^ turn_k<D>(r)) << 4));
+        for (int nb = 0; nb < 2 * kPages; ++nb) {
+          const int r = (nb & 1) * 8 + g;
+          const uint4 raw = *reinterpret_cast<const uint4*>(page_at[nb >> 1] + r * D + (((4 * grp + t) ^ turn_k<D>(r)) << 4));
           const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -290,23 +298,24 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
         }
       }
     } else {
+      bf16* ks = reinterpret_cast<bf16*>(const_cast<uint8_t*>(page_at[0]));
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         uint32_t b[4];
         ldsm_x4(b, tile_ptr<D>(ks, (j >> 1) * 8 + (lane & 7), 2 * kk + (j & 1)));
-        mma_16<KV8>(s[0], qf[kk], b[0], b[1]);
-        mma_16<KV8>(s[1], qf[kk], b[2], b[3]);
+        mma_bf16(s[0], qf[kk], b[0], b[1]);
+        mma_bf16(s[1], qf[kk], b[2], b[3]);
       }
     }
     float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
+    for (int nb = 0; nb < 2 * kPages; ++nb) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v = s[nb][e] * (e >= 2 ? f1 : f0);
         if (p.softcap > 0.f) v = p.softcap * tanhf(v / (p.softcap * kLog2e)) * kLog2e;
-        if (!full) {
-          const int tok = tok0 + nb * 8 + 2 * t + (e & 1);
+        if (!full[nb >> 1]) {
+          const int tok = tok0[nb >> 1] + (nb & 1) * 8 + 2 * t + (e & 1);
           if (!(e >= 2 ? span_sees(p, tok, base1, beg1, bits1) : span_sees(p, tok, base0, beg0, bits0))) v = -INFINITY;
         }
         s[nb][e] = v;
@@ -315,8 +324,8 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
       }
     }
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
     const float mn0 = fmaxf(m[0], mx0), mn1 = fmaxf(m[1], mx1);
     constexpr float lift = KV8 ? kF16Lift : 0.f;
@@ -333,23 +342,23 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
       m[0] = mn0;
       m[1] = mn1;
     }
-    uint32_t pf[4];
+    uint32_t pf[kPages][4];
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
+    for (int nb = 0; nb < 2 * kPages; ++nb) {
       const float p0 = ex2(s[nb][0] - r0), p1 = ex2(s[nb][1] - r0), p2 = ex2(s[nb][2] - r1), p3 = ex2(s[nb][3] - r1);
       l[0] += p0 + p1;
       l[1] += p2 + p3;
-      pf[2 * nb] = pack_16<KV8>(p0, p1);
-      pf[2 * nb + 1] = pack_16<KV8>(p2, p3);
+      pf[nb >> 1][2 * (nb & 1)] = pack_16<KV8>(p0, p1);
+      pf[nb >> 1][2 * (nb & 1) + 1] = pack_16<KV8>(p2, p3);
     }
     // infinities and NaN of V in a page that not every row sees whole: value(token, column block, which of the lane's two columns)
-    auto add_odd = [&](auto value) {
+    auto add_odd = [&](int h, auto value) {
       for (int tk = 0; tk < kPage; ++tk) {
         const int src = (lane & ~3) | (tk & 7) >> 1;
-        const float2 a = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[0] : pf[2], src));
-        const float2 b = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[1] : pf[3], src));
+        const float2 a = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[h][0] : pf[h][2], src));
+        const float2 b = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[h][1] : pf[h][3], src));
         const float w0 = tk & 1 ? a.y : a.x, w1 = tk & 1 ? b.y : b.x;
-        const bool sees0 = span_sees(p, tok0 + tk, base0, beg0, bits0), sees1 = span_sees(p, tok0 + tk, base1, beg1, bits1);
+        const bool sees0 = span_sees(p, tok0[h] + tk, base0, beg0, bits0), sees1 = span_sees(p, tok0[h] + tk, base1, beg1, bits1);
 #pragma unroll
         for (int db = 0; db < D / 8; ++db) {
 #pragma unroll
@@ -365,55 +374,65 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
     };
     if constexpr (KV8) {
       constexpr int kWords = D == 64 ? 2 : 4, kParts = D == 256 ? 2 : 1;
-      uint32_t nan = 0;
 #pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        uint32_t w[4][kWords];             // rows 2t, 2t + 1, 2t + 8, 2t + 9
+      for (int h = 0; h < kPages; ++h) {
+        const uint8_t* v8 = page_at[h] + S::kPageBytes;
+        uint32_t nan = 0;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int r = 2 * t + (h & 1) + 8 * (h >> 1);
-          if constexpr (D == 64) {
-            const uint2 x = *reinterpret_cast<const uint2*>(v8 + r * D + (((g >> 1) ^ turn_v<D>(r)) << 4) + (g & 1) * 8);
-            w[h][0] = x.x; w[h][1] = x.y;
-          } else {
-            const uint4 x = *reinterpret_cast<const uint4*>(v8 + r * D + (((8 * part + g) ^ turn_v<D>(r)) << 4));
-            w[h][0] = x.x; w[h][1] = x.y; w[h][2] = x.z; w[h][3] = x.w;
-          }
-        }
-        if (!full) {
+        for (int part = 0; part < kParts; ++part) {
+          uint32_t w[4][kWords];           // rows 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-          for (int h = 0; h < 4; ++h)
-#pragma unroll
-            for (int k = 0; k < kWords; ++k) {
-              const uint32_t n = e4m3_nan(w[h][k]);
-              nan |= n;
-              w[h][k] &= ~((n >> 7) * 0xFFu);
+          for (int i = 0; i < 4; ++i) {
+            const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+            if constexpr (D == 64) {
+              const uint2 x = *reinterpret_cast<const uint2*>(v8 + r * D + (((g >> 1) ^ turn_v<D>(r)) << 4) + (g & 1) * 8);
+              w[i][0] = x.x; w[i][1] = x.y;
+            } else {
+              const uint4 x = *reinterpret_cast<const uint4*>(v8 + r * D + (((8 * part + g) ^ turn_v<D>(r)) << 4));
+              w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
             }
-          if (__any_sync(0xffffffffu, nan) && part == kParts - 1)
-            add_odd([&](int tk, int db, int e) {
-              const int d = dim_of<D>(db, 2 * t + e);
-              const uint8_t x = v8[tk * D + (((d >> 4) ^ turn_v<D>(tk)) << 4) + (d & 15)];
-              return (x & 0x7F) == 0x7F ? __int_as_float(0x7FC00000) : 0.f;
-            });
-        }
+          }
+          if (tok0[h] == INT_MAX / 2) {    // what lies there is of another page
 #pragma unroll
-        for (int k = 0; k < kWords; ++k) {
-          const uint2 a = e4m3x4_to_f16(__byte_perm(w[0][k], w[1][k], 0x5140)), b = e4m3x4_to_f16(__byte_perm(w[0][k], w[1][k], 0x7362));
-          const uint2 c = e4m3x4_to_f16(__byte_perm(w[2][k], w[3][k], 0x5140)), d = e4m3x4_to_f16(__byte_perm(w[2][k], w[3][k], 0x7362));
-          mma_f16(o[16 * part + 4 * k], pf, a.x, c.x);
-          mma_f16(o[16 * part + 4 * k + 1], pf, a.y, c.y);
-          mma_f16(o[16 * part + 4 * k + 2], pf, b.x, d.x);
-          mma_f16(o[16 * part + 4 * k + 3], pf, b.y, d.y);
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int k = 0; k < kWords; ++k) w[i][k] = 0;
+          } else if (!full[h]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int k = 0; k < kWords; ++k) {
+                const uint32_t n = e4m3_nan(w[i][k]);
+                nan |= n;
+                w[i][k] &= ~((n >> 7) * 0xFFu);
+              }
+            if (__any_sync(0xffffffffu, nan) && part == kParts - 1)
+              add_odd(h, [&](int tk, int db, int e) {
+                const int d = dim_of<D>(db, 2 * t + e);
+                const uint8_t x = v8[tk * D + (((d >> 4) ^ turn_v<D>(tk)) << 4) + (d & 15)];
+                return (x & 0x7F) == 0x7F ? __int_as_float(0x7FC00000) : 0.f;
+              });
+          }
+#pragma unroll
+          for (int k = 0; k < kWords; ++k) {
+            const uint2 a = e4m3x4_to_f16(__byte_perm(w[0][k], w[1][k], 0x5140)), b = e4m3x4_to_f16(__byte_perm(w[0][k], w[1][k], 0x7362));
+            const uint2 c = e4m3x4_to_f16(__byte_perm(w[2][k], w[3][k], 0x5140)), d = e4m3x4_to_f16(__byte_perm(w[2][k], w[3][k], 0x7362));
+            mma_f16(o[16 * part + 4 * k], pf[h], a.x, c.x);
+            mma_f16(o[16 * part + 4 * k + 1], pf[h], a.y, c.y);
+            mma_f16(o[16 * part + 4 * k + 2], pf[h], b.x, d.x);
+            mma_f16(o[16 * part + 4 * k + 3], pf[h], b.y, d.y);
+          }
         }
       }
     } else {
-      if (!full) {
+      bf16* vs = reinterpret_cast<bf16*>(const_cast<uint8_t*>(page_at[0])) + S::kPageElems;
+      if (!full[0]) {
         uint32_t* vw = reinterpret_cast<uint32_t*>(vs);
         bool odd = false;
 #pragma unroll 4
         for (int i = lane; i < kPage * D / 2; i += 32) odd |= odd_bf16x2(vw[i]);
         if (__any_sync(0xffffffffu, odd)) {
-          add_odd([&](int tk, int db, int e) { return __bfloat162float(tile_ptr<D>(vs, tk, db)[2 * t + e]); });
+          add_odd(0, [&](int tk, int db, int e) { return __bfloat162float(tile_ptr<D>(vs, tk, db)[2 * t + e]); });
           for (int i = lane; i < kPage * D / 2; i += 32) {
             const uint32_t w = vw[i];
             if (odd_bf16x2(w)) vw[i] = (odd_bf16x2(w & 0xFFFFu) ? 0u : w & 0xFFFFu) | (odd_bf16x2(w & 0xFFFF0000u) ? 0u : w & 0xFFFF0000u);
@@ -425,8 +444,8 @@ __global__ void __launch_bounds__(128) span_rows_kernel(const __grid_constant__ 
       for (int db = 0; db < D / 8; db += 2) {
         uint32_t b[4];
         ldsm_x4_t(b, tile_ptr<D>(vs, (j & 1) * 8 + (lane & 7), db + (j >> 1)));
-        mma_16<KV8>(o[db], pf, b[0], b[1]);
-        mma_16<KV8>(o[db + 1], pf, b[2], b[3]);
+        mma_bf16(o[db], pf[0], b[0], b[1]);
+        mma_bf16(o[db + 1], pf[0], b[2], b[3]);
       }
     }
     __syncwarp();
@@ -612,7 +631,7 @@ SpanPlan attention_span_plan(const SpanParams& p) {
     // As many splits as leave all CTAs on the SMs at once, a page for each of a CTA's warps at least: a CTA's way in and out is some 5 us (64 sequences
     // under a window of 4096, 8 key heads of 128: 170 us whole, 182 in two, 202 in four; 16 under one of 1024: 24, 17, 24). Up to eight are a
     // cluster and join in it; more, where few sequences are long, leave their rows to a kernel behind.
-    const int resident = p.head_dim == 256 ? 1 : p.head_dim == 64 ? 4 : p.kv_fp8 ? 3 : 2;      // CTAs of an SM, by registers and shared memory
+    const int resident = p.head_dim == 256 ? 1 : p.head_dim == 64 ? rows_resident<64, false>() : p.kv_fp8 ? rows_resident<128, true>() : rows_resident<128, false>();
     plan.min_pages = 4;
     long long splits = std::min<long long>((long long)resident * sm_count() / ctas, (pages + plan.min_pages - 1) / plan.min_pages);
     if (splits > 8 && pages < 8 * 64) splits = 8;
