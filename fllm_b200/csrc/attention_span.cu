@@ -72,7 +72,7 @@ __device__ __forceinline__ void store_row(const SpanParams& p, int q0, int row, 
 // An e4m3 page stays as it is in shared memory and becomes operands in registers, which needs no order of columns that memory does not have: a lane
 // takes 16 bytes of a key row for four k-steps (queries lie in the same order), and 16 bytes of each of four value rows, two tokens of a dim to a
 // register. So of column block i of O, column n is dim i of the n-th piece of 16 (or 8, at D = 64) values. (Through f16 tiles in shared memory, ldmatrix
-// behind them, 48 sequences under a window of 1000 with 130 first tokens, 64 query and 8 key heads of 64, took 42 us, ROWS8_US so.)
+// behind them, 48 sequences under a window of 1000 with 130 first tokens, 64 query and 8 key heads of 64, took 42 us, 31 so.)
 template <int D>
 __device__ __forceinline__ int dim_of(int i, int n) {
   if constexpr (D == 64) return 8 * n + i;
@@ -121,13 +121,10 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
   pdl_launch_dependents();
   pdl_wait();
   // (what follows is the same for all splits, which are a cluster where they join in one: all of them leave, or none)
-  const int q0 = p.q_starts[seq], qn = p.q_starts[seq + 1] - q0, kv_len = max(p.kv_lens[seq], 0);
-  const int all_rows = qn > 0 && qn <= p.max_q_len ? qn * G : 0, row0 = tile * kSpanRows;
-  if (all_rows <= p.rows_from || all_rows > p.rows_to || row0 >= all_rows) return;
-  if (q0 < 0 || q0 + qn > p.tokens) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
-    return;
-  }
+  int q0, qn, kv_len;
+  if (!span_lengths(p, seq, threadIdx.x == 0, q0, qn, kv_len)) return;
+  const int all_rows = qn * G, row0 = tile * kSpanRows;
+  if (all_rows > p.rows_to || row0 >= all_rows) return;
   const int n_rows = min(kSpanRows, all_rows - row0);
 
   // Every warp finds out what the rows see for itself (a lane to a row), so that its pages are on their way before the queries are.
@@ -221,9 +218,9 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
       }
 #pragma unroll
       for (int o = (D / 8 < 32 ? D / 8 : 32) / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int up = top ? min(max(127 + 14 - (int)top, -100), 100) : 0;
+      const int up = min(127 + 14 - (int)top, 126);
       const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-      factor *= __uint_as_float((uint32_t)(127 - up) << 23);
+      factor = span_factor(factor, up);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 x = unpack_bf16x2(w[e]);
@@ -530,7 +527,7 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
   }
 }
 
-// Joins the splits of a row: one warp per (token, head). `some`: only sequences of p.rows_from < packed rows <= p.rows_to were split.
+// Joins the splits of a row: one warp per (token, head). `some`: sequences of at most p.rows_from packed rows were another kernel's.
 template <int D>
 __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__ SpanParams p, int some) {
   pdl_launch_dependents();
@@ -547,7 +544,7 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
       else hi = mid;
     }
     const int rows = (p.q_starts[lo + 1] - p.q_starts[lo]) * p.group;
-    if (rows <= p.rows_from || rows > p.rows_to) return;
+    if (rows <= p.rows_from) return;
   }
   const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + (size_t)pair * p.splits;
   const float* part = p.ws_o + (size_t)pair * p.splits * D + lane;
@@ -634,7 +631,7 @@ SpanPlan attention_span_plan(const SpanParams& p) {
     const int resident = p.head_dim == 256 ? 1 : p.head_dim == 64 ? rows_resident<64, false>() : p.kv_fp8 ? rows_resident<128, true>() : rows_resident<128, false>();
     plan.min_pages = 4;
     long long splits = std::min<long long>((long long)resident * sm_count() / ctas, (pages + plan.min_pages - 1) / plan.min_pages);
-    if (splits > 8 && pages < 8 * 64) splits = 8;
+    if (splits > 8 && (pages < 8 * 64 || (tc && most > kSpanRows))) splits = 8;      // (their workspace would have room for the other kernel's rows, too)
     plan.rows_splits = (int)std::max<long long>(1, std::min<long long>(splits, 128));
     plan.in_cluster = plan.rows_splits > 1 && plan.rows_splits <= 8;
   }
@@ -649,7 +646,6 @@ SpanPlan attention_span_plan(const SpanParams& p) {
 
 int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStream_t s) {
   int n = 0;
-  const bool both = plan.rows_splits > 0 && plan.tile_splits > 0;
   p.min_pages = plan.min_pages;
   p.sms = sm_count();
   auto take = [&](int splits) {
@@ -660,11 +656,11 @@ int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStre
   };
   if (plan.tile_splits > 0) {
     take(plan.tile_splits);
-    p.rows_from = kSpanRows;
+    p.rows_from = plan.rows_splits > 0 ? kSpanRows : 0;
     p.rows_to = INT_MAX;
     attention_span_tc(p, s);
     ++n;
-    if (p.splits > 1) { merge(p, both, s); ++n; }
+    if (p.splits > 1) { merge(p, plan.rows_splits > 0, s); ++n; }
   }
   if (plan.rows_splits > 0) {
     take(plan.rows_splits);
@@ -677,7 +673,7 @@ int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStre
       default: p.kv_fp8 ? launch_rows<256, true>(p, s) : launch_rows<256, false>(p, s); break;
     }
     ++n;
-    if (p.splits > 1 && !p.in_cluster) { merge(p, both, s); ++n; }
+    if (p.splits > 1 && !p.in_cluster) { merge(p, false, s); ++n; }      // (the only kernel then)
   }
   cuda_check(cudaGetLastError(), "attention_span launch");
   return n;

@@ -8,6 +8,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "fllm_ops.h"
@@ -75,6 +76,22 @@ __device__ __forceinline__ SpanRange span_range(const SpanParams& p, int unit, i
   s.count = end > 0 ? s.head + max((end + unit - 1) / unit - s.lo, 0) : 0;
   return s;
 }
+
+// Query rows of a sequence and its length, no longer than its row of the table reaches (a walk is then bounded by the table, whatever the lengths on
+// the device say); false where they are none to compute with, which is reported, as is a length out of reach.
+__device__ __forceinline__ bool span_lengths(const SpanParams& p, int seq, bool report, int& q0, int& qn, int& kv_len) {
+  q0 = p.q_starts[seq];
+  const int end = p.q_starts[seq + 1], len = p.kv_lens[seq];
+  const bool good = q0 >= 0 && end >= q0 && end <= p.tokens && end - q0 <= p.max_q_len;
+  qn = good ? end - q0 : 0;
+  kv_len = min(max(len, 0), p.reach);
+  if ((!good || (qn > 0 && len > p.reach)) && report && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
+  return qn > 0;
+}
+
+// The factor of a row's scores whose queries were multiplied by 2^up, -126 <= up <= 126. Never 0, which an infinity would make a NaN: scores whose
+// factor is below the smallest normal number are below 2^-100, whatever it is.
+__device__ __forceinline__ float span_factor(float scale, int up) { return fmaxf(scale * __uint_as_float((uint32_t)(127 - up) << 23), FLT_MIN); }
 
 // Block id of the 16 tokens from 16 * page on, or -1 where the table does not reach or the entry names no block of the pool.
 __device__ __forceinline__ int span_block(const SpanParams& p, const int* table, int page) {

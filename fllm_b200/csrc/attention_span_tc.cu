@@ -262,7 +262,7 @@ __device__ __forceinline__ void load_q(const SpanParams& p, int tid, uint8_t* sq
         for (int o = C / 2; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
         const int top = (int)(max(most & 0xFFFFu, most >> 16) >> 7);      // largest exponent field of the row
         const bool odd = top == 0xFF;                  // an infinity or a NaN: no score of the row is a number
-        const int up = top && !odd ? min(max(127 + 7 - top, -100), 100) : 0;
+        const int up = odd ? 0 : min(127 + 7 - top, 126);
         const float f = odd ? __int_as_float(0x7FC00000) : __uint_as_float((uint32_t)(127 + up) << 23);
         uint32_t high[2] = {0, 0}, low[2] = {0, 0};
 #pragma unroll
@@ -280,7 +280,7 @@ __device__ __forceinline__ void load_q(const SpanParams& p, int tid, uint8_t* sq
         uint8_t* at8 = sq + (r >> 7) * tile_bytes<D>() + rr * D + (((c >> 1) ^ (D == 128 ? rr & 7 : (rr >> 1) & 3)) << 4) + (c & 1) * 8;
         *reinterpret_cast<uint2*>(at8) = make_uint2(high[0], high[1]);
         *reinterpret_cast<uint2*>(at8 + kRows * D) = make_uint2(low[0], low[1]);
-        if (c == 0) factors[r] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+        if (c == 0) factors[r] = span_factor(p.scale_log2, up);
       }
     }
   }
@@ -359,8 +359,10 @@ __device__ __forceinline__ int pieces_of(const SpanParams& p, int n_rows, int ti
     const int s = s0 + (threadIdx.x & 31);
     float mine = 0.f;
     if (s < p.num_seqs) {
-      const int qn = p.q_starts[s + 1] - p.q_starts[s], rows = qn > 0 && qn <= p.max_q_len ? qn * p.group : 0, whole = rows / kTcRows;
-      if (rows > p.rows_from) mine = (2.f * whole + (rows > whole * kTcRows ? weight_of_rows(rows - whole * kTcRows) : 0.f)) * tiles_of(p, qn, max(p.kv_lens[s], 0));
+      int q0, qn, kv_len;
+      span_lengths(p, s, false, q0, qn, kv_len);
+      const int rows = qn * p.group, whole = rows / kTcRows;
+      if (rows > p.rows_from) mine = (2.f * whole + (rows > whole * kTcRows ? weight_of_rows(rows - whole * kTcRows) : 0.f)) * tiles_of(p, qn, kv_len);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -439,13 +441,10 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const int kvh = rest % p.hkv;
   rest /= p.hkv;
   const int seq = rest % p.num_seqs, tile = row_tiles - 1 - rest / p.num_seqs;      // the tiles that see the most first
-  const int q0 = p.q_starts[seq], qn = p.q_starts[seq + 1] - q0, kv_len = max(p.kv_lens[seq], 0), G = p.group;
-  const int all_rows = qn > 0 && qn <= p.max_q_len ? qn * G : 0, row0 = tile * kTcRows;
+  int q0, qn, kv_len;
+  if (!span_lengths(p, seq, threadIdx.x == 0, q0, qn, kv_len)) return;
+  const int G = p.group, all_rows = qn * G, row0 = tile * kTcRows;
   if (all_rows <= p.rows_from || row0 >= all_rows) return;
-  if (q0 < 0 || q0 + qn > p.tokens) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
-    return;
-  }
   const int n_rows = min(kTcRows, all_rows - row0);
   const int pieces = p.splits > 1 ? pieces_of(p, n_rows, tiles_of(p, qn, kv_len)) : 1;
   if (split >= pieces) return;

@@ -46,7 +46,7 @@ std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cach
   check_ints(block_tables, q, 0, "block_tables");
   check_ints(q_starts, q, num_seqs + 1, "q_starts");
   check_ints(kv_lens, q, num_seqs, "kv_lens");
-  TORCH_CHECK(std::isfinite(scale) && scale > 0 && std::isfinite(softcap) && softcap >= 0, "attention: scale must be positive, softcap not negative");
+  TORCH_CHECK(std::isfinite((float)scale) && scale >= 2e-38 && std::isfinite(softcap) && softcap >= 0, "attention: scale must be positive, softcap not negative");
   TORCH_CHECK(window >= 0 && first >= 0 && window < INT32_MAX && first < INT32_MAX, "attention: window and first must not be negative");
   if (sinks.has_value() && sinks->defined()) {
     TORCH_CHECK(sinks->is_cuda() && sinks->device() == q.device() && sinks->scalar_type() == at::kFloat && sinks->is_contiguous() && sinks->numel() == hq,
@@ -77,6 +77,7 @@ std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cach
   p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv); p.head_dim = (int)head_dim;
   p.kv_fp8 = is_e4m3(k_cache);
   p.max_q_len = (int)std::min<int64_t>(max_q_len, q.size(0)); p.min_q_len = (int)min_q_len; p.max_kv_len = (int)max_kv_len;
+  p.reach = (int)std::min<int64_t>(block_tables.size(1) * k_cache.size(2), INT32_MAX / 2 - 4096);
   p.window = (int)window; p.first = window > 0 ? (int)first : 0;
   p.scale = (float)scale; p.scale_log2 = (float)(scale * 1.4426950408889634); p.softcap = (float)softcap;
   c10::cuda::CUDAGuard guard(q.device());

@@ -308,12 +308,13 @@ struct SpanParams {
   int* status;
   int tokens, num_seqs, hq, hkv, group, head_dim, kv_fp8;
   int max_q_len, min_q_len, max_kv_len;
+  int reach;                   // tokens that a row of block_tables has room for
   int window, first;           // window 0: no limit (first is 0 then)
   float scale, scale_log2, softcap;
   // set by the planner, for one kernel
   int splits, min_pages, sms;  // pieces of what a sequence's rows see, at most; fewest pages in one; SMs
   bool in_cluster;             // the pieces join in a cluster
-  int rows_from, rows_to;      // packed rows (query rows x group) of the sequences that the kernel takes: from < rows <= to
+  int rows_from, rows_to;      // packed rows (query rows x group): the tensor-memory kernel takes sequences of more than `from`, the other of at most `to`
   float* ws_o;                 // [tokens][hq][splits][head_dim]
   float* ws_ml;                // [tokens][hq][splits][2]
 };

@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(kMoveThreads) kv_compact_kernel(const __grid_c
   pdl_wait();
   const int count = min(counts[seq], depth), b0 = base[seq];
   const int* table = tables + (size_t)seq * max_blocks;
-  auto place = [&](int tok, long long& row) {                  // block and offset of a token; false: there is no such page
-    const int page = tok / p.block_size;
+  auto place = [&](long long tok, long long& row) {            // block and offset of a token; false: there is no such page
+    const long long page = tok / p.block_size;
     if (tok < 0 || page >= max_blocks) return false;
     const int block = table[page];
     if (block < 0 || block >= p.blocks) return false;
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_compact_kernel(const __grid_c
       const int i = s0 + threadIdx.x, n = path[(size_t)seq * depth + i];
       long long f = 0, t = -1;
       if (n != i) {
-        if (n < i || b0 < 0 || !place(b0 + n, f) || !place(b0 + i, t)) {
+        if (n < i || b0 < 0 || !place((long long)b0 + n, f) || !place((long long)b0 + i, t)) {
           t = -1;
           if (status) atomicCAS(status, FLLM_OK, FLLM_ERR_BAD_ARGS);
         }

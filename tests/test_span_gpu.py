@@ -447,3 +447,251 @@ def test_tree_step_and_the_plain_step_after_it(ops, window, first):
         o, b = so.attend(q1.view(1, hq, D), k, v, so.seen_rows(n - 1, 1, window, first), D ** -0.5)
         so.check(y.view(1, hq, D), o, b)
     assert ops.check_status() == 0
+
+
+# ------------------------------------------------------------------------------------------ the tensor-memory kernel
+# (few rows in all go to the kernel for few rows: what follows is large enough for the other one)
+def _trees(n, nodes, hq, hkv, D, kv="bf16", ctx=700, seed=0, fill=0.0, words=1):
+    par = [-1] + [max(0, i - 4) for i in range(1, nodes)]              # a root with four chains
+    return so.setup([nodes] * n, [ctx + 17 * i for i in range(n)], hq, hkv, D, kv, words=words, trees=[par] * n, seed=seed, fill=fill), par
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,D", [(8, 2, 128), (40, 2, 64), (6, 2, 64)])
+@pytest.mark.parametrize("n", [2, 30])
+def test_infinities_and_nan_of_other_branches_in_many_rows(ops, hq, hkv, D, kv, n):
+    """One and two row tiles, whole and cut items: NaN and infinities in one sequence's nodes reach only the rows that see them."""
+    nodes, ctx = 60, 2500
+    c, par = _trees(n, nodes, hq, hkv, D, kv, ctx, seed=21, fill=float("nan"))
+    o, bound = so.want(c, D ** -0.5, 0, 0)
+    where = n - 1
+    bad = {9: float("nan"), 22: float("inf") if kv == "bf16" else float("nan")}
+    for node, x in bad.items():
+        tok = c.ctx[where] + node
+        c.v[int(c.tables[where, tok // 16]), :, tok % 16, 5] = x
+    tok = c.ctx[where] + 31
+    c.k[int(c.tables[where, tok // 16]), :, tok % 16, 3] = float("nan")
+    y = _tree(ops, c)
+    first = where * nodes
+    so.check(y[:first], o[:first], bound[:first])
+    seen = so.seen_rows(c.ctx[where], nodes, 0, 0, par)
+    mine = y[first:].view(nodes, hq, D)
+    o, bound = o[first:].view(nodes, hq, D), bound[first:].view(nodes, hq, D)
+    hit = {m: [i for i in range(nodes) if seen[i, c.ctx[where] + m]] for m in (9, 22, 31)}
+    clean = [i for i in range(nodes) if not any(i in h for h in hit.values())]
+    assert clean and all(hit.values())
+    so.check(mine[clean], o[clean], bound[clean])
+    rest = [d for d in range(D) if d != 5]
+    for m, x in bad.items():
+        got = mine[hit[m]][:, :, 5].float()
+        assert (torch.isnan(got) if math.isnan(x) else got == x).all()
+        so.check(mine[hit[m]][:, :, rest], o[hit[m]][:, :, rest], bound[hit[m]][:, :, rest])
+    assert torch.isnan(mine[hit[31]]).all()
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,D", [(8, 128), (32, 64)])
+def test_stale_values_around_prompts(ops, hq, D, kv):
+    """NaN in pages that the window has passed, in tokens in front of it and behind the last one; freed pages; several row tiles."""
+    rows, ctx, window, first = [600, 333], [900, 1501], 190, 20
+    c = so.setup(rows, ctx, hq, 2, D, kv, seed=8, fill=float("nan"))
+    o, bound = so.want(c, D ** -0.5, window, first)
+    for s in range(2):
+        for tok in range(first, ctx[s] + 1 - window):
+            blk, off = int(c.tables[s, tok // 16]), tok % 16
+            c.v[blk, :, off] = float("nan")
+            c.k[blk, :, off] = float("nan")
+        for page in range(2, (ctx[s] + 1 - window) // 16):
+            c.tables[s, page] = -1
+    so.check(_window(ops, c, window, first), o, bound)
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_rows_that_see_nothing_among_many(ops, kv):
+    c, _ = _trees(40, 30, 8, 2, 128, kv, ctx=200, seed=3)
+    c.base.zero_()                                      # no context: what the masks name is all there is
+    c.masks.zero_()
+    c.masks[::3] = 7
+    y = _tree(ops, c)
+    empty = torch.ones(len(y), dtype=torch.bool, device="cuda")
+    empty[::3] = False
+    assert (y[empty] == 0).all() and torch.isfinite(y).all()
+    for i in (0, 3, 597, 1197):
+        s = i // 30
+        o, b = so.attend(c.q[i:i + 1].view(1, 8, 128), c.keys[s][:3], c.values[s][:3], torch.ones(1, 3, dtype=torch.bool), 128 ** -0.5)
+        so.check(y[i].view(1, 8, 128), o, b)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_prompts_in_pools_of_more_than_32_bits(ops, kv):
+    blocks = (1 << 31) // (8 * 16 * 128) + 500
+    c = so.setup([500], [300], 32, 8, 128, kv, seed=6, pool_blocks=blocks)
+    assert int(c.tables.min()) * 8 * 16 * 128 > 1 << 31
+    so.check(_window(ops, c, 200, 30), *so.want(c, 128 ** -0.5, 200, 30))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_prompt_pages_that_are_not_there(ops, kv):
+    from fllm_b200.ops.native import NativeOps
+    mine = NativeOps(torch.device("cuda:0"), 1 << 20)
+    c = so.setup([700], [300], 16, 2, 128, kv, seed=9)
+    good = c.tables.clone()
+    for entry in (-1, c.k.shape[0], 1 << 30):
+        c.tables.copy_(good)
+        c.tables[0, 40] = entry
+        _window(mine, c, 200, 4)
+        assert mine.check_status() == 3
+    c.tables.copy_(good)
+    _window(mine, c, 200, 4)
+    assert mine.check_status() == 0
+    c.meta.seq_lens += 1 << 20
+    _window(mine, c, 100, 4)
+    assert mine.check_status() == 3
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("sink", [False, True])
+def test_long_sequences_beside_short_ones(ops, kv, sink):
+    """Trees of which some are cut into pieces and some are not, decode rows of one long sequence, and both in one call."""
+    s = _sinks(8) if sink else None
+    nodes, ctx = [40, 33, 5, 64, 2, 4, 1], [9000, 50, 700, 300, 0, 3000, 20]
+    c = so.setup(nodes, ctx, 8, 1, 128, kv, words=1, trees=[so.grow(n, n) for n in nodes], seed=31, fill=float("nan"))
+    so.check(_tree(ops, c, sinks=s), *so.want(c, 128 ** -0.5, 0, 0, s))
+    one = so.setup([1], [20000], 8, 1, 128, kv, seed=32)
+    so.check(_window(ops, one, 19000, 100, s), *so.want(one, 128 ** -0.5, 19000, 100, s))
+    both = so.setup([1, 1, 900], [15000, 7, 500], 8, 1, 128, kv, seed=33)
+    so.check(_window(ops, both, 12000, 64, s), *so.want(both, 128 ** -0.5, 12000, 64, s))
+    assert ops.check_status() == 0
+
+
+def test_prompts_in_graphs_and_on_streams(ops):
+    """Two captured graphs of the tensor-memory kernel replayed in turn and on two streams at once, then on other lengths."""
+    c = so.setup([500, 40, 3], [600, 1100, 2000], 16, 2, 128, seed=12)
+    t, _ = _trees(24, 50, 16, 2, 128, ctx=500, seed=13)
+    w1, w2 = so.want(c, 128 ** -0.5, 300, 4), so.want(t, 128 ** -0.5, 0, 0)
+    graphs, outs = [], []
+    for f in (lambda: _window(ops, c, 300, 4), lambda: _tree(ops, t)):
+        f()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(f())
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    so.check(outs[0], *w1)
+    so.check(outs[1], *w2)
+    short = so.setup([500, 40, 3], [0, 77, 1999], 16, 2, 128, seed=14)
+    c.q.copy_(short.q)
+    c.tables.fill_(-1)
+    c.tables[:, :short.tables.shape[1]].copy_(short.tables)
+    c.meta.seq_lens.copy_(short.meta.seq_lens)
+    c.k[:short.k.shape[0]].copy_(short.k)
+    c.v[:short.k.shape[0]].copy_(short.v)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    so.check(outs[0], *so.want(short, 128 ** -0.5, 300, 4))
+    assert ops.check_status() == 0
+
+
+def test_large_magnitudes_beside_an_8_bit_cache(ops):
+    """Queries of very different magnitudes from row to row, up to 2^120 and down to 2^-130 with a scale that makes up for it, zero rows, and rows with
+    an infinity or a NaN, which are NaN and disturb no other."""
+    for rows, ctx in ([3, 1], [200, 90]), ([500, 333], [300, 700]):
+        c = so.setup(rows, ctx, 16, 2, 128, "e4m3", seed=41)
+        T = sum(rows)
+        c.q[::5] = 0
+        for up, scale in ((2.0 ** 118, 2.0 ** -118), (2.0 ** -118, 2.0 ** 118)):
+            q = (c.q.float() * up).bfloat16()
+            d = SimpleNamespace(**{**vars(c), "q": q})
+            call = lambda x: ops.attention(x, c.k, c.v, c.tables, c.row_seq, c.positions, 16, 2, 128, 128 ** -0.5 * scale, 150, meta=c.meta, first=9)
+            o, bound = so.want(d, 128 ** -0.5 * scale, 150, 9)
+            so.check(call(q), o, bound)
+            q2 = q.clone()
+            q2[T - 1, 3] = float("inf")
+            q2[1, 200] = float("nan")
+            y = call(q2)
+            assert torch.isnan(y[T - 1, :128]).all() and torch.isnan(y[1, 128:256]).all()
+            keep = torch.ones(T, dtype=torch.bool, device="cuda")
+            keep[[1, T - 1]] = False
+            so.check(y[keep], o[keep], bound[keep])
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("rows,ctx", [([3, 1], [200, 90]), ([300, 290], [300, 700])])
+def test_lengths_that_the_batch_does_not_announce(rows, ctx):
+    """More rows in a sequence than the batch says, rows behind the query's, a length that no table reaches: reported. Fewer rows than it says: right."""
+    from fllm_b200.ops.native import NativeOps
+    mine = NativeOps(torch.device("cuda:0"), 1 << 20)
+    c = so.setup(rows, ctx, 16, 2, 128, seed=51, fill=float("nan"))
+    o, bound = so.want(c, 128 ** -0.5, 150, 9)
+    c.meta.max_q_len -= 1
+    c.meta.min_q_len = min(c.meta.min_q_len, c.meta.max_q_len)
+    y = _window(mine, c, 150, 9)
+    assert mine.check_status() == 3
+    so.check(y[rows[0]:], o[rows[0]:], bound[rows[0]:])
+    c.meta.max_q_len += 1
+    c.meta.min_q_len = c.meta.max_q_len
+    so.check(_window(mine, c, 150, 9), o, bound)
+    assert mine.check_status() == 0
+    good = c.meta.q_starts.clone()
+    for bad in ([-1, rows[0], sum(rows)], [0, sum(rows), rows[0]], [0, rows[0], sum(rows) + 1]):
+        c.meta.q_starts.copy_(torch.tensor(bad))
+        c.meta.max_q_len = sum(rows) + 1
+        _window(mine, c, 150, 9)
+        assert mine.check_status() == 3, bad
+    c.meta.q_starts.copy_(good)
+    c.meta.seq_lens[1] = 2 ** 31 - 1
+    y = _window(mine, c, 150, 9)
+    assert mine.check_status() == 3
+    so.check(y[:rows[0]], o[:rows[0]], bound[:rows[0]])
+
+
+def test_compaction_beyond_every_table():
+    from fllm_b200.ops.native import NativeOps
+    mine = NativeOps(torch.device("cuda:0"), 1 << 20)
+    pool = torch.randn(2, 4, 2, 16, 64, device="cuda").bfloat16()
+    before = pool.clone()
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    for base, node in ((2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31 - 8, 20), (-5, 9), (0, 64)):
+        mine.kv_compact([pool], i32([[0, 1, 2, 3]]), i32([base]), i32([[node]]), i32([1]))
+        assert mine.check_status() == 3 and torch.equal(pool, before)
+    mine.kv_compact([pool], i32([[0, 1, 2, 3]]), i32([1]), i32([[5, 5, 7]]), i32([3]))         # the same node twice: copied twice
+    assert mine.check_status() == 0
+    for to, node in ((1, 6), (2, 6), (3, 8)):
+        assert torch.equal(pool[:, 0, :, to], before[:, 0, :, node])
+
+
+def test_served_model_keeps_its_first_tokens():
+    """An engine whose windows leave the first tokens visible: prompts in chunks, decode steps from captured graphs, the blocks between freed; the
+    tokens are those of an engine that frees nothing, and the logits follow the PyTorch operators."""
+    from fllm_b200.config import EngineConfig, preset
+    from fllm_b200.models.decoder import Decoder, KVCache, StepBatch
+    from fllm_b200.ops.reference import RefOps
+    from fllm_b200.runtime import LLMEngine, SamplingParams
+    cfg = preset("qwen3-tiny")
+    cfg.sliding_window, cfg.window_first = 40, 20
+    prompt = [(7 * i) % 50 + 1 for i in range(150)]
+    outs = []
+    for free in (True, False):
+        eng = LLMEngine(cfg, EngineConfig(max_num_seqs=4, num_kv_blocks=96, max_model_len=256, max_num_batched_tokens=64), device="cuda:0")
+        if not free:
+            eng.scheduler.window = 0
+        outs.append(eng.generate([prompt, prompt[:30]], SamplingParams(max_tokens=12)))
+    assert outs[0] == outs[1]
+    n = len(prompt)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    b = StepBatch(i32(prompt), i32(list(range(n))), i32(list(range(n))), i32([0] * n), i32([list(range(16))]), i32([n - 1]), num_seqs=1, num_tokens=n,
+                  max_kv_len=n, max_q_len=n, min_q_len=n, seq_lens=i32([n]), q_starts=i32([0, n]))
+    logits = []
+    for o in (eng.ops, RefOps()):
+        kv = KVCache(cfg.num_layers, 20, cfg.num_kv_heads, 16, cfg.head_dim, "cuda")
+        logits.append(Decoder(cfg, eng.weights, kv, o, eng.spec).forward(b).float())
+    assert (logits[0] - logits[1]).abs().max() <= 0.05 * logits[1].abs().max()
