@@ -20,7 +20,7 @@ constexpr int kSpanWords = 4;              // 64-bit words of a tree mask: at mo
 
 struct SpanRow {
   int base;                                // context tokens are those in front of it
-  int beg;                                 // where the window begins
+  int beg;                                 // where the window begins, its end at most
 };
 
 // Row `qi` of the qn rows of a sequence; `bits` (trees): its mask, trimmed, p.words of them.
@@ -54,6 +54,7 @@ __device__ __forceinline__ SpanRow span_row(const SpanParams& p, int q0, int qn,
       }
       bits[w] = keep;
     }
+    r.beg = r.base;                        // no context is left in the window, and nodes that stay may lie anywhere behind it
   }
   return r;
 }

@@ -449,6 +449,18 @@ def test_tree_step_and_the_plain_step_after_it(ops, window, first):
     assert ops.check_status() == 0
 
 
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq", [2, 16])
+@pytest.mark.parametrize("n", [1, 40])
+def test_first_nodes_that_lie_far_behind(ops, kv, hq, n):
+    """Two deep branches of a tree in a text that begins with it: the second one's upper nodes are among the first tokens, but stored behind the first one."""
+    par = [-1] + list(range(0, 50)) + [0] + list(range(51, 150))
+    c = so.setup([151] * n, [0, 3, 1, 9] * (n // 4) if n > 1 else [0], hq, 2, 128, kv, words=3, trees=[par] * n, seed=77)
+    for window, first in ((4, 4), (20, 7)):
+        so.check(_tree(ops, c, window, first), *so.want(c, 128 ** -0.5, window, first))
+    assert ops.check_status() == 0
+
+
 # ------------------------------------------------------------------------------------------ the tensor-memory kernel
 # (few rows in all go to the kernel for few rows: what follows is large enough for the other one)
 def _trees(n, nodes, hq, hkv, D, kv="bf16", ctx=700, seed=0, fill=0.0, words=1):
