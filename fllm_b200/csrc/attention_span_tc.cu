@@ -87,7 +87,7 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return hi <= lo ? 0u : (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
 }
 
-// What a row sees of the 128 tokens from tok0 on: its context, and (trees, out of line: few tiles hold nodes, and what a mask needs would be held in
+// What a row sees of the walk's 128 tokens from tok0 on (base and beg in the walk's places): its context, and (trees, out of line: few tiles hold nodes, and what a mask needs would be held in
 // registers beside the scores of those that do not) the nodes that row `qi` of the sequence sees.
 __device__ __forceinline__ uint4 context_bits(const SpanParams& p, int base, int beg, int tok0) {
   uint32_t vis[4];
@@ -98,9 +98,11 @@ __device__ __forceinline__ uint4 context_bits(const SpanParams& p, int base, int
   }
   return make_uint4(vis[0], vis[1], vis[2], vis[3]);
 }
-__device__ __noinline__ uint4 tree_bits(const SpanParams& p, int q0, int qn, int kv_len, int qi, int tok0) {
+__device__ __noinline__ uint4 tree_bits(const SpanParams& p, int q0, int qn, int kv_len, int gap, int qi, int tok0) {
   unsigned long long b[kSpanWords + 1] = {0, 0, 0, 0, 0};
-  const SpanRow row = span_row(p, q0, qn, kv_len, qi, b);
+  SpanRow row = span_row(p, q0, qn, kv_len + gap, qi, b);
+  row.base -= gap;
+  row.beg -= gap;
   const uint4 context = context_bits(p, row.base, row.beg, tok0);
   uint32_t vis[4] = {context.x, context.y, context.z, context.w};
 #pragma unroll
@@ -111,9 +113,9 @@ __device__ __noinline__ uint4 tree_bits(const SpanParams& p, int q0, int qn, int
   }
   return make_uint4(vis[0], vis[1], vis[2], vis[3]);
 }
-__device__ __forceinline__ uint4 row_bits(const SpanParams& p, int q0, int qn, int kv_len, int qi, int tok0) {
+__device__ __forceinline__ uint4 row_bits(const SpanParams& p, int q0, int qn, int kv_len, int gap, int qi, int tok0) {
   if (qi < 0) return make_uint4(0, 0, 0, 0);
-  if (p.tree_mask) return tree_bits(p, q0, qn, kv_len, qi, tok0);
+  if (p.tree_mask) return tree_bits(p, q0, qn, kv_len, gap, qi, tok0);
   const int base = max(kv_len - qn + qi + 1, 0);
   return context_bits(p, base, p.window > 0 ? max(0, base - p.window) : 0, tok0);
 }
@@ -300,10 +302,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 struct PageRows {
   const SpanParams& p;
   const int* table;
-  int kvh, head_end, lo, end, none;        // pages [0, head_end) and [lo, end) are seen
-  __device__ __forceinline__ int operator()(int page, bool& bad) const {
-    if (!(page < head_end || (page >= lo && page < end))) return none;
-    const int b = span_block(p, table, page);
+  int kvh, head, gap, count, none;         // of the walk's `count` pages those from `head` on lie `gap` further in the text
+  __device__ __forceinline__ int page_of(int i) const { return i < head ? i : i + gap; }
+  __device__ __forceinline__ int operator()(int i, bool& bad) const {
+    if (i >= count) return none;
+    const int page = page_of(i), b = span_block(p, table, page);
     bad |= b < 0;
     return b < 0 ? none : (int)span_pool_row(p, b, kvh, page);
   }
@@ -313,15 +316,14 @@ struct PageRows {
 // all lanes, in front of every tile, the producers took longer than the products.)
 struct PagesAhead {
   const PageRows& rows;
-  const SpanRange& range;
   int t0, n_tiles, now, next;
   bool bad;
-  __device__ __forceinline__ PagesAhead(const PageRows& r, const SpanRange& s, int first, int n) : rows(r), range(s), t0(first), n_tiles(n), now(0), next(0), bad(false) {
+  __device__ __forceinline__ PagesAhead(const PageRows& r, int first, int n) : rows(r), t0(first), n_tiles(n), now(0), next(0), bad(false) {
     next = look(0);
   }
   __device__ __forceinline__ int look(int it) {
     const int at = it + ((threadIdx.x & 31) >> 3);
-    return at < n_tiles ? rows(range.piece(t0 + at) * kTilePages + (threadIdx.x & 7), bad) : rows.none;
+    return at < n_tiles ? rows((t0 + at) * kTilePages + (threadIdx.x & 7), bad) : rows.none;
   }
   __device__ __forceinline__ void to(int it) {         // tile after tile
     if ((it & 3) == 0) { now = next; next = look(it + 4); }
@@ -350,7 +352,7 @@ __device__ __forceinline__ uint32_t without_odd_f16(uint32_t w) {
 // 157 by this rule, 172 where two pieces begin at 1.35 SMs.
 __device__ __forceinline__ int tiles_of(const SpanParams& p, int qn, int kv_len) {
   const int tiles = max((kv_len + kTile - 1) / kTile, 1);
-  return p.window > 0 ? (int)min((long long)tiles, ((long long)p.window + p.first + min(qn, kTcRows)) / kTile + 3) : tiles;
+  return p.window > 0 ? (int)min((long long)tiles, ((long long)p.window + p.first + min(qn, kTcRows / p.group + 2) + 2 * kPage) / kTile + 1) : tiles;
 }
 __device__ __forceinline__ float weight_of_rows(int rows) { return rows > kRows ? 2.f : 1.f; }
 __device__ __forceinline__ int pieces_of(const SpanParams& p, int n_rows, int tiles) {
@@ -446,7 +448,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const int G = p.group, all_rows = qn * G, row0 = tile * kTcRows;
   if (all_rows <= p.rows_from || row0 >= all_rows) return;
   const int n_rows = min(kTcRows, all_rows - row0);
-  const int pieces = p.splits > 1 ? pieces_of(p, n_rows, tiles_of(p, qn, kv_len)) : 1;
+  const int walk = tiles_of(p, qn, kv_len), pieces = p.splits > 1 ? pieces_of(p, n_rows, walk) : 1;
   if (split >= pieces) return;
   const bool two = n_rows > kRows;                     // two row tiles that share K and V, or two groups that share a row tile
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
@@ -464,15 +466,20 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const int r_first = (two ? group * kRows : 0) + (warp & 3) * 32, r = r_first + lane;
   const int qi = warp < 8 && r < n_rows ? (row0 + r) / G : -1;
   const TileSees sees = tile_sees(p, q0, qn, kv_len, row0, n_rows);
-  const int min_base = sees.min_base, max_beg = sees.max_beg, end = sees.end;
-  const SpanRange range = span_range(p, kTile, sees.min_beg, end);
-  const int per_piece = (tiles_of(p, qn, kv_len) + pieces - 1) / pieces;      // (the last one goes on to the end, should that be further)
-  const int t0 = min(split * per_piece, range.count), n_tiles = split == pieces - 1 ? range.count - t0 : min(per_piece, range.count - t0);
+  // The walk goes over the first tokens' pages and those from the window on as if they lay one behind the other: from here on places are the walk's,
+  // in which context, windows and lengths are what they are in a text without the `gap`. (A text with a gap has its context behind it, so no first
+  // token lies elsewhere. Tiles of 128 tokens of the text each, 3 x 777 rows under a window of 512 with 16 first tokens, 64 query and 8 key heads of 64,
+  // e4m3: 90 us; so: 81.)
+  const SpanRange range = span_range(p, kPage, sees.min_beg, sees.end);
+  const int gap = (range.lo - range.head) * kPage, min_base = sees.min_base - gap, max_beg = sees.max_beg - gap;
+  kv_len -= gap;
+  const int per_piece = (walk + pieces - 1) / pieces;      // (the last one goes on to the end, should that be further)
+  const int n_all = (range.count + kTilePages - 1) / kTilePages, t0 = min(split * per_piece, n_all), n_tiles = split == pieces - 1 ? n_all - t0 : min(per_piece, n_all - t0);
   const int shift = two ? 1 : 0, n_items = n_tiles << shift;
   // not every row of the CTA sees the whole tile
   auto partial = [&](int tok0) { return !(tok0 + kTile <= min_base && (tok0 >= max_beg || tok0 + kTile <= p.first)); };
-  const PageRows page_rows{p, p.block_tables + (size_t)seq * p.max_blocks, kvh, (min(p.first, end) + kPage - 1) / kPage, sees.min_beg / kPage,
-                           (end + kPage - 1) / kPage, (int)(p.num_blocks * p.hkv * p.block_pages * kPage)};
+  const PageRows page_rows{p, p.block_tables + (size_t)seq * p.max_blocks, kvh, range.head, range.lo - range.head, range.count,
+                           (int)(p.num_blocks * p.hkv * p.block_pages * kPage)};
 
   // The block was launched with 168 registers a thread (e4m3: 128): 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128.
   if (warp >= 8) {
@@ -565,7 +572,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     } else if constexpr (!KV8) {
       const bool is_v = warp == 11;
       const int half = warp == 10 ? 1 : 0;
-      PagesAhead pages(page_rows, range, t0, n_tiles);
+      PagesAhead pages(page_rows, t0, n_tiles);
       auto ask = [&](int it) {                         // all lanes; false: gave up
         const int b = it & 1;
         int rows[kTilePages];
@@ -597,7 +604,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           const int b = it & 1;
           ok = ok && mbar_wait_warp(&v_full[b], (it >> 1) & 1, abort_flag);
           if (!ok) break;
-          if (partial(range.piece(t0 + it) * kTile)) {
+          if (partial((t0 + it) * kTile)) {
             uint4* v = reinterpret_cast<uint4*>(sv + b * TB);
             uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll 8
@@ -626,7 +633,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       const int part = warp - 10;
       const int slots = two ? 4 : 8, turn = two ? 2 : 3, pieces = 2 * n_tiles;
       auto slot_at = [&](int s) { return s < 4 ? smem + 6 * TB + s * S::kRaw : sq + TB + (s - 4) * S::kRaw; };      // the unused tile of Q
-      PagesAhead pages(page_rows, range, t0, warp == 8 ? n_tiles : 0);
+      PagesAhead pages(page_rows, t0, warp == 8 ? n_tiles : 0);
       auto ask_k = [&](int it) {                       // warp 8
         const int b = it & (KS - 1);
         int rows[kTilePages];
@@ -679,7 +686,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
 #pragma unroll
         for (int u = 0; u < kMost; ++u)
           if (part + kWideners * u < kTurns) raw[u] = *reinterpret_cast<const uint4*>(src + (part + kWideners * u) * 512);
-        const bool look = partial(range.piece(t0 + it) * kTile);
+        const bool look = partial((t0 + it) * kTile);
         uint32_t sum[2] = {0, 0};
 #pragma unroll
         for (int u = 0; u < kMost; ++u) {
@@ -731,12 +738,12 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int n = group; n < n_items; n += 2) {
-      const int k = n >> 1, tok0 = range.piece(t0 + (n >> shift)) * kTile;
+      const int k = n >> 1, tok0 = (t0 + (n >> shift)) * kTile;
       if (!mbar_wait(&s_full[group], k & 1, abort_flag)) { ok = false; break; }
       tc_fence_after_sync();
       const bool whole = tok0 + kTile <= w_base && (tok0 >= w_beg || tok0 + kTile <= p.first);
       uint4 vis = make_uint4(0, 0, 0, 0);
-      if (!whole) vis = row_bits(p, q0, qn, kv_len, qi, tok0);
+      if (!whole) vis = row_bits(p, q0, qn, kv_len, gap, qi, tok0);
       if (p.softcap > 0.f) cap_scores(t_s, factor / (p.softcap * kLog2e));
       softmax_tile<D, KV8>(t_s, t_o, whole, vis, scale, k > 0, &p_half[group], m_used, l);
       tc_fence_before_sync();
@@ -847,13 +854,13 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         // infinities and NaN that were taken out of tiles, added to the rows that see them
         for (int it = 0; it < n_tiles; ++it) {
-          const int tok0 = range.piece(t0 + it) * kTile;
+          const int tok0 = (t0 + it) * kTile;
           if (!partial(tok0)) continue;
-          const uint4 visible = row_bits(p, q0, qn, kv_len, qi, tok0);
+          const uint4 visible = row_bits(p, q0, qn, kv_len, gap, qi, tok0);
           const uint32_t vis[4] = {visible.x, visible.y, visible.z, visible.w};
           for (int i = 0; i < kTile; ++i) {
             if (!(vis[i >> 5] >> (i & 31) & 1)) continue;
-            const int page = (tok0 + i) / kPage, b = span_block(p, page_rows.table, page);
+            const int page = page_rows.page_of((tok0 + i) / kPage), b = span_block(p, page_rows.table, page);
             if (b < 0) continue;
             const size_t at = (size_t)(span_pool_row(p, b, kvh, page) + (i & 15)) * D;
             for (int d = 0; d < D; ++d) {
