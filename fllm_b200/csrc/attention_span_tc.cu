@@ -404,7 +404,7 @@ __device__ __forceinline__ TileSees tile_sees(const SpanParams& p, int q0, int q
 
 template <int D, bool KV8>
 __global__ void __launch_bounds__(tc_threads<KV8>(), 1)
-span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ SpanParams p, int row_tiles) {
+span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ SpanParams p, int row_tiles, int halved) {
   using S = TcSmem<D, KV8>;
   constexpr int TB = S::kT;
   extern __shared__ uint8_t smem_raw[];
@@ -439,15 +439,24 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   if (warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); if (!KV8) tma_prefetch_desc(&tma_v); }
   pdl_wait();
   const int split = blockIdx.y;
-  int rest = blockIdx.x;
+  // Whole tiles of the longest sequence come first, those that see the most before others; then what is left of the rows. The last `halved` of the whole
+  // ones are two CTAs of half the rows each.
+  int rest = blockIdx.x, half = -1;
+  const int from_halves = row_tiles * p.num_seqs * p.hkv - halved;
+  if (rest >= from_halves + 2 * halved) {
+    rest -= halved;
+  } else if (rest >= from_halves) {
+    half = (rest - from_halves) & 1;
+    rest = from_halves + ((rest - from_halves) >> 1);
+  }
   const int kvh = rest % p.hkv;
   rest /= p.hkv;
-  const int seq = rest % p.num_seqs, tile = row_tiles - 1 - rest / p.num_seqs;      // the tiles that see the most first
+  const int seq = rest % p.num_seqs, at_tile = rest / p.num_seqs, tile = at_tile < row_tiles ? row_tiles - 1 - at_tile : at_tile;
   int q0, qn, kv_len;
   if (!span_lengths(p, seq, threadIdx.x == 0, q0, qn, kv_len)) return;
-  const int G = p.group, all_rows = qn * G, row0 = tile * kTcRows;
+  const int G = p.group, all_rows = qn * G, row0 = tile * kTcRows + (half > 0 ? kRows : 0);
   if (all_rows <= p.rows_from || row0 >= all_rows) return;
-  const int n_rows = min(kTcRows, all_rows - row0);
+  const int n_rows = min(half < 0 ? kTcRows : kRows, all_rows - row0);
   const int walk = tiles_of(p, qn, kv_len), pieces = p.splits > 1 ? pieces_of(p, n_rows, walk) : 1;
   if (split >= pieces) return;
   const bool two = n_rows > kRows;                     // two row tiles that share K and V, or two groups that share a row tile
@@ -902,10 +911,15 @@ void launch_tc(const SpanParams& p, cudaStream_t s) {
     mk = make_tmap_2d(p.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, D, D * 2, kPage, 64, true);
     mv = make_tmap_parts(p.v_cache, rows, D, kPage, D / 64);
   }
-  const long long tiles = ((long long)p.max_q_len * p.group + kTcRows - 1) / kTcRows;
-  const long long ctas = tiles * p.num_seqs * p.hkv;
+  // (What is left of the longest sequence's rows is a whole tile from 129 rows on.)
+  const long long most = (long long)p.max_q_len * p.group, row_tiles = (most + kRows - 1) / kTcRows, whole = row_tiles * p.num_seqs * p.hkv;
+  // Where the last round of whole tiles, and what is left of rows behind it, would leave half of the SMs or more without work, two SMs share each of its
+  // tiles by rows. (2 x 2048 rows under a window of 1024, 32 query and 8 key heads of 128, three rounds and 68 tiles: 99 us, 105 without.)
+  const long long left = most > row_tiles * kTcRows ? (long long)p.num_seqs * p.hkv : 0;
+  const int last = (int)(whole % p.sms), halved = p.splits == 1 && 2 * last + left <= p.sms ? last : 0;
+  const long long ctas = whole + halved + left;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
-  launch_pdl(span_tc_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(tc_threads<KV8>()), smem, s, mk, mv, p, (int)tiles);
+  launch_pdl(span_tc_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(tc_threads<KV8>()), smem, s, mk, mv, p, (int)row_tiles, halved);
 }
 }  // namespace
 

@@ -579,6 +579,16 @@ def test_long_sequences_beside_short_ones(ops, kv, sink):
     assert ops.check_status() == 0
 
 
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows,hq,hkv", [([704, 640], 16, 2), ([2400], 8, 1), ([1500, 20, 1400], 8, 2)])
+def test_last_rounds_of_prompts(ops, kv, rows, hq, hkv):
+    """Whole tiles that two blocks share, tiles of what is left of rows, sequences that end where others go on; first tokens in the window's tiles."""
+    c = so.setup(rows, [400 + 77 * i for i in range(len(rows))], hq, hkv, 64, kv, seed=61, fill=float("nan"))
+    for window, first in ((130, 3), (65, 40), (500, 1)):
+        so.check(_window(ops, c, window, first), *so.want(c, 0.125, window, first))
+    assert ops.check_status() == 0
+
+
 def test_prompts_in_graphs_and_on_streams(ops):
     """Two captured graphs of the tensor-memory kernel replayed in turn and on two streams at once, then on other lengths."""
     c = so.setup([500, 40, 3], [600, 1100, 2000], 16, 2, 128, seed=12)
