@@ -50,6 +50,12 @@ __device__ __forceinline__ float2 unpack_16(uint32_t w) {
   if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   else return unpack_bf16x2(w);
 }
+// A lane's two 16-bit values of an 8 x 8 matrix, row lane / 4 and columns 2 (lane % 4), for those of the transposed one.
+__device__ __forceinline__ uint32_t transposed(uint32_t w) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(w));
+  return d;
+}
 __device__ __forceinline__ void cp_async16_or_zero(void* smem, const void* gmem, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(there ? 16 : 0) : "memory");
 }
@@ -72,7 +78,7 @@ __device__ __forceinline__ void store_row(const SpanParams& p, int q0, int row, 
 // An e4m3 page stays as it is in shared memory and becomes operands in registers, which needs no order of columns that memory does not have: a lane
 // takes 16 bytes of a key row for four k-steps (queries lie in the same order), and 16 bytes of each of four value rows, two tokens of a dim to a
 // register. So of column block i of O, column n is dim i of the n-th piece of 16 (or 8, at D = 64) values. (Through f16 tiles in shared memory, ldmatrix
-// behind them, 48 sequences under a window of 1000 with 130 first tokens, 64 query and 8 key heads of 64, took 42 us, 31 so.)
+// behind them, 48 sequences under a window of 1000 with 130 first tokens, 64 query and 8 key heads of 64, took 42 us, 31 so, both with all 16 rows.)
 template <int D>
 __device__ __forceinline__ int dim_of(int i, int n) {
   if constexpr (D == 64) return 8 * n + i;
@@ -101,7 +107,11 @@ struct RowsSmem {
 // CTAs of an SM, by registers and shared memory.
 template <int D, bool KV8> constexpr int rows_resident() { return D == 256 ? 1 : D == 64 ? 4 : KV8 ? 3 : 2; }
 
-template <int D, bool KV8>
+// NARROW: up to 8 packed rows, for which scores and sums are transposed, S^T = K Q^T and O^T = V^T P^T: the products' 16 rows are tokens and dims, their
+// 8 columns the rows, and nothing is computed for rows 8 to 15. A lane's operands are the same registers in another order; it holds scores of rows 2t and
+// 2t + 1 and tokens g and g + 8 (otherwise rows g and g + 8 and tokens 2t, 2t + 1 of each half). us of decode rows, so and with 16 rows: 48 sequences of an
+// e4m3 cache under 1000 with 130 first tokens, 64 query and 8 key heads of 64: 22.6, 28.8; one under 256, 32 and 8 of 128: 6.3, 6.8; 64 under 4096: 166 both.
+template <int D, bool KV8, bool NARROW>
 __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel(const __grid_constant__ SpanParams p) {
   using S = RowsSmem<D, KV8>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -249,13 +259,17 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
     for (int kk = 0; kk < D / 16; ++kk) ldsm_x4(qf[kk], tile_ptr<D>(qtile, lane & 15, 2 * kk + (lane >> 4)));
   }
 
-  const int base0 = bases[g], base1 = bases[g + 8], beg0 = begs[g], beg1 = begs[g + 8];
-  const float f0 = factors[g], f1 = factors[g + 8];
-  const unsigned long long *bits0 = bits + g * kSpanWords, *bits1 = bits + (g + 8) * kSpanWords;
+  const int row_a = NARROW ? 2 * t : g, row_b = NARROW ? 2 * t + 1 : g + 8;           // a lane's rows
+  const int base0 = bases[row_a], base1 = bases[row_b], beg0 = begs[row_a], beg1 = begs[row_b];
+  const float f0 = factors[row_a], f1 = factors[row_b];
+  const unsigned long long *bits0 = bits + row_a * kSpanWords, *bits1 = bits + row_b * kSpanWords;
 
-  float o[D / 8][4];
+  constexpr int kO = NARROW ? D / 16 : D / 8, kS = NARROW ? kPages : 2 * kPages;      // accumulators of O and of S
+  // value `x` of a lane (0 to 3) in an accumulator: which of its rows, which of the two places (tokens, column blocks) along the other side
+  constexpr auto second_row = [](int x) { return NARROW ? x & 1 : x >> 1; };
+  float o[kO][4];
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < kO; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
   // kPages pages at a time: with two there are two chains of products and one maximum for both. (One that is not there any more has no token that
@@ -275,22 +289,33 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
       tok0[h] = there ? range.piece(pg0 + warp + 4 * (it + h)) * kPage : INT_MAX / 2;
       full[h] = tok0[h] + kPage <= min_base && (tok0[h] >= max_beg || tok0[h] + kPage <= p.first);
     }
-    float s[2 * kPages][4];
+    float s[kS][4];
 #pragma unroll
-    for (int i = 0; i < 2 * kPages; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int i = 0; i < kS; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
     const int j = lane >> 3;
     if constexpr (KV8) {
 #pragma unroll
       for (int grp = 0; grp < D / 64; ++grp) {
 #pragma unroll
-        for (int nb = 0; nb < 2 * kPages; ++nb) {
-          const int r = (nb & 1) * 8 + g;
-          const uint4 raw = *reinterpret_cast<const uint4*>(page_at[nb >> 1] + r * D + (((4 * grp + t) ^ turn_k<D>(r)) << 4));
-          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        for (int h = 0; h < kPages; ++h) {
+          uint32_t w[2][4];                // tokens g and g + 8
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int r = 8 * half + g;
+            const uint4 raw = *reinterpret_cast<const uint4*>(page_at[h] + r * D + (((4 * grp + t) ^ turn_k<D>(r)) << 4));
+            w[half][0] = raw.x; w[half][1] = raw.y; w[half][2] = raw.z; w[half][3] = raw.w;
+          }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint2 h = e4m3x4_to_f16(w[k]);
-            mma_f16(s[nb], qf[4 * grp + k], h.x, h.y);
+            const uint2 x = e4m3x4_to_f16(w[0][k]), y = e4m3x4_to_f16(w[1][k]);
+            const uint32_t(&q)[4] = qf[4 * grp + k];
+            if constexpr (NARROW) {
+              const uint32_t a[4] = {x.x, y.x, x.y, y.y};
+              mma_f16(s[h], a, q[0], q[2]);
+            } else {
+              mma_f16(s[2 * h], q, x.x, x.y);
+              mma_f16(s[2 * h + 1], q, y.x, y.y);
+            }
           }
         }
       }
@@ -300,30 +325,38 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
       for (int kk = 0; kk < D / 16; ++kk) {
         uint32_t b[4];
         ldsm_x4(b, tile_ptr<D>(ks, (j >> 1) * 8 + (lane & 7), 2 * kk + (j & 1)));
-        mma_bf16(s[0], qf[kk], b[0], b[1]);
-        mma_bf16(s[1], qf[kk], b[2], b[3]);
+        if constexpr (NARROW) {
+          const uint32_t a[4] = {b[0], b[2], b[1], b[3]};
+          mma_bf16(s[0], a, qf[kk][0], qf[kk][2]);
+        } else {
+          mma_bf16(s[0], qf[kk], b[0], b[1]);
+          mma_bf16(s[1], qf[kk], b[2], b[3]);
+        }
       }
     }
     float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-    for (int nb = 0; nb < 2 * kPages; ++nb) {
+    for (int i = 0; i < kS; ++i) {
+      const int h = NARROW ? i : i >> 1;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = s[nb][e] * (e >= 2 ? f1 : f0);
+        float v = s[i][e] * (second_row(e) ? f1 : f0);
         if (p.softcap > 0.f) v = p.softcap * tanhf(v / (p.softcap * kLog2e)) * kLog2e;
-        if (!full[nb >> 1]) {
-          const int tok = tok0[nb >> 1] + (nb & 1) * 8 + 2 * t + (e & 1);
-          if (!(e >= 2 ? span_sees(p, tok, base1, beg1, bits1) : span_sees(p, tok, base0, beg0, bits0))) v = -INFINITY;
+        if (!full[h]) {
+          const int tok = tok0[h] + (NARROW ? g + 8 * (e >> 1) : (i & 1) * 8 + 2 * t + (e & 1));
+          if (!(second_row(e) ? span_sees(p, tok, base1, beg1, bits1) : span_sees(p, tok, base0, beg0, bits0))) v = -INFINITY;
         }
-        s[nb][e] = v;
-        if (e >= 2) mx1 = fmaxf(mx1, v);
+        s[i][e] = v;
+        if (second_row(e)) mx1 = fmaxf(mx1, v);
         else mx0 = fmaxf(mx0, v);
       }
     }
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+    constexpr int kNext = NARROW ? 4 : 1, kLast = NARROW ? 16 : 2;       // a row's lanes
+#pragma unroll
+    for (int x = kNext; x <= kLast; x *= 2) {
+      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
+      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+    }
     const float mn0 = fmaxf(m[0], mx0), mn1 = fmaxf(m[1], mx1);
     constexpr float lift = KV8 ? kF16Lift : 0.f;
     const float r0 = mn0 == -INFINITY ? 0.f : mn0 - lift, r1 = mn1 == -INFINITY ? 0.f : mn1 - lift;
@@ -332,43 +365,56 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
       l[0] *= c0;
       l[1] *= c1;
 #pragma unroll
-      for (int db = 0; db < D / 8; ++db) {
-        o[db][0] *= c0; o[db][1] *= c0;
-        o[db][2] *= c1; o[db][3] *= c1;
-      }
+      for (int i = 0; i < kO; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[i][x] *= second_row(x) ? c1 : c0;
       m[0] = mn0;
       m[1] = mn1;
     }
-    uint32_t pf[kPages][4];
+    uint32_t pf[kPages][NARROW ? 2 : 4];               // narrow: of tokens g and g + 8, both rows
 #pragma unroll
-    for (int nb = 0; nb < 2 * kPages; ++nb) {
-      const float p0 = ex2(s[nb][0] - r0), p1 = ex2(s[nb][1] - r0), p2 = ex2(s[nb][2] - r1), p3 = ex2(s[nb][3] - r1);
-      l[0] += p0 + p1;
-      l[1] += p2 + p3;
-      pf[nb >> 1][2 * (nb & 1)] = pack_16<KV8>(p0, p1);
-      pf[nb >> 1][2 * (nb & 1) + 1] = pack_16<KV8>(p2, p3);
+    for (int i = 0; i < kS; ++i) {
+      float e[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) e[x] = ex2(s[i][x] - (second_row(x) ? r1 : r0));
+      l[0] += e[0] + e[NARROW ? 2 : 1];
+      l[1] += e[NARROW ? 1 : 2] + e[3];
+      uint32_t* w = NARROW ? pf[i] : pf[i >> 1] + 2 * (i & 1);
+      w[0] = pack_16<KV8>(e[0], e[1]);
+      w[1] = pack_16<KV8>(e[2], e[3]);
     }
-    // infinities and NaN of V in a page that not every row sees whole: value(token, column block, which of the lane's two columns)
+    // infinities and NaN of V in a page that not every row sees whole: value(token, column block, column of it)
     auto add_odd = [&](int h, auto value) {
       for (int tk = 0; tk < kPage; ++tk) {
-        const int src = (lane & ~3) | (tk & 7) >> 1;
-        const float2 a = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[h][0] : pf[h][2], src));
-        const float2 b = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[h][1] : pf[h][3], src));
-        const float w0 = tk & 1 ? a.y : a.x, w1 = tk & 1 ? b.y : b.x;
+        float w0, w1;
+        if constexpr (NARROW) {
+          const float2 a = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[h][0] : pf[h][1], (tk & 7) << 2 | t));
+          w0 = a.x; w1 = a.y;
+        } else {
+          const int src = (lane & ~3) | (tk & 7) >> 1;
+          const float2 a = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[h][0] : pf[h][2], src));
+          const float2 b = unpack_16<KV8>(__shfl_sync(0xffffffffu, tk < 8 ? pf[h][1] : pf[h][3], src));
+          w0 = tk & 1 ? a.y : a.x; w1 = tk & 1 ? b.y : b.x;
+        }
         const bool sees0 = span_sees(p, tok0[h] + tk, base0, beg0, bits0), sees1 = span_sees(p, tok0[h] + tk, base1, beg1, bits1);
 #pragma unroll
-        for (int db = 0; db < D / 8; ++db) {
+        for (int i = 0; i < kO; ++i) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float v = value(tk, db, e);
+            const float v = NARROW ? value(tk, 2 * i + e, g) : value(tk, i, 2 * t + e);
             if (isfinite(v)) continue;
-            if (sees0) o[db][e] += w0 * v;
-            if (sees1) o[db][2 + e] += w1 * v;
+            if (sees0) o[i][NARROW ? 2 * e : e] += w0 * v;
+            if (sees1) o[i][NARROW ? 2 * e + 1 : 2 + e] += w1 * v;
           }
         }
       }
       __syncwarp();
     };
+    uint32_t pt[kPages][2];
+    if constexpr (NARROW) {
+#pragma unroll
+      for (int h = 0; h < kPages; ++h) { pt[h][0] = transposed(pf[h][0]); pt[h][1] = transposed(pf[h][1]); }
+    }
     if constexpr (KV8) {
       constexpr int kWords = D == 64 ? 2 : 4, kParts = D == 256 ? 2 : 1;
 #pragma unroll
@@ -404,8 +450,8 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
                 w[i][k] &= ~((n >> 7) * 0xFFu);
               }
             if (__any_sync(0xffffffffu, nan) && part == kParts - 1)
-              add_odd(h, [&](int tk, int db, int e) {
-                const int d = dim_of<D>(db, 2 * t + e);
+              add_odd(h, [&](int tk, int db, int col) {
+                const int d = dim_of<D>(db, col);
                 const uint8_t x = v8[tk * D + (((d >> 4) ^ turn_v<D>(tk)) << 4) + (d & 15)];
                 return (x & 0x7F) == 0x7F ? __int_as_float(0x7FC00000) : 0.f;
               });
@@ -414,10 +460,16 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
           for (int k = 0; k < kWords; ++k) {
             const uint2 a = e4m3x4_to_f16(__byte_perm(w[0][k], w[1][k], 0x5140)), b = e4m3x4_to_f16(__byte_perm(w[0][k], w[1][k], 0x7362));
             const uint2 c = e4m3x4_to_f16(__byte_perm(w[2][k], w[3][k], 0x5140)), d = e4m3x4_to_f16(__byte_perm(w[2][k], w[3][k], 0x7362));
-            mma_f16(o[16 * part + 4 * k], pf[h], a.x, c.x);
-            mma_f16(o[16 * part + 4 * k + 1], pf[h], a.y, c.y);
-            mma_f16(o[16 * part + 4 * k + 2], pf[h], b.x, d.x);
-            mma_f16(o[16 * part + 4 * k + 3], pf[h], b.y, d.y);
+            if constexpr (NARROW) {
+              const uint32_t v0[4] = {a.x, a.y, c.x, c.y}, v1[4] = {b.x, b.y, d.x, d.y};
+              mma_f16(o[8 * part + 2 * k], v0, pt[h][0], pt[h][1]);
+              mma_f16(o[8 * part + 2 * k + 1], v1, pt[h][0], pt[h][1]);
+            } else {
+              mma_f16(o[16 * part + 4 * k], pf[h], a.x, c.x);
+              mma_f16(o[16 * part + 4 * k + 1], pf[h], a.y, c.y);
+              mma_f16(o[16 * part + 4 * k + 2], pf[h], b.x, d.x);
+              mma_f16(o[16 * part + 4 * k + 3], pf[h], b.y, d.y);
+            }
           }
         }
       }
@@ -429,7 +481,7 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
 #pragma unroll 4
         for (int i = lane; i < kPage * D / 2; i += 32) odd |= odd_bf16x2(vw[i]);
         if (__any_sync(0xffffffffu, odd)) {
-          add_odd(0, [&](int tk, int db, int e) { return __bfloat162float(tile_ptr<D>(vs, tk, db)[2 * t + e]); });
+          add_odd(0, [&](int tk, int db, int col) { return __bfloat162float(tile_ptr<D>(vs, tk, db)[col]); });
           for (int i = lane; i < kPage * D / 2; i += 32) {
             const uint32_t w = vw[i];
             if (odd_bf16x2(w)) vw[i] = (odd_bf16x2(w & 0xFFFFu) ? 0u : w & 0xFFFFu) | (odd_bf16x2(w & 0xFFFF0000u) ? 0u : w & 0xFFFF0000u);
@@ -441,8 +493,13 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
       for (int db = 0; db < D / 8; db += 2) {
         uint32_t b[4];
         ldsm_x4_t(b, tile_ptr<D>(vs, (j & 1) * 8 + (lane & 7), db + (j >> 1)));
-        mma_bf16(o[db], pf[0], b[0], b[1]);
-        mma_bf16(o[db + 1], pf[0], b[2], b[3]);
+        if constexpr (NARROW) {
+          const uint32_t a[4] = {b[0], b[2], b[1], b[3]};
+          mma_bf16(o[db / 2], a, pt[0][0], pt[0][1]);
+        } else {
+          mma_bf16(o[db], pf[0], b[0], b[1]);
+          mma_bf16(o[db + 1], pf[0], b[2], b[3]);
+        }
       }
     }
     __syncwarp();
@@ -451,8 +508,8 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
   if (bad && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+#pragma unroll
+    for (int x = NARROW ? 4 : 1; x <= (NARROW ? 16 : 2); x *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
   }
   if constexpr (KV8) { m[0] -= kF16Lift; m[1] -= kF16Lift; }
 
@@ -463,8 +520,15 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
   float4* part_ml = reinterpret_cast<float4*>(part_o + kSpanRows * D);      // [16]
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float* row = mo + ((size_t)warp * 16 + g + 8 * h) * D;
-    if constexpr (KV8) {                               // a lane has four neighbouring dims in four neighbouring column blocks
+    const int r = h ? row_b : row_a;
+    float* row = mo + ((size_t)warp * 16 + r) * D;
+    if constexpr (NARROW && KV8) {
+#pragma unroll
+      for (int i = 0; i < kO; i += 2) *reinterpret_cast<float4*>(row + dim_of<D>(2 * i, g)) = make_float4(o[i][h], o[i][2 + h], o[i + 1][h], o[i + 1][2 + h]);
+    } else if constexpr (NARROW) {
+#pragma unroll
+      for (int i = 0; i < kO; ++i) { row[16 * i + g] = o[i][h]; row[16 * i + 8 + g] = o[i][2 + h]; }
+    } else if constexpr (KV8) {                        // a lane has four neighbouring dims in four neighbouring column blocks
 #pragma unroll
       for (int db = 0; db < D / 8; db += 4)
 #pragma unroll
@@ -474,7 +538,7 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
 #pragma unroll
       for (int db = 0; db < D / 8; ++db) *reinterpret_cast<float2*>(row + db * 8 + 2 * t) = make_float2(o[db][2 * h], o[db][2 * h + 1]);
     }
-    if (t == 0) *reinterpret_cast<float2*>(mml + (warp * 16 + g + 8 * h) * 2) = make_float2(m[h], l[h]);
+    if ((NARROW ? g : t) == 0) *reinterpret_cast<float2*>(mml + (warp * 16 + r) * 2) = make_float2(m[h], l[h]);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n_rows * (D / 4); i += 128) {
@@ -589,17 +653,23 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
   for (int e = 0; e < D / 32; ++e) dst[32 * e] = __float2bfloat16(a[e] * inv);
 }
 
-template <int D, bool KV8>
+long long most_rows(const SpanParams& p) { return std::min<long long>((long long)p.max_q_len * p.group, p.rows_to); }
+template <int D, bool KV8, bool NARROW>
 void launch_rows(const SpanParams& p, cudaStream_t s) {
   static bool configured[kMaxDevices] = {};
   if (first_call_on_device(configured))
-    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D, KV8>::kTotal), "span_rows smem");
-  const long long most = (long long)p.max_q_len * p.group < p.rows_to ? (long long)p.max_q_len * p.group : p.rows_to;
+    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D, KV8>::kTotal), "span_rows smem");
+  const long long most = most_rows(p);
   const long long tiles = (most + kSpanRows - 1) / kSpanRows;
   const long long ctas = tiles * p.num_seqs * p.hkv * p.splits;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
-  if (p.in_cluster) launch_cluster(true, span_rows_kernel<D, KV8>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, (unsigned)p.splits, p);
-  else launch_pdl(span_rows_kernel<D, KV8>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, p);
+  if (p.in_cluster) launch_cluster(true, span_rows_kernel<D, KV8, NARROW>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, (unsigned)p.splits, p);
+  else launch_pdl(span_rows_kernel<D, KV8, NARROW>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, p);
+}
+template <int D>
+void launch_rows_of(const SpanParams& p, cudaStream_t s) {
+  if (most_rows(p) <= 8) p.kv_fp8 ? launch_rows<D, true, true>(p, s) : launch_rows<D, false, true>(p, s);
+  else p.kv_fp8 ? launch_rows<D, true, false>(p, s) : launch_rows<D, false, false>(p, s);
 }
 template <int D>
 void launch_merge(const SpanParams& p, bool some, cudaStream_t s) {
@@ -668,9 +738,9 @@ int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStre
     p.rows_from = 0;
     p.rows_to = plan.tile_splits > 0 ? kSpanRows : INT_MAX;
     switch (p.head_dim) {
-      case 64: p.kv_fp8 ? launch_rows<64, true>(p, s) : launch_rows<64, false>(p, s); break;
-      case 128: p.kv_fp8 ? launch_rows<128, true>(p, s) : launch_rows<128, false>(p, s); break;
-      default: p.kv_fp8 ? launch_rows<256, true>(p, s) : launch_rows<256, false>(p, s); break;
+      case 64: launch_rows_of<64>(p, s); break;
+      case 128: launch_rows_of<128>(p, s); break;
+      default: launch_rows_of<256>(p, s); break;
     }
     ++n;
     if (p.splits > 1 && !p.in_cluster) { merge(p, false, s); ++n; }      // (the only kernel then)

@@ -461,6 +461,48 @@ def test_first_nodes_that_lie_far_behind(ops, kv, hq, n):
     assert ops.check_status() == 0
 
 
+# ------------------------------------------------------------------------------------------ up to eight packed rows
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,D", [(8, 1, 64), (6, 2, 128), (4, 4, 256), (7, 1, 128), (2, 2, 64), (16, 2, 256)])
+@pytest.mark.parametrize("n,longest", [(1, 900), (5, 1500), (90, 700), (1, 16000)])
+def test_decode_rows(ops, hq, hkv, D, kv, n, longest):
+    """One row a sequence, some of no row, from one to many splits; places that a row does not see hold NaN."""
+    rows, ctx = [1 if i % 4 != 2 else 0 for i in range(n)], [(i * 397) % longest if i else longest for i in range(n)]
+    c = so.setup(rows, ctx, hq, hkv, D, kv, seed=n + D, fill=float("nan"))
+    for window, first, s, cap in ((50, 3, None, 0.0), (longest // 2, 100, _sinks(hq), 0.0), (1, 1, None, 20.0), (0, 0, None, 0.0) if n == 1 else (33, 40, None, 0.0)):
+        window = window or 1 << 20
+        so.check(_window(ops, c, window, max(first, 1), s, cap), *so.want(c, D ** -0.5, window, max(first, 1), s, cap))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("G,D", [(1, 128), (2, 64), (4, 256), (2, 128)])
+def test_trees_of_few_rows(ops, G, D, kv):
+    """Trees of up to 8 / G nodes: infinities and NaN of a node's values reach the nodes below it and no others; masks of no bits."""
+    nodes = 8 // G
+    par = [-1] + [0] * (nodes - 1)
+    for n, ctx in ((1, 37), (3, 700), (70, 90)):
+        c = so.setup([nodes] * n, [ctx + i for i in range(n)], 2 * G, 2, D, kv, words=1, trees=[par] * n, seed=n, fill=float("nan"))
+        so.check(_tree(ops, c, 60, 5), *so.want(c, D ** -0.5, 60, 5))
+        o, bound = so.want(c, D ** -0.5, 0, 0)
+        so.check(_tree(ops, c), o, bound)
+        tok = c.ctx[n - 1] + 1                          # the last sequence's second node: its own row alone sees it
+        for at, x in ((7, float("nan")), (D - 2, float("inf") if kv == "bf16" else float("nan"))):
+            c.v[int(c.tables[n - 1, tok // 16]), :, tok % 16, at] = x
+        y = _tree(ops, c)
+        mine = (n - 1) * nodes + 1
+        keep = torch.arange(n * nodes, device="cuda") != mine
+        so.check(y[keep], o[keep], bound[keep])
+        got = y[mine].view(2 * G, D).float()
+        assert torch.isnan(got[:, 7]).all() and (torch.isnan(got[:, D - 2]) if kv == "e4m3" else got[:, D - 2] == float("inf")).all()
+        rest = [d for d in range(D) if d not in (7, D - 2)]
+        so.check(y[mine].view(2 * G, D)[:, rest], o[mine].view(2 * G, D)[:, rest], bound[mine].view(2 * G, D)[:, rest])
+        c.masks.zero_()
+        c.base.zero_()
+        assert (_tree(ops, c) == 0).all()
+    assert ops.check_status() == 0
+
+
 # ------------------------------------------------------------------------------------------ the tensor-memory kernel
 # (few rows in all go to the kernel for few rows: what follows is large enough for the other one)
 def _trees(n, nodes, hq, hkv, D, kv="bf16", ctx=700, seed=0, fill=0.0, words=1):
