@@ -69,15 +69,19 @@ class KVCache:
 
     def pools(self) -> List[torch.Tensor]:
         """The pool as [planes, blocks, heads, block_size, width], what the operators that move rows and blocks take."""
-        return [self.store.flatten(0, 1)]
+        return [self.store.flatten(0, 1)] if self.store.shape[0] else []
 
     def copy_blocks(self, pairs, ops) -> None:
         """Blocks (source, destination) of all layers, as if one after the other."""
-        ops.kv_copy_blocks(self.pools(), pairs)
+        pools = self.pools()
+        if pools:                                # a pipeline stage may cache nothing
+            ops.kv_copy_blocks(pools, pairs)
 
     def compact(self, block_tables, base, path, counts, ops) -> None:
         """The accepted rows of draft trees to the places behind their contexts (``ops.kv_compact``)."""
-        ops.kv_compact(self.pools(), block_tables, base, path, counts)
+        pools = self.pools()
+        if pools:
+            ops.kv_compact(pools, block_tables, base, path, counts)
 
     @staticmethod
     def bytes_per_block(num_layers, kv_heads, block_size, head_dim, elem=2) -> int:

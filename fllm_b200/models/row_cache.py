@@ -62,11 +62,15 @@ class RowCache:
 
     def copy_blocks(self, pairs, ops) -> None:
         """Blocks (source, destination) of all layers, as if one after the other."""
-        ops.kv_copy_blocks(self.pools(), pairs)
+        pools = self.pools()
+        if pools:                                # a pipeline stage may cache nothing
+            ops.kv_copy_blocks(pools, pairs)
 
     def compact(self, block_tables, base, path, counts, ops) -> None:
         """The accepted rows of draft trees to the places behind their contexts (``ops.kv_compact``)."""
-        ops.kv_compact(self.pools(), block_tables, base, path, counts)
+        pools = self.pools()
+        if pools:
+            ops.kv_compact(pools, block_tables, base, path, counts)
 
     @staticmethod
     def specs(cfg: ModelConfig, layer_range) -> List[RowSpec]:

@@ -137,3 +137,13 @@ def test_cow_of_a_fork_runs_as_one_copy():
     ops = SimpleNamespace(kv_copy_blocks=lambda pools, pairs: calls.append((len(pools), list(pairs))))
     kv.copy_blocks(ScheduledStep(cow=[(0, 1), (2, 3)]).cow, ops)
     assert calls == [(1, [(0, 1), (2, 3)])]
+
+
+def test_a_stage_without_caches_copies_nothing():
+    from fllm_b200.models.decoder import KVCache
+    from fllm_b200.models.row_cache import RowCache
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32)
+    for kv in (KVCache(0, 4, 2, 16, 64, "cpu"), RowCache([], 4, 16, "cpu")):
+        assert kv.pools() == []
+        kv.copy_blocks([(0, 1), (1, 2)], RefOps())
+        kv.compact(i32([[0, 1]]), i32([3]), i32([[1, 2]]), i32([2]), RefOps())
