@@ -133,9 +133,10 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
   const int split = blockIdx.x - work * p.splits;
   const int kvh = work % p.hkv;
   work /= p.hkv;
-  const int seq = work % p.num_seqs, tile = work / p.num_seqs;
   pdl_launch_dependents();
   pdl_wait();
+  int seq = work % p.num_seqs, tile = work / p.num_seqs;
+  if (p.search && !span_find(p, kSpanRows, 0, p.rows_to, work, blockIdx.x == gridDim.x - 1, seq, tile)) return;
   // (what follows is the same for all splits, which are a cluster where they join in one: all of them leave, or none)
   int q0, qn, kv_len;
   if (!span_lengths(p, seq, threadIdx.x == 0, q0, qn, kv_len)) return;
@@ -661,13 +662,11 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
 
 long long most_rows(const SpanParams& p) { return std::min<long long>((long long)p.max_q_len * p.group, p.rows_to); }
 template <int D, bool KV8, bool NARROW>
-void launch_rows(const SpanParams& p, cudaStream_t s) {
+void launch_rows(SpanParams p, cudaStream_t s) {
   static bool configured[kMaxDevices] = {};
   if (first_call_on_device(configured))
     cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D, KV8>::kTotal), "span_rows smem");
-  const long long most = most_rows(p);
-  const long long tiles = (most + kSpanRows - 1) / kSpanRows;
-  const long long ctas = tiles * p.num_seqs * p.hkv * p.splits;
+  const long long ctas = span_tiles(p, most_rows(p), kSpanRows, p.search) * p.hkv * p.splits;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
   if (p.in_cluster) launch_cluster(true, span_rows_kernel<D, KV8, NARROW>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, (unsigned)p.splits, p);
   else launch_pdl(span_rows_kernel<D, KV8, NARROW>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, p);
@@ -696,10 +695,11 @@ SpanPlan attention_span_plan(const SpanParams& p) {
   // Sequences of more than 16 packed rows go to the tensor-memory kernel, unless all there is to do is less than 28 pages of 16 rows for each SM: its way
   // in and out is longer (one tree of 8, 12, 32 and 64 nodes behind 900 tokens, 32 query and 8 key heads of 128: 10.6, 11.0, 13.9, 20.4 us here, 15.5, 15.6,
   // 16.1, 18.6 there; 12 nodes behind 4000: 19.2 and 18.6).
-  const long long all_tiles = (most + kSpanRows - 1) / kSpanRows * p.num_seqs * p.hkv;
+  bool search;
+  const long long all_tiles = span_tiles(p, most, kSpanRows, search) * p.hkv;
   const bool tc = attention_span_tc_supported(p) && all_tiles * ((span + kPage - 1) / kPage) > 28LL * sm_count();
   if (!tc || (long long)p.min_q_len * p.group <= kSpanRows) {
-    const long long ctas = ((tc ? std::min<long long>(most, kSpanRows) : most) + kSpanRows - 1) / kSpanRows * p.num_seqs * p.hkv;
+    const long long ctas = span_tiles(p, tc ? std::min<long long>(most, kSpanRows) : most, kSpanRows, search) * p.hkv;
     const long long pages = (span + kPage - 1) / kPage;
     // As many splits as leave all CTAs on the SMs at once, a page for each of a CTA's warps at least: a CTA's way in and out is some 5 us (64 sequences
     // under a window of 4096, 8 key heads of 128: 170 us whole, 182 in two, 202 in four; 16 under one of 1024: 24, 17, 24). Up to eight are a
@@ -713,7 +713,7 @@ SpanPlan attention_span_plan(const SpanParams& p) {
   }
   if (tc && most > kSpanRows) {
     // at most four places for a piece to each SM: those that the kernel finds no work for cost a start all the same
-    const long long ctas = (most + 255) / 256 * p.num_seqs * p.hkv, tiles = (span + 127) / 128 + 2;
+    const long long ctas = span_tiles(p, most, 256, search) * p.hkv, tiles = (span + 127) / 128 + 2;
     plan.tile_splits = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(4LL * sm_count() / ctas, tiles), 32));
   }
   plan.bytes = (partial_floats(p, plan.in_cluster ? 1 : plan.rows_splits) + partial_floats(p, plan.tile_splits)) * sizeof(float);

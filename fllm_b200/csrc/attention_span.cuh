@@ -94,6 +94,51 @@ __device__ __forceinline__ bool span_lengths(const SpanParams& p, int seq, bool 
 // factor is below the smallest normal number are below 2^-100, whatever it is.
 __device__ __forceinline__ float span_factor(float scale, int up) { return fmaxf(scale * __uint_as_float((uint32_t)(127 - up) << 23), FLT_MIN); }
 
+// Which sequence's which tile of `unit` rows is the item-th one, sequences of `from` < packed rows <= `to` counted, a sequence's last tile first; by a warp.
+// `report`: lengths that are none to compute with are reported, of all sequences.
+__device__ __forceinline__ bool span_find(const SpanParams& p, int unit, int from, int to, int item, bool report, int& seq, int& tile) {
+  constexpr int kEach = 4;                 // sequences of a lane at a time
+  const int lane = threadIdx.x & 31;
+  bool found = false;
+  for (int s0 = 0; s0 < p.num_seqs && (report || !found); s0 += 32 * kEach) {
+    int mine[kEach], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int s = s0 + lane * kEach + i;
+      int q0, qn = 0, kv_len;
+      if (s < p.num_seqs) span_lengths(p, s, report, q0, qn, kv_len);
+      const int rows = qn * p.group;
+      mine[i] = rows > from && rows <= to ? (rows + unit - 1) / unit : 0;
+      sum += mine[i];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned behind = __ballot_sync(0xffffffffu, item < upto);
+    if (!found && behind) {
+      found = true;
+      int left = item - (upto - sum), at = -1;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (at < 0 && left < mine[i]) {
+          at = i;
+          left = mine[i] - 1 - left;
+        } else if (at < 0) {
+          left -= mine[i];
+        }
+      }
+      const int who = __ffs(behind) - 1;
+      seq = s0 + who * kEach + __shfl_sync(0xffffffffu, at, who);
+      tile = __shfl_sync(0xffffffffu, left, who);
+    }
+    item -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return found;
+}
+
 // Block id of the 16 tokens from 16 * page on, or -1 where the table does not reach or the entry names no block of the pool.
 __device__ __forceinline__ int span_block(const SpanParams& p, const int* table, int page) {
   const int at = page / p.block_pages;

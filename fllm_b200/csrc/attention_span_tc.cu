@@ -448,7 +448,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   // Whole tiles of the longest sequence come first, those that see the most before others; then what is left of the rows. The last `halved` of the whole
   // ones are two CTAs of half the rows each.
   int rest = blockIdx.x, half = -1;
-  const int from_halves = row_tiles * p.num_seqs * p.hkv - halved;
+  const int from_halves = p.search ? INT_MAX / 2 : row_tiles * p.num_seqs * p.hkv - halved;
   if (rest >= from_halves + 2 * halved) {
     rest -= halved;
   } else if (rest >= from_halves) {
@@ -457,7 +457,9 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   }
   const int kvh = rest % p.hkv;
   rest /= p.hkv;
-  const int seq = rest % p.num_seqs, at_tile = rest / p.num_seqs, tile = at_tile < row_tiles ? row_tiles - 1 - at_tile : at_tile;
+  const int at_tile = rest / p.num_seqs;
+  int seq = rest % p.num_seqs, tile = at_tile < row_tiles ? row_tiles - 1 - at_tile : at_tile;
+  if (p.search && !span_find(p, kTcRows, p.rows_from, INT_MAX, rest, blockIdx.x == gridDim.x - 1 && split == 0, seq, tile)) return;
   int q0, qn, kv_len;
   if (!span_lengths(p, seq, threadIdx.x == 0, q0, qn, kv_len)) return;
   const int G = p.group, all_rows = qn * G, row0 = tile * kTcRows + (half > 0 ? kRows : 0);
@@ -902,7 +904,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
 }
 
 template <int D, bool KV8>
-void launch_tc(const SpanParams& p, cudaStream_t s) {
+void launch_tc(SpanParams p, cudaStream_t s) {
   static bool configured[kMaxDevices] = {};
   constexpr int smem = TcSmem<D, KV8>::kTotal;
   static_assert(smem <= 227 * 1024, "shared memory");
@@ -922,8 +924,9 @@ void launch_tc(const SpanParams& p, cudaStream_t s) {
   // Where the last round of whole tiles, and what is left of rows behind it, would leave half of the SMs or more without work, two SMs share each of its
   // tiles by rows. (2 x 2048 rows under a window of 1024, 32 query and 8 key heads of 128, three rounds and 68 tiles: 99 us, 105 without.)
   const long long left = most > row_tiles * kTcRows ? (long long)p.num_seqs * p.hkv : 0;
-  const int last = (int)(whole % p.sms), halved = p.splits == 1 && 2 * last + left <= p.sms ? last : 0;
-  const long long ctas = whole + halved + left;
+  const long long tiles = span_tiles(p, most, kTcRows, p.search);
+  const int last = (int)(whole % p.sms), halved = p.splits == 1 && !p.search && 2 * last + left <= p.sms ? last : 0;
+  const long long ctas = tiles * p.hkv + halved;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
   launch_pdl(span_tc_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(tc_threads<KV8>()), smem, s, mk, mv, p, (int)row_tiles, halved);
 }

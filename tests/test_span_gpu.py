@@ -631,6 +631,46 @@ def test_last_rounds_of_prompts(ops, kv, rows, hq, hkv):
     assert ops.check_status() == 0
 
 
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,D", [(8, 2, 128), (16, 2, 64), (8, 4, 256)])
+@pytest.mark.parametrize("n,at", [(10, [9]), (150, [0, 131]), (400, [128, 255, 399])])
+def test_a_few_prompts_among_many_rows(ops, hq, hkv, D, kv, n, at):
+    """Prompts at the ends of the ranges in which blocks look their sequence up, beside decode rows and sequences of no row."""
+    rows, ctx = [(1, 1, 0, 3, 1)[i % 5] for i in range(n)], [37 * i % 300 for i in range(n)]
+    for k, i in enumerate(at):
+        rows[i] = 700 - 121 * k
+    c = so.setup(rows, ctx, hq, hkv, D, kv, seed=n + D, fill=float("nan"))
+    so.check(_window(ops, c, 100, 5), *so.want(c, D ** -0.5, 100, 5))
+    assert ops.check_status() == 0
+    nodes = [min(r, 100) for r in rows]
+    t = so.setup(nodes, ctx, hq, hkv, D, kv, words=2, trees=[so.grow(m, m) for m in nodes], seed=n, fill=float("nan"))
+    so.check(_tree(ops, t), *so.want(t, D ** -0.5, 0, 0))
+    assert ops.check_status() == 0
+
+
+def test_lengths_that_a_ragged_batch_does_not_announce():
+    from fllm_b200.ops.native import NativeOps
+    mine = NativeOps(torch.device("cuda:0"), 1 << 20)
+    n, at = 300, 140
+    rows = [1] * n
+    rows[at] = 900
+    for D in (128, 256):
+        c = so.setup(rows, [50] * n, 8, 2, D, seed=5)
+        o, bound = so.want(c, D ** -0.5, 60, 5)
+        good = c.meta.q_starts.clone()
+        for s, delta in ((299, 5), (at, -3), (0, -1)):
+            c.meta.q_starts.copy_(good)
+            c.meta.q_starts[s + (s == 299)] += delta
+            y = _window(mine, c, 60, 5)
+            assert mine.check_status() == 3, (D, s)
+        c.meta.q_starts.copy_(good)
+        c.meta.max_q_len = 899
+        y = _window(mine, c, 60, 5)
+        assert mine.check_status() == 3
+        so.check(y[:at], o[:at], bound[:at])
+        so.check(y[at + 900:], o[at + 900:], bound[at + 900:])
+
+
 def test_prompts_in_graphs_and_on_streams(ops):
     """Two captured graphs of the tensor-memory kernel replayed in turn and on two streams at once, then on other lengths."""
     c = so.setup([500, 40, 3], [600, 1100, 2000], 16, 2, 128, seed=12)
