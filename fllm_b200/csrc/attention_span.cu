@@ -117,7 +117,8 @@ template <int D, bool KV8> constexpr int rows_resident() { return D == 256 ? 1 :
 // 8 columns the rows, and nothing is computed for rows 8 to 15. A lane's operands are the same registers in another order; it holds scores of rows 2t and
 // 2t + 1 and tokens g and g + 8 (otherwise rows g and g + 8 and tokens 2t, 2t + 1 of each half). us of decode rows, so and with 16 rows: 48 sequences of an
 // e4m3 cache under 1000 with 130 first tokens, 64 query and 8 key heads of 64: 22.6, 28.8; one under 256, 32 and 8 of 128: 6.3, 6.8; 64 under 4096: 166 both.
-template <int D, bool KV8, bool NARROW>
+// SEARCH: p.search. (Its code in all calls cost the smallest 3 %.)
+template <int D, bool KV8, bool NARROW, bool SEARCH>
 __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel(const __grid_constant__ SpanParams p) {
   using S = RowsSmem<D, KV8>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -136,7 +137,9 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
   pdl_launch_dependents();
   pdl_wait();
   int seq = work % p.num_seqs, tile = work / p.num_seqs;
-  if (p.search && !span_find(p, kSpanRows, 0, p.rows_to, work, blockIdx.x == gridDim.x - 1, seq, tile)) return;
+  if constexpr (SEARCH) {
+    if (!span_find(p, kSpanRows, 0, p.rows_to, work, blockIdx.x == gridDim.x - 1, seq, tile)) return;
+  }
   // (what follows is the same for all splits, which are a cluster where they join in one: all of them leave, or none)
   int q0, qn, kv_len;
   if (!span_lengths(p, seq, threadIdx.x == 0, q0, qn, kv_len)) return;
@@ -663,13 +666,20 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
 long long most_rows(const SpanParams& p) { return std::min<long long>((long long)p.max_q_len * p.group, p.rows_to); }
 template <int D, bool KV8, bool NARROW>
 void launch_rows(SpanParams p, cudaStream_t s) {
+  constexpr int smem = RowsSmem<D, KV8>::kTotal;
   static bool configured[kMaxDevices] = {};
-  if (first_call_on_device(configured))
-    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D, KV8>::kTotal), "span_rows smem");
+  if (first_call_on_device(configured)) {
+    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_rows smem");
+    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_rows smem");
+  }
   const long long ctas = span_tiles(p, most_rows(p), kSpanRows, p.search) * p.hkv * p.splits;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
-  if (p.in_cluster) launch_cluster(true, span_rows_kernel<D, KV8, NARROW>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, (unsigned)p.splits, p);
-  else launch_pdl(span_rows_kernel<D, KV8, NARROW>, dim3((unsigned)ctas), dim3(128), RowsSmem<D, KV8>::kTotal, s, p);
+  auto go = [&](auto kernel) {
+    if (p.in_cluster) launch_cluster(true, kernel, dim3((unsigned)ctas), dim3(128), smem, s, (unsigned)p.splits, p);
+    else launch_pdl(kernel, dim3((unsigned)ctas), dim3(128), smem, s, p);
+  };
+  if (p.search) go(span_rows_kernel<D, KV8, NARROW, true>);
+  else go(span_rows_kernel<D, KV8, NARROW, false>);
 }
 template <int D>
 void launch_rows_of(const SpanParams& p, cudaStream_t s) {

@@ -408,7 +408,7 @@ __device__ __forceinline__ TileSees tile_sees(const SpanParams& p, int q0, int q
   return t;
 }
 
-template <int D, bool KV8>
+template <int D, bool KV8, bool SEARCH>
 __global__ void __launch_bounds__(tc_threads<KV8>(), 1)
 span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ SpanParams p, int row_tiles, int halved) {
   using S = TcSmem<D, KV8>;
@@ -448,7 +448,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   // Whole tiles of the longest sequence come first, those that see the most before others; then what is left of the rows. The last `halved` of the whole
   // ones are two CTAs of half the rows each.
   int rest = blockIdx.x, half = -1;
-  const int from_halves = p.search ? INT_MAX / 2 : row_tiles * p.num_seqs * p.hkv - halved;
+  const int from_halves = SEARCH ? INT_MAX / 2 : row_tiles * p.num_seqs * p.hkv - halved;
   if (rest >= from_halves + 2 * halved) {
     rest -= halved;
   } else if (rest >= from_halves) {
@@ -459,7 +459,9 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   rest /= p.hkv;
   const int at_tile = rest / p.num_seqs;
   int seq = rest % p.num_seqs, tile = at_tile < row_tiles ? row_tiles - 1 - at_tile : at_tile;
-  if (p.search && !span_find(p, kTcRows, p.rows_from, INT_MAX, rest, blockIdx.x == gridDim.x - 1 && split == 0, seq, tile)) return;
+  if constexpr (SEARCH) {
+    if (!span_find(p, kTcRows, p.rows_from, INT_MAX, rest, blockIdx.x == gridDim.x - 1 && split == 0, seq, tile)) return;
+  }
   int q0, qn, kv_len;
   if (!span_lengths(p, seq, threadIdx.x == 0, q0, qn, kv_len)) return;
   const int G = p.group, all_rows = qn * G, row0 = tile * kTcRows + (half > 0 ? kRows : 0);
@@ -908,8 +910,10 @@ void launch_tc(SpanParams p, cudaStream_t s) {
   static bool configured[kMaxDevices] = {};
   constexpr int smem = TcSmem<D, KV8>::kTotal;
   static_assert(smem <= 227 * 1024, "shared memory");
-  if (first_call_on_device(configured))
-    cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
+  if (first_call_on_device(configured)) {
+    cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
+    cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
+  }
   const uint64_t rows = (uint64_t)p.num_blocks * p.hkv * p.block_pages * kPage;
   // encoded for every call: they cost less than looking up by an address what another tensor may since have
   CUtensorMap mk{}, mv{};
@@ -928,7 +932,9 @@ void launch_tc(SpanParams p, cudaStream_t s) {
   const int last = (int)(whole % p.sms), halved = p.splits == 1 && !p.search && 2 * last + left <= p.sms ? last : 0;
   const long long ctas = tiles * p.hkv + halved;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
-  launch_pdl(span_tc_kernel<D, KV8>, dim3((unsigned)ctas, p.splits), dim3(tc_threads<KV8>()), smem, s, mk, mv, p, (int)row_tiles, halved);
+  auto go = [&](auto kernel) { launch_pdl(kernel, dim3((unsigned)ctas, p.splits), dim3(tc_threads<KV8>()), smem, s, mk, mv, p, (int)row_tiles, halved); };
+  if (p.search) go(span_tc_kernel<D, KV8, true>);
+  else go(span_tc_kernel<D, KV8, false>);
 }
 }  // namespace
 
