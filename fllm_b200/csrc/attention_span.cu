@@ -66,12 +66,13 @@ __device__ __forceinline__ void cp_async16_or_zero(void* smem, const void* gmem,
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(there ? 16 : 0) : "memory");
 }
 
-// Four values of a row, normalised with the head's sink.
+// Four values of a row, normalised with the head's sink. (A row that saw nothing has m = -inf and l = 0, not NaN as one of NaN scores: no sink is added to
+// it, where e^(sink - m) of a sink of -inf would be a NaN.)
 template <int D>
 __device__ __forceinline__ void store_row(const SpanParams& p, int q0, int row, int kvh, int d, float4 a, float mm, float ll) {
   const int qi = row / p.group, head = kvh * p.group + row - qi * p.group;
   float c = 1.f;
-  if (p.sinks) {
+  if (p.sinks && (mm != -INFINITY || ll != 0.f)) {
     const float sk = p.sinks[head] * kLog2e, mn = fmaxf(mm, sk);
     c = mm == -INFINITY ? 0.f : ex2(mm - mn);
     ll = ll * c + ex2(sk - mn);
@@ -627,7 +628,8 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
   const float sk = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
   float mm = mine.x;
   for (int s = lane + 32; s < p.splits; s += 32) mm = fmaxf(mm, __ldcg(ml + s).x);
-  mm = fmaxf(warp_max(mm), sk);
+  const float top = warp_max(mm);
+  mm = fmaxf(top, sk);
   float ll = 0.f, a[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) a[e] = 0.f;
@@ -656,7 +658,8 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
       }
     }
   }
-  ll = warp_sum(ll) + (p.sinks ? ex2(sk - mm) : 0.f);
+  ll = warp_sum(ll);
+  if (p.sinks && (top != -INFINITY || ll != 0.f)) ll += ex2(sk - mm);        // (see store_row)
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
   bf16* dst = static_cast<bf16*>(p.out) + (size_t)tok * p.ldo + (size_t)head * D + lane;
 #pragma unroll

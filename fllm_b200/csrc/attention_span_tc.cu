@@ -815,7 +815,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       // shared memory of the warp's own (Q and K have been read) and asks for it to be copied.
       if (!splits) {
         float ll = l, less = 1.f;
-        if (p.sinks && qi >= 0) {
+        if (p.sinks && qi >= 0 && (m_used != -INFINITY || l != 0.f)) {       // (a row that saw nothing stays 0, whatever the sink)
           const float mn = fmaxf(m_used, sink);
           less = m_used == -INFINITY ? 0.f : ex2(m_used - mn);
           ll = ll * less + ex2(sink - mn);

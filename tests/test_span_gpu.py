@@ -799,3 +799,23 @@ def test_served_model_keeps_its_first_tokens():
         kv = KVCache(cfg.num_layers, 20, cfg.num_kv_heads, 16, cfg.head_dim, "cuda")
         logits.append(Decoder(cfg, eng.weights, kv, o, eng.spec).forward(b).float())
     assert (logits[0] - logits[1]).abs().max() <= 0.05 * logits[1].abs().max()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,nodes,ctx", [(2, 2, [3], [200]), (2, 1, [3, 5], [900, 40]), (2, 2, [2], [9500]), (16, 2, [64], [6000]), (32, 8, [33] * 40, [800] * 40)])
+def test_rows_that_see_nothing_have_no_sink_either(ops, hq, hkv, nodes, ctx, kv):
+    """A row that sees nothing is 0 whatever its head's sink is; a sink of -inf, or of a magnitude that log2 e takes to -inf, is none for the others.
+    Few rows whole, in a cluster and over a merge; many rows in pieces and whole."""
+    c = so.setup(nodes, ctx, hq, hkv, 64, kv, words=1, trees=[so.grow(n, n) for n in nodes], seed=hq, fill=float("nan"))
+    blind = [c.starts[s] + n - 1 for s, n in enumerate(nodes)]
+    c.masks[blind] = 0
+    c.base[blind] = 0
+    keep = [i for i in range(sum(nodes)) if i not in blind]
+    low = torch.finfo(torch.float32).min
+    for values in ([-math.inf, low], [low, -math.inf, 1.0, -2.0], [-1e38, math.inf], [math.nan, -math.inf]):
+        s = torch.tensor((values * hq)[:hq], device="cuda")
+        o, bound = so.want(c, 64 ** -0.5, 0, 0, s)
+        y = _tree(ops, c, sinks=s)
+        so.check(y[keep], o[keep], bound[keep])
+        assert (y[blind] == 0).all()
+    assert ops.check_status() == 0
