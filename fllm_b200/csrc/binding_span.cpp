@@ -76,15 +76,18 @@ std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cach
   p.tokens = (int)q.size(0); p.num_seqs = (int)num_seqs;
   p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv); p.head_dim = (int)head_dim;
   p.kv_fp8 = is_e4m3(k_cache);
-  p.max_q_len = (int)std::min<int64_t>(max_q_len, q.size(0)); p.min_q_len = (int)min_q_len; p.max_kv_len = (int)max_kv_len;
+  // No sequence has more rows than there are, and none may be said to have none: one that has more than announced is reported by a kernel.
+  p.max_q_len = (int)std::max<int64_t>(1, std::min<int64_t>(max_q_len, q.size(0)));
+  p.min_q_len = (int)std::min<int64_t>(min_q_len, p.max_q_len); p.max_kv_len = (int)max_kv_len;
   p.reach = (int)std::min<int64_t>(block_tables.size(1) * k_cache.size(2), INT32_MAX / 2 - 4096);
   p.window = (int)window; p.first = window > 0 ? (int)first : 0;
   p.scale = (float)scale; p.scale_log2 = (float)(scale * 1.4426950408889634); p.softcap = (float)softcap;
   c10::cuda::CUDAGuard guard(q.device());
   Tensor out = at::empty({q.size(0), q.size(1)}, q.options());
-  if (p.tokens == 0 || num_seqs == 0 || p.max_q_len == 0) return {out, 0};
+  if (p.tokens == 0 || num_seqs == 0) return {out, 0};
   p.out = out.data_ptr(); p.ldo = out.stride(0);
   const fllm::SpanPlan plan = fllm::attention_span_plan(p);
+  TORCH_CHECK(plan.rows_splits > 0 || plan.tile_splits > 0, "attention: no kernel was planned for the rows");
   Tensor ws;                                  // of this call alone: two streams or two captured graphs do not share it
   if (plan.bytes) ws = at::empty({(int64_t)plan.bytes}, q.options().dtype(at::kByte));
   const int n = fllm::attention_span(p, plan, plan.bytes ? ws.data_ptr() : nullptr, cur_stream());

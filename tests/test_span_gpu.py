@@ -819,3 +819,25 @@ def test_rows_that_see_nothing_have_no_sink_either(ops, hq, hkv, nodes, ctx, kv)
         so.check(y[keep], o[keep], bound[keep])
         assert (y[blind] == 0).all()
     assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows,ctx", [([1], [9000]), ([2, 1], [16000, 8800]), ([1], [40])])
+def test_batches_that_announce_more_rows_than_there_are(ops, rows, ctx, kv):
+    """Every sequence is said to have more rows than the batch has, so that both kernels' rows are spoken for: answered all the same. A batch that is said
+    to have none is answered or reported."""
+    c = so.setup(rows, ctx, 32, 8, 64, kv, seed=sum(ctx))
+    o, bound = so.want(c, 0.125, 20000, 4)
+    for most, least in ((20, 20), (5000, 300), (17, 5)):
+        c.meta.max_q_len, c.meta.min_q_len = most, least
+        torch.full((sum(rows), 32 * 64), math.nan, dtype=torch.bfloat16, device="cuda")        # (what an output would otherwise begin as)
+        so.check(_window(ops, c, 20000, 4), o, bound)
+        assert ops.check_status() == 0
+    c.meta.max_q_len = c.meta.min_q_len = 0
+    y = _window(ops, c, 20000, 4)
+    if max(rows) == 1:
+        so.check(y, o, bound)
+        assert ops.check_status() == 0
+    else:
+        assert ops.check_status() != 0
+    ops.status.zero_()
