@@ -19,7 +19,8 @@
 // power of two per row that puts the row's largest magnitude between 2^14 and 2^15: what a bf16 value loses is below 2^-38 of that magnitude.
 //
 // Values in places that a row does not see may be anything: a weight of zero times a NaN would be a NaN, so in pages that not every row
-// sees whole, infinities and NaN of V are taken out of the tile in front of the product and added to the rows that see them.
+// sees whole, infinities and NaN of V are taken out of the tile in front of the product and added to the rows that see them. Those that a row sees show
+// in its output even where their weight is 0 in 32 bits, whichever part of the walk they are in.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <limits.h>
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
       const float c = ml.x == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : ex2(ml.x - mm);
       const float4 v = *reinterpret_cast<const float4*>(mo + ((size_t)w * 16 + r) * D + d);
       ll += ml.y * c;
-      if (c != 0.f) { a.x += v.x * c; a.y += v.y * c; a.z += v.z * c; a.w += v.w * c; }
+      a.x += v.x * c; a.y += v.y * c; a.z += v.z * c; a.w += v.w * c;      // (a factor of 0 too: 0 x NaN is what one warp would have made of it)
     }
     if (p.splits == 1) {
       store_row<D>(p, q0, row0 + r, kvh, d, a, mm, ll);
@@ -637,7 +638,8 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
     if (s0) mine = s0 + lane < p.splits ? __ldcg(ml + s0 + lane) : make_float2(-INFINITY, 0.f);
     const float w = mine.x == -INFINITY ? (mm == -INFINITY && mine.y != 0.f ? 1.f : 0.f) : ex2(mine.x - mm);
     ll += mine.y * w;
-    unsigned live = __ballot_sync(0xffffffffu, w != 0.f);     // (of the others there are no rows)
+    // A part that saw nothing has no row to read. One whose factor is 0 has: an infinity or a NaN of its values shows as it does within a part.
+    unsigned live = __ballot_sync(0xffffffffu, mine.x != -INFINITY || mine.y != 0.f);
     while (live) {
       int at[4];
       float x[4][D / 32];

@@ -841,3 +841,26 @@ def test_batches_that_announce_more_rows_than_there_are(ops, rows, ctx, kv):
     else:
         assert ops.check_status() != 0
     ops.status.zero_()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,rows,ctx", [(2, [1], [70]), (8, [2], [500]), (2, [1], [9500]), (32, [40], [6000]), (32, [64] * 40, [700] * 40)])
+def test_nan_of_values_with_weights_below_every_number(ops, hq, rows, ctx, kv):
+    """A NaN that a row sees shows wherever its page is summed, though e^x of its score is 0 beside the others': in another warp, split or piece."""
+    c = so.setup(rows, ctx, hq, 2, 64, kv, seed=hq)
+    c.q.fill_(4.0)
+    for s, n in enumerate(ctx):
+        for at, n_at in ((n // 3, 3), (2, 5)):           # (token, dim)
+            tok = torch.arange(c.lens[s], device="cuda")
+            c.keys[s].fill_(4.0)
+            c.keys[s][:n // 2] = -4.0
+            c.values[s][at, :, n_at] = math.nan
+        page = c.tables[s, tok // 16].long()
+        c.k[page, :, tok % 16] = c.keys[s].to(c.k.dtype)
+        c.v[page, :, tok % 16] = c.values[s].to(c.v.dtype)
+    window = max(c.lens)                                 # everything is seen, the first tokens by `first` at the latest
+    y = _window(ops, c, window, 16).view(-1, hq, 64)
+    nan = torch.zeros_like(y, dtype=torch.bool)
+    nan[..., 3] = nan[..., 5] = True
+    assert torch.equal(torch.isnan(y), nan)
+    assert ops.check_status() == 0
