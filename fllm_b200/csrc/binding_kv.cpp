@@ -59,6 +59,25 @@ int64_t kv_copy_blocks(const std::vector<Tensor>& pools, const Tensor& pairs, co
   return n;
 }
 
+// Pairs that the host lists, one behind the other: source, destination, source, ...
+int64_t kv_copy_listed(const std::vector<Tensor>& pools, const std::vector<int64_t>& pairs, const optional<Tensor>& status) {
+  check_pools(pools);
+  TORCH_CHECK(pairs.size() % 2 == 0 && pairs.size() < INT32_MAX, "pairs must be sources and destinations");
+  std::vector<int> of32;
+  of32.reserve(pairs.size());
+  for (const int64_t b : pairs) {
+    TORCH_CHECK(b >= 0 && b < pools[0].size(1), "copy of block ", b, ": the pool has ", pools[0].size(1));
+    of32.push_back((int)b);
+  }
+  int* st = nullptr;
+  if (status.has_value() && status->defined()) { check_ints(*status, pools[0], 1, "status"); st = status->data_ptr<int>(); }
+  c10::cuda::CUDAGuard guard(pools[0].device());
+  int64_t n = 0;
+  for (size_t i = 0; i < pools.size(); i += fllm::kMaxKvPools)
+    n += fllm::kv_copy_listed(make_pools(pools, i), of32.data(), (int)(of32.size() / 2), st, cur_stream());
+  return n;
+}
+
 int64_t kv_compact(const std::vector<Tensor>& pools, const Tensor& block_tables, const Tensor& base, const Tensor& path, const Tensor& counts,
                    const optional<Tensor>& status) {
   check_pools(pools);
@@ -86,5 +105,6 @@ int64_t kv_compact(const std::vector<Tensor>& pools, const Tensor& block_tables,
 
 TORCH_LIBRARY_FRAGMENT(fllm_b200, m) {
   m.def("kv_copy_blocks(Tensor(a!)[] pools, Tensor pairs, Tensor? status=None) -> int", &kv_copy_blocks);
+  m.def("kv_copy_listed(Tensor(a!)[] pools, int[] pairs, Tensor? status=None) -> int", &kv_copy_listed);
   m.def("kv_compact(Tensor(a!)[] pools, Tensor block_tables, Tensor base, Tensor path, Tensor counts, Tensor? status=None) -> int", &kv_compact);
 }

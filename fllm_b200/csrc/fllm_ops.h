@@ -350,7 +350,9 @@ struct KvPools {
   int count, block_size, planes;      // planes: of all pools together
   long long blocks;
 };
-int kv_copy_blocks(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s);
+constexpr int kListedPairs = 96;     // of a launch
+int kv_copy_blocks(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s);       // pairs on the device
+int kv_copy_listed(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s);       // pairs of the host
 int kv_compact(const KvPools& p, const int* block_tables, int max_blocks, const int* base, const int* path, int depth, const int* counts,
                int seqs, int* status, cudaStream_t s);
 

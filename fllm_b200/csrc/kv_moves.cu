@@ -30,6 +30,18 @@ struct SomePools {
 };
 constexpr int kFewPools = 4;
 
+// Pairs (source, destination) in memory of the device, or in the launch itself: what the host lists needs no memory that has to outlive the call, no copy
+// that the host waits for, and a captured graph keeps it. (One listed pair, us a call: 6.4; through a tensor made of the list 19.9, and behind 100 ms of
+// other work as long as that; a copy by PyTorch 8.2.)
+struct PairsAt {
+  const int* at;
+  __device__ __forceinline__ int2 operator()(int i) const { return make_int2(at[2 * i], at[2 * i + 1]); }
+};
+struct PairsListed {
+  int2 pair[kListedPairs];
+  __device__ __forceinline__ int2 operator()(int i) const { return pair[i]; }
+};
+
 template <int N>
 __device__ __forceinline__ const KvPool& pool_of_plane(const SomePools<N>& p, int& plane) {
   int i = 0;
@@ -39,8 +51,8 @@ __device__ __forceinline__ const KvPool& pool_of_plane(const SomePools<N>& p, in
 
 constexpr int kCopyThreads = 256, kCopyEach = 4;       // accesses of a thread, all on their way at once
 
-template <int V, int N>
-__global__ void __launch_bounds__(kCopyThreads) kv_copy_blocks_kernel(const __grid_constant__ SomePools<N> p, const int* pairs, int n, int chunks, int* status) {
+template <int V, int N, class Pairs>
+__global__ void __launch_bounds__(kCopyThreads) kv_copy_blocks_kernel(const __grid_constant__ SomePools<N> p, const __grid_constant__ Pairs pairs, int n, int chunks, int* status) {
   using T = typename Wide<V>::type;
   int plane = blockIdx.x / chunks;
   const int chunk = blockIdx.x - plane * chunks;
@@ -49,7 +61,8 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_blocks_kernel(const __gr
   pdl_launch_dependents();
   pdl_wait();
   for (int i = blockIdx.y; i < n; i += gridDim.y) {
-    const int src = pairs[2 * i], dst = pairs[2 * i + 1];
+    const int2 pair = pairs(i);
+    const int src = pair.x, dst = pair.y;
     if (src < 0 || dst < 0 || src >= p.blocks || dst >= p.blocks) {
       if (threadIdx.x == 0 && status) atomicCAS(status, FLLM_OK, FLLM_ERR_BAD_ARGS);
       continue;
@@ -139,9 +152,9 @@ int access_width(const KvPools& p, bool blocks) {
   }
   return v;
 }
-}  // namespace
 
-int kv_copy_blocks(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s) {
+template <class Pairs>
+int copy_blocks(const KvPools& p, const Pairs& pairs, int n, int* status, cudaStream_t s) {
   if (n <= 0 || p.planes <= 0) return 0;
   const int v = access_width(p, true);
   long long most = 0;
@@ -150,12 +163,27 @@ int kv_copy_blocks(const KvPools& p, const int* pairs, int n, int* status, cudaS
   if (chunks * p.planes > 0x7fffffffLL) throw std::runtime_error("kv_copy_blocks: pools too large");
   const dim3 grid((unsigned)(chunks * p.planes), (unsigned)min(n, 65535));
   auto go = [&](auto kernel, auto pools) { launch_pdl(kernel, grid, dim3(kCopyThreads), 0, s, pools, pairs, n, (int)chunks, status); };
-  if (v == 16 && p.count <= kFewPools) go(kv_copy_blocks_kernel<16, kFewPools>, SomePools<kFewPools>(p));
-  else if (v == 16) go(kv_copy_blocks_kernel<16, kMaxKvPools>, SomePools<kMaxKvPools>(p));
-  else if (v == 4) go(kv_copy_blocks_kernel<4, kMaxKvPools>, SomePools<kMaxKvPools>(p));
-  else go(kv_copy_blocks_kernel<1, kMaxKvPools>, SomePools<kMaxKvPools>(p));
+  if (v == 16 && p.count <= kFewPools) go(kv_copy_blocks_kernel<16, kFewPools, Pairs>, SomePools<kFewPools>(p));
+  else if (v == 16) go(kv_copy_blocks_kernel<16, kMaxKvPools, Pairs>, SomePools<kMaxKvPools>(p));
+  else if (v == 4) go(kv_copy_blocks_kernel<4, kMaxKvPools, Pairs>, SomePools<kMaxKvPools>(p));
+  else go(kv_copy_blocks_kernel<1, kMaxKvPools, Pairs>, SomePools<kMaxKvPools>(p));
   cuda_check(cudaGetLastError(), "kv_copy_blocks launch");
   return 1;
+}
+static_assert(sizeof(SomePools<kMaxKvPools>) + sizeof(PairsListed) + 32 <= 4096, "a kernel's parameters");
+}  // namespace
+
+int kv_copy_blocks(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s) { return copy_blocks(p, PairsAt{pairs}, n, status, s); }
+
+int kv_copy_listed(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s) {
+  int launches = 0;
+  for (int i = 0; i < n; i += kListedPairs) {
+    PairsListed some{};
+    const int here = min(n - i, kListedPairs);
+    for (int k = 0; k < here; ++k) some.pair[k] = make_int2(pairs[2 * (i + k)], pairs[2 * (i + k) + 1]);
+    launches += copy_blocks(p, some, here, status, s);
+  }
+  return launches;
 }
 
 int kv_compact(const KvPools& p, const int* block_tables, int max_blocks, const int* base, const int* path, int depth, const int* counts,

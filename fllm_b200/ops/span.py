@@ -118,12 +118,13 @@ class SpanNative:
     def kv_copy_blocks(self, pools, pairs):
         """Blocks ``pairs[i][0]`` of all planes to ``pairs[i][1]``. A host list is carried out as if pair after pair; an int32 tensor [n, 2] on the
         device in one launch: it names no block as a destination twice, or as a source and a destination (pairs out of range are skipped and
-        reported in ``status``)."""
+        reported in ``status``). Both are queued without waiting for the stream, and may be captured: a graph keeps the pairs of a list, and
+        reads those of a tensor when it is replayed."""
         if isinstance(pairs, torch.Tensor):
             self.launches += self.k.kv_copy_blocks(pools, pairs, self.status)
             return
         for g in ordered_copies(pairs, pools[0].shape[1] if pools else 0):
-            self.launches += self.k.kv_copy_blocks(pools, torch.tensor(g, dtype=torch.int32).to(pools[0].device), self.status)
+            self.launches += self.k.kv_copy_listed(pools, [b for pair in g for b in pair], self.status)
 
     def kv_compact(self, pools, block_tables, base, path, counts):
         """For every sequence b the row of position ``base[b] + path[b, i]`` to position ``base[b] + i``, for i < counts[b], in this order: what is

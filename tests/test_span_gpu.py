@@ -864,3 +864,47 @@ def test_nan_of_values_with_weights_below_every_number(ops, hq, rows, ctx, kv):
     nan[..., 3] = nan[..., 5] = True
     assert torch.equal(torch.isnan(y), nan)
     assert ops.check_status() == 0
+
+
+def test_a_list_of_copies_does_not_wait_for_the_stream(ops):
+    """The copies of a host list are queued behind what the stream has to do, however often; their source is read when they run."""
+    pool = torch.zeros(4, 64, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    pool[:, 0] = 1
+    ops.kv_copy_blocks([pool], [(0, 1)])
+    a = torch.randn(8192, 8192, device="cuda")
+    torch.cuda.synchronize()
+    b = a
+    for _ in range(6):                                 # some 100 ms in fp32
+        b = a @ a
+    pool[:, 2] = b[0, 0].bfloat16()
+    for i in range(40):
+        ops.kv_copy_blocks([pool], [(2, 3 + i), (3 + i, 60)])
+    done = torch.cuda.Event()
+    done.record()
+    assert not done.query(), "the call waited for the stream"
+    torch.cuda.synchronize()
+    assert all(torch.equal(pool[:, i], pool[:, 2]) for i in list(range(3, 43)) + [60])
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kind,n", [("kv", 1), ("kv", 96), ("rows", 97), ("odd", 200), ("many", 250)])
+def test_lists_of_many_copies(ops, kind, n):
+    """More pairs than a launch holds, chains among them, and the same list from a captured graph."""
+    from fllm_b200.ops.reference import RefOps
+    pools = _pools(kind, 2 * n + 3)
+    pairs = [(2 * i, 2 * i + 1) for i in range(n)] + [(1, 2 * n), (2 * n, 2 * n + 2)]
+    for graph in (False, True):
+        ref = [t.clone() for t in pools]
+        RefOps().kv_copy_blocks(ref, pairs)
+        if graph:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                ops.kv_copy_blocks(pools, list(pairs))
+            g.replay()
+        else:
+            ops.kv_copy_blocks(pools, pairs)
+        torch.cuda.synchronize()
+        assert _same(pools, ref)
+        for t in pools:                                # other sources for the graph
+            t[:, 0:2 * n:2] = t[:, 1:2 * n:2].flip(1)
+    assert ops.check_status() == 0
