@@ -278,6 +278,17 @@ class BlockManager:
         sb.first_live_block = max(sb.first_live_block, first_needed)
         return freed
 
+    def drop_absent(self, seq_id: int, live: Iterable[int], num_tokens: int) -> None:
+        """Of a fresh table's blocks of the first `num_tokens` tokens, give back those that are not among `live`: a
+        sequence that comes back from elsewhere has nothing to put there, and what they hold is not its text."""
+        sb = self.seqs[seq_id]
+        live = set(live)
+        for i in range(self.blocks_needed(num_tokens)):
+            if i not in live and sb.table[i] >= 0:
+                self._release(sb.table[i])
+                sb.table[i] = -1
+                sb._np_dirty = True
+
     def truncate(self, seq_id: int, new_total: int) -> None:
         """Roll back KV past `new_total` tokens (rejected speculative tokens)."""
         sb = self.seqs[seq_id]

@@ -316,6 +316,7 @@ class LLMEngine:
         if live:
             dst = torch.tensor([table[i] for i in live], dtype=torch.long, device=self.device)
             self.kv.store.index_copy_(2, dst, kv.to(self.device))
+        self.blocks.drop_absent(req.seq_id, live, n)            # before their hashes are registered
         self.blocks.commit_tokens(req.seq_id, req.all_tokens, n, params.cache_salt.encode())
         req.status = RequestStatus.RUNNING
         self.scheduler.running.append(req)
@@ -1175,6 +1176,7 @@ class _KvSwapper:
         if live:
             dst = torch.tensor([table[i] for i in live], dtype=torch.long, device=eng.device)
             eng.kv.store.index_copy_(2, dst, host.to(eng.device, non_blocking=False))
+        eng.blocks.drop_absent(req.seq_id, live, req.num_computed)
         self.stats["swapped_in"] += 1
 
     def drop(self, req) -> None:

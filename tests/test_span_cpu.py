@@ -147,3 +147,51 @@ def test_a_stage_without_caches_copies_nothing():
         assert kv.pools() == []
         kv.copy_blocks([(0, 1), (1, 2)], RefOps())
         kv.compact(i32([[0, 1]]), i32([3]), i32([[1, 2]]), i32([2]), RefOps())
+
+
+@pytest.mark.parametrize("first", [0, 20])
+@pytest.mark.parametrize("how", ["import", "swap"])
+def test_blocks_freed_behind_a_window_stay_absent_when_the_sequence_comes_back(first, how):
+    """A sequence that is handed over, or comes back from the host, has holes where its window had passed. Fresh blocks hold other text there, which
+    must not be found under this text's name."""
+    from fllm_b200.config import EngineConfig, preset
+    from fllm_b200.runtime import LLMEngine, SamplingParams
+    from fllm_b200.runtime.scheduler import ScheduledStep
+    cfg = preset("qwen3-tiny")
+    cfg.sliding_window, cfg.window_first = 24, first
+    make = lambda: LLMEngine(cfg, EngineConfig(max_num_seqs=4, num_kv_blocks=64, max_model_len=256, preemption="swap"), device="cpu")
+    prompt = [(7 * i) % 50 + 1 for i in range(120)]
+    other = prompt[:70] + [3, 9, 4]
+    params = SamplingParams(max_tokens=6)
+    want = [make().generate([p], params)[0] for p in (prompt, other)]
+    eng = make()
+    if how == "import":
+        blob, _ = eng.prefill_only(prompt, params)
+        eng = make()
+        eng.kv.store.normal_()                          # blocks that were others' before
+        rid = eng.import_request(blob)
+        live = blob["live_blocks"]
+    else:
+        rid = eng.add_request(prompt, params)
+        while not eng.requests[rid].output:
+            eng.step()
+        eng.drain()
+        assert eng.scheduler._preempt_one(ScheduledStep(), None) and eng.requests[rid].swapped
+        live = eng.scheduler.swapper.parked[eng.requests[rid].seq_id][1]
+        eng.blocks.reset_prefix_cache()
+        eng.kv.store.normal_()
+        eng.step()
+        eng.drain()
+    r = eng.requests[rid]
+    head = -(-first // 16)
+    assert live == list(range(head)) + [6, 7]
+    table = eng.blocks.table(r.seq_id)
+    assert [i for i, b in enumerate(table) if b >= 0] == live and eng.blocks.num_used() == len(live)
+    assert eng.blocks.np_table(r.seq_id).tolist() == table
+    got = {}
+    follow = eng.add_request(other, params)
+    while eng.has_unfinished():
+        for e in eng.step():
+            got.setdefault(e.request_id, []).extend(e.token_ids)
+    assert got[follow] == want[1] and r.output == want[0]
+    assert eng.blocks.num_used() == 0
