@@ -297,7 +297,17 @@ class ModelConfig:
 
     @classmethod
     def from_hf_config(cls, hf: Dict[str, Any]) -> "ModelConfig":
-        """Map a ``config.json`` (Hugging Face keys, or those of a native design) to the decoder description."""
+        """Map a ``config.json`` (Hugging Face keys, or those of a native design) to the decoder description. ``window_first``, a key of this
+        project, may stand beside those of any model: so many first tokens stay visible behind its windows."""
+        cfg = cls._from_hf_keys(hf)
+        inner = hf.get("text_config")
+        cfg.window_first = int(hf.get("window_first", inner.get("window_first") if isinstance(inner, dict) else 0) or 0)
+        if cfg.window_first < 0:
+            raise ValueError("window_first must not be negative")
+        return cfg
+
+    @classmethod
+    def _from_hf_keys(cls, hf: Dict[str, Any]) -> "ModelConfig":
         if hf.get("architecture") == "Sovanex":
             return sovanex_from_config(cls, hf)
         if hf.get("architecture") == "Divanex":

@@ -98,8 +98,13 @@ def config_from_gguf(r: GgufReader) -> ModelConfig:
                               truncate=bool(m.get("fllm.rope.yarn_truncate", True)), attn_factor=m.get("fllm.rope.yarn_attn_factor"))
     elif "rope_freqs.weight" in r.tensors:         # one divisor per frequency (Llama-3 style scaling, stored as a tensor)
         scaling = RopeScaling(kind="factors", freq_factors=[float(v) for v in r.tensor_f32("rope_freqs.weight").reshape(-1)])
+    windows = {}
+    if int(m.get("fllm.attention.window_first", 0)):      # written together with the window and its layers
+        pattern = m.get("fllm.attention.window_pattern")
+        windows = dict(sliding_window=int(g("attention.sliding_window")), window_first=int(m["fllm.attention.window_first"]),
+                       window_pattern=[int(v) for v in pattern] if pattern is not None else None)
     return ModelConfig(
-        rope_scaling=scaling, rotary_dim=int(rot) if rot is not None and int(rot) != head_dim else None,
+        **windows, rope_scaling=scaling, rotary_dim=int(rot) if rot is not None and int(rot) != head_dim else None,
         arch="llama" if arch not in ("qwen3", "gpt_oss") else arch, name=str(m.get("general.name", arch)),
         vocab_size=int(vocab), hidden_size=hidden, num_layers=int(g("block_count")), num_heads=heads,
         num_kv_heads=int(g("attention.head_count_kv", heads)), head_dim=int(g("attention.key_length", hidden // heads)),
@@ -116,6 +121,8 @@ class CpuEngine:
         self.reader = GgufReader(gguf_path)
         self.cfg = config_from_gguf(self.reader)
         c = self.cfg
+        if c.window_first:
+            raise ValueError("the CPU engine attends to the whole text: it has no windows with first tokens")
         self.block_size, self.num_blocks = block_size, num_blocks
         cc = _CpuConfig(c.num_layers, c.hidden_size, c.num_heads, c.num_kv_heads, c.head_dim, c.intermediate_size,
                         c.vocab_size, block_size, num_blocks, 0 if c.rope_style == "neox" else 1,

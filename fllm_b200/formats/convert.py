@@ -144,6 +144,10 @@ def convert_checkpoint(directory: str, out_path: str, out_type: str = "F16") -> 
         w.add(f"{arch}.expert_used_count", int(cfg.experts_per_token))
     if cfg.sliding_window:
         w.add(f"{arch}.attention.sliding_window", int(cfg.sliding_window))
+        if cfg.window_first:
+            w.add("fllm.attention.window_first", int(cfg.window_first))
+            if cfg.window_pattern is not None:
+                w.add("fllm.attention.window_pattern", [int(v) for v in cfg.window_pattern])
     w.add(f"{arch}.attention.layer_norm_rms_epsilon", float(cfg.rms_eps))
     w.add(f"{arch}.rope.freq_base", float(cfg.rope_theta))
     w.add("fllm.rope_style", 0 if cfg.rope_style == "neox" else 1)

@@ -157,3 +157,39 @@ def test_block_codecs_round_trip(name, tol):
     gguf = pytest.importorskip("gguf")            # bit-exact against the format's own numpy decoder when it is installed
     ref = gguf.quants.dequantize(packed, getattr(gguf.GGMLQuantizationType, name))
     assert np.array_equal(ref.astype(np.float32), y)
+
+
+@pytest.mark.parametrize("pattern", [None, [1, 0]])
+def test_convert_keeps_the_first_tokens_of_a_window(hf_dir, tmp_path, pattern):
+    """`window_first` beside a checkpoint's keys reaches the model, and the converted file serves the same tokens as the directory."""
+    from fllm_b200.config import EngineConfig
+    from fllm_b200.cpu_engine import CpuEngine
+    from fllm_b200.runtime import LLMEngine, SamplingParams
+    d, _ = hf_dir
+    d2 = str(tmp_path / "windowed")
+    os.makedirs(d2)
+    os.symlink(os.path.join(d, "model.safetensors"), os.path.join(d2, "model.safetensors"))
+    hf = json.load(open(os.path.join(d, "config.json")))
+    hf.update(sliding_window=24, use_sliding_window=True)
+    if pattern:
+        hf["layer_types"] = ["sliding_attention" if pattern[i % 2] else "full_attention" for i in range(hf["num_hidden_layers"])]
+    prompt = [(7 * i) % 50 + 1 for i in range(90)]
+    out = {}
+    for first in (0, 20):
+        json.dump(dict(hf, window_first=first), open(os.path.join(d2, "config.json"), "w"))
+        gguf = str(tmp_path / f"first{first}.gguf")
+        convert_checkpoint(d2, gguf, "BF16")
+        for what, (cfg, w, _) in dict(hf=load_hf_checkpoint(d2, "cpu"), gguf=load_gguf(gguf, "cpu")).items():
+            if first:
+                assert (cfg.window_first, cfg.sliding_window) == (first, 24) and [cfg.layer_window(i) for i in range(cfg.num_layers)] == [
+                    24 if pattern is None or pattern[i % 2] else 0 for i in range(cfg.num_layers)]
+            else:
+                assert cfg.window_first == 0
+            eng = LLMEngine(cfg, EngineConfig(max_num_seqs=1, num_kv_blocks=16, max_model_len=128), weights=w, device="cpu")
+            out[what, first] = eng.generate([prompt], SamplingParams(max_tokens=6))
+    assert out["hf", 20] == out["gguf", 20] != out["hf", 0]
+    with pytest.raises(ValueError):
+        CpuEngine(gguf)
+    json.dump(dict(hf, window_first=-1), open(os.path.join(d2, "config.json"), "w"))
+    with pytest.raises(ValueError):
+        load_hf_checkpoint(d2, "cpu")
