@@ -149,8 +149,9 @@ class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNa
         """bidirectional: no causal mask (encoders); `positions` must then hold the last position of each row's
         sequence (the generic kernel's visibility limit), the tensor-core kernels take the flag. `first`: so many tokens
         at the start of the text stay visible when the window has moved past them (causal, with `meta`; the rows of a
-        sequence are its last ones)."""
-        if first or window < 0:
+        sequence are its last ones; head dims 64, 128 and 256, blocks of a multiple of 16 tokens). No window: 0, or, without
+        `first`, any negative one."""
+        if first:
             _check_span(window, first, bidirectional)
         if first and window:
             return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta)
@@ -211,7 +212,6 @@ class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNa
         if meta is not None:
             return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta,
                                         tree_mask, tree_base)
-        _check_span(window, first)
         if first:
             raise ValueError("attention_tree: first tokens need the step batch (meta)")
         out = torch.empty(q.shape[0], hq * head_dim, dtype=q.dtype, device=q.device)

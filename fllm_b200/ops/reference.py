@@ -124,7 +124,7 @@ class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef, SpanRef):
                   scale, window=0, sinks=None, softcap=0.0, meta=None, bidirectional=False, first=0):
         """`positions[t]` is the last visible token of row t: a causal decoder passes the row's own position, an
         encoder (bidirectional) the last position of the row's sequence. `first`: so many tokens at the start of the
-        text stay visible when the window has moved past them."""
+        text stay visible when the window has moved past them. (A negative window, which the kernels take as none, is refused here.)"""
         _check_span(window, first, bidirectional)
         if first and window:
             return self.attention_first(q, k_cache, v_cache, block_tables, row_seq, positions, hq, hkv, head_dim, scale, window, first,
@@ -182,8 +182,8 @@ class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef, SpanRef):
                        head_dim, scale, window=0, sinks=None, softcap=0.0, first=0, meta=None):
         """Rows are nodes of draft trees: the context plus the ancestors named by a 64-bit mask per row (with `meta`: by one
         or more words, under a window and first tokens)."""
-        _check_span(window, first)
         if meta is not None:
+            _check_span(window, first)
             return self.attention_tree_span(q, k_cache, v_cache, block_tables, tree_mask, tree_base, hq, hkv, head_dim, scale, window,
                                             sinks, softcap, first, meta)
         if first:

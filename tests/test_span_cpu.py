@@ -195,3 +195,12 @@ def test_blocks_freed_behind_a_window_stay_absent_when_the_sequence_comes_back(f
             got.setdefault(e.request_id, []).extend(e.token_ids)
     assert got[follow] == want[1] and r.output == want[0]
     assert eng.blocks.num_used() == 0
+
+
+def test_trees_without_a_step_batch_take_any_window_below_one():
+    c = so.setup([5], [9], 2, 2, 64, device="cpu", words=1, trees=[so.grow(5, 1)])
+    tree = lambda **kw: RefOps().attention_tree(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.masks.view(-1), c.base, 2, 2, 64, 0.125, **kw)
+    assert torch.equal(tree(window=-3), tree())
+    for kw in (dict(first=-1), dict(first=2), dict(window=-3, meta=c.meta)):
+        with pytest.raises(ValueError):
+            tree(**kw)

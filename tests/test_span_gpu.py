@@ -908,3 +908,17 @@ def test_lists_of_many_copies(ops, kind, n):
         for t in pools:                                # other sources for the graph
             t[:, 0:2 * n:2] = t[:, 1:2 * n:2].flip(1)
     assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [[1, 1], [40, 3]])
+def test_windows_below_zero_are_none(ops, rows, kv):
+    """Without first tokens, and for trees without a step batch, a negative window is no window."""
+    c = so.setup(rows, [300, 77], 8, 2, 128, kv, seed=3)
+    for meta in (c.meta, None):
+        call = lambda window: ops.attention(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, 8, 2, 128, 128 ** -0.5, window, meta=meta)
+        assert torch.equal(call(-1), call(0))
+    t = so.setup(rows, [300, 77], 8, 2, 128, words=1, trees=[so.grow(n, n) for n in rows], seed=4)
+    tree = lambda window: ops.attention_tree(t.q, t.k, t.v, t.tables, t.row_seq, t.positions, t.masks.view(-1), t.base, 8, 2, 128, 128 ** -0.5, window)
+    assert torch.equal(tree(-7), tree(0))
+    assert ops.check_status() == 0
