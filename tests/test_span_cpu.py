@@ -204,3 +204,55 @@ def test_trees_without_a_step_batch_take_any_window_below_one():
     for kw in (dict(first=-1), dict(first=2), dict(window=-3, meta=c.meta)):
         with pytest.raises(ValueError):
             tree(**kw)
+
+
+def test_a_forked_sequence_writes_into_a_block_of_its_own():
+    """Two sequences share a partly filled block and go on with different tokens: the engine's step copies it for one of them, both read what they would
+    have alone."""
+    import copy
+    from fllm_b200.config import EngineConfig, preset
+    from fllm_b200.runtime import LLMEngine, SamplingParams
+    cfg = preset("qwen3-tiny")
+    make = lambda: LLMEngine(cfg, EngineConfig(max_num_seqs=4, num_kv_blocks=64, max_model_len=256), device="cpu")
+    prompt = [(7 * i) % 50 + 1 for i in range(40)]
+    params = SamplingParams(max_tokens=8)
+
+    def start(eng):
+        rid = eng.add_request(prompt, params)
+        r = eng.requests[rid]
+        while len(r.output) < 2:
+            eng.step()
+        eng.drain()
+        return r
+    want = []
+    for turn in (0, 1):                                  # alone: the first as it is, the second with another last token
+        eng = make()
+        r = start(eng)
+        if turn:
+            r.output[-1] = 17
+        while eng.has_unfinished():
+            eng.step()
+        want.append(list(r.output))
+    eng = make()
+    parent = start(eng)
+    child = copy.copy(parent)
+    child.request_id, child.seq_id, child.output = "child", next(eng._seq_ids), list(parent.output)
+    child.output[-1] = 17
+    eng.blocks.fork(parent.seq_id, child.seq_id)
+    eng.scheduler.running.append(child)
+    eng.requests["child"] = child
+    shared = list(eng.blocks.table(parent.seq_id))
+    assert parent.num_computed % 16 and shared == eng.blocks.table(child.seq_id)
+    calls = []
+    copies = eng.ops.kv_copy_blocks
+    eng.ops.kv_copy_blocks = lambda pools, pairs: (calls.append((len(pools), list(pairs))), copies(pools, pairs))
+    eng.step()
+    eng.drain()
+    tables = [eng.blocks.table(r.seq_id) for r in (parent, child)]
+    (pools, ((src, dst),)), = calls
+    assert pools == 1 and eng.blocks.stats["cow"] == 1 and src == shared[-1] and {src, dst} == {t[len(shared) - 1] for t in tables}
+    assert all(t[:len(shared) - 1] == shared[:-1] for t in tables)
+    while eng.has_unfinished():
+        eng.step()
+    assert [parent.output, child.output] == want and want[0] != want[1] and len(calls) == 1
+    assert eng.blocks.num_used() == 0
