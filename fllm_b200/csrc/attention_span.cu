@@ -9,12 +9,13 @@
 // those of up to eight splits in that of their cluster, of more by span_merge_kernel. Sequences with more than 16 packed rows go to attention_span_tc.cu
 // where that has a kernel, and enough to do.
 //
-// What bounds it: memory, where there is enough to read (one row of 64 sequences under a window of 4096, 32 query and 8 key heads of 128: 166 us, 6.5 TB/s);
+// What bounds it (times of passes in a captured graph, where the host is not waited for; a single call of a few us is some 4 us longer): memory, where there
+// is enough to read (one row of 64 sequences under a window of 4096, 32 query and 8 key heads of 128: 169 us, 6.4 TB/s);
 // a CTA's way in and out, some 5 us, where there is little (one sequence, a window of 256: 6.3 us); in between the latency of each warp's chain of
 // products, maxima and exponentials, of which ten warps an SM hide less than half (48 sequences of an e4m3 cache under 1000 with 130 first tokens, 64 query
 // and 8 key heads of 64: 22.6 us, 2.5 TB/s).
 //
-// Scores and sums are fp32. Weights are rounded to the operands' 16 bits for the product with the values (bf16, at most 2^-9 each and of
+// Scores and sums are fp32. Weights are rounded to the operands' 16 bits for the product with the values (bf16, at most 2^-8 of each and of
 // either sign; f16 beside an e4m3 cache). An e4m3 cache is widened to f16, which holds all of its values; queries are f16 there as well, times a
 // power of two per row that puts the row's largest magnitude between 2^14 and 2^15: what a bf16 value loses is below 2^-38 of that magnitude.
 //

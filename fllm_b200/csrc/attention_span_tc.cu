@@ -13,7 +13,7 @@
 //   bf16 cache    warps 8, 10 ask for K by TMA, warp 11 for V; it also looks through V where not every row sees the whole tile
 //   e4m3 cache    K is an operand as it is, with queries in two e4m3 pieces; V travels as f16: warp 8 asks for both, warps 10 - 15 widen V
 //
-// What bounds it: two tiles of 128 x 128 scores take the softmax groups some 3200 clocks, the tensor pipe 2048 at heads of 128; and a CTA's way in (lengths,
+// What bounds it (times from captured graphs): two tiles of 128 x 128 scores take the softmax groups some 3200 clocks, the tensor pipe 2048 at heads of 128; and a CTA's way in (lengths,
 // table, queries, keys, first products: 9000 clocks) and out (4000), which nothing on its SM runs under. 2 x 2048 rows behind 4096 tokens without a window, 32
 // query and 8 key heads of 128: 1097 TFLOP/s, e4m3 1007; under a window of 1024 with 64 first tokens 735, of the products that the window leaves. (CTAs
 // that stay and take item after item hid the way in, but missed the instruction cache 7000 times an SM for 2800: 146 us for 115 at that
@@ -269,7 +269,7 @@ __device__ __forceinline__ void load_q(const SpanParams& p, int tid, uint8_t* sq
 #pragma unroll
         for (int o = C / 2; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
         const int top = (int)(max(most & 0xFFFFu, most >> 16) >> 7);      // largest exponent field of the row
-        const bool odd = top == 0xFF;                  // an infinity or a NaN: no score of the row is a number
+        const bool odd = top == 0xFF;                  // an infinity or a NaN: no score of the row is a number (a soft-cap would make 1 of an infinite one: NaN here)
         const int up = odd ? 0 : min(127 + 7 - top, 126);
         const float f = odd ? __int_as_float(0x7FC00000) : __uint_as_float((uint32_t)(127 + up) << 23);
         uint32_t high[2] = {0, 0}, low[2] = {0, 0};
@@ -355,7 +355,7 @@ __device__ __forceinline__ uint32_t without_odd_f16(uint32_t w) {
 // SMs is the number of SMs that it could keep; a piece costs a start, partial sums and their way through memory, so that is rounded down, but for
 // items that would hold two SMs almost. us of 32 query and 8 key heads of 128: 16 trees of 64 nodes behind 6000 tokens: 107 in one piece each,
 // 137 in two, 161 in four; 4 of 32: 67 in one, 36 in four, 49 in six; 16 of 64 behind 1000 to 12,000: 182 in one each, 201 in pieces of up to 13 tiles,
-// 157 by this rule, 172 where two pieces begin at 1.35 SMs.
+// 157 by this rule, 172 where two pieces begin at 1.35 SMs (from captured graphs, before the last steps: 152 by the rule since).
 __device__ __forceinline__ int tiles_of(const SpanParams& p, int qn, int kv_len) {
   const int tiles = max((kv_len + kTile - 1) / kTile, 1);
   return p.window > 0 ? (int)min((long long)tiles, ((long long)p.window + p.first + min(qn, kTcRows / p.group + 2) + 2 * kPage) / kTile + 1) : tiles;

@@ -81,7 +81,7 @@ std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cach
   p.min_q_len = (int)std::min<int64_t>(min_q_len, p.max_q_len); p.max_kv_len = (int)max_kv_len;
   p.reach = (int)std::min<int64_t>(block_tables.size(1) * k_cache.size(2), INT32_MAX / 2 - 4096);
   p.window = (int)window; p.first = window > 0 ? (int)first : 0;
-  p.scale = (float)scale; p.scale_log2 = (float)(scale * 1.4426950408889634); p.softcap = (float)softcap;
+  p.scale_log2 = (float)(scale * 1.4426950408889634); p.softcap = (float)softcap;
   c10::cuda::CUDAGuard guard(q.device());
   Tensor out = at::empty({q.size(0), q.size(1)}, q.options());
   if (p.tokens == 0 || num_seqs == 0) return {out, 0};

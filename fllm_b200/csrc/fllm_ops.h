@@ -310,7 +310,7 @@ struct SpanParams {
   int max_q_len, min_q_len, max_kv_len;
   int reach;                   // tokens that a row of block_tables has room for
   int window, first;           // window 0: no limit (first is 0 then)
-  float scale, scale_log2, softcap;
+  float scale_log2, softcap;   // of the scores, to base 2; 0: no soft-cap
   // set by the planner, for one kernel
   int splits, min_pages, sms;  // pieces of what a sequence's rows see, at most; fewest pages in one; SMs
   bool in_cluster;             // the pieces join in a cluster
