@@ -28,60 +28,17 @@
 
 #include <algorithm>
 
-#include "attention_span.cuh"
+#include "attention_span_rows.cuh"
 #include "attention_util.cuh"
 #include "tma_host.h"
 
 namespace fllm {
 namespace {
-constexpr int kSpanRows = 16;
 // Weights in f16 are taken to a reference 2^12 below the row's maximum: below 2^-14 of their unit they would lose bits.
 constexpr float kF16Lift = 12.f;
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <bool F16>
-__device__ __forceinline__ uint32_t pack_16(float lo, float hi) {
-  if constexpr (F16) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    return pack_bf16x2(lo, hi);
-  }
-}
-template <bool F16>
-__device__ __forceinline__ float2 unpack_16(uint32_t w) {
-  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  else return unpack_bf16x2(w);
-}
-// A lane's two 16-bit values of an 8 x 8 matrix, row lane / 4 and columns 2 (lane % 4), for those of the transposed one.
-__device__ __forceinline__ uint32_t transposed(uint32_t w) {
-  uint32_t d;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(w));
-  return d;
-}
 __device__ __forceinline__ void cp_async16_or_zero(void* smem, const void* gmem, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(there ? 16 : 0) : "memory");
-}
-
-// Four values of a row, normalised with the head's sink. (A row that saw nothing has m = -inf and l = 0, not NaN as one of NaN scores: no sink is added to
-// it, where e^(sink - m) of a sink of -inf would be a NaN.)
-template <int D>
-__device__ __forceinline__ void store_row(const SpanParams& p, int q0, int row, int kvh, int d, float4 a, float mm, float ll) {
-  const int qi = row / p.group, head = kvh * p.group + row - qi * p.group;
-  float c = 1.f;
-  if (p.sinks && (mm != -INFINITY || ll != 0.f)) {
-    const float sk = p.sinks[head] * kLog2e, mn = fmaxf(mm, sk);
-    c = mm == -INFINITY ? 0.f : ex2(mm - mn);
-    ll = ll * c + ex2(sk - mn);
-  }
-  const float inv = ll == 0.f ? 0.f : c / ll;
-  *reinterpret_cast<uint2*>(static_cast<bf16*>(p.out) + (size_t)(q0 + qi) * p.ldo + (size_t)head * D + d) =
-      make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
 }
 
 // An e4m3 page stays as it is in shared memory and becomes operands in registers, which needs no order of columns that memory does not have: a lane
@@ -120,8 +77,9 @@ template <int D, bool KV8> constexpr int rows_resident() { return D == 256 ? 1 :
 // 8 columns the rows, and nothing is computed for rows 8 to 15. A lane's operands are the same registers in another order; it holds scores of rows 2t and
 // 2t + 1 and tokens g and g + 8 (otherwise rows g and g + 8 and tokens 2t, 2t + 1 of each half). us of decode rows, so and with 16 rows: 48 sequences of an
 // e4m3 cache under 1000 with 130 first tokens, 64 query and 8 key heads of 64: 22.6, 28.8; one under 256, 32 and 8 of 128: 6.3, 6.8; 64 under 4096: 166 both.
-// SEARCH: p.search. (Its code in all calls cost the smallest 3 %.)
-template <int D, bool KV8, bool NARROW, bool SEARCH>
+// MODE: whose rows a CTA's are, as its place says, looked up (p.search; its code in all calls cost the smallest 3 %), or one row's, which reads selected
+// blocks (p.picks; up to 16 heads at a time).
+template <int D, bool KV8, bool NARROW, int MODE>
 __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel(const __grid_constant__ SpanParams p) {
   using S = RowsSmem<D, KV8>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -139,16 +97,8 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
   work /= p.hkv;
   pdl_launch_dependents();
   pdl_wait();
-  int seq = work % p.num_seqs, tile = work / p.num_seqs;
-  if constexpr (SEARCH) {
-    if (!span_find(p, kSpanRows, 0, p.rows_to, work, blockIdx.x == gridDim.x - 1, seq, tile)) return;
-  }
-  // (what follows is the same for all splits, which are a cluster where they join in one: all of them leave, or none)
-  int q0, qn, kv_len;
-  if (!span_lengths(p, seq, threadIdx.x == 0, q0, qn, kv_len)) return;
-  const int all_rows = qn * G, row0 = tile * kSpanRows;
-  if (all_rows > p.rows_to || row0 >= all_rows) return;
-  const int n_rows = min(kSpanRows, all_rows - row0);
+  int seq, row0, n_rows, q0, qn, kv_len;
+  if (!span_rows_of_cta<MODE>(p, work, split, seq, row0, n_rows, q0, qn, kv_len)) return;
 
   // Every warp finds out what the rows see for itself (a lane to a row), so that its pages are on their way before the queries are.
   int min_base = INT_MAX, max_base = 0, min_beg = INT_MAX, max_beg = 0;      // what they see between them, and what all of them see
@@ -171,7 +121,7 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
   max_base = __reduce_max_sync(0xffffffffu, max_base);
   min_beg = __reduce_min_sync(0xffffffffu, min_beg);
   max_beg = __reduce_max_sync(0xffffffffu, max_beg);
-  const SpanRange range = span_range(p, kPage, min_beg, p.tree_mask ? kv_len : max_base);
+  const SpanWalk<MODE> range = span_walk<MODE>(p, q0, row0, kvh, min_beg, max_base, kv_len, warp == 0 && split == 0);
   const int per_split = max(p.min_pages, (range.count + p.splits - 1) / p.splits);
   const int pg0 = min(split * per_split, range.count), pg1 = min(pg0 + per_split, range.count);
 
@@ -553,55 +503,7 @@ __global__ void __launch_bounds__(128, rows_resident<D, KV8>()) span_rows_kernel
     }
     if ((NARROW ? g : t) == 0) *reinterpret_cast<float2*>(mml + (warp * 16 + r) * 2) = make_float2(m[h], l[h]);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n_rows * (D / 4); i += 128) {
-    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mml[(w * 16 + r) * 2]);
-    float ll = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float2 ml = *reinterpret_cast<const float2*>(mml + (w * 16 + r) * 2);
-      const float c = ml.x == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : ex2(ml.x - mm);
-      const float4 v = *reinterpret_cast<const float4*>(mo + ((size_t)w * 16 + r) * D + d);
-      ll += ml.y * c;
-      a.x += v.x * c; a.y += v.y * c; a.z += v.z * c; a.w += v.w * c;      // (a factor of 0 too: 0 x NaN is what one warp would have made of it)
-    }
-    if (p.splits == 1) {
-      store_row<D>(p, q0, row0 + r, kvh, d, a, mm, ll);
-    } else if (p.in_cluster) {
-      *reinterpret_cast<float4*>(part_o + r * D + d) = a;
-      if (d == 0) part_ml[r] = make_float4(mm, ll, 0.f, 0.f);
-    } else {
-      const int qi = (row0 + r) / G, head = kvh * G + (row0 + r) - qi * G;
-      const size_t at = ((size_t)(q0 + qi) * p.hq + head) * p.splits + split;
-      *reinterpret_cast<float4*>(p.ws_o + at * D + d) = a;
-      if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(mm, ll);
-    }
-  }
-  if (p.in_cluster) {
-    // the splits are a cluster: each CTA takes a share of the row's values from all of them
-    cluster_sync();
-    for (int i = split * 128 + threadIdx.x; i < n_rows * (D / 4); i += 128 * p.splits) {
-      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-      float mm = -INFINITY, ll = 0.f;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int c = 0; c < p.splits; ++c) {
-        const float4 ml = ld_dsmem_f4(smem_u32(part_ml + r), c), v = ld_dsmem_f4(smem_u32(part_o + r * D + d), c);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        const float mn = fmaxf(mm, ml.x);
-        const float w0 = mm == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : ex2(mm - mn), w1 = ml.x == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : ex2(ml.x - mn);
-        mm = mn;
-        ll = ll * w0 + ml.y * w1;
-        a.x = a.x * w0 + v.x * w1; a.y = a.y * w0 + v.y * w1; a.z = a.z * w0 + v.z * w1; a.w = a.w * w0 + v.w * w1;
-      }
-      store_row<D>(p, q0, row0 + r, kvh, d, a, mm, ll);
-    }
-    cluster_sync();                                    // no CTA leaves while another reads its rows
-  }
+  span_join<D>(p, mo, mml, part_o, part_ml, q0, row0, n_rows, kvh, split);
 }
 
 // Joins the splits of a row: one warp per (token, head). `some`: sequences of at most p.rows_from packed rows were another kernel's.
@@ -669,23 +571,25 @@ __global__ void __launch_bounds__(128) span_merge_kernel(const __grid_constant__
   for (int e = 0; e < D / 32; ++e) dst[32 * e] = __float2bfloat16(a[e] * inv);
 }
 
-long long most_rows(const SpanParams& p) { return std::min<long long>((long long)p.max_q_len * p.group, p.rows_to); }
+long long most_rows(const SpanParams& p) { return p.picks ? p.group : std::min<long long>((long long)p.max_q_len * p.group, p.rows_to); }
 template <int D, bool KV8, bool NARROW>
 void launch_rows(SpanParams p, cudaStream_t s) {
   constexpr int smem = RowsSmem<D, KV8>::kTotal;
   static bool configured[kMaxDevices] = {};
   if (first_call_on_device(configured)) {
-    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_rows smem");
-    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_rows smem");
+    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW, kAsked>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_rows smem");
+    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW, kSearch>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_rows smem");
+    cuda_check(cudaFuncSetAttribute(span_rows_kernel<D, KV8, NARROW, kPicked>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_rows smem");
   }
-  const long long ctas = span_tiles(p, most_rows(p), kSpanRows, p.search) * p.hkv * p.splits;
+  const long long ctas = span_rows_ctas(p) * p.splits;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
   auto go = [&](auto kernel) {
     if (p.in_cluster) launch_cluster(true, kernel, dim3((unsigned)ctas), dim3(128), smem, s, (unsigned)p.splits, p);
     else launch_pdl(kernel, dim3((unsigned)ctas), dim3(128), smem, s, p);
   };
-  if (p.search) go(span_rows_kernel<D, KV8, NARROW, true>);
-  else go(span_rows_kernel<D, KV8, NARROW, false>);
+  if (p.picks) go(span_rows_kernel<D, KV8, NARROW, kPicked>);
+  else if (p.search) go(span_rows_kernel<D, KV8, NARROW, kSearch>);
+  else go(span_rows_kernel<D, KV8, NARROW, kAsked>);
 }
 template <int D>
 void launch_rows_of(const SpanParams& p, cudaStream_t s) {
@@ -704,23 +608,34 @@ void merge(const SpanParams& p, bool some, cudaStream_t s) {
 size_t partial_floats(const SpanParams& p, int splits) { return splits > 1 ? (size_t)p.tokens * p.hq * splits * (p.head_dim + 2) : 0; }
 }  // namespace
 
+long long span_rows_ctas(SpanParams& p) {
+  if (p.picks) {
+    p.search = false;
+    return (long long)p.tokens * p.hkv * ((p.group + kSpanRows - 1) / kSpanRows);
+  }
+  return span_tiles(p, most_rows(p), kSpanRows, p.search) * p.hkv;
+}
+
 SpanPlan attention_span_plan(const SpanParams& p) {
   SpanPlan plan{};
   const long long most = (long long)p.max_q_len * p.group;
-  const long long span = std::min<long long>(p.window > 0 ? (long long)p.window + p.first + p.max_q_len : p.max_kv_len, p.max_kv_len);
+  const long long reach = p.picks ? (long long)p.pick_count * kPage * p.block_pages : p.window > 0 ? (long long)p.window + p.first + p.max_q_len : p.max_kv_len;
+  const long long span = std::min<long long>(reach, p.max_kv_len);
   // Sequences of more than 16 packed rows go to the tensor-memory kernel, unless all there is to do is less than 28 pages of 16 rows for each SM: its way
   // in and out is longer (one tree of 8, 12, 32 and 64 nodes behind 900 tokens, 32 query and 8 key heads of 128: 10.6, 11.0, 13.9, 20.4 us here, 15.5, 15.6,
   // 16.1, 18.6 there; 12 nodes behind 4000: 19.2 and 18.6).
   bool search;
   const long long all_tiles = span_tiles(p, most, kSpanRows, search) * p.hkv;
-  const bool tc = attention_span_tc_supported(p) && all_tiles * ((span + kPage - 1) / kPage) > 28LL * sm_count();
+  const bool tc = !p.picks && attention_span_tc_supported(p) && all_tiles * ((span + kPage - 1) / kPage) > 28LL * sm_count();
   if (!tc || (long long)p.min_q_len * p.group <= kSpanRows) {
-    const long long ctas = span_tiles(p, tc ? std::min<long long>(most, kSpanRows) : most, kSpanRows, search) * p.hkv;
+    SpanParams rows = p;
+    rows.rows_to = tc ? kSpanRows : INT_MAX;
+    const long long ctas = span_rows_ctas(rows);
     const long long pages = (span + kPage - 1) / kPage;
     // As many splits as leave all CTAs on the SMs at once, a page for each of a CTA's warps at least: a CTA's way in and out is some 5 us (64 sequences
     // under a window of 4096, 8 key heads of 128: 170 us whole, 182 in two, 202 in four; 16 under one of 1024: 24, 17, 24). Up to eight are a
     // cluster and join in it; more, where few sequences are long, leave their rows to a kernel behind.
-    const int resident = p.head_dim == 256 ? 1 : p.head_dim == 64 ? rows_resident<64, false>() : p.kv_fp8 ? rows_resident<128, true>() : rows_resident<128, false>();
+    const int resident = p.kv4 ? attention_kv4_resident(rows) : p.head_dim == 256 ? 1 : p.head_dim == 64 ? rows_resident<64, false>() : p.kv_fp8 ? rows_resident<128, true>() : rows_resident<128, false>();
     plan.min_pages = 4;
     long long splits = std::min<long long>((long long)resident * sm_count() / ctas, (pages + plan.min_pages - 1) / plan.min_pages);
     if (splits > 8 && (pages < 8 * 64 || (tc && most > kSpanRows))) splits = 8;      // (their workspace would have room for the other kernel's rows, too)
@@ -759,7 +674,8 @@ int attention_span(SpanParams p, const SpanPlan& plan, void* workspace, cudaStre
     p.in_cluster = plan.in_cluster;
     p.rows_from = 0;
     p.rows_to = plan.tile_splits > 0 ? kSpanRows : INT_MAX;
-    switch (p.head_dim) {
+    if (p.kv4) attention_kv4_rows(p, s);
+    else switch (p.head_dim) {
       case 64: launch_rows_of<64>(p, s); break;
       case 128: launch_rows_of<128>(p, s); break;
       default: launch_rows_of<256>(p, s); break;

@@ -139,6 +139,31 @@ __device__ __forceinline__ bool span_find(const SpanParams& p, int unit, int fro
   return found;
 }
 
+// Which sequence a query row is of, by a warp: the last one that begins at or before it. False where the batch has no such row.
+__device__ __forceinline__ bool span_seq_of(const SpanParams& p, int row, int& seq) {
+  int n = 0;
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 32) {
+    const int s = s0 + (threadIdx.x & 31);
+    const unsigned at = __ballot_sync(0xffffffffu, s < p.num_seqs && p.q_starts[s] <= row);
+    n += __popc(at);
+    if (at != 0xffffffffu) break;
+  }
+  seq = n - 1;
+  return n > 0;
+}
+
+// Blocks that a row reads of one key head, by a warp: those in front of the first that is negative (or that the row's last token lies in front of: reported).
+__device__ __forceinline__ int span_count_picks(const SpanParams& p, const int* picks, int blocks, bool report) {
+  for (int i0 = 0; i0 < p.pick_count; i0 += 32) {
+    const int i = i0 + (threadIdx.x & 31);
+    const int b = i < p.pick_count ? picks[i] : -1;
+    const unsigned end = __ballot_sync(0xffffffffu, b < 0 || b >= blocks);
+    if (__any_sync(0xffffffffu, b >= blocks) && report && p.status && (threadIdx.x & 31) == 0) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
+    if (end) return min(i0 + __ffs(end) - 1, p.pick_count);
+  }
+  return p.pick_count;
+}
+
 // Block id of the 16 tokens from 16 * page on, or -1 where the table does not reach or the entry names no block of the pool.
 __device__ __forceinline__ int span_block(const SpanParams& p, const int* table, int page) {
   const int at = page / p.block_pages;

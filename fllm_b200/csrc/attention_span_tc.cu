@@ -939,7 +939,7 @@ void launch_tc(SpanParams p, cudaStream_t s) {
 }  // namespace
 
 bool attention_span_tc_supported(const SpanParams& p) {
-  return (p.head_dim == 64 || p.head_dim == 128) && p.num_blocks * p.hkv * p.block_pages * kPage <= INT_MAX - kTile;
+  return !p.kv4 && (p.head_dim == 64 || p.head_dim == 128) && p.num_blocks * p.hkv * p.block_pages * kPage <= INT_MAX - kTile;
 }
 void attention_span_tc(const SpanParams& p, cudaStream_t s) {
   if (p.head_dim == 64) p.kv_fp8 ? launch_tc<64, true>(p, s) : launch_tc<64, false>(p, s);

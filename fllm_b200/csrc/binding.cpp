@@ -157,13 +157,23 @@ void rmsnorm(Tensor residual, const optional<Tensor>& delta, const Tensor& w, Te
                      cur_stream());
 }
 
+// Whether the caches hold rows of 4 bits: uint8, head_dim / 2 + 4 to a row
+bool is_kv4(const Tensor& k_cache, const Tensor& v_cache, int64_t hkv, int64_t head_dim) {
+  const bool kv4 = k_cache.scalar_type() == at::kByte && k_cache.dim() == 4 && k_cache.size(3) == head_dim / 2 + 4;
+  TORCH_CHECK(!kv4 || (v_cache.sizes() == k_cache.sizes() && v_cache.scalar_type() == at::kByte && k_cache.size(1) == hkv &&
+                       ((reinterpret_cast<uintptr_t>(k_cache.data_ptr()) | reinterpret_cast<uintptr_t>(v_cache.data_ptr())) & 3) == 0),
+              "caches of 4-bit rows must be alike, uint8 [blocks, hkv, block_size, head_dim / 2 + 4]");
+  return kv4;
+}
+
 void rope_kv_write(Tensor qkv, const Tensor& positions, const optional<Tensor>& slots,
                    const Tensor& inv_freq, const optional<Tensor>& q_norm_w,
                    const optional<Tensor>& k_norm_w, Tensor k_cache, Tensor v_cache, int64_t hq,
                    int64_t hkv, int64_t head_dim, int64_t rot_dim, int64_t rope_style, double eps,
                    double attn_factor) {
   check_bf16(qkv, "qkv"); check_rows(qkv, "qkv"); check_i32(positions, "positions");
-  const bool kv_fp8 = k_cache.element_size() == 1;            // e4m3 cache
+  const bool kv_fp8 = k_cache.element_size() == 1;            // e4m3 cache, or one of 4-bit rows
+  const bool kv4 = is_kv4(k_cache, v_cache, hkv, head_dim);
   TORCH_CHECK(k_cache.is_cuda() && k_cache.element_size() == v_cache.element_size() &&
               (kv_fp8 || k_cache.scalar_type() == at::kBFloat16), "caches must be bf16 or 1-byte e4m3 tensors");
   TORCH_CHECK(inv_freq.scalar_type() == at::kFloat && inv_freq.is_cuda(), "inv_freq must be fp32 CUDA");
@@ -176,7 +186,7 @@ void rope_kv_write(Tensor qkv, const Tensor& positions, const optional<Tensor>& 
       inv_freq.data_ptr<float>(), opt_ptr<void>(q_norm_w), opt_ptr<void>(k_norm_w),
       k_cache.data_ptr(), v_cache.data_ptr(), (int)qkv.size(0), (int)hq, (int)hkv, (int)head_dim,
       (int)k_cache.size(2), (int)rot_dim, (int)rope_style, (float)eps, (float)attn_factor,
-      cur_stream(), kv_fp8 ? 1 : 0);
+      cur_stream(), kv4 ? fllm::kKv4 : kv_fp8 ? 1 : 0);
 }
 
 // QK-norm + RoPE + KV write reading the q|k|v heads from split-K partials; rotated queries go to q_out
@@ -187,6 +197,7 @@ void rope_kv_write_splitk(const Tensor& workspace, int64_t splits, const optiona
                           int64_t rope_style, double eps, double attn_factor) {
   check_bf16(q_out, "q_out"); check_rows(q_out, "q_out"); check_i32(positions, "positions");
   const bool kv_fp8 = k_cache.element_size() == 1;
+  const bool kv4 = is_kv4(k_cache, v_cache, hkv, head_dim);
   TORCH_CHECK(k_cache.is_cuda() && k_cache.element_size() == v_cache.element_size() &&
               (kv_fp8 || k_cache.scalar_type() == at::kBFloat16), "caches must be bf16 or 1-byte e4m3 tensors");
   TORCH_CHECK(inv_freq.scalar_type() == at::kFloat && inv_freq.is_cuda(), "inv_freq must be fp32 CUDA");
@@ -200,7 +211,7 @@ void rope_kv_write_splitk(const Tensor& workspace, int64_t splits, const optiona
       nullptr, 0, positions.data_ptr<int>(), opt_ptr<int>(slots), inv_freq.data_ptr<float>(),
       opt_ptr<void>(q_norm_w), opt_ptr<void>(k_norm_w), k_cache.data_ptr(), v_cache.data_ptr(), tokens, (int)hq,
       (int)hkv, (int)head_dim, (int)k_cache.size(2), (int)rot_dim, (int)rope_style, (float)eps, (float)attn_factor,
-      cur_stream(), kv_fp8 ? 1 : 0, ws, (int)splits, opt_ptr<void>(bias), q_out.data_ptr(), q_out.stride(0));
+      cur_stream(), kv4 ? fllm::kKv4 : kv_fp8 ? 1 : 0, ws, (int)splits, opt_ptr<void>(bias), q_out.data_ptr(), q_out.stride(0));
 }
 
 // glu with a column layout (0 natural, 16 blocked) and, when splits > 0, split-K partials as the source

@@ -25,18 +25,20 @@ inline bool is_e4m3(const Tensor& t) { return t.scalar_type() == at::kFloat8_e4m
 std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_tables, const Tensor& q_starts,
                        const Tensor& kv_lens, int64_t num_seqs, int64_t max_q_len, int64_t min_q_len, int64_t max_kv_len, int64_t hq,
                        int64_t hkv, int64_t head_dim, double scale, int64_t window, int64_t first, const optional<Tensor>& sinks, double softcap,
-                       const optional<Tensor>& tree_mask, const optional<Tensor>& tree_base, const optional<Tensor>& status) {
+                       const optional<Tensor>& tree_mask, const optional<Tensor>& tree_base, const optional<Tensor>& status, const optional<Tensor>& picks) {
   fllm::SpanParams p{};
   TORCH_CHECK(hq > 0 && hkv > 0 && hq % hkv == 0 && hq <= 65536, "attention: query heads must be a multiple of the key heads");
   TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "attention: head_dim must be 64, 128 or 256");
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 2 && q.stride(1) == 1 && q.size(1) == hq * head_dim && q.stride(0) % 8 == 0 &&
                   (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) == 0,
               "q must be bf16 rows of hq * head_dim values on 16-byte boundaries");
+  p.kv4 = k_cache.scalar_type() == at::kByte && k_cache.dim() == 4 && k_cache.size(3) == head_dim / 2 + 4;
   auto pool = [&](const Tensor& t, const char* name) {
     TORCH_CHECK(t.is_cuda() && t.device() == q.device() && t.dim() == 4 && t.is_contiguous() && t.sizes() == k_cache.sizes() &&
                     t.scalar_type() == k_cache.scalar_type() && (t.scalar_type() == at::kBFloat16 || is_e4m3(t)) && t.size(1) == hkv &&
-                    t.size(2) % 16 == 0 && t.size(2) > 0 && t.size(3) == head_dim && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
-                name, " must be a contiguous bf16 or e4m3 pool [blocks, hkv, block_size, head_dim], block_size a multiple of 16");
+                    t.size(2) % 16 == 0 && t.size(2) > 0 && (p.kv4 || t.size(3) == head_dim) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
+                name, " must be a contiguous bf16 or e4m3 pool [blocks, hkv, block_size, head_dim] or one of 4-bit rows (uint8, head_dim / 2 + 4 of them), block_size a "
+                "multiple of 16");
   };
   pool(k_cache, "k_cache");
   pool(v_cache, "v_cache");
@@ -68,6 +70,14 @@ std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cach
     check_ints(*status, q, 1, "status");
     p.status = status->data_ptr<int>();
   }
+  if (picks.has_value() && picks->defined()) {
+    TORCH_CHECK(!p.tree_mask && window == 0, "attention_blocks: selected blocks have no window and no tree");
+    TORCH_CHECK(picks->dim() == 3 && picks->size(0) == q.size(0) && picks->size(1) == hkv && picks->size(2) > 0 && picks->size(2) < (1 << 24),
+                "attention_blocks: blocks must be int32 [rows, hkv, count]");
+    check_ints(*picks, q, 0, "blocks");
+    p.picks = picks->data_ptr<int>();
+    p.pick_count = (int)picks->size(2);
+  }
   p.q = q.data_ptr(); p.ldq = q.stride(0);
   p.k_cache = k_cache.data_ptr(); p.v_cache = v_cache.data_ptr();
   p.block_tables = block_tables.data_ptr<int>(); p.max_blocks = (int)block_tables.size(1);
@@ -75,7 +85,7 @@ std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cach
   p.q_starts = q_starts.data_ptr<int>(); p.kv_lens = kv_lens.data_ptr<int>();
   p.tokens = (int)q.size(0); p.num_seqs = (int)num_seqs;
   p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv); p.head_dim = (int)head_dim;
-  p.kv_fp8 = is_e4m3(k_cache);
+  p.kv_fp8 = is_e4m3(k_cache) && !p.kv4;
   // No sequence has more rows than there are, and none may be said to have none: one that has more than announced is reported by a kernel.
   p.max_q_len = (int)std::max<int64_t>(1, std::min<int64_t>(max_q_len, q.size(0)));
   p.min_q_len = (int)std::min<int64_t>(min_q_len, p.max_q_len); p.max_kv_len = (int)max_kv_len;
@@ -98,5 +108,5 @@ std::tuple<Tensor, int64_t> attention_span(const Tensor& q, const Tensor& k_cach
 TORCH_LIBRARY_FRAGMENT(fllm_b200, m) {
   m.def("attention_span(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor q_starts, Tensor kv_lens, int num_seqs, "
         "int max_q_len, int min_q_len, int max_kv_len, int hq, int hkv, int head_dim, float scale, int window, int first, Tensor? sinks, float softcap, "
-        "Tensor? tree_mask=None, Tensor? tree_base=None, Tensor? status=None) -> (Tensor, int)", &attention_span);
+        "Tensor? tree_mask=None, Tensor? tree_base=None, Tensor? status=None, Tensor? picks=None) -> (Tensor, int)", &attention_span);
 }

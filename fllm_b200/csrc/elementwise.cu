@@ -11,6 +11,7 @@
 #include <algorithm>
 
 #include "fllm_ops.h"
+#include "kv4.cuh"
 #include "ptx.cuh"
 #include "tma_host.h"
 
@@ -278,7 +279,8 @@ void rmsnorm_splitk_bf16(void* residual, long long ld_res, const float* partials
 // 2048 x 24 heads of 256 in 48.7 us (32 registers: 24.2), 2048 x 48 of 128, interleaved, in 38.7 (27.2).
 template <int D, Sums SUMS>
 constexpr int kRopeCtas = SUMS == Sums::batch ? (D == 64 ? 10 : D == 128 ? 7 : 4) : SUMS == Sums::loop ? (D == 64 ? 16 : D == 128 ? 9 : 7) : 16;
-template <int D, Sums SUMS>
+// KV4: the caches hold rows of 4 bits (kv4.cuh) of what a bf16 cache would hold.
+template <int D, Sums SUMS, bool KV4 = false>
 __global__ void __launch_bounds__(128, kRopeCtas<D, SUMS>)
 rope_kv_kernel(__nv_bfloat16* __restrict__ qkv, long long ld_qkv, const int* __restrict__ positions,
                const int* __restrict__ slots, const float* __restrict__ inv_freq,
@@ -320,6 +322,25 @@ rope_kv_kernel(__nv_bfloat16* __restrict__ qkv, long long ld_qkv, const int* __r
     if (slot < 0) return;
     const int kvh = h - hq - hkv;
     const int blk = slot / block_size, off = slot - blk * block_size;
+    if constexpr (KV4) {
+      float a[EPL];
+      int at[EPL];
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) at[j] = 2 * (lane + 32 * (j / 2)) + (j & 1);
+      if constexpr (ADD) {
+        sum_splits_at<EPL, SUMS == Sums::batch>(a, wsrc, plane, splits, at);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) a[j] = __bfloat162float(__float2bfloat16(bias ? a[j] + __bfloat162float(bias[h * D + at[j]]) : a[j]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < EPL; j += 2) {
+          const float2 f = unpack_bf16x2(reinterpret_cast<const uint32_t*>(src)[lane + 32 * (j / 2)]);
+          a[j] = f.x; a[j + 1] = f.y;
+        }
+      }
+      kv4_store_row<D, true>(a, reinterpret_cast<uint8_t*>(v_cache) + (((size_t)blk * hkv + kvh) * block_size + off) * kKv4Row<D>, lane);
+      return;
+    }
     __nv_bfloat16* dst = v_cache + (((size_t)blk * hkv + kvh) * block_size + off) * D;
     if (kv_fp8) {                  // e4m3 cache: one byte per value, same [block][head][slot][dim] order
       uint8_t* d8 = reinterpret_cast<uint8_t*>(v_cache) + (((size_t)blk * hkv + kvh) * block_size + off) * D;
@@ -459,6 +480,14 @@ rope_kv_kernel(__nv_bfloat16* __restrict__ qkv, long long ld_qkv, const int* __r
     if (slot < 0) return;
     const int kvh = h - hq;
     const int blk = slot / block_size, off = slot - blk * block_size;
+    if constexpr (KV4) {
+      uint8_t* row = reinterpret_cast<uint8_t*>(k_cache) + (((size_t)blk * hkv + kvh) * block_size + off) * kKv4Row<D>;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) v[j] = __bfloat162float(__float2bfloat16(v[j]));
+      if (rope_style == 0) kv4_store_row<D, false>(v, row, lane);
+      else kv4_store_row<D, true>(v, row, lane);
+      return;
+    }
     dst = k_cache + (((size_t)blk * hkv + kvh) * block_size + off) * D;
     if (kv_fp8) {
       uint8_t* d8 = reinterpret_cast<uint8_t*>(k_cache) + (((size_t)blk * hkv + kvh) * block_size + off) * D;
@@ -488,7 +517,7 @@ rope_kv_kernel(__nv_bfloat16* __restrict__ qkv, long long ld_qkv, const int* __r
 // sines of its position once (a warp per head computes them for every head: 48 accurate sincosf of a token instead of one took
 // 44 us of 2048 x 48 heads of 128, whose 50 MB move in 8); then D / 8 lanes take a head, eight values each: four neighbours and
 // their partners half a head further, so that a rotation stays in its lane and every access is 8 bytes.
-template <int D>
+template <int D, bool KV4 = false>
 __global__ void __launch_bounds__(256)
 rope_kv_rows_kernel(__nv_bfloat16* __restrict__ qkv, long long ld_qkv, const int* __restrict__ positions, const int* __restrict__ slots,
                     const float* __restrict__ inv_freq, const __nv_bfloat16* __restrict__ q_norm_w, const __nv_bfloat16* __restrict__ k_norm_w,
@@ -551,6 +580,20 @@ rope_kv_rows_kernel(__nv_bfloat16* __restrict__ qkv, long long ld_qkv, const int
       a = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
       b = make_uint2(pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
     }
+    if constexpr (KV4) {
+      const float2 p0 = unpack_bf16x2(a.x), p1 = unpack_bf16x2(a.y), p2 = unpack_bf16x2(b.x), p3 = unpack_bf16x2(b.y);
+      const float r[8] = {p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+      const Kv4Scale s = kv4_scale<8, LANES>(r);          // (of all heads: the lanes of a warp hold several)
+      if (in && !is_q && slot >= 0) {
+        uint8_t* row = reinterpret_cast<uint8_t*>(is_v ? v_cache : k_cache) + (((size_t)blk * hkv + (is_v ? h - hq - hkv : h - hq)) * block_size + off) * kKv4Row<D>;
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+          *reinterpret_cast<uint16_t*>(row + (part * D / 2 + e) / 2) = (uint16_t)(kv4_code(r[4 * part], s) | kv4_code(r[4 * part + 1], s) << 4 |
+                                                                                  kv4_code(r[4 * part + 2], s) << 8 | kv4_code(r[4 * part + 3], s) << 12);
+        if (sub == 0) *reinterpret_cast<uint32_t*>(row + D / 2) = s.packed();
+      }
+      if (!in || !is_q) continue;
+    }
     if (!in || (!is_q && slot < 0)) continue;
     __nv_bfloat16* dst = src;
     if (!is_q) dst = (is_v ? v_cache : k_cache) + (((size_t)blk * hkv + (is_v ? h - hq - hkv : h - hq)) * block_size + off) * D;
@@ -583,19 +626,19 @@ void rope_qknorm_kvwrite_bf16(void* qkv, long long ld_qkv, const int* positions,
   // One block per token needs as many tokens as there are SMs; below, a warp per head finishes sooner.
   const uintptr_t align = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w) |
                           reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache);
-  if (tokens >= sm_count() && !partials && !q_out && !kv_fp8 && rope_style == 0 && rot_dim == head_dim && (head_dim == 64 || head_dim == 128) &&
+  const bool kv4 = kv_fp8 == kKv4;
+  if (tokens >= sm_count() && !partials && !q_out && (!kv_fp8 || kv4) && rope_style == 0 && rot_dim == head_dim && (head_dim == 64 || head_dim == 128) &&
       (ld_qkv & 3) == 0 && (align & 7) == 0) {
-    if (head_dim == 64)
-      launch_pdl(rope_kv_rows_kernel<64>, dim3(tokens), dim3(256), 0, s, x, ld_qkv, positions, slots, inv_freq, qn, kn, kc, vc, hq, hkv, block_size, eps,
-                 attn_factor);
-    else
-      launch_pdl(rope_kv_rows_kernel<128>, dim3(tokens), dim3(256), 0, s, x, ld_qkv, positions, slots, inv_freq, qn, kn, kc, vc, hq, hkv, block_size, eps,
-                 attn_factor);
+    auto go = [&](auto kernel) {
+      launch_pdl(kernel, dim3(tokens), dim3(256), 0, s, x, ld_qkv, positions, slots, inv_freq, qn, kn, kc, vc, hq, hkv, block_size, eps, attn_factor);
+    };
+    if (head_dim == 64) kv4 ? go(rope_kv_rows_kernel<64, true>) : go(rope_kv_rows_kernel<64>);
+    else kv4 ? go(rope_kv_rows_kernel<128, true>) : go(rope_kv_rows_kernel<128>);
     return;
   }
   const Sums sums = !partials ? Sums::none : rope_sums(splits, head_dim);
 #define FLLM_ROPE_SUMS(DD, SS)                                                                                     \
-  launch_pdl(rope_kv_kernel<DD, SS>, dim3(blocks), dim3(128), 0, s, x, ld_qkv, positions, slots, inv_freq, qn, kn, kc, \
+  launch_pdl(kv4 ? rope_kv_kernel<DD, SS, true> : rope_kv_kernel<DD, SS>, dim3(blocks), dim3(128), 0, s, x, ld_qkv, positions, slots, inv_freq, qn, kn, kc, \
              vc, tokens, hq, hkv, block_size, rot_dim, rope_style, eps, attn_factor, kv_fp8, partials, splits,    \
              (const __nv_bfloat16*)bias, (__nv_bfloat16*)q_out, ld_q)
 #define FLLM_ROPE(DD)                                                   \

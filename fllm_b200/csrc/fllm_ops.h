@@ -234,6 +234,7 @@ void moe_combine(const void* y, long long ldy, const int* row_of, const float* w
                  long long ldo, int hidden, cudaStream_t s, const void* add = nullptr, long long ld_add = 0, int f32 = 0,
                  const float* add_gate = nullptr);
 
+constexpr int kKv4 = 2;        // of a cache's kind, beside 0 (bf16) and 1 (e4m3): rows of 4 bits (kv4.cuh)
 // ---- elementwise --------------------------------------------------------------------
 void embed_bf16(const int* ids, const void* table, void* out, int tokens, int hidden, int vocab,
                 float scale, cudaStream_t s);
@@ -244,7 +245,7 @@ void rope_qknorm_kvwrite_bf16(void* qkv, long long ld_qkv, const int* positions,
                               const float* inv_freq, const void* q_norm_w, const void* k_norm_w,
                               void* k_cache, void* v_cache, int tokens, int hq, int hkv,
                               int head_dim, int block_size, int rot_dim, int rope_style, float eps,
-                              float attn_factor, cudaStream_t s, int kv_fp8 = 0,   // kv_fp8: caches hold e4m3 bytes
+                              float attn_factor, cudaStream_t s, int kv_fp8 = 0,   // kv_fp8: caches hold e4m3 bytes, or (kKv4) rows of 4 bits
                               // optional: read the heads from fp32 split-K partials [splits][tokens][width]
                               // (+ bias) instead of qkv, and write the rotated query heads to q_out
                               const float* partials = nullptr, int splits = 0, const void* bias = nullptr,
@@ -293,7 +294,7 @@ size_t attention_tc_workspace_bytes(int tokens, int hq, int head_dim, int max_sp
 struct SpanParams {
   const void* q;               // bf16 [tokens, hq * head_dim], pitch ldq
   long long ldq;
-  const void *k_cache, *v_cache;      // [num_blocks, hkv, 16 * block_pages, head_dim], bf16 or e4m3
+  const void *k_cache, *v_cache;      // [num_blocks, hkv, 16 * block_pages, head_dim], bf16 or e4m3, or rows of 4 bits (kv4)
   const int* block_tables;     // [num_seqs, max_blocks]
   int max_blocks, block_pages;
   long long num_blocks;
@@ -310,6 +311,9 @@ struct SpanParams {
   int max_q_len, min_q_len, max_kv_len;
   int reach;                   // tokens that a row of block_tables has room for
   int window, first;           // window 0: no limit (first is 0 then)
+  const int* picks;            // [tokens][hkv][pick_count] or null: a row reads these of its sequence's blocks only (each once, none behind the first negative one)
+  int pick_count;
+  bool kv4;
   float scale_log2, softcap;   // of the scores, to base 2; 0: no soft-cap
   // set by the planner, for one kernel
   int splits, min_pages, sms;  // pieces of what a sequence's rows see, at most; fewest pages in one; SMs
@@ -337,6 +341,9 @@ inline long long span_tiles(const SpanParams& p, long long most, int rows, bool&
   return search ? all : each;
 }
 void attention_span_tc(const SpanParams& p, cudaStream_t s);
+long long span_rows_ctas(SpanParams& p);               // of the kernels of few rows, for each split; finds out whether they search
+int attention_kv4_resident(const SpanParams& p);       // CTAs of an SM
+void attention_kv4_rows(const SpanParams& p, cudaStream_t s);
 
 // ---- rows of the cache pools (kv_moves.cu) ------------------------------------------
 struct KvPool {                // [planes][blocks][heads][block_size][row_bytes], a block's bytes contiguous
@@ -355,6 +362,40 @@ int kv_copy_blocks(const KvPools& p, const int* pairs, int n, int* status, cudaS
 int kv_copy_listed(const KvPools& p, const int* pairs, int n, int* status, cudaStream_t s);       // pairs of the host
 int kv_compact(const KvPools& p, const int* block_tables, int max_blocks, const int* base, const int* path, int depth, const int* counts,
                int seqs, int* status, cudaStream_t s);
+
+// ---- caches held in 4 bits (kv4.cu) --------------------------------------------------
+struct Kv4Rows {
+  const void *k, *v;           // bf16 [rows, hkv * head_dim], pitches ldk and ldv
+  long long ldk, ldv;
+  const int* slots;            // [rows]: block * block_size + offset, negative: none
+  uint8_t *k_cache, *v_cache;  // [num_blocks, hkv, block_size, head_dim / 2 + 4]
+  int* status;
+  int rows, hkv, head_dim, block_size, num_blocks;
+};
+void kv4_write(const Kv4Rows& p, cudaStream_t s);
+void kv4_read(const Kv4Rows& p, float* out, cudaStream_t s);      // rows of k_cache as fp32 [rows, hkv * head_dim]; 0 where there is no slot
+
+// ---- blocks that a query row reads (block_select.cu) ----------------------------------
+struct BoundsParams {
+  const void* k_cache;         // [num_blocks, hkv, block_size, row of head_dim values]
+  int8_t* bounds;              // [num_blocks, hkv, 2 * head_dim + 16]
+  const int* slots;            // [rows]
+  int* status;
+  int rows, hkv, head_dim, block_size, num_blocks;
+};
+void kv_bounds(const BoundsParams& p, int kind, cudaStream_t s);      // kind: 0 bf16, 1 e4m3, kKv4
+constexpr int kMostSelectBlocks = 48 * 1024;           // of a text
+struct SelectParams {
+  SpanParams rows;             // q, block_tables, q_starts, kv_lens, status and sizes; group 1
+  const int8_t* bounds;
+  int group, block_size, count, lead, tail;
+  int stride;                  // blocks of the longest text, at most
+  float* scores;               // [rows][hkv][stride]
+  int* out;                    // [rows][hkv][count]
+  int row_from;
+  int pieces;                  // set by the launcher
+};
+int select_blocks(SelectParams p, cudaStream_t s);     // kernels launched
 
 // ---- sampling -----------------------------------------------------------------------
 struct SampleRow {

@@ -12,6 +12,8 @@ from typing import Optional
 import torch
 
 from ._lib import load_cuda
+from .blocks import BlocksNative
+from .kv4 import Kv4Native, is_kv4
 from .latent import LatentNative
 from .maps import MapsNative
 from .prenorm import PreNormNative
@@ -35,7 +37,7 @@ class Deferred:
         return (self.rows, self.cols)
 
 
-class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNative, SpanNative):
+class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNative, SpanNative, Kv4Native, BlocksNative):
     name = "sm100a"
 
     def __init__(self, device: torch.device, workspace_bytes: int = 96 << 20, part: str = ""):
@@ -150,9 +152,13 @@ class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNa
         sequence (the generic kernel's visibility limit), the tensor-core kernels take the flag. `first`: so many tokens
         at the start of the text stay visible when the window has moved past them (causal, with `meta`; the rows of a
         sequence are its last ones; head dims 64, 128 and 256, blocks of a multiple of 16 tokens). No window: 0, or, without
-        `first`, any negative one."""
+        `first`, any negative one. A cache of 4-bit rows (uint8, head_dim / 2 + 4 to a row) needs `meta` as well."""
         if first:
             _check_span(window, first, bidirectional)
+        if is_kv4(k_cache, head_dim):
+            if bidirectional:
+                raise ValueError("attention over a 4-bit cache is causal")
+            return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, max(window, 0), first, sinks, softcap, meta)
         if first and window:
             return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta)
         out = torch.empty(q.shape[0], hq * head_dim, dtype=q.dtype, device=q.device)
@@ -212,8 +218,8 @@ class NativeOps(RecurrentNative, LatentNative, TiedNative, MapsNative, PreNormNa
         if meta is not None:
             return self._attention_span(q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta,
                                         tree_mask, tree_base)
-        if first:
-            raise ValueError("attention_tree: first tokens need the step batch (meta)")
+        if first or is_kv4(k_cache, head_dim):
+            raise ValueError("attention_tree: first tokens and caches of 4 bits need the step batch (meta)")
         out = torch.empty(q.shape[0], hq * head_dim, dtype=q.dtype, device=q.device)
         self.k.attention_generic(q, k_cache, v_cache, block_tables, row_seq, positions, out, hq, hkv, head_dim,
                                  float(scale), int(window), sinks, float(softcap), tree_mask, tree_base)

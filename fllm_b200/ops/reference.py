@@ -11,6 +11,8 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from .blocks import BlocksRef
+from .kv4 import Kv4Ref, cache_rows, cache_values
 from .latent import LatentRef
 from .maps import MapsRef
 from .prenorm import PreNormRef
@@ -19,7 +21,7 @@ from .tied import TiedRef
 from .recurrent import RecurrentRef
 
 
-class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef, SpanRef):
+class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef, SpanRef, Kv4Ref, BlocksRef):
     name = "reference"
 
     # ---------------------------------------------------------------- dense
@@ -87,8 +89,8 @@ class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef, SpanRef):
             ok = slots >= 0
             sl = slots[ok].long()
             blk, off = sl // bs, sl % bs
-            k_cache[blk, :, off] = k[ok].to(k_cache.dtype)
-            v_cache[blk, :, off] = v[ok].to(v_cache.dtype)
+            k_cache[blk, :, off] = cache_rows(k[ok], k_cache)
+            v_cache[blk, :, off] = cache_rows(v[ok], v_cache)
         return qkv[:, : hq * head_dim]
 
     def glu(self, x, act_kind=0, alpha=1.702, limit=7.0, layout=0):
@@ -140,8 +142,8 @@ class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef, SpanRef):
             begin = max(0, n - window) if window > 0 else 0
             nblk = (n + bs - 1) // bs
             blocks = block_tables[seq, :nblk].long()
-            k = k_cache[blocks].float().permute(1, 0, 2, 3).reshape(hkv, nblk * bs, head_dim)[:, begin:n]
-            v = v_cache[blocks].float().permute(1, 0, 2, 3).reshape(hkv, nblk * bs, head_dim)[:, begin:n]
+            k = cache_values(k_cache[blocks], head_dim).permute(1, 0, 2, 3).reshape(hkv, nblk * bs, head_dim)[:, begin:n]
+            v = cache_values(v_cache[blocks], head_dim).permute(1, 0, 2, 3).reshape(hkv, nblk * bs, head_dim)[:, begin:n]
             k = k.repeat_interleave(g, 0)
             v = v.repeat_interleave(g, 0)
             s = torch.einsum("hd,hnd->hn", qf[t], k) * scale
@@ -197,8 +199,8 @@ class RefOps(RecurrentRef, LatentRef, TiedRef, MapsRef, PreNormRef, SpanRef):
             seq, n, base, mask = int(row_seq[t]), int(positions[t]) + 1, int(tree_base[t]), int(tree_mask[t]) & ((1 << 64) - 1)
             nblk = (n + bs - 1) // bs
             blocks = block_tables[seq, :nblk].long()
-            k = k_cache[blocks].float().permute(1, 0, 2, 3).reshape(hkv, nblk * bs, head_dim)[:, :n]
-            v = v_cache[blocks].float().permute(1, 0, 2, 3).reshape(hkv, nblk * bs, head_dim)[:, :n]
+            k = cache_values(k_cache[blocks], head_dim).permute(1, 0, 2, 3).reshape(hkv, nblk * bs, head_dim)[:, :n]
+            v = cache_values(v_cache[blocks], head_dim).permute(1, 0, 2, 3).reshape(hkv, nblk * bs, head_dim)[:, :n]
             vis = torch.tensor([j < base or ((mask >> (j - base)) & 1) == 1 for j in range(n)], device=q.device)
             s = torch.einsum("hd,hnd->hn", qf[t], k.repeat_interleave(g, 0)) * scale
             if softcap > 0:

@@ -15,6 +15,8 @@ from typing import List, Sequence, Tuple
 
 import torch
 
+from .kv4 import cache_values
+
 
 def ordered_copies(pairs: Sequence[Tuple[int, int]], blocks: int) -> List[List[Tuple[int, int]]]:
     """Copies of blocks that are meant one after the other, in groups that may run at once: no group writes a block that it reads or writes
@@ -53,8 +55,7 @@ class SpanRef:
             if not len(tok):
                 continue                                   # nothing is seen: 0, whatever the sink
             page = tables[s, tok // bs].long()
-            k = k_cache[page, :, tok % bs].float().repeat_interleave(g, 1)
-            v = v_cache[page, :, tok % bs].float().repeat_interleave(g, 1)
+            k, v = (cache_values(c[page, :, tok % bs], head_dim).repeat_interleave(g, 1) for c in (k_cache, v_cache))
             x = torch.einsum("hd,nhd->hn", q[t].float().view(hq, head_dim), k) * scale
             if softcap > 0:
                 x = softcap * torch.tanh(x / softcap)
@@ -107,11 +108,11 @@ class SpanRef:
 
 
 class SpanNative:
-    def _attention_span(self, q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta, tree_mask=None, tree_base=None):
+    def _attention_span(self, q, k_cache, v_cache, block_tables, hq, hkv, head_dim, scale, window, first, sinks, softcap, meta, tree_mask=None, tree_base=None, picks=None):
         if meta is None or meta.q_starts is None or meta.seq_lens is None:
             raise ValueError("this attention takes its rows from the step batch: q_starts, seq_lens and their bounds")
         out, n = self.k.attention_span(q, k_cache, v_cache, block_tables, meta.q_starts, meta.seq_lens, meta.num_seqs, meta.max_q_len, meta.min_q_len,
-                                       meta.max_kv_len, hq, hkv, head_dim, scale, window, first, sinks, softcap, tree_mask, tree_base, self.status)
+                                       meta.max_kv_len, hq, hkv, head_dim, scale, window, first, sinks, softcap, tree_mask, tree_base, self.status, picks)
         self.launches += n
         return out
 
