@@ -3,10 +3,11 @@
 //
 // A key is z + s c with codes c of 0 to 15, so q . k = s (q . c) + z sum(q): the product is one of queries with codes, step and lowest value come to a
 // score once for each token. In the same way o = sum_t (p_t s_t) (c_t - 8) + sum_t p_t (z_t + 8 s_t): the step goes into the weight, the second sum is one
-// number a row. So codes are never widened to values. Of keys a code is a 16-bit operand as it lies in a word: the bits of c are those of the f16 number
-// c 2^-24 (a denormal, which the tensor cores multiply exactly), those of c << 4 are c 2^-20. A word's eight codes are four registers of two, by a mask each
-// and a shift for the last two; registers of odd codes hold 16 times as much, which queries (times 1/16 there) or the sums of odd dims make up for. Codes of
-// values are counted from the middle of their range, one subtraction more to a register: sums of c alone grow with the text where those of values do
+// number a row. So codes are never widened to values: a code is a 16-bit operand as it lies in a word. The bits of c are those of the f16 number c 2^-24 (a
+// denormal, which the tensor cores multiply exactly), those of c << 4 are c 2^-20. A word's eight codes are four registers of two, by a mask each and a
+// shift for the last two; registers of odd codes hold 16 times as much, which queries (times 1/16 there) or the sums of odd dims make up for. (e4m3 operands,
+// of which a byte with a code in it is one as it is, took a quarter longer.) Codes of values are counted from the middle of their range, in that 8 times
+// the sum of the weights, a product with ones, is taken off the sums every eighth turn: sums of c alone grow with the text where those of values do
 // not, and what the tensor cores cut off of each (it is not rounded) grew to 7e-4 of the outputs over 18,000 tokens.
 //
 // Scores are transposed, S^T = K Q^T and O^T = V^T P^T: the products' 16 rows are tokens and dims, their 8 columns packed rows, so that nothing is computed
@@ -24,6 +25,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_span_rows.cuh"
 #include "kv4.cuh"
@@ -38,8 +40,10 @@ constexpr int kWeightLift = 6;                           // weights are below 2^
 template <int D, int NB>
 struct Kv4Smem {
   static constexpr int kRow = kKv4Row<D>, kPageBytes = kPage * kRow;
-  static constexpr int kPages = D == 256 ? 1 : 2;        // of a turn of a warp
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  // Pages of a turn of a warp. More of them share its maxima, votes and barriers and leave more to do while a result is waited for, fewer leave registers for
+  // more CTAs (64 sequences of 4000 to 32,000 tokens, 8 key heads of 128: 4 and three CTAs an SM 291 us, 2 and four 302, 2 and three 323, 1 and four 355).
+  static constexpr int kPages = D == 256 ? 1 : NB == 1 ? 4 : 2;
+  static constexpr int kStages = D == 256 ? 3 : NB == 1 && D == 128 ? 2 : 3;
   static constexpr int kStage = 2 * kPages * kPageBytes; // K and V
   static constexpr int kRing = 4 * kStages * kStage;
   static constexpr int kMerge = 4 * kSpanRows * (D + 2) * 4 + kSpanRows * (D + 4) * 4;
@@ -51,19 +55,25 @@ struct Kv4Smem {
   static constexpr int kTotal = kInfo + (kBars + 15) / 16 * 16 + kBody + 128;
   static_assert(kPageBytes % 16 == 0 && kQ % 16 == 0 && kInfo % 16 == 0, "shared memory");
 };
-template <int D, int NB> constexpr int kv4_resident() { return D == 256 ? 2 : NB == 2 ? 3 : 4; }
+template <int D, int NB> constexpr int kv4_resident() { return D == 256 || NB == 2 ? 2 : 3; }
 
+__device__ __forceinline__ float pow2_field(int field) { return __uint_as_float((uint32_t)field << 23); }
 __device__ __forceinline__ uint32_t lds32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
 __device__ __forceinline__ void bulk_in(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
                "r"(smem_u32(bar)) : "memory");
 }
-// Codes from the middle of their range, c - 8 (ODD: 16 times that), of bits 0 to 3 (4 to 7) of either half: 1024 + c is a f16 number as it lies.
-template <int ODD>
-__device__ __forceinline__ uint32_t centred(uint32_t w) {
-  const uint32_t up = (w & (ODD ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u, mid = ODD ? 0x64806480u : 0x64086408u;      // 1152, 1032
-  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&up), *reinterpret_cast<const __half2*>(&mid));
-  return *reinterpret_cast<const uint32_t*>(&d);
+// As mma_f16, free to be moved by the compiler; and the first product of a sum.
+__device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 // Which token of a page is row i of the products (0 to 7, and 8 more: + 4). Rows of a page lie 4 bytes next to a multiple of 32, so neighbouring rows share
 // banks; in this order two of 32 lanes meet at most, for keys (a lane's rows i = lane / 4) and for values (i = 2 (lane % 4)).
@@ -73,7 +83,7 @@ template <int D, int NB, int MODE>
 __global__ void __launch_bounds__(128, kv4_resident<D, NB>()) kv4_rows_kernel(const __grid_constant__ SpanParams p) {
   using S = Kv4Smem<D, NB>;
   constexpr int kPages = S::kPages, kStages = S::kStages, RB = S::kRow, W = D / 32;       // W: words of a key row that a lane takes
-  constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
+  constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, kOnes = 0x3C003C00u;
   extern __shared__ __align__(128) uint8_t smem[];
   unsigned long long* bits = reinterpret_cast<unsigned long long*>(smem);                 // [16][4]
   int* bases = reinterpret_cast<int*>(bits + kSpanRows * kSpanWords);
@@ -133,34 +143,36 @@ __global__ void __launch_bounds__(128, kv4_resident<D, NB>()) kv4_rows_kernel(co
   bool bad = false;
   // A warp's pages are kPages neighbours at a time. Their blocks are looked up 32 pages at a time, a lane to a page, ahead of their use.
   constexpr int kTurns = 32 / kPages;
-  auto look = [&](int it, int& page) {
+  auto look = [&](int it, int& tok) {                    // first row in the pool, first token; -1 and kNowhere of a page that is not there
     const int pg = pg0 + (warp + 4 * (it + lane / kPages)) * kPages + lane % kPages;
-    page = -1;
-    if (pg >= pg1) return -1;
-    page = range.piece(pg);
-    const int block = span_block(p, table, page);
+    tok = kNowhere;
+    if (pg >= pg1) return -1LL;
+    const int page = range.piece(pg), block = span_block(p, table, page);
     bad |= block < 0;
-    return block;
+    if (block < 0) return -1LL;
+    tok = page * kPage;
+    return span_pool_row(p, block, kvh, page) * RB;
   };
-  int pages, blocks, pages_next, blocks_next = look(0, pages_next);
+  int toks_now, toks_next;
+  long long at_now, at_next = look(0, toks_next);
   const int my_turns = pg1 > pg0 + warp * kPages ? (pg1 - pg0 - warp * kPages + 4 * kPages - 1) / (4 * kPages) : 0;
   __syncthreads();                                       // the barriers are there
+  int to = 0;                                            // stage of the next turn that is asked for
   auto issue = [&](int it) {
     if (it >= my_turns) return;
-    if (it % kTurns == 0) { blocks = blocks_next; pages = pages_next; blocks_next = look(it + kTurns, pages_next); }
-    const int s = it % kStages, h = lane - it % kTurns * kPages;
-    const bool mine = h >= 0 && h < kPages;
-    const bool there = mine && blocks >= 0;
+    if (it % kTurns == 0) { at_now = at_next; toks_now = toks_next; at_next = look(it + kTurns, toks_next); }
+    const int h = lane - it % kTurns * kPages;
+    const bool mine = (unsigned)h < (unsigned)kPages, there = mine && at_now >= 0;
     const unsigned asked = __ballot_sync(0xffffffffu, there);
-    if (mine) my_tok[s * kPages + h] = there ? pages * kPage : kNowhere;
-    if (lane == 0) mbar_expect_tx(my_bars + s, __popc(asked) * 2 * S::kPageBytes);
+    if (mine) my_tok[to * kPages + h] = toks_now;
+    if (lane == 0) mbar_expect_tx(my_bars + to, __popc(asked) * 2 * S::kPageBytes);
     __syncwarp();
     if (there) {
-      const size_t off = (size_t)span_pool_row(p, blocks, kvh, pages) * RB;
-      uint8_t* st = my_ring + s * S::kStage + h * 2 * S::kPageBytes;
-      bulk_in(st, static_cast<const uint8_t*>(p.k_cache) + off, S::kPageBytes, my_bars + s);
-      bulk_in(st + S::kPageBytes, static_cast<const uint8_t*>(p.v_cache) + off, S::kPageBytes, my_bars + s);
+      uint8_t* st = my_ring + to * S::kStage + h * 2 * S::kPageBytes;
+      bulk_in(st, static_cast<const uint8_t*>(p.k_cache) + at_now, S::kPageBytes, my_bars + to);
+      bulk_in(st + S::kPageBytes, static_cast<const uint8_t*>(p.v_cache) + at_now, S::kPageBytes, my_bars + to);
     }
+    to = to + 1 == kStages ? 0 : to + 1;
   };
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) issue(s);
@@ -227,124 +239,107 @@ __global__ void __launch_bounds__(128, kv4_resident<D, NB>()) kv4_rows_kernel(co
     }
   const int k_at = token_of(g) * RB, v_at = token_of(2 * t) * RB;
 
-  float o[NB][D / 16][4];
-  float m[NB][2], l[NB][2], zs[NB][2];     // reference, sum of weights, sum of weights times the middles of ranges
+  float o[NB][D / 16][4], sum[NB][4];      // sum: of the operands of a row's weights, since it was taken off o
+  float m[NB][2], ref[NB][2], l[NB][2], zs[NB][2];       // reference (0 as long as there is none), sum of weights, sum of weights times the middles of ranges
   int unit = 8;                            // U: exponent field that all steps are below, with some room
+  float step_limit = pow2_field(unit + 1), of_step = pow2_field(2 * 127 + kWeightLift - unit);
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) { m[n][h] = -INFINITY; l[n][h] = zs[n][h] = 0.f; }
+    for (int h = 0; h < 2; ++h) { m[n][h] = -INFINITY; ref[n][h] = l[n][h] = zs[n][h] = 0.f; }
   }
-  bool ok = true;
-  int it = 0;
-  for (; it < my_turns; ++it) {
-    issue(it + kStages - 1);
-    const int s = it % kStages;
-    if (!mbar_wait_warp(my_bars + s, (it / kStages) & 1, abort_flag)) { ok = false; break; }
-    const uint8_t* st = my_ring + s * S::kStage;
+  // One turn: the pages at `st`. FULL: all rows see all of it, and there is no soft-cap.
+  auto turn = [&](const uint8_t* st, const int* toks, auto full_turn) {
+    constexpr bool FULL = decltype(full_turn)::value;
     float x[NB][kPages][4];
-    int tok0[kPages];
-    bool full = true;
-#pragma unroll
-    for (int h = 0; h < kPages; ++h) {
-      tok0[h] = my_tok[s * kPages + h];
-      full = full && tok0[h] + kPage <= min_base && (tok0[h] >= max_beg || tok0[h] + kPage <= p.first);
-#pragma unroll
-      for (int n = 0; n < NB; ++n) x[n][h][0] = x[n][h][1] = x[n][h][2] = x[n][h][3] = 0.f;
-    }
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int h = 0; h < kPages; ++h) {
-        const uint8_t* row = st + h * 2 * S::kPageBytes + k_at + (t + 4 * i) * 4;
-        uint32_t a = lds32(row), b = lds32(row + 4 * RB);
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int h = 0; h < kPages; ++h) {
+          const uint8_t* row = st + h * 2 * S::kPageBytes + k_at + (t + 4 * i) * 4;
+          const uint32_t a = lds32(row) >> 8 * k, b = lds32(row + 4 * RB) >> 8 * k;
           const uint32_t op[4] = {a & kLow, b & kLow, a & kHigh, b & kHigh};
 #pragma unroll
-          for (int n = 0; n < NB; ++n) mma_f16(x[n][h], op, qf[n][i][2 * k], qf[n][i][2 * k + 1]);
-          a >>= 8;
-          b >>= 8;
+          for (int n = 0; n < NB; ++n) {
+            if (i == 0 && k == 0) mma_first(x[n][h], op, qf[n][0][0], qf[n][0][1]);
+            else mma_add(x[n][h], op, qf[n][i][2 * k], qf[n][i][2 * k + 1]);
+          }
         }
-      }
     Kv4Scale vs[kPages][2];                // of values, the middle of the range instead of its lowest value
-    bool more = false;                     // a score or a step is out of reach of its reference
 #pragma unroll
     for (int h = 0; h < kPages; ++h) {
       const uint8_t* tail = st + h * 2 * S::kPageBytes + k_at + D / 2;
-      const Kv4Scale ks[2] = {kv4_scale_of(lds32(tail)), kv4_scale_of(lds32(tail + 4 * RB))};
-      vs[h][0] = kv4_scale_of(lds32(tail + S::kPageBytes));
-      vs[h][1] = kv4_scale_of(lds32(tail + S::kPageBytes + 4 * RB));
-      vs[h][0].low = fmaf(8.f, vs[h][0].step, vs[h][0].low);
-      vs[h][1].low = fmaf(8.f, vs[h][1].step, vs[h][1].low);
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = e & 1, tk = e >> 1;
-          float v = fmaf(x[n][h][e], ks[tk].step, ks[tk].low * qs[n][r]) * fac[n][r];
-          if (p.softcap > 0.f) v = p.softcap * tanhf(v / (p.softcap * kLog2e)) * kLog2e;
-          if (!full) {
-            const int tok = tok0[h] + token_of(g) + 4 * tk;
-            if (!span_sees(p, tok, base[n][r], beg[n][r], bits + (8 * n + 2 * t + r) * kSpanWords)) v = -INFINITY;
-          }
-          x[n][h][e] = v;
-          more |= v > m[n][r] + kRefSlack;
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < kPages; ++h)
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk) {
-        const int e = __float_as_uint(vs[h][tk].step) >> 23 & 0xFF;
-        if (full) {
-          more |= e > unit && e != 0xFF;
-        } else {
-          bool seen = false;
+        const Kv4Scale ks = kv4_scale_of(lds32(tail + 4 * tk * RB));
+        vs[h][tk] = kv4_scale_of(lds32(tail + S::kPageBytes + 4 * tk * RB));
+        vs[h][tk].low = fmaf(8.f, vs[h][tk].step, vs[h][tk].low);
+        bool any = false;
 #pragma unroll
-          for (int n = 0; n < NB; ++n) seen |= x[n][h][2 * tk] != -INFINITY || x[n][h][2 * tk + 1] != -INFINITY;
-          if (!seen) vs[h][tk] = {0.f, 0.f};             // of a place that none of the lane's rows sees
-          more |= seen && e > unit && e != 0xFF;
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float v = fmaf(x[n][h][2 * tk + r], ks.step, ks.low * qs[n][r]) * fac[n][r];
+            if constexpr (!FULL) {
+              if (p.softcap > 0.f) v = p.softcap * tanhf(v / (p.softcap * kLog2e)) * kLog2e;
+              const int tok = toks[h] + token_of(g) + 4 * tk;
+              const bool sees = span_sees(p, tok, base[n][r], beg[n][r], bits + (8 * n + 2 * t + r) * kSpanWords);
+              if (!sees) v = -INFINITY;
+              any |= sees;
+            }
+            x[n][h][2 * tk + r] = v;
+          }
+        if constexpr (!FULL) {
+          if (!any) vs[h][tk] = {0.f, 0.f};              // of a place that none of the lane's rows sees
         }
       }
+    }
+    float top[NB][2], steepest = fmaxf(vs[0][0].step, vs[0][1].step);      // largest scores and steps of a lane
+#pragma unroll
+    for (int h = 1; h < kPages; ++h) steepest = fmaxf(fmaxf(steepest, vs[h][0].step), vs[h][1].step);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        top[n][r] = fmaxf(x[n][0][r], x[n][0][2 + r]);
+#pragma unroll
+        for (int h = 1; h < kPages; ++h) top[n][r] = fmaxf(fmaxf(top[n][r], x[n][h][r]), x[n][h][2 + r]);
+      }
+    bool more = steepest >= step_limit;    // a score or a step is out of reach of its reference
+#pragma unroll
+    for (int n = 0; n < NB; ++n) more |= top[n][0] > m[n][0] + kRefSlack || top[n][1] > m[n][1] + kRefSlack;
     if (__any_sync(0xffffffffu, more)) {
-      int top = 0;
-#pragma unroll
-      for (int h = 0; h < kPages; ++h)
-#pragma unroll
-        for (int tk = 0; tk < 2; ++tk) {
-          const int e = __float_as_uint(vs[h][tk].step) >> 23 & 0xFF;
-          if (e != 0xFF) top = max(top, e);
-        }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const int was = unit;
-      if (top > unit) unit = min(top + 2, 254);
-      const float shrink = unit == was ? 1.f : __uint_as_float((uint32_t)max(127 + was - unit, 0) << 23);
+      const int field = __reduce_max_sync(0xffffffffu, (int)(__float_as_uint(steepest) >> 23)), was = unit;
+      if (field > unit) unit = min(field + 2, 254);
+      const float shrink = unit == was ? 1.f : pow2_field(max(127 + was - unit, 0));
+      step_limit = unit == 254 ? INFINITY : pow2_field(unit + 1);
+      of_step = pow2_field(2 * 127 + kWeightLift - unit);
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int h = 0; h < kPages; ++h) mx = fmaxf(mx, fmaxf(x[n][h][r], x[n][h][2 + r]));
+          float mx = top[n][r];
 #pragma unroll
           for (int d = 4; d <= 16; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           const float mn = fmaxf(m[n][r], mx);
           const float c = mn == -INFINITY ? 1.f : ex2(m[n][r] - mn);
           m[n][r] = mn;
+          ref[n][r] = mn == -INFINITY ? 0.f : mn;
           l[n][r] *= c;
           zs[n][r] *= c;
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) { o[n][i][r] *= c * shrink; o[n][i][2 + r] *= c * shrink; }
+          sum[n][r] *= c * shrink;
         }
     }
-    const float of_step = __uint_as_float((uint32_t)min(127 + 127 + kWeightLift - unit, 254) << 23);
     uint32_t pt[NB][kPages][2];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const float ref[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
 #pragma unroll
       for (int h = 0; h < kPages; ++h)
 #pragma unroll
@@ -352,16 +347,26 @@ __global__ void __launch_bounds__(128, kv4_resident<D, NB>()) kv4_rows_kernel(co
           float w[2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float v = x[n][h][2 * tk + r], e = ex2(v - ref[r]);
+            const float v = x[n][h][2 * tk + r], e = ex2(v - ref[n][r]);
             l[n][r] += e;
             w[r] = e * (vs[h][tk].step * of_step);
-            float z = e * vs[h][tk].low;
-            if (!full && v == -INFINITY) w[r] = z = 0.f;
-            zs[n][r] += z;
+            if constexpr (FULL) {
+              zs[n][r] = fmaf(e, vs[h][tk].low, zs[n][r]);
+            } else {
+              if (v == -INFINITY) w[r] = 0.f;
+              else zs[n][r] = fmaf(e, vs[h][tk].low, zs[n][r]);
+            }
           }
           pt[n][h][tk] = transposed(pack_16<true>(w[0], w[1]));
         }
     }
+#pragma unroll
+    for (int h = 0; h < kPages; ++h)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const uint32_t ones[4] = {kOnes, kOnes, kOnes, kOnes};
+        mma_add(sum[n], ones, pt[n][h][0], pt[n][h][1]);
+      }
 #pragma unroll
     for (int h = 0; h < kPages; ++h)
 #pragma unroll
@@ -371,21 +376,54 @@ __global__ void __launch_bounds__(128, kv4_resident<D, NB>()) kv4_rows_kernel(co
         uint32_t a = __byte_perm(w0, w1, 0x5410), b = __byte_perm(w0, w1, 0x7632), c = __byte_perm(w2, w3, 0x5410), d = __byte_perm(w2, w3, 0x7632);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint32_t even[4] = {centred<0>(a), centred<0>(b), centred<0>(c), centred<0>(d)};
-          const uint32_t odd[4] = {centred<1>(a), centred<1>(b), centred<1>(c), centred<1>(d)};
+          const uint32_t even[4] = {a & kLow, b & kLow, c & kLow, d & kLow}, odd[4] = {a & kHigh, b & kHigh, c & kHigh, d & kHigh};
 #pragma unroll
           for (int n = 0; n < NB; ++n) {
-            mma_f16(o[n][4 * i + 2 * k], even, pt[n][h][0], pt[n][h][1]);
-            mma_f16(o[n][4 * i + 2 * k + 1], odd, pt[n][h][0], pt[n][h][1]);
+            mma_add(o[n][4 * i + 2 * k], even, pt[n][h][0], pt[n][h][1]);
+            mma_add(o[n][4 * i + 2 * k + 1], odd, pt[n][h][0], pt[n][h][1]);
           }
           a >>= 8; b >>= 8; c >>= 8; d >>= 8;
         }
       }
+  };
+  // Sums of codes become sums of codes from the middle of their range.
+  auto centre = [&] {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const float unit8 = 8.f / (i & 1 ? 1 << 20 : 1 << 24);
+          o[n][i][r] = fmaf(sum[n][r], -unit8, o[n][i][r]);
+          o[n][i][2 + r] = fmaf(sum[n][r], -unit8, o[n][i][2 + r]);
+        }
+        sum[n][r] = 0.f;
+      }
+  };
+  bool ok = true;
+  int it = 0, from = 0, phase = 0;
+  for (; it < my_turns; ++it) {
+    issue(it + kStages - 1);
+    if (!mbar_wait_warp(my_bars + from, phase, abort_flag)) { ok = false; break; }
+    const uint8_t* st = my_ring + from * S::kStage;
+    int toks[kPages];
+    bool full = p.softcap <= 0.f;
+#pragma unroll
+    for (int h = 0; h < kPages; ++h) {
+      toks[h] = my_tok[from * kPages + h];
+      full = full && toks[h] + kPage <= min_base && (toks[h] >= max_beg || toks[h] + kPage <= p.first);
+    }
+    if (full) turn(st, toks, std::true_type{});
+    else turn(st, toks, std::false_type{});
+    if ((it & 7) == 7) centre();
     __syncwarp();                          // the stage is free
+    if (++from == kStages) { from = 0; phase ^= 1; }
   }
+  centre();
   if (!ok) {                               // copies that are on their way land before the memory is another CTA's
     for (int k = 1; k < kStages; ++k)
-      if (it + k < my_turns && it + k <= it + kStages - 1) {
+      if (it + k < my_turns) {
         int none = 0;
         mbar_wait_warp(my_bars + (it + k) % kStages, ((it + k) / kStages) & 1, &none);
       }
@@ -398,8 +436,8 @@ __global__ void __launch_bounds__(128, kv4_resident<D, NB>()) kv4_rows_kernel(co
   float* mml = mo + 4 * kSpanRows * D;                   // [4][16][2]
   float* part_o = mml + 4 * kSpanRows * 2;               // [16][D]: the CTA's
   float4* part_ml = reinterpret_cast<float4*>(part_o + kSpanRows * D);      // [16]
-  // of a row's dims a lane has 8 (g + 8 i) + 0 to 7; products were with c - 8 (16 times that of odd dims), weights times 2^(kWeightLift + 127 - unit)
-  const float back = __uint_as_float((uint32_t)unit << 23), even = 1.f / (1 << kWeightLift), odd = even * 0.0625f;
+  // of a row's dims a lane has 8 (g + 8 i) + 0 to 7; products were with c 2^-24 (2^-20 of odd dims), weights times 2^(kWeightLift + 127 - unit)
+  const float back = pow2_field(unit), even = (float)(1 << (24 - kWeightLift)), odd = even * 0.0625f;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll

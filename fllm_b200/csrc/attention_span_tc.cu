@@ -12,6 +12,7 @@
 //   warps 0 - 7   softmax        warp 9   issuer
 //   bf16 cache    warps 8, 10 ask for K by TMA, warp 11 for V; it also looks through V where not every row sees the whole tile
 //   e4m3 cache    K is an operand as it is, with queries in two e4m3 pieces; V travels as f16: warp 8 asks for both, warps 10 - 15 widen V
+//   4-bit cache   warps 10 - 15 widen K and V (kv4.cuh) to f16, which warp 8 asks for tile by tile; queries are f16
 //
 // What bounds it (times from captured graphs): two tiles of 128 x 128 scores take the softmax groups some 3200 clocks, the tensor pipe 2048 at heads of 128; and a CTA's way in (lengths,
 // table, queries, keys, first products: 9000 clocks) and out (4000), which nothing on its SM runs under. 2 x 2048 rows behind 4096 tokens without a window, 32
@@ -31,29 +32,33 @@
 
 #include "attention_span.cuh"
 #include "attention_util.cuh"
+#include "kv4.cuh"
 #include "tma_host.h"
 
 namespace fllm {
 namespace {
 constexpr int kTcRows = 256, kWideners = 6;       // packed rows of a CTA; warps that widen V of an e4m3 cache
-template <bool KV8> constexpr int tc_threads() { return KV8 ? 512 : 384; }
-template <bool KV8> constexpr int kQThreads = KV8 ? 384 : 256;      // that load queries
+constexpr int kBf16 = 0, kE4m3 = 1;        // kinds of caches, and kKv4
+template <int KV> constexpr int tc_threads() { return KV == kBf16 ? 384 : 512; }
+template <int KV> constexpr int kQThreads = KV == kE4m3 ? 384 : 256;      // that load queries
 constexpr float kTcLift = 6.f;             // f16 weights: their reference lies so far below the row's (their largest is 2^14 then)
 constexpr int kTilePages = kTile / kPage;
 template <int N> using Int = std::integral_constant<int, N>;
 template <bool B> using Bool = std::integral_constant<bool, B>;
 
 constexpr int kRawTokens = 64;             // of a piece of an e4m3 tile
-constexpr int kTcFlags = 384;              // bytes of barriers and flags
+constexpr int kKv4Slots = 3;               // of tiles of 4-bit rows
+constexpr int kKv4Top = -6;                // their largest magnitude is below 2 to this as f16 (kv4_widen_f16)
+constexpr int kTcFlags = 400;              // bytes of barriers and flags
 
 // Shared memory: two tiles of Q, two stages of K and of V, 16-bit values in rows of 128 bytes. e4m3: Q in two e4m3 pieces, four stages of K as it
-// is, V in 16 bits behind four slots of raw halves of tiles (eight where there is one tile of Q).
-template <int D, bool KV8>
+// is, V in 16 bits behind four slots of raw halves of tiles (eight where there is one tile of Q). 4 bits: three slots of raw tiles of K or V.
+template <int D, int KV>
 struct TcSmem {
   static constexpr int kT = tile_bytes<D>();           // a 128-row tile of 16-bit values
-  static constexpr int kStages = KV8 ? 4 : 2, kK = KV8 ? kTile * D : kT;      // of K
-  static constexpr int kRaw = KV8 ? kRawTokens * D : 0;
-  static constexpr int kTiles = 6 * kT + 4 * kRaw;
+  static constexpr int kStages = KV == kE4m3 ? 4 : 2, kK = KV == kE4m3 ? kTile * D : kT;      // of K
+  static constexpr int kRaw = KV == kE4m3 ? kRawTokens * D : KV == kKv4 ? kTile * kKv4Row<D> : 0;
+  static constexpr int kTiles = 6 * kT + (KV == kKv4 ? kKv4Slots : 4) * kRaw;
   static constexpr int kTotal = kTiles + kTcFlags + kTcRows * 4 + 1024;
 };
 
@@ -86,6 +91,7 @@ __device__ __forceinline__ uint32_t pack_16(float lo, float hi) {
     return pack_bf16x2(lo, hi);
   }
 }
+__device__ __forceinline__ float pow2_of(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // bits [lo, hi) of 32
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   lo = max(lo, 0);
@@ -141,11 +147,11 @@ __device__ __noinline__ void cap_scores(uint32_t t_s, float cap_in) {
 }
 
 // A row's softmax over one tile of 128 tokens: scores in registers, weights as 16-bit values over the scores' first columns, the first 64 of them
-// handed over before the others are computed; O of the warp is rescaled when a row's maximum has moved by more than 2^8. Scores that the row
+// handed over before the others are computed; O of the warp is rescaled when a row's maximum has moved by more than 2^8, or its unit by `shrink`. Scores that the row
 // does not see become -inf first, 32 columns at a time where some row of the warp does not see them all.
 template <int D, bool F16>
 __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, bool whole, const uint4& visible, float scale, bool have_o, uint64_t* p_half,
-                                             float& m_used, float& l) {
+                                             float& m_used, float& l, float shrink = 1.f) {
   uint32_t s[4][32];
 #pragma unroll
   for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, s[c]);
@@ -167,7 +173,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, bool wh
   // the scale is positive, so it commutes with the maximum
   const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
   const bool grow = m > m_used + kLazyRescale || (m_used == -INFINITY && m > -INFINITY);
-  if (__any_sync(0xffffffffu, grow)) {
+  if (__any_sync(0xffffffffu, grow || shrink != 1.f)) {
     const float m_new = fmaxf(m_used, m);
     const float corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
     m_used = m_new;
@@ -179,7 +185,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, bool wh
         tmem_ld_32x16(t_o + 16 * c, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * (corr * shrink));
         tmem_st_32x16(t_o + 16 * c, o);
       }
     }
@@ -235,14 +241,15 @@ __device__ __forceinline__ uint64_t desc_k_major(uint32_t saddr) {
 
 // Queries of rows [0, tiles x 128) to shared memory in swizzled rows, by THREADS threads, `tid` of them this one. Beside an e4m3 cache: two e4m3
 // pieces, of the value times a power of two per row (its largest magnitude is between 2^7 and 2^8 then) and of what that leaves, four bits each of
-// a bf16's eight. Exact down to 2^-9 of the row's largest value, within 2^-17 of that value below. bf16: asynchronous copies.
-template <int D, bool F16, int THREADS>
+// a bf16's eight. Exact down to 2^-9 of the row's largest value, within 2^-17 of that value below. 4 bits: f16, times a power of two per row (between 2^14 and
+// 2^15; within 2^-38 of the largest), dims in the order of kv4_widen_f16. bf16: asynchronous copies.
+template <int D, int KV, int THREADS>
 __device__ __forceinline__ void load_q(const SpanParams& p, int tid, uint8_t* sq, float* factors, int tiles, int q0, int row0, int n_rows, int kvh) {
   constexpr int C = D / 8, kStep = THREADS / C;        // rows between those of a thread
   const int c = tid % C, r0 = tid / C;
   RowWalk at(row0 + r0, kStep, p.group);
   const bf16* head = static_cast<const bf16*>(p.q) + (size_t)q0 * p.ldq + (size_t)kvh * p.group * D + c * 8;
-  if constexpr (!F16) {
+  if constexpr (KV == kBf16) {
 #pragma unroll 2
     for (int r = r0; r < tiles * kRows; r += kStep, at.next()) {
       const bool valid = r < n_rows;
@@ -270,8 +277,21 @@ __device__ __forceinline__ void load_q(const SpanParams& p, int tid, uint8_t* sq
         for (int o = C / 2; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
         const int top = (int)(max(most & 0xFFFFu, most >> 16) >> 7);      // largest exponent field of the row
         const bool odd = top == 0xFF;                  // an infinity or a NaN: no score of the row is a number (a soft-cap would make 1 of an infinite one: NaN here)
-        const int up = odd ? 0 : min(127 + 7 - top, 126);
+        const int up = odd ? 0 : min(127 + (KV == kKv4 ? 14 : 7) - top, 126);
         const float f = odd ? __int_as_float(0x7FC00000) : __uint_as_float((uint32_t)(127 + up) << 23);
+        if constexpr (KV == kKv4) {
+          if (r >= tiles * kRows) continue;
+          uint32_t h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = unpack_bf16x2(w[e]);
+            h[e] = pack_16<true>(x.x * f, x.y * f);
+          }
+          *reinterpret_cast<uint4*>(sq + (r >> 7) * tile_bytes<D>() + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) =
+              make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
+          if (c == 0) factors[r] = span_factor(p.scale_log2, up);
+          continue;
+        }
         uint32_t high[2] = {0, 0}, low[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -408,11 +428,12 @@ __device__ __forceinline__ TileSees tile_sees(const SpanParams& p, int q0, int q
   return t;
 }
 
-template <int D, bool KV8, bool SEARCH>
-__global__ void __launch_bounds__(tc_threads<KV8>(), 1)
+template <int D, int KV, bool SEARCH>
+__global__ void __launch_bounds__(tc_threads<KV>(), 1)
 span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ SpanParams p, int row_tiles, int halved) {
-  using S = TcSmem<D, KV8>;
+  using S = TcSmem<D, KV>;
   constexpr int TB = S::kT;
+  constexpr bool KV8 = KV == kE4m3, KV4 = KV == kKv4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sq = smem, *sk = smem + 2 * TB, *sv = smem + 4 * TB;
@@ -426,23 +447,24 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* odd_met = reinterpret_cast<int*>(tmem_slot + 2);     // values were taken out of tiles of V
+  volatile int *k_up = odd_met + 1, *v_up = k_up + 4;       // [4] by tile: keys and values of a 4-bit cache are times 2 to this
   float* factors = reinterpret_cast<float*>(smem + S::kTiles + kTcFlags);
-  static_assert(38 * 8 + 3 * 4 <= kTcFlags, "barriers and flags");
+  static_assert(38 * 8 + 11 * 4 <= kTcFlags && kTcFlags % 16 == 0, "barriers and flags");
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV8 ? kWideners : 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV == kBf16 ? 1 : kWideners);
     }
-    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], KV8 ? 1 : D / 64); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], KV8 ? 1 : KV4 ? kWideners : D / 64); mbar_init(&k_empty[i], 1); }
     for (int i = 0; i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], kWideners); }
-    mbar_init(o_done, 1); mbar_init(q_full, kQThreads<KV8> / 32);
+    mbar_init(o_done, 1); mbar_init(q_full, kQThreads<KV> / 32);
     *abort_flag = 0;
     *odd_met = 0;
     fence_barrier_init();
   }
-  if (warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); if (!KV8) tma_prefetch_desc(&tma_v); }
+  if (!KV4 && warp == 8 && lane == 0) { tma_prefetch_desc(&tma_k); if (!KV8) tma_prefetch_desc(&tma_v); }
   pdl_wait();
   const int split = blockIdx.y;
   // Whole tiles of the longest sequence come first, those that see the most before others; then what is left of the rows. The last `halved` of the whole
@@ -479,7 +501,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   // Queries: the softmax groups, and beside an e4m3 cache, where there is more to it than to copy them, four of the warps that wait for V. (Whoever
   // asks for K and V is not among them.)
   const bool q_too = KV8 && warp >= 12;
-  if (warp < 8 || q_too) load_q<D, KV8, kQThreads<KV8>>(p, warp < 8 ? (int)threadIdx.x : (int)threadIdx.x - 128, sq, factors, two ? 2 : 1, q0, row0, n_rows, kvh);
+  if (warp < 8 || q_too) load_q<D, KV, kQThreads<KV>>(p, warp < 8 ? (int)threadIdx.x : (int)threadIdx.x - 128, sq, factors, two ? 2 : 1, q0, row0, n_rows, kvh);
 
   const int group = warp >> 2;                         // of softmax warps
   const int r_first = (two ? group * kRows : 0) + (warp & 3) * 32, r = r_first + lane;
@@ -492,6 +514,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const SpanRange range = span_range(p, kPage, sees.min_beg, sees.end);
   const int gap = (range.lo - range.head) * kPage, min_base = sees.min_base - gap, max_beg = sees.max_beg - gap;
   kv_len -= gap;
+  const int any_beg = sees.min_beg - gap, any_end = sees.end - gap;      // tokens that some row sees, the first ones aside
   const int per_piece = (walk + pieces - 1) / pieces;      // (the last one goes on to the end, should that be further)
   const int n_all = (range.count + kTilePages - 1) / kTilePages, t0 = min(split * per_piece, n_all), n_tiles = split == pieces - 1 ? n_all - t0 : min(per_piece, n_all - t0);
   const int shift = two ? 1 : 0, n_items = n_tiles << shift;
@@ -500,9 +523,9 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const PageRows page_rows{p, p.block_tables + (size_t)seq * p.max_blocks, kvh, range.head, range.lo - range.head, range.count,
                            (int)(p.num_blocks * p.hkv * p.block_pages * kPage)};
 
-  // The block was launched with 168 registers a thread (e4m3: 128): 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128.
+  // The block was launched with 168 registers a thread (e4m3 and 4 bits: 128): 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128.
   if (warp >= 8) {
-    if constexpr (KV8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (KV != kBf16) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     bool bad = false;
     if (q_too) {
@@ -512,7 +535,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       asm volatile("bar.arrive 2, 384;" ::: "memory");
     }
     if (warp == 9) {
-      constexpr int fmt = KV8 ? 0 : 1;
+      constexpr int fmt = KV == kBf16 ? 1 : 0;
       constexpr uint32_t idesc_s = make_idesc(128, 128, fmt, fmt);      // (e4m3 x e4m3 has the same bits as f16 x f16)
       constexpr uint32_t idesc_pv = make_idesc(128, D, fmt, fmt) | (1u << 16);     // B is MN-major
       const uint64_t dq = desc_k_major<D, KV8>(smem_u32(sq)), dk = desc_k_major<D, KV8>(smem_u32(sk));
@@ -588,6 +611,118 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         else walk(Bool<false>{});
       }
       __syncwarp();
+    } else if constexpr (KV4) {
+      // Warp 8 asks for tiles, of K one tile ahead of V, through a ring of slots: K0, K1, V0, K2, V1, ... Each of six other warps widens a part of every one.
+      const int part = warp - 10, pieces = 2 * n_tiles;
+      auto piece_at = [&](int x, int& it, bool& is_v) {            // the x-th piece: of which tile, and whether of V
+        const bool last = x == pieces - 1;
+        is_v = last || (x >= 2 && (x & 1) == 0);
+        it = last ? n_tiles - 1 : is_v ? x / 2 - 1 : (x + 1) / 2;
+      };
+      PagesAhead pages_k(page_rows, t0, warp == 8 ? n_tiles : 0), pages_v(page_rows, t0, warp == 8 ? n_tiles : 0);
+      int slot = 0, turn = 0;
+      auto next_slot = [&] { if (++slot == kKv4Slots) { slot = 0; turn ^= 1; } };
+      constexpr int kPageBytes = kPage * kKv4Row<D>;
+      bool ok = true;
+      for (int x = 0; ok && warp == 8 && x < pieces; ++x, next_slot()) {
+        int it;
+        bool is_v;
+        piece_at(x, it, is_v);
+        if (is_v) pages_v.to(it);
+        else pages_k.to(it);
+        if (x >= kKv4Slots && !mbar_wait_warp(&raw_empty[slot], turn ^ 1, abort_flag)) { ok = false; break; }
+        const int now = is_v ? pages_v.now : pages_k.now;
+        uint8_t* at = smem + 6 * TB + slot * S::kRaw;
+        // A page is 16 rows in one piece: the lanes that looked the tile's pages up ask for one each. One that nobody sees, or that is not there, is zeros.
+        const int pg = lane - (it & 3) * kTilePages;
+        const bool mine = pg >= 0 && pg < kTilePages && now != page_rows.none;
+        const uint32_t asked = __ballot_sync(0xffffffffu, mine) >> ((it & 3) * kTilePages);
+        if (asked != (1u << kTilePages) - 1) {
+          for (int i = lane; i < S::kRaw / 16; i += 32)
+            if (!(asked >> (i / (kPageBytes / 16)) & 1)) *reinterpret_cast<uint4*>(at + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();                    // (a later tile comes by a bulk copy)
+          __syncwarp();
+        }
+        if (lane == 0) mbar_expect_tx(&raw_full[slot], __popc(asked) * kPageBytes);
+        __syncwarp();
+        if (mine) bulk_load(at + pg * kPageBytes, static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache) + (size_t)now * kKv4Row<D>, kPageBytes, &raw_full[slot]);
+        __syncwarp();
+      }
+      // A lane takes two words of a row, half a row apart.
+      constexpr int kWords = D / 16, kTurnRows = 32 / kWords, kTurns = kTile / kTurnRows;
+      constexpr int kMost = (kTurns + kWideners - 1) / kWideners, kBatch = 4;
+      const int word = lane % kWords, sub = lane / kWords;
+      int up_v = 127;                                  // values are times 2^up_v
+      for (int x = 0; ok && warp >= 10 && x < pieces; ++x, next_slot()) {
+        int it;
+        bool is_v;
+        piece_at(x, it, is_v);
+        const int b = it & 1, tile0 = (t0 + it) * kTile;
+        ok = mbar_wait_warp(&raw_full[slot], turn, abort_flag) && (it < 2 || mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag));
+        if (!ok) break;
+        const uint8_t* src = smem + 6 * TB + slot * S::kRaw;
+        const bool look = partial(tile0);
+        auto seen = [&](int tok) { return tok < any_end && (tok >= any_beg || tok < p.first); };
+        // The largest magnitude of the tile that some row sees, by every warp for itself, a lane to four rows. It goes below 2^kKv4Top; that of values, whose
+        // sums go over all tiles, only where it is above that of those before, with room for four times as much.
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Kv4Scale k = kv4_scale_of(*reinterpret_cast<const uint32_t*>(src + (32 * i + lane) * kKv4Row<D> + D / 2));
+          const uint32_t field = __float_as_uint(fmaxf(fabsf(k.low), fabsf(fmaf(15.f, k.step, k.low)))) >> 23;
+          if ((!look || seen(tile0 + 32 * i + lane)) && field < 255) most = max(most, field);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        int up = 126 + kKv4Top - (int)most;
+        if (is_v) up = up_v = up < up_v ? up - 2 : up_v;
+        up = min(up, 120);
+        if (part == 0 && lane == 0) (is_v ? v_up : k_up)[it & 3] = up;
+        const float f1 = pow2_of(up >> 1), f2 = pow2_of(up - (up >> 1));
+        bool met = false;
+        uint8_t* const to = is_v ? sv + b * TB : sk + b * TB;
+#pragma unroll 1
+        for (int u0 = 0; u0 < kMost; u0 += kBatch) {
+          uint32_t w[kBatch][2], scale[kBatch];
+          const uint8_t* from = src + ((part + kWideners * u0) * kTurnRows + sub) * kKv4Row<D>;
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u)
+            if (part + kWideners * (u0 + u) < kTurns) {
+              const uint8_t* row = from + u * kWideners * kTurnRows * kKv4Row<D>;
+              w[u][0] = *reinterpret_cast<const uint32_t*>(row + word * 4);
+              w[u][1] = *reinterpret_cast<const uint32_t*>(row + (word + kWords) * 4);
+              scale[u] = *reinterpret_cast<const uint32_t*>(row + D / 2);
+            }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            if (part + kWideners * (u0 + u) >= kTurns) continue;
+            const int tok = (part + kWideners * (u0 + u)) * kTurnRows + sub;
+            const Kv4Scale k = kv4_scale_of(scale[u]);
+            const float step = k.step * f1 * f2, low = k.low * f1 * f2;
+            const uint32_t low2 = pack_16<true>(low, low), even = pack_16<true>(step * 16777216.f, step * 16777216.f), odd = pack_16<true>(step * 1048576.f, step * 1048576.f);
+            uint4 y[2] = {kv4_widen_f16(w[u][0], even, odd, low2), kv4_widen_f16(w[u][1], even, odd, low2)};
+            if (look && is_v) {
+              const bool nan = (scale[u] & 0x7F80u) == 0x7F80u, there = seen(tile0 + tok);      // a row that reads as NaN, one that anybody sees
+              if (nan || !there) y[0] = y[1] = make_uint4(0, 0, 0, 0);
+              met |= nan && there;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = word + h * kWords;
+              uint8_t* line = is_v ? to + (tok >> 4) * (D / 64) * 2048 + (c >> 3) * 2048 + (tok & 15) * 128 : to + (c >> 3) * kHalf + tok * 128;      // V: [page][half][16][64]
+              *reinterpret_cast<uint4*>(line + (((c & 7) ^ (tok & 7)) << 4)) = y[h];
+            }
+          }
+        }
+        if (met) atomicOr(odd_met, 1);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&raw_empty[slot]);
+          mbar_arrive(is_v ? &v_ready[b] : &k_full[b]);
+        }
+        __syncwarp();
+      }
+      bad = pages_k.bad;
     } else if constexpr (!KV8) {
       const bool is_v = warp == 11;
       const int half = warp == 10 ? 1 : 0;
@@ -737,7 +872,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     }
     if (bad && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
   } else {
-    if constexpr (KV8) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if constexpr (KV != kBf16) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     q_loaded();
@@ -745,7 +880,9 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     if (lane == 0) mbar_arrive(q_full);
     if constexpr (KV8) asm volatile("bar.sync 2, 384;" ::: "memory");
     else asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float factor = factors[r], scale = p.softcap > 0.f ? p.softcap * kLog2e : factor;
+    float factor = factors[r], scale = p.softcap > 0.f ? p.softcap * kLog2e : factor;
+    const float row_factor = factor;
+    int up_v = 0;                                      // O is in units of 2^-up_v
     const uint32_t t_s = tmem_base + 128 * group + lane_off, t_o = tmem_base + 256 + 128 * group + lane_off;
     // tokens [w_beg, w_base) are seen by all rows of this warp
     int w_base = min_base, w_beg = max_beg;
@@ -760,16 +897,26 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       const int k = n >> 1, tok0 = (t0 + (n >> shift)) * kTile;
       if (!mbar_wait(&s_full[group], k & 1, abort_flag)) { ok = false; break; }
       tc_fence_after_sync();
+      float shrink = 1.f;
+      if constexpr (KV4) {
+        const int t = n >> shift;
+        if (!mbar_wait(&v_ready[t & 1], (t >> 1) & 1, abort_flag)) { ok = false; break; }      // (done by now, as a rule)
+        const int up = k_up[t & 3], now = v_up[t & 3];
+        factor = row_factor * pow2_of(-(up >> 1)) * pow2_of((up >> 1) - up);
+        if (p.softcap <= 0.f) scale = factor;
+        if (k > 0 && now != up_v) shrink = pow2_of(max(now - up_v, -126));
+        up_v = now;
+      }
       const bool whole = tok0 + kTile <= w_base && (tok0 >= w_beg || tok0 + kTile <= p.first);
       uint4 vis = make_uint4(0, 0, 0, 0);
       if (!whole) vis = row_bits(p, q0, qn, kv_len, gap, qi, tok0);
       if (p.softcap > 0.f) cap_scores(t_s, factor / (p.softcap * kLog2e));
-      softmax_tile<D, KV8>(t_s, t_o, whole, vis, scale, k > 0, &p_half[group], m_used, l);
+      softmax_tile<D, KV != kBf16>(t_s, t_o, whole, vis, scale, k > 0, &p_half[group], m_used, l, shrink);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[group]);
     }
-    if (KV8) m_used -= kTcLift;
+    if (KV != kBf16) m_used -= kTcLift;
     const bool splits = pieces > 1;
     const int G_row = qi >= 0 ? kvh * G + (row0 + r) - qi * G : 0;
     const float sink = p.sinks && qi >= 0 ? p.sinks[G_row] * kLog2e : -INFINITY;
@@ -792,7 +939,11 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
             tmem_ld_32x32(t_o + 32 * c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) swap[(32 * c + i) * kRows + at] = __uint_as_float(o[i]);
+            for (int i = 0; i < 32; ++i) {
+              float v = __uint_as_float(o[i]);
+              if constexpr (KV4) v = v * pow2_of(-(up_v >> 1)) * pow2_of((up_v >> 1) - up_v);
+              swap[(32 * c + i) * kRows + at] = v;
+            }
           }
         }
         swap_ml[at] = make_float2(have ? m_used : -INFINITY, have ? l : 0.f);
@@ -844,10 +995,22 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
             tmem_ld_32x32(t_o + c0 + h, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c_mine);
+            for (int i = 0; i < 32; ++i) {
+              float v = __uint_as_float(o[i]) * c_mine;
+              if constexpr (KV4) v = v * pow2_of(-(up_v >> 1)) * pow2_of((up_v >> 1) - up_v);
+              o[i] = __float_as_uint(v);
+            }
             if (other) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + swap[(c0 + h + i) * kRows + at] * c_other);
+            }
+            if constexpr (KV4) {                       // of eight columns the dims (kv4_widen_f16)
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                const uint32_t d[8] = {o[i], o[i + 2], o[i + 4], o[i + 6], o[i + 1], o[i + 3], o[i + 5], o[i + 7]};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[i + e] = d[e];
+              }
             }
           } else {
 #pragma unroll
@@ -881,10 +1044,15 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
             if (!(vis[i >> 5] >> (i & 31) & 1)) continue;
             const int page = page_rows.page_of((tok0 + i) / kPage), b = span_block(p, page_rows.table, page);
             if (b < 0) continue;
-            const size_t at = (size_t)(span_pool_row(p, b, kvh, page) + (i & 15)) * D;
+            const size_t at = (size_t)(span_pool_row(p, b, kvh, page) + (i & 15)) * (KV4 ? kKv4Row<D> : D);
+            if constexpr (KV4) {                       // a row is NaN as a whole, or a number
+              if ((static_cast<const uint16_t*>(p.v_cache)[(at + D / 2) / 2] & 0x7F80u) != 0x7F80u) continue;
+            }
             for (int d = 0; d < D; ++d) {
               float x;
-              if constexpr (KV8) {
+              if constexpr (KV4) {
+                x = __int_as_float(0x7FC00000);
+              } else if constexpr (KV8) {
                 x = (static_cast<const uint8_t*>(p.v_cache)[at + d] & 0x7F) == 0x7F ? __int_as_float(0x7FC00000) : 0.f;
               } else {
                 x = __bfloat162float(static_cast<const bf16*>(p.v_cache)[at + d]);
@@ -905,21 +1073,21 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   if (threadIdx.x == 0 && *abort_flag && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_MBAR_TIMEOUT);
 }
 
-template <int D, bool KV8>
+template <int D, int KV>
 void launch_tc(SpanParams p, cudaStream_t s) {
   static bool configured[kMaxDevices] = {};
-  constexpr int smem = TcSmem<D, KV8>::kTotal;
+  constexpr int smem = TcSmem<D, KV>::kTotal;
   static_assert(smem <= 227 * 1024, "shared memory");
   if (first_call_on_device(configured)) {
-    cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
-    cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
+    cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
+    cuda_check(cudaFuncSetAttribute(span_tc_kernel<D, KV, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "span_tc smem");
   }
   const uint64_t rows = (uint64_t)p.num_blocks * p.hkv * p.block_pages * kPage;
   // encoded for every call: they cost less than looking up by an address what another tensor may since have
   CUtensorMap mk{}, mv{};
-  if (KV8) {
+  if (KV == kE4m3) {
     mk = make_tmap_bytes(p.k_cache, rows, D, kPage);
-  } else {
+  } else if (KV == kBf16) {
     mk = make_tmap_2d(p.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, D, D * 2, kPage, 64, true);
     mv = make_tmap_parts(p.v_cache, rows, D, kPage, D / 64);
   }
@@ -932,17 +1100,18 @@ void launch_tc(SpanParams p, cudaStream_t s) {
   const int last = (int)(whole % p.sms), halved = p.splits == 1 && !p.search && 2 * last + left <= p.sms ? last : 0;
   const long long ctas = tiles * p.hkv + halved;
   if (ctas > INT_MAX) throw std::runtime_error("attention_span: too many query rows");
-  auto go = [&](auto kernel) { launch_pdl(kernel, dim3((unsigned)ctas, p.splits), dim3(tc_threads<KV8>()), smem, s, mk, mv, p, (int)row_tiles, halved); };
-  if (p.search) go(span_tc_kernel<D, KV8, true>);
-  else go(span_tc_kernel<D, KV8, false>);
+  auto go = [&](auto kernel) { launch_pdl(kernel, dim3((unsigned)ctas, p.splits), dim3(tc_threads<KV>()), smem, s, mk, mv, p, (int)row_tiles, halved); };
+  if (p.search) go(span_tc_kernel<D, KV, true>);
+  else go(span_tc_kernel<D, KV, false>);
 }
 }  // namespace
 
 bool attention_span_tc_supported(const SpanParams& p) {
-  return !p.kv4 && (p.head_dim == 64 || p.head_dim == 128) && p.num_blocks * p.hkv * p.block_pages * kPage <= INT_MAX - kTile;
+  return (p.head_dim == 64 || p.head_dim == 128) && p.num_blocks * p.hkv * p.block_pages * kPage <= INT_MAX - kTile;
 }
 void attention_span_tc(const SpanParams& p, cudaStream_t s) {
-  if (p.head_dim == 64) p.kv_fp8 ? launch_tc<64, true>(p, s) : launch_tc<64, false>(p, s);
-  else p.kv_fp8 ? launch_tc<128, true>(p, s) : launch_tc<128, false>(p, s);
+  if (p.kv4) p.head_dim == 64 ? launch_tc<64, kKv4>(p, s) : launch_tc<128, kKv4>(p, s);
+  else if (p.head_dim == 64) p.kv_fp8 ? launch_tc<64, kE4m3>(p, s) : launch_tc<64, kBf16>(p, s);
+  else p.kv_fp8 ? launch_tc<128, kE4m3>(p, s) : launch_tc<128, kBf16>(p, s);
 }
 }  // namespace fllm

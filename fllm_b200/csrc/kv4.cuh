@@ -48,6 +48,17 @@ __device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Scale& s) {
 }
 __device__ __forceinline__ float kv4_value(uint32_t code, const Kv4Scale& s) { return fmaf((float)code, s.step, s.low); }
 
+// Eight codes, of dims 0 to 7, as f16 values z + s c, rounded once, dims in the order 0, 4, 1, 5, 2, 6, 3, 7. The bits of c are those of the f16 number
+// c 2^-24, those of c << 4 are c 2^-20: `even` is s 2^24, `odd` s 2^20, `low` z, in both halves of a word (so values are below 2^-6, where s 2^24 is a number).
+__device__ __forceinline__ uint4 kv4_widen_f16(uint32_t codes, uint32_t even, uint32_t odd, uint32_t low) {
+  uint4 v;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v.x) : "r"(codes & 0x000F000Fu), "r"(even), "r"(low));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v.y) : "r"(codes & 0x00F000F0u), "r"(odd), "r"(low));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v.z) : "r"(codes >> 8 & 0x000F000Fu), "r"(even), "r"(low));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v.w) : "r"(codes >> 8 & 0x00F000F0u), "r"(odd), "r"(low));
+  return v;
+}
+
 // A warp's row of D values, EPL to a lane (bf16 values in fp32): PAIRS: v[2i], v[2i + 1] are dims 2 (lane + 32 i) and the next; otherwise v[i] is dim
 // lane + 32 i. All lanes take part.
 template <int D, bool PAIRS>

@@ -4,7 +4,16 @@ Its bound holds here as well. Weights are f16, times a step s, for a product wit
 magnitude): an error of 2^-11 w s 8 for each token at most, and what is added to it for the middle of the range is exact in fp32. A row of bf16 values has
 s <= (max - min) / 15 (1 + 2^-7), so 8 s 2^-11 <= 2^-11.8 (max - min): below 2^-8 A where A = sum_j w_j |v_j| >= (max - min) / 13 or so. The rows here are normal
 values, of which no channel is near 0 in all tokens: A is about 0.8 where max - min is at most 8. Short rows see few tokens, whose weights are then large; the
-bound's factor of 1.1 and `slack` (2^-11 x 8 s, summed over the weights) stand for those."""
+bound's factor of 1.1 and `slack` (2^-11 x 8 s, summed over the weights) stand for those.
+
+The kernel of prompts widens keys and values to f16 (times a power of two), each z + s c rounded once: relative 2^-11 of those within 2^-8 of a tile's largest,
+2^-25 + 2^-26 of the unit in which that is above 2^-9 otherwise. Let o' be the formula's output for keys and values rounded to f16 as they are (normal values
+here, for which that is 2^-11 as well); an error of either can be that of o' and, rounded the other way, twice it. The kernel's other errors are those of an
+8-bit cache's kernel, so |y - o| <= bound' + 2 |o' - o|, both of which are computed here, and 2^-10 A for values whose roundings cancel in o' (A >= |o|, of
+normal values about 0.8, is bound' / 2^-8 or less). Which kernel a row meets is the planner's
+business: the other one's |y - o| <= bound is within that, up to bound - bound', so the larger of the two bounds is taken."""
+from types import SimpleNamespace
+
 import torch
 
 import span_oracle as so
@@ -25,7 +34,9 @@ def slack(c):
 
 def want(c, *args, **more):
     o, bound = so.want(c, *args, **more)
-    return o, bound + slack(c)
+    rounded = SimpleNamespace(**{**vars(c), "keys": [k.half() for k in c.keys], "values": [v.half() for v in c.values]})
+    o2, bound2 = so.want(rounded, *args, **more)
+    return o, torch.maximum(bound, bound2) * (1 + 2.0 ** -2) + 2 * (o2 - o).abs() + slack(c)
 
 
 def blocks_of_head(c, picks, block, row, head):
