@@ -48,6 +48,7 @@ template <bool B> using Bool = std::integral_constant<bool, B>;
 
 constexpr int kRawTokens = 64;             // of a piece of an e4m3 tile
 constexpr int kKv4Slots = 3;               // of tiles of 4-bit rows
+constexpr int kKv4Team = 3;                // warps that widen K, and V
 constexpr int kKv4Top = -6;                // their largest magnitude is below 2 to this as f16 (kv4_widen_f16)
 constexpr int kTcFlags = 400;              // bytes of barriers and flags
 
@@ -444,6 +445,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   uint64_t *s_full = bars + 14, *p_half = bars + 16, *p_ready = bars + 18;                    // [2] by softmax group
   uint64_t *o_done = bars + 20, *q_full = bars + 21;
   uint64_t *raw_full = bars + 22, *raw_empty = bars + 30;                                     // [8] by slot
+  uint64_t* v_unit = raw_full + 4;         // [2] by stage of V: a 4-bit cache has three raw slots, and units that softmax has to know
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* odd_met = reinterpret_cast<int*>(tmem_slot + 2);     // values were taken out of tiles of V
@@ -455,10 +457,10 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV == kBf16 ? 1 : kWideners);
+      mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_ready[i], 4); mbar_init(&v_ready[i], KV4 ? kKv4Team : KV8 ? kWideners : 1);
     }
-    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], KV8 ? 1 : KV4 ? kWideners : D / 64); mbar_init(&k_empty[i], 1); }
-    for (int i = 0; i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], kWideners); }
+    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], KV8 ? 1 : KV4 ? kKv4Team : D / 64); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], KV4 ? kKv4Team : kWideners); }
     mbar_init(o_done, 1); mbar_init(q_full, kQThreads<KV> / 32);
     *abort_flag = 0;
     *odd_met = 0;
@@ -612,25 +614,18 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       }
       __syncwarp();
     } else if constexpr (KV4) {
-      // Warp 8 asks for tiles, of K one tile ahead of V, through a ring of slots: K0, K1, V0, K2, V1, ... Each of six other warps widens a part of every one.
-      const int part = warp - 10, pieces = 2 * n_tiles;
-      auto piece_at = [&](int x, int& it, bool& is_v) {            // the x-th piece: of which tile, and whether of V
-        const bool last = x == pieces - 1;
-        is_v = last || (x >= 2 && (x & 1) == 0);
-        it = last ? n_tiles - 1 : is_v ? x / 2 - 1 : (x + 1) / 2;
-      };
+      // Warp 8 asks for tiles, K0, V0, K1, V1, ..., through a ring of slots. Three warps widen those of K, three those of V, each a part of every one. (All six
+      // one tile after the other, each with its waits and its search for a unit: 600 us where so 534, 2 x 2048 rows behind 2500 and 6143 tokens.)
+      const int part = (warp - 10) % kKv4Team, pieces = 2 * n_tiles;
       PagesAhead pages_k(page_rows, t0, warp == 8 ? n_tiles : 0), pages_v(page_rows, t0, warp == 8 ? n_tiles : 0);
-      int slot = 0, turn = 0;
-      auto next_slot = [&] { if (++slot == kKv4Slots) { slot = 0; turn ^= 1; } };
       constexpr int kPageBytes = kPage * kKv4Row<D>;
       bool ok = true;
-      for (int x = 0; ok && warp == 8 && x < pieces; ++x, next_slot()) {
-        int it;
-        bool is_v;
-        piece_at(x, it, is_v);
+      for (int x = 0; ok && warp == 8 && x < pieces; ++x) {
+        const int it = x >> 1, slot = x % kKv4Slots;
+        const bool is_v = x & 1;
         if (is_v) pages_v.to(it);
         else pages_k.to(it);
-        if (x >= kKv4Slots && !mbar_wait_warp(&raw_empty[slot], turn ^ 1, abort_flag)) { ok = false; break; }
+        if (x >= kKv4Slots && !mbar_wait_warp(&raw_empty[slot], (x / kKv4Slots - 1) & 1, abort_flag)) { ok = false; break; }
         const int now = is_v ? pages_v.now : pages_k.now;
         uint8_t* at = smem + 6 * TB + slot * S::kRaw;
         // A page is 16 rows in one piece: the lanes that looked the tile's pages up ask for one each. One that nobody sees, or that is not there, is zeros.
@@ -648,20 +643,17 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         if (mine) bulk_load(at + pg * kPageBytes, static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache) + (size_t)now * kKv4Row<D>, kPageBytes, &raw_full[slot]);
         __syncwarp();
       }
-      // A lane takes two words of a row, half a row apart.
-      constexpr int kWords = D / 16, kTurnRows = 32 / kWords, kTurns = kTile / kTurnRows;
-      constexpr int kMost = (kTurns + kWideners - 1) / kWideners, kBatch = 4;
+      // A lane takes two words of a row, half a row apart. Steps and lowest values of the warp's rows are made ready a lane to a row.
+      constexpr int kWords = D / 16, kTurnRows = 32 / kWords, kTurns = kTile / kTurnRows, kMost = (kTurns + kKv4Team - 1) / kKv4Team;
+      constexpr int kBatch = 32 / kTurnRows;           // turns whose rows 32 lanes have
       const int word = lane % kWords, sub = lane / kWords;
+      const bool is_v = warp >= 10 + kKv4Team;
       int up_v = 127;                                  // values are times 2^up_v
-      for (int x = 0; ok && warp >= 10 && x < pieces; ++x, next_slot()) {
-        int it;
-        bool is_v;
-        piece_at(x, it, is_v);
-        const int b = it & 1, tile0 = (t0 + it) * kTile;
-        ok = mbar_wait_warp(&raw_full[slot], turn, abort_flag) && (it < 2 || mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag));
-        if (!ok) break;
-        const uint8_t* src = smem + 6 * TB + slot * S::kRaw;
+      for (int it = 0; ok && warp >= 10 && it < n_tiles; ++it) {
+        const int x = 2 * it + is_v, slot = x % kKv4Slots, b = it & 1, tile0 = (t0 + it) * kTile;
         const bool look = partial(tile0);
+        if (!mbar_wait_warp(&raw_full[slot], x / kKv4Slots & 1, abort_flag)) { ok = false; break; }
+        const uint8_t* src = smem + 6 * TB + slot * S::kRaw;
         auto seen = [&](int tok) { return tok < any_end && (tok >= any_beg || tok < p.first); };
         // The largest magnitude of the tile that some row sees, by every warp for itself, a lane to four rows. It goes below 2^kKv4Top; that of values, whose
         // sums go over all tiles, only where it is above that of those before, with room for four times as much.
@@ -676,44 +668,54 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         int up = 126 + kKv4Top - (int)most;
         if (is_v) up = up_v = up < up_v ? up - 2 : up_v;
         up = min(up, 120);
-        if (part == 0 && lane == 0) (is_v ? v_up : k_up)[it & 3] = up;
         const float f1 = pow2_of(up >> 1), f2 = pow2_of(up - (up >> 1));
-        bool met = false;
+        if (it >= 2 && !mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+        if (part == 0 && lane == 0) {
+          (is_v ? v_up : k_up)[it & 3] = up;
+          if (is_v) mbar_arrive(&v_unit[b]);
+        }
         uint8_t* const to = is_v ? sv + b * TB : sk + b * TB;
-#pragma unroll 1
+        // of row tok: V: [page][half][16][64]
+        const int line_of_page = is_v ? (D / 64) * 2048 : 16 * 128, line_of_half = is_v ? 2048 : kHalf;
+#pragma unroll
         for (int u0 = 0; u0 < kMost; u0 += kBatch) {
-          uint32_t w[kBatch][2], scale[kBatch];
-          const uint8_t* from = src + ((part + kWideners * u0) * kTurnRows + sub) * kKv4Row<D>;
+          uint32_t even = 0, odd = 0, low2 = 0;        // of a row of values that reads as NaN, or that nobody sees: 0
+          const int mine = (part + kKv4Team * (u0 + lane / kTurnRows)) * kTurnRows + lane % kTurnRows;
+          if (mine < kTile) {
+            const Kv4Scale k = kv4_scale_of(*reinterpret_cast<const uint32_t*>(src + mine * kKv4Row<D> + D / 2));
+            const bool there = !look || seen(tile0 + mine), nan = !(fabsf(k.step) < INFINITY);
+            if (!is_v || (there && !(look && nan))) {
+              const float step = k.step * f1 * f2, low = k.low * f1 * f2;
+              even = pack_16<true>(step * 16777216.f, step * 16777216.f);
+              odd = pack_16<true>(step * 1048576.f, step * 1048576.f);
+              low2 = pack_16<true>(low, low);
+            }
+            if (is_v && look && there && nan) *reinterpret_cast<volatile int*>(odd_met) = 1;
+          }
+          constexpr int kHere = kBatch;
+          uint32_t w[kHere][2];
+          const uint8_t* from = src + ((part + kKv4Team * u0) * kTurnRows + sub) * kKv4Row<D> + word * 4;
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u)
-            if (part + kWideners * (u0 + u) < kTurns) {
-              const uint8_t* row = from + u * kWideners * kTurnRows * kKv4Row<D>;
-              w[u][0] = *reinterpret_cast<const uint32_t*>(row + word * 4);
-              w[u][1] = *reinterpret_cast<const uint32_t*>(row + (word + kWords) * 4);
-              scale[u] = *reinterpret_cast<const uint32_t*>(row + D / 2);
+          for (int u = 0; u < kHere; ++u)
+            if (u0 + u < kMost && part + kKv4Team * (u0 + u) < kTurns) {
+              w[u][0] = *reinterpret_cast<const uint32_t*>(from + u * kKv4Team * kTurnRows * kKv4Row<D>);
+              w[u][1] = *reinterpret_cast<const uint32_t*>(from + u * kKv4Team * kTurnRows * kKv4Row<D> + kWords * 4);
             }
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            if (part + kWideners * (u0 + u) >= kTurns) continue;
-            const int tok = (part + kWideners * (u0 + u)) * kTurnRows + sub;
-            const Kv4Scale k = kv4_scale_of(scale[u]);
-            const float step = k.step * f1 * f2, low = k.low * f1 * f2;
-            const uint32_t low2 = pack_16<true>(low, low), even = pack_16<true>(step * 16777216.f, step * 16777216.f), odd = pack_16<true>(step * 1048576.f, step * 1048576.f);
-            uint4 y[2] = {kv4_widen_f16(w[u][0], even, odd, low2), kv4_widen_f16(w[u][1], even, odd, low2)};
-            if (look && is_v) {
-              const bool nan = (scale[u] & 0x7F80u) == 0x7F80u, there = seen(tile0 + tok);      // a row that reads as NaN, one that anybody sees
-              if (nan || !there) y[0] = y[1] = make_uint4(0, 0, 0, 0);
-              met |= nan && there;
-            }
+          for (int u = 0; u < kHere; ++u) {
+            if (u0 + u >= kMost) continue;
+            const uint32_t e = __shfl_sync(0xffffffffu, even, u * kTurnRows + sub), o = __shfl_sync(0xffffffffu, odd, u * kTurnRows + sub);
+            const uint32_t l = __shfl_sync(0xffffffffu, low2, u * kTurnRows + sub);
+            if (part + kKv4Team * (u0 + u) >= kTurns) continue;
+            const int tok = (part + kKv4Team * (u0 + u)) * kTurnRows + sub;
+            uint8_t* line = to + (tok >> 4) * line_of_page + (tok & 15) * 128;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int c = word + h * kWords;
-              uint8_t* line = is_v ? to + (tok >> 4) * (D / 64) * 2048 + (c >> 3) * 2048 + (tok & 15) * 128 : to + (c >> 3) * kHalf + tok * 128;      // V: [page][half][16][64]
-              *reinterpret_cast<uint4*>(line + (((c & 7) ^ (tok & 7)) << 4)) = y[h];
+              *reinterpret_cast<uint4*>(line + (c >> 3) * line_of_half + (((c & 7) ^ (tok & 7)) << 4)) = kv4_widen_f16(w[u][h], e, o, l);
             }
           }
         }
-        if (met) atomicOr(odd_met, 1);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -900,7 +902,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       float shrink = 1.f;
       if constexpr (KV4) {
         const int t = n >> shift;
-        if (!mbar_wait(&v_ready[t & 1], (t >> 1) & 1, abort_flag)) { ok = false; break; }      // (done by now, as a rule)
+        if (!mbar_wait(&v_unit[t & 1], (t >> 1) & 1, abort_flag)) { ok = false; break; }
         const int up = k_up[t & 3], now = v_up[t & 3];
         factor = row_factor * pow2_of(-(up >> 1)) * pow2_of((up >> 1) - up);
         if (p.softcap <= 0.f) scale = factor;
