@@ -25,7 +25,11 @@ def _add_engine_flags(p: argparse.ArgumentParser) -> None:
     p.add_argument("--gpu-memory-utilization", type=float, default=0.90)
     p.add_argument("--dtype", default="bf16", choices=["bf16", "fp32"],
                    help="weights, activations and cache; fp32 for the families whose kernels exist in 32-bit")
-    p.add_argument("--kv-cache-type", default="bf16")
+    p.add_argument("--kv-cache-type", default="bf16", help="bf16, fp8_e4m3 or int4 (rows of 4-bit codes)")
+    p.add_argument("--sparse-blocks", type=int, default=0,
+                   help="blocks of its text that a row reads in layers without a window, the best by a bound of their scores (0: all)")
+    p.add_argument("--sparse-lead", type=int, default=1, help="of them the first of the text")
+    p.add_argument("--sparse-tail", type=int, default=2, help="of them the last, the row's own among them")
     p.add_argument("--kv-blocks", type=int, default=0)
     p.add_argument("--no-prefix-cache", action="store_true")
     p.add_argument("--no-cuda-graphs", action="store_true")
@@ -62,7 +66,8 @@ def build_engine(args):
         use_cuda_graphs=not args.no_cuda_graphs, scheduling_policy=args.scheduling_policy,
         preemption=args.preemption, speculative=args.speculative, draft_tokens=args.draft_tokens, seed=args.seed,
         kv_tier_host_gb=args.kv_tier_host_gb, kv_tier_disk_dir=args.kv_tier_disk_dir, kv_tier_disk_gb=args.kv_tier_disk_gb,
-        state_cache_gb=getattr(args, "state_cache_gb", 0.0))
+        state_cache_gb=getattr(args, "state_cache_gb", 0.0), sparse_blocks=args.sparse_blocks, sparse_lead=args.sparse_lead,
+        sparse_tail=args.sparse_tail)
     par = ParallelConfig(tp=args.tp, pp=args.pp, expert_parallel=args.expert_parallel, ep_dispatch=args.ep_dispatch,
                          distributed_backend=args.distributed_backend)
     weights, tok_path = None, args.tokenizer

@@ -1310,7 +1310,10 @@ class EngineConfig:
     gpu_memory_utilization: float = 0.90
     max_model_len: int = 8192
     dtype: str = "bf16"                  # bf16 | fp32 (families whose kernels exist in 32-bit: weights, activations and cache)
-    kv_cache_dtype: str = "bf16"         # bf16 | fp8_e4m3
+    kv_cache_dtype: str = "bf16"         # bf16 | fp8_e4m3 | int4 (rows of 4-bit codes: 68 bytes a token and head of 128)
+    sparse_blocks: int = 0               # blocks of its text that a row reads in layers without a window, the best by a bound of their scores (0 = all)
+    sparse_lead: int = 1                 # of them the first of the text
+    sparse_tail: int = 2                 # and the last, the row's own among them
     spare_state_rows: int = 8            # recurrent models: state rows beyond one per running sequence
     enable_prefix_caching: bool = True
     scheduling_policy: str = "fcfs"      # fcfs | priority

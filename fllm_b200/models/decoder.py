@@ -18,6 +18,8 @@ from typing import List, Optional
 import torch
 
 from ..config import ModelConfig, RopeScaling, rope_inv_freq, scaled_inv_freq
+from ..ops.blocks import bounds_width
+from ..ops.kv4 import kv4_width
 from ..ops.prenorm import TokenShift
 from .maps import MAPS_MIXERS
 from .moe import ACT_KIND
@@ -51,12 +53,16 @@ class KVCache:
     [num_blocks, kv_heads_local, block_size, head_dim]."""
 
     def __init__(self, num_layers: int, num_blocks: int, kv_heads: int, block_size: int, head_dim: int,
-                 device, dtype=torch.bfloat16):
+                 device, dtype=torch.bfloat16, sparse=None):
         """dtype torch.float8_e4m3fn halves the pool (values stored unscaled; written by the rope kernel,
-        read by the generic attention kernel)."""
-        self.num_blocks, self.block_size = num_blocks, block_size
-        self.store = torch.zeros(num_layers, 2, num_blocks, kv_heads, block_size, head_dim,
-                                 device=device, dtype=dtype)
+        read by the generic attention kernel); "int4": rows of 4-bit codes with a step and a lowest value of their own
+        (``ops.kv4``), in a uint8 pool. ``sparse``: (blocks that a row reads, first and last ones among them) of layers without a window;
+        the pool then has the bounds of every block's keys beside it (``ops.blocks``)."""
+        self.num_blocks, self.block_size, self.head_dim, self.sparse = num_blocks, block_size, head_dim, sparse
+        self.four_bit = dtype == "int4"
+        self.store = torch.zeros(num_layers, 2, num_blocks, kv_heads, block_size, kv4_width(head_dim) if self.four_bit else head_dim,
+                                 device=device, dtype=torch.uint8 if self.four_bit else dtype)
+        self.bounds = torch.zeros(num_layers, num_blocks, kv_heads, bounds_width(head_dim), device=device, dtype=torch.int8) if sparse else None
 
     def k(self, layer: int) -> torch.Tensor:
         return self.store[layer, 0]
@@ -66,6 +72,8 @@ class KVCache:
 
     def copy_block(self, src: int, dst: int) -> None:
         self.store[:, :, dst].copy_(self.store[:, :, src])
+        if self.bounds is not None:
+            self.bounds[:, dst].copy_(self.bounds[:, src])
 
     def pools(self) -> List[torch.Tensor]:
         """The pool as [planes, blocks, heads, block_size, width], what the operators that move rows and blocks take."""
@@ -76,16 +84,55 @@ class KVCache:
         pools = self.pools()
         if pools:                                # a pipeline stage may cache nothing
             ops.kv_copy_blocks(pools, pairs)
+            if self.bounds is not None:          # of a block and head: one row
+                ops.kv_copy_blocks([self.bounds[:, :, :, None]], pairs)
 
     def compact(self, block_tables, base, path, counts, ops) -> None:
         """The accepted rows of draft trees to the places behind their contexts (``ops.kv_compact``)."""
         pools = self.pools()
         if pools:
             ops.kv_compact(pools, block_tables, base, path, counts)
+            if self.bounds is not None:          # of blocks whose last row is among those that were moved to
+                step = torch.arange(path.shape[1], dtype=torch.int32, device=path.device)
+                at = base[:, None] + step
+                page = (at // self.block_size).clamp(0, block_tables.shape[1] - 1).long()
+                slots = block_tables[:path.shape[0]].gather(1, page) * self.block_size + at % self.block_size
+                self._find_bounds(torch.where(step < counts[:, None], slots, -1).flatten().to(torch.int32), ops)
+
+    def put_blocks(self, blocks: torch.Tensor, kv: torch.Tensor, ops) -> None:
+        """Contents of whole blocks, [layers, 2, blocks, kv heads, block_size, row] of a pool of this kind, or of a bf16 one beside a 4-bit one
+        (encoded) or the other way round (what the codes stand for, rounded to bf16)."""
+        kv = kv.to(self.store.device)
+        if kv.dtype == self.store.dtype and kv.shape[3:] == self.store.shape[3:]:
+            self.store.index_copy_(2, blocks, kv)
+        elif tuple(kv.shape[3:5]) == tuple(self.store.shape[3:5]) and {kv.dtype, self.store.dtype} == {torch.bfloat16, torch.uint8}:
+            n, heads = kv.shape[2], kv.shape[3]
+            slots = torch.arange(n * self.block_size, dtype=torch.int32, device=kv.device)
+            there = (blocks[:, None] * self.block_size + torch.arange(self.block_size, device=kv.device)).flatten().to(torch.int32)
+            for layer, (k, v) in enumerate(kv):
+                if self.four_bit:
+                    ops.kv4_write(*(x.transpose(1, 2).reshape(n * self.block_size, -1) for x in (k, v)), there, self.k(layer), self.v(layer))
+                else:
+                    for x, pool in ((k, self.k(layer)), (v, self.v(layer))):
+                        rows = ops.kv4_read(x.contiguous(), slots).to(torch.bfloat16)
+                        pool[blocks] = rows.view(n, self.block_size, heads, -1).transpose(1, 2)
+        else:
+            raise ValueError(f"blocks of {tuple(kv.shape[3:])} {kv.dtype} do not fit a pool of {tuple(self.store.shape[3:])} {self.store.dtype}")
+        self.find_bounds(blocks, ops)
+
+    def find_bounds(self, blocks: torch.Tensor, ops) -> None:
+        """Bounds of blocks whose rows came from elsewhere than a step."""
+        if self.bounds is not None:
+            self._find_bounds((blocks * self.block_size + self.block_size - 1).to(torch.int32), ops)
+
+    def _find_bounds(self, slots: torch.Tensor, ops) -> None:
+        for layer in range(self.store.shape[0]):
+            ops.kv_bounds(self.k(layer), self.bounds[layer], slots)
 
     @staticmethod
-    def bytes_per_block(num_layers, kv_heads, block_size, head_dim, elem=2) -> int:
-        return num_layers * 2 * kv_heads * block_size * head_dim * elem
+    def bytes_per_block(num_layers, kv_heads, block_size, head_dim, elem=2, four_bit=False, sparse=False) -> int:
+        row = kv4_width(head_dim) if four_bit else head_dim * elem
+        return num_layers * kv_heads * (2 * block_size * row + (bounds_width(head_dim) if sparse else 0))
 
 
 class Decoder:
@@ -217,12 +264,22 @@ class Decoder:
         q = ops.rope_kv_write(qkv, b.positions, b.slots, inv, lw.q_norm, lw.k_norm,
                               kc, vc, sp.hq_local, sp.hkv_local, cfg.head_dim, cfg.rot_dim, self.rope_style,
                               cfg.rms_eps, 1.0 if local_rope else self.attn_factor)
-        a = ops.attention(q, kc, vc, b.block_tables, b.row_seq, b.positions, sp.hq_local, sp.hkv_local,
-                          cfg.head_dim, self.scale, cfg.layer_window(li), lw.sinks, cfg.attn_softcap,
-                          meta=b, first=cfg.window_first)
+        a = self._attend(li, lw, local, q, b)
         if gated:                                # the attention output passes through a sigmoid gate of its own projection
             a = (a.float() * torch.sigmoid(ops.linear(h, lw.w_attn_gate).float())).to(a.dtype)
         return ops.linear(a, lw.wo, lw.bo, defer=defer_out and self._defer_out(lw.post_attn_norm))
+
+    def _attend(self, li: int, lw, local: int, q: torch.Tensor, b: StepBatch) -> torch.Tensor:
+        """Attention of a layer whose rows are in the cache: over what its window shows, or over the blocks that each row selects."""
+        cfg, sp, ops, kv = self.cfg, self.spec, self.ops, self.kv
+        kc, vc, window = kv.k(local), kv.v(local), cfg.layer_window(li)
+        if kv.sparse and not window:
+            count, lead, tail = kv.sparse
+            ops.kv_bounds(kc, kv.bounds[local], b.slots)
+            blocks = ops.select_blocks(q, kv.bounds[local], b.block_tables, sp.hq_local, sp.hkv_local, cfg.head_dim, kv.block_size, count, b, lead, tail)
+            return ops.attention_blocks(q, kc, vc, b.block_tables, blocks, sp.hq_local, sp.hkv_local, cfg.head_dim, self.scale, b, lw.sinks, cfg.attn_softcap)
+        return ops.attention(q, kc, vc, b.block_tables, b.row_seq, b.positions, sp.hq_local, sp.hkv_local, cfg.head_dim, self.scale, window, lw.sinks,
+                             cfg.attn_softcap, meta=b, first=cfg.window_first)
 
     def _defer_out(self, post_norm) -> bool:
         """May a row-parallel projection hand its split-K partials to the next norm? Only when nothing
@@ -475,9 +532,7 @@ class Decoder:
             q = ops.rope_kv_write(qkv, b.positions, b.slots, self.inv_freq, lw.q_norm, lw.k_norm, kc, vc,
                                   sp.hq_local, sp.hkv_local, cfg.head_dim, cfg.rot_dim, self.rope_style,
                                   cfg.rms_eps, self.attn_factor)
-            a = ops.attention(q, kc, vc, b.block_tables, b.row_seq, b.positions, sp.hq_local, sp.hkv_local,
-                              cfg.head_dim, self.scale, cfg.layer_window(li), lw.sinks, cfg.attn_softcap, meta=b,
-                              first=cfg.window_first)
+            a = self._attend(li, lw, local, q, b)
             tp.linear_rs(a, lw.wo, lw.bo, bc)
             tp.norm(x, T, True, lw.ffn_norm, cfg.rms_eps, cfg.norm_weight_offset, bc)
             layout = getattr(lw, "glu_layout", 0)

@@ -28,6 +28,7 @@ from ..config import EngineConfig, ModelConfig, ParallelConfig
 from ..models.decoder import Decoder, KVCache, StepBatch
 from ..models.weights import DecoderWeights, init_random_weights, make_shard_spec
 from ..ops import get_ops
+from ..ops.kv4 import kv4_width
 from .block_manager import BlockManager
 from .request import Request, RequestStatus, SamplingParams, TokenEvent
 from .scheduler import ScheduledSeq, ScheduledStep, Scheduler
@@ -108,10 +109,9 @@ class LLMEngine:
             release_scale_atoms(self.weights.layers)
             torch.cuda.empty_cache()                     # the pool is sized by what the device has free
         num_blocks = self.cfg.num_kv_blocks or self._size_kv_pool()
-        if self.cfg.kv_cache_dtype not in ("bf16", "fp8", "fp8_e4m3", "fp32"):
-            raise ValueError("kv_cache_dtype must be bf16 or fp8_e4m3")
+        self._check_cache_kind()
         # fp32: with the PyTorch operators (exact comparisons against other implementations), or a family with fp32 kernels
-        kv_dtype = {"bf16": torch.bfloat16, "fp32": torch.float32}.get(self.cfg.kv_cache_dtype, torch.float8_e4m3fn)
+        kv_dtype = {"bf16": torch.bfloat16, "fp32": torch.float32, "int4": "int4"}.get(self.cfg.kv_cache_dtype, torch.float8_e4m3fn)
         if kv_dtype == torch.float32 and hasattr(self.ops, "k") and not (model_cfg.native_f32 and self.weights.embed.dtype == torch.float32):
             raise ValueError("an fp32 KV pool is for the reference operators and for models served in fp32")
         if model_cfg.has_row_cache:
@@ -121,7 +121,7 @@ class LLMEngine:
             self.kv = RowCache(RowCache.specs(model_cfg, self.layer_range), num_blocks, self.block_size, self.device, kv_dtype)
         else:
             self.kv = KVCache(self._kv_layers(), num_blocks, self.spec.hkv_local, self.block_size,
-                              model_cfg.head_dim, self.device, kv_dtype)
+                              model_cfg.head_dim, self.device, kv_dtype, self._sparse())
         self.rstate = None
         if model_cfg.has_recurrent:
             # one state row per running sequence, a few spare for sequences between two owners, and the scratch
@@ -204,6 +204,28 @@ class LLMEngine:
         self._out_host = torch.empty(self.cfg.max_num_batched_tokens + 64, dtype=torch.int32,
                                      pin_memory=self.is_cuda)
 
+    # ------------------------------------------------------------------ kind of cache
+    def _sparse(self) -> "Optional[tuple[int, int, int]]":
+        c = self.cfg
+        return (c.sparse_blocks, c.sparse_lead, c.sparse_tail) if c.sparse_blocks else None
+
+    def _check_cache_kind(self) -> None:
+        c, m = self.cfg, self.model_cfg
+        if c.kv_cache_dtype not in ("bf16", "fp8", "fp8_e4m3", "fp32", "int4"):
+            raise ValueError("kv_cache_dtype must be bf16, fp8_e4m3 or int4")
+        native = hasattr(self.ops, "k")
+        for on, what in ((c.kv_cache_dtype == "int4", "a 4-bit cache"), (c.sparse_blocks, "attention over selected blocks")):
+            if not on:
+                continue
+            if m.has_row_cache or not any(m.has_kv(li) for li in range(m.num_layers)):
+                raise ValueError(f"{what} is for layers that cache keys and values")
+            if m.head_dim not in (64, 128, 256) and (native or c.kv_cache_dtype == "int4"):
+                raise ValueError(f"{what} needs head dims of 64, 128 or 256")
+            if native and (c.block_size % 16 or c.dtype != "bf16"):
+                raise ValueError(f"{what} needs blocks of a multiple of 16 tokens and a model in bf16")
+        if c.sparse_blocks and (c.sparse_tail < 1 or c.sparse_lead < 0 or c.sparse_blocks < c.sparse_lead + c.sparse_tail):
+            raise ValueError("sparse_blocks must have room for the first and the last blocks, one of the last at least")
+
     # ------------------------------------------------------------------ sizing
     def _state_rows(self) -> int:
         """Rows of the recurrent-state pools: one per running sequence, the spare ones, and the scratch row."""
@@ -216,7 +238,8 @@ class LLMEngine:
     def _size_kv_pool(self) -> int:
         per_block = KVCache.bytes_per_block(self._kv_layers(), self.spec.hkv_local,
                                             self.block_size, self.model_cfg.head_dim,
-                                            {"bf16": 2, "fp32": 4}.get(self.cfg.kv_cache_dtype, 1))
+                                            {"bf16": 2, "fp32": 4}.get(self.cfg.kv_cache_dtype, 1),
+                                            self.cfg.kv_cache_dtype == "int4", self._sparse() is not None)
         if self.model_cfg.has_row_cache:
             from ..models.row_cache import RowCache
             per_block = max(1, RowCache.bytes_per_block(RowCache.specs(self.model_cfg, self.layer_range), self.block_size,
@@ -293,12 +316,15 @@ class LLMEngine:
         """Decode side: adopt an exported request. Its KV is copied into freshly allocated blocks and
         the request continues as a running decode sequence."""
         kv = blob["kv"]
-        if blob["kv_dtype"] != str(self.kv.store.dtype) or blob["block_size"] != self.block_size:
+        # (a 4-bit cache and a bf16 one take each other's blocks)
+        converts = {blob["kv_dtype"], str(self.kv.store.dtype)} == {"torch.bfloat16", "torch.uint8"}
+        if (blob["kv_dtype"] != str(self.kv.store.dtype) and not converts) or blob["block_size"] != self.block_size:
             raise ValueError("KV layout mismatch between the exporting and the importing engine")
-        if kv.element_size() == 1 and kv.dtype != self.kv.store.dtype:
+        if not converts and kv.element_size() == 1 and kv.dtype != self.kv.store.dtype:
             kv = kv.view(self.kv.store.dtype)
-        want = self.kv.store.shape
-        if tuple(kv.shape[:2]) != tuple(want[:2]) or tuple(kv.shape[3:]) != tuple(want[3:]):
+        want, last = self.kv.store.shape, 5 if converts else 6
+        if kv.dim() != 6 or tuple(kv.shape[:2]) != tuple(want[:2]) or tuple(kv.shape[3:last]) != tuple(want[3:last]) or \
+                (converts and kv.shape[5] != (self.kv.head_dim if self.kv.four_bit else kv4_width(self.kv.head_dim))):
             raise ValueError(f"KV shape {tuple(kv.shape)} does not fit this engine's pool {tuple(want)}")
         params = SamplingParams(**blob["params"])
         params.validate(self.model_cfg.vocab_size)
@@ -315,7 +341,7 @@ class LLMEngine:
         live = list(blob["live_blocks"])
         if live:
             dst = torch.tensor([table[i] for i in live], dtype=torch.long, device=self.device)
-            self.kv.store.index_copy_(2, dst, kv.to(self.device))
+            self.kv.put_blocks(dst, kv, self.ops)
         self.blocks.drop_absent(req.seq_id, live, n)            # before their hashes are registered
         self.blocks.commit_tokens(req.seq_id, req.all_tokens, n, params.cache_salt.encode())
         req.status = RequestStatus.RUNNING
@@ -1031,7 +1057,8 @@ class LLMEngine:
         for t in probe:
             fp.update(t.detach().reshape(-1)[:4096].float().cpu().numpy().tobytes())
         sig = (f"{mc.name}|{tuple(st[:, :, 0].shape)}|{st.dtype}|bs{self.block_size}|tp{self.tp_rank}|"
-               f"theta{mc.rope_theta}|{mc.rope_scaling.kind}:{mc.rope_scaling.factor}|w{fp.hexdigest()[:16]}")
+               f"theta{mc.rope_theta}|{mc.rope_scaling.kind}:{mc.rope_scaling.factor}|w{fp.hexdigest()[:16]}"
+               + (f"|blocks{self._sparse()}" if self._sparse() else ""))      # (what rows read decides what is cached of them in the next layer)
         if self.tp_group is not None and getattr(self.tp_group, "size", 1) > 1:
             # ranks must take identical hit / miss decisions to keep their block tables equal: the host tier is
             # deterministic, a file that fails to read on one rank is not, so the disk tier is single-rank only
@@ -1047,6 +1074,7 @@ class LLMEngine:
             if blob is None:
                 return False
             st[:, :, block].copy_(blob.view(st.dtype).view(st[:, :, block].shape).to(st.device))
+            self.kv.find_bounds(torch.tensor([block], device=st.device), self.ops)
             return True
         self.blocks.on_evict, self.blocks.tier_has, self.blocks.tier_restore = evict, self.kv_tier.has, restore
 
@@ -1175,7 +1203,7 @@ class _KvSwapper:
         table = eng.blocks.table(req.seq_id)
         if live:
             dst = torch.tensor([table[i] for i in live], dtype=torch.long, device=eng.device)
-            eng.kv.store.index_copy_(2, dst, host.to(eng.device, non_blocking=False))
+            eng.kv.put_blocks(dst, host, eng.ops)
         eng.blocks.drop_absent(req.seq_id, live, req.num_computed)
         self.stats["swapped_in"] += 1
 
