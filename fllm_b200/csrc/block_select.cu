@@ -197,24 +197,31 @@ __global__ void __launch_bounds__(128) block_score_kernel(const __grid_constant_
 
   const int* table = s.block_tables + (size_t)seq * s.max_blocks;
   constexpr int J = 2 * D / 64;             // pieces of 16 bytes of a lane
-  for (int b0 = first + warp * kScoreBlocks; b0 < stop; b0 += 4 * kScoreBlocks) {
+  // The block of lane & 15 of a step is looked up two steps ahead of its use.
+  bool missing = false;
+  auto look = [&](int b0) {
     const int at = b0 + (lane & 15);
     const int id = at < stop && at < s.max_blocks ? table[at] : 0;
     const bool there = (unsigned)id < (unsigned)s.num_blocks;
-    const int8_t* mine = p.bounds + ((size_t)(there ? id : 0) * s.hkv + kvh) * (2 * D + kTail);
-    const int e_at = there ? (int)mine[2 * D] : -128;
-    if (!there && s.status) atomicCAS(s.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
-    const int8_t* of[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int other = __shfl_sync(0xffffffffu, there ? id : 0, g + 8 * h);
-      of[h] = p.bounds + ((size_t)other * s.hkv + kvh) * (2 * D + kTail) + 16 * t;
-    }
+    missing |= !there;
+    return there ? id : -1;
+  };
+  constexpr int kStep = 4 * kScoreBlocks;
+  const int mine0 = first + warp * kScoreBlocks;
+  int id = mine0 < stop ? look(mine0) : 0, id1 = mine0 + kStep < stop ? look(mine0 + kStep) : 0;
+  for (int b0 = mine0; b0 < stop; b0 += kStep) {
+    const int id2 = b0 + 2 * kStep < stop ? look(b0 + 2 * kStep) : 0;
+    const int e_at = id >= 0 ? (int)p.bounds[((size_t)id * s.hkv + kvh) * (2 * D + kTail) + 2 * D] : -128;
     uint4 a[2][J];
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int h = 0; h < 2; ++h) {
+      const int other = __shfl_sync(0xffffffffu, max(id, 0), g + 8 * h);
+      const int8_t* of = p.bounds + ((size_t)other * s.hkv + kvh) * (2 * D + kTail) + 16 * t;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) a[h][j] = __ldg(reinterpret_cast<const uint4*>(of[h] + 64 * j));
+      for (int j = 0; j < J; ++j) a[h][j] = __ldg(reinterpret_cast<const uint4*>(of + 64 * j));
+    }
+    id = id1;
+    id1 = id2;
     const int e0 = __shfl_sync(0xffffffffu, e_at, g), e1 = __shfl_sync(0xffffffffu, e_at, g + 8);
 #pragma unroll 1
     for (int n = 0; n < NQ; ++n) {
@@ -234,6 +241,7 @@ __global__ void __launch_bounds__(128) block_score_kernel(const __grid_constant_
       }
     }
   }
+  if (missing && s.status) atomicCAS(s.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
 }
 
 // ---------------------------------------------------------------------------- the best
@@ -265,8 +273,8 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
   return before + upto - v;
 }
 
-// One CTA per (row, key head): the key of the last block that is taken digit by digit (11, 11 and 10 bits, from the largest), then what is above it, and of
-// what equals it as many as are left, from the lowest block on.
+// One CTA per (row, key head): the key of the last block that is taken digit by digit, from the largest, then what is above it, and of what equals it as many
+// as are left, from the lowest block on.
 __global__ void __launch_bounds__(kSelectThreads) block_choose_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ uint32_t keys_s[];
   __shared__ uint32_t hist[kBins];
@@ -290,27 +298,43 @@ __global__ void __launch_bounds__(kSelectThreads) block_choose_kernel(const __gr
   if (want == 0) return;
   const int n = most - p.lead - p.tail;
   const float* scores = p.scores + ((size_t)local * s.hkv + kvh) * p.stride + p.lead;
-  for (int i = tid; i < n; i += kSelectThreads) keys_s[i] = key_of(scores[i]);
+  uint32_t least = 0xFFFFFFFFu, most_key = 0;
+  for (int i = tid; i < n; i += kSelectThreads) {
+    const uint32_t k = key_of(scores[i]);
+    keys_s[i] = k;
+    least = min(least, k);
+    most_key = max(most_key, k);
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most_key = __reduce_max_sync(0xffffffffu, most_key);
+  if ((tid & 31) == 0) sums[tid >> 5] = (unsigned long long)most_key << 32 | least;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelectThreads / 32; ++w) {
+    least = min(least, (uint32_t)sums[w]);
+    most_key = max(most_key, (uint32_t)(sums[w] >> 32));
+  }
+  // Digits are of what a key is above the least, from its 11 highest bits down, so that scores of one magnitude do not all meet in one counter.
   uint32_t prefix = 0, mask = 0;
+  int upper = 32 - __clz(most_key - least);            // bits that are still open
 #pragma unroll 1
-  for (int shift = 21; ; shift = max(shift - 11, 0)) {
-    const int bits = shift ? 11 : 10;
+  while (true) {
+    const int bits = 11, shift = max(upper - bits, 0);
     for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += kSelectThreads) {
-      const uint32_t k = keys_s[i];
-      if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
+      const uint32_t k = keys_s[i] - least;
+      if ((k & mask) == prefix) atomicAdd(&hist[(k & ~mask) >> shift], 1u);
     }
     __syncthreads();
     // from the largest digit down: a thread has kBins / 256 of them
     constexpr int kEach = kBins / kSelectThreads;
-    const int from = (1 << bits) - 1 - tid * ((1 << bits) / kSelectThreads);
-    const int each = (1 << bits) / kSelectThreads;
+    const int from = kBins - 1 - tid * kEach;
     uint32_t mine[kEach];
     uint32_t sum = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      mine[i] = i < each ? hist[from - i] : 0;
+      mine[i] = hist[from - i];
       sum += mine[i];
     }
     unsigned long long total;
@@ -322,11 +346,13 @@ __global__ void __launch_bounds__(kSelectThreads) block_choose_kernel(const __gr
     }
     __syncthreads();
     prefix |= found[0] << shift;
-    mask |= ((1u << bits) - 1) << shift;
+    mask = 0xFFFFFFFFu << shift;
     want -= (int)found[1];                  // of those with this digit
+    upper = shift;
     if (!shift) break;
     __syncthreads();
   }
+  prefix += least;
   // A thread has neighbouring blocks, an odd number of them: its place among the others' is a sum over the threads in front of it.
   const int each = ((n + kSelectThreads - 1) / kSelectThreads) | 1;
   const int from = min(tid * each, n), to = min(from + each, n);
@@ -359,9 +385,10 @@ void launch_bounds(const BoundsParams& p, int kind, cudaStream_t s) {
 template <int D, int NQ>
 void launch_scores(SelectParams p, cudaStream_t s) {
   const long long tiles = span_tiles(p.rows, p.rows.max_q_len, 8 * NQ, p.rows.search) * p.rows.hkv;
-  // Pieces of the text as long as there are SMs without a tile, four CTAs to an SM, a step of each warp at least.
+  // Pieces of the text for two rounds of CTAs, so that long texts do not hold their SMs alone in the end (64 decode rows of 4000 to 32,000 tokens, 8 key heads of
+  // 128: 48 us with half as many, 34, 37 with twice, 42 with four times as many), a step of each warp at least.
   const long long steps = (std::max(p.stride - p.lead - p.tail, 1) + 4 * kScoreBlocks - 1) / (4 * kScoreBlocks);
-  p.pieces = (int)std::max<long long>(1, std::min<long long>(8LL * sm_count() / tiles, steps));
+  p.pieces = (int)std::max<long long>(1, std::min<long long>(16LL * sm_count() / tiles, steps));
   if (tiles * p.pieces > INT_MAX) throw std::runtime_error("select_blocks: too many query rows");
   if (p.rows.search) launch_pdl(block_score_kernel<D, NQ, true>, dim3((unsigned)(tiles * p.pieces)), dim3(128), 0, s, p);
   else launch_pdl(block_score_kernel<D, NQ, false>, dim3((unsigned)(tiles * p.pieces)), dim3(128), 0, s, p);

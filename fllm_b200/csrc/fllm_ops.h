@@ -371,6 +371,7 @@ struct Kv4Rows {
   uint8_t *k_cache, *v_cache;  // [num_blocks, hkv, block_size, head_dim / 2 + 4]
   int* status;
   int rows, hkv, head_dim, block_size, num_blocks;
+  int block_shift;             // set by the launcher: of a block size that is a power of two
 };
 void kv4_write(const Kv4Rows& p, cudaStream_t s);
 void kv4_read(const Kv4Rows& p, float* out, cudaStream_t s);      // rows of k_cache as fp32 [rows, hkv * head_dim]; 0 where there is no slot

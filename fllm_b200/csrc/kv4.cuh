@@ -42,9 +42,27 @@ __device__ __forceinline__ Kv4Scale kv4_scale(const float (&v)[N]) {
   s.step = fine ? __uint_as_float((__float_as_uint(__fdiv_rn(range, 15.f)) + 0xFFFFu) & 0xFFFF0000u) : __int_as_float(0x7FC00000);
   return s;
 }
+// Step and lowest value of a row from its lowest and largest one (infinite or NaN where some value is).
+__device__ __forceinline__ Kv4Scale kv4_scale_between(float lo, float hi) {
+  const float range = hi - lo;
+  const bool fine = fabsf(lo) < INFINITY && fabsf(hi) < INFINITY && range < INFINITY;
+  Kv4Scale s;
+  s.low = fine ? lo : 0.f;
+  s.step = fine ? __uint_as_float((__float_as_uint(__fdiv_rn(range, 15.f)) + 0xFFFFu) & 0xFFFF0000u) : __int_as_float(0x7FC00000);
+  return s;
+}
 __device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Scale& s) {
   if (!(s.step > 0.f)) return 0;
   return (uint32_t)fminf(rintf(__fdiv_rn(x - s.low, s.step)), 15.f);
+}
+// The same without a division, `inv` 1 / step or near it, for steps of 2^-100 to 2^100: what c leaves of x - z is exact, and says whether c is the nearest
+// (of two as near, the even one).
+__device__ __forceinline__ uint32_t kv4_code_by(float x, const Kv4Scale& s, float inv) {
+  const float d = x - s.low, t = fmaf(d, inv, 8388608.f);       // 2^23: a sum's last bit is that of ones
+  float c = t - 8388608.f;
+  const float r = fmaf(-c, s.step, d), off = fabsf(r) - 0.5f * s.step;
+  if (off > 0.f || (off == 0.f && (__float_as_uint(t) & 1))) c += r > 0.f ? 1.f : -1.f;
+  return (uint32_t)fminf(c, 15.f);
 }
 __device__ __forceinline__ float kv4_value(uint32_t code, const Kv4Scale& s) { return fmaf((float)code, s.step, s.low); }
 
