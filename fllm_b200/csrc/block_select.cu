@@ -13,8 +13,13 @@
 // between; one of fewer blocks reads all. A block with a value that is not finite (or 2^107 and above) scores infinity: it is read, so that it shows.
 // Values of a query that are not finite count as 0.
 //
-// The scores of a step go through memory, tile of rows by tile; scores are products of 16 blocks and 8 rows on mma.sync of int8 (a block's codes are read
-// once for a tile of rows, in pieces of 16 bytes). Decode rows are bounded by that read.
+// The scores of a step go through memory; scores are products of 16 blocks and 8 rows on mma.sync of int8 (a block's codes are read once for a tile of rows, in
+// pieces of 16 bytes), the choice is a search for the last key that is taken, digit by digit.
+//
+// What bounds them (us from captured graphs, scores and choice together): reading the codes, where there are many (64 decode rows of 4000 to 32,000 tokens, 8 key heads
+// of 128, 139 MB: 61, some 45 of them for the scores, 3.1 TB/s: a warp waits for table and codes with 16 blocks on their way); trips to memory one behind the other and
+// the barriers of a choice where there are few (one row of 30,000 tokens: 18); the choices of prompts, one CTA for each row and head (602 rows of 3000 to 6300
+// tokens: 64, some 40 for them). Bounds: 1 to 4.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <limits.h>
@@ -160,18 +165,38 @@ __global__ void __launch_bounds__(128) block_score_kernel(const __grid_constant_
   const int first = p.lead + piece * each * 4 * kScoreBlocks, stop = min(end, first + each * 4 * kScoreBlocks);
   if (first >= stop) return;
 
-  // u and -w of the rows: a warp to a row
-  for (int r = warp; r < kTileRows; r += 4) {
+  const int* table = s.block_tables + (size_t)seq * s.max_blocks;
+  constexpr int J = 2 * D / 64;             // pieces of 16 bytes of a lane
+  // The block of lane & 15 of a step is looked up two steps ahead of its use.
+  bool missing = false;
+  auto look = [&](int b0) {
+    const int at = b0 + (lane & 15);
+    const int id = at < stop && at < s.max_blocks ? table[at] : 0;
+    const bool there = (unsigned)id < (unsigned)s.num_blocks;
+    missing |= !there;
+    return there ? id : -1;
+  };
+  constexpr int kStep = 4 * kScoreBlocks;
+  const int mine0 = first + warp * kScoreBlocks;
+  int id = mine0 < stop ? look(mine0) : 0, id1 = mine0 + kStep < stop ? look(mine0 + kStep) : 0;
+  // u and -w of the rows: a warp to a row (what the products have of rows that are not there goes nowhere)
+  for (int r = warp; r < n_rows; r += 4) {
     constexpr int CH = D / 32;
     float u[CH], w[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) u[i] = w[i] = 0.f;
-    if (r < n_rows) {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const bf16*>(s.q) + (size_t)(q0 + row0 + r) * s.ldq + (size_t)kvh * p.group * D) + lane * (CH / 2);
-      for (int h = 0; h < p.group; ++h, src += D / 2) {
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const bf16*>(s.q) + (size_t)(q0 + row0 + r) * s.ldq + (size_t)kvh * p.group * D) + lane * (CH / 2);
+    for (int h0 = 0; h0 < p.group; h0 += 4) {           // heads in their order, four on their way at once
+      uint32_t q4[4][CH / 2];
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) q4[h][i] = h0 + h < p.group ? src[(h0 + h) * (D / 2) + i] : 0u;
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
 #pragma unroll
         for (int i = 0; i < CH / 2; ++i) {
-          const float2 f = unpack_bf16x2(src[i]);
+          const float2 f = unpack_bf16x2(q4[h][i]);
           const float x[2] = {isfinite(f.x) ? f.x : 0.f, isfinite(f.y) ? f.y : 0.f};
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
@@ -179,7 +204,6 @@ __global__ void __launch_bounds__(128) block_score_kernel(const __grid_constant_
             w[2 * i + k] = fminf(w[2 * i + k] + fmaxf(-x[k], 0.f), FLT_MAX);
           }
         }
-      }
     }
     float top = 0.f;
 #pragma unroll
@@ -195,20 +219,6 @@ __global__ void __launch_bounds__(128) block_score_kernel(const __grid_constant_
   }
   __syncthreads();
 
-  const int* table = s.block_tables + (size_t)seq * s.max_blocks;
-  constexpr int J = 2 * D / 64;             // pieces of 16 bytes of a lane
-  // The block of lane & 15 of a step is looked up two steps ahead of its use.
-  bool missing = false;
-  auto look = [&](int b0) {
-    const int at = b0 + (lane & 15);
-    const int id = at < stop && at < s.max_blocks ? table[at] : 0;
-    const bool there = (unsigned)id < (unsigned)s.num_blocks;
-    missing |= !there;
-    return there ? id : -1;
-  };
-  constexpr int kStep = 4 * kScoreBlocks;
-  const int mine0 = first + warp * kScoreBlocks;
-  int id = mine0 < stop ? look(mine0) : 0, id1 = mine0 + kStep < stop ? look(mine0 + kStep) : 0;
   for (int b0 = mine0; b0 < stop; b0 += kStep) {
     const int id2 = b0 + 2 * kStep < stop ? look(b0 + 2 * kStep) : 0;
     const int e_at = id >= 0 ? (int)p.bounds[((size_t)id * s.hkv + kvh) * (2 * D + kTail) + 2 * D] : -128;
@@ -218,7 +228,7 @@ __global__ void __launch_bounds__(128) block_score_kernel(const __grid_constant_
       const int other = __shfl_sync(0xffffffffu, max(id, 0), g + 8 * h);
       const int8_t* of = p.bounds + ((size_t)other * s.hkv + kvh) * (2 * D + kTail) + 16 * t;
 #pragma unroll
-      for (int j = 0; j < J; ++j) a[h][j] = __ldg(reinterpret_cast<const uint4*>(of + 64 * j));
+      for (int j = 0; j < J; ++j) a[h][j] = *reinterpret_cast<const uint4*>(of + 64 * j);
     }
     id = id1;
     id1 = id2;
@@ -251,25 +261,21 @@ __device__ __forceinline__ uint32_t key_of(float f) {
   const uint32_t b = __float_as_uint(f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-// Exclusive sums of two counts below 2^16 each in one word... of 256 threads; `total` of all.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* sums, unsigned long long& total) {
+// Exclusive sum over the threads. `sums` is free again behind the next barrier.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned long long upto = v;
+  uint32_t upto = v;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
-    const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+    const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += x;
   }
   if (lane == 31) sums[warp] = upto;
   __syncthreads();
-  unsigned long long before = 0;
-  total = 0;
+  uint32_t before = 0;
 #pragma unroll
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
+  for (int w = 0; w < kSelectThreads / 32; ++w)
     if (w < warp) before += sums[w];
-    total += sums[w];
-  }
-  __syncthreads();
   return before + upto - v;
 }
 
@@ -279,6 +285,7 @@ __global__ void __launch_bounds__(kSelectThreads) block_choose_kernel(const __gr
   extern __shared__ uint32_t keys_s[];
   __shared__ uint32_t hist[kBins];
   __shared__ unsigned long long sums[kSelectThreads / 32];
+  __shared__ uint32_t parts[kSelectThreads / 32];
   __shared__ uint32_t found[2];
   const SpanParams& s = p.rows;
   const int local = blockIdx.x / s.hkv, kvh = blockIdx.x - local * s.hkv, row = p.row_from + local, tid = threadIdx.x;
@@ -299,6 +306,7 @@ __global__ void __launch_bounds__(kSelectThreads) block_choose_kernel(const __gr
   const int n = most - p.lead - p.tail;
   const float* scores = p.scores + ((size_t)local * s.hkv + kvh) * p.stride + p.lead;
   uint32_t least = 0xFFFFFFFFu, most_key = 0;
+#pragma unroll 8
   for (int i = tid; i < n; i += kSelectThreads) {
     const uint32_t k = key_of(scores[i]);
     keys_s[i] = k;
@@ -322,6 +330,7 @@ __global__ void __launch_bounds__(kSelectThreads) block_choose_kernel(const __gr
     const int bits = 11, shift = max(upper - bits, 0);
     for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
     __syncthreads();
+#pragma unroll 8
     for (int i = tid; i < n; i += kSelectThreads) {
       const uint32_t k = keys_s[i] - least;
       if ((k & mask) == prefix) atomicAdd(&hist[(k & ~mask) >> shift], 1u);
@@ -337,8 +346,7 @@ __global__ void __launch_bounds__(kSelectThreads) block_choose_kernel(const __gr
       mine[i] = hist[from - i];
       sum += mine[i];
     }
-    unsigned long long total;
-    uint32_t above = (uint32_t)block_scan(sum, sums, total);
+    uint32_t above = block_scan(sum, parts);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       if (above < (uint32_t)want && (uint32_t)want <= above + mine[i]) { found[0] = (uint32_t)(from - i); found[1] = above; }
@@ -353,22 +361,35 @@ __global__ void __launch_bounds__(kSelectThreads) block_choose_kernel(const __gr
     __syncthreads();
   }
   prefix += least;
-  // A thread has neighbouring blocks, an odd number of them: its place among the others' is a sum over the threads in front of it.
-  const int each = ((n + kSelectThreads - 1) / kSelectThreads) | 1;
-  const int from = min(tid * each, n), to = min(from + each, n);
-  unsigned long long counts = 0;            // above the last key, and equal to it
-  for (int i = from; i < to; ++i) {
-    const uint32_t k = keys_s[i];
-    counts += (k > prefix ? 1ull << 32 : 0ull) + (k == prefix ? 1ull : 0ull);
+  // A warp has neighbouring blocks, 32 at a time: the place of one among the others' is a sum over the warps in front of it, and a count of lanes.
+  const int warp = tid >> 5, lane = tid & 31, each = ((n + kSelectThreads - 1) / kSelectThreads) * 32;
+  const int from = min(warp * each, n), to = min(from + each, n);
+  int over = 0, equal = 0;
+#pragma unroll 4
+  for (int i0 = from; i0 < to; i0 += 32) {
+    const uint32_t k = i0 + lane < to ? keys_s[i0 + lane] : 0;
+    over += __popc(__ballot_sync(0xffffffffu, i0 + lane < to && k > prefix));
+    equal += __popc(__ballot_sync(0xffffffffu, i0 + lane < to && k == prefix));
   }
-  unsigned long long total;
-  const unsigned long long before = block_scan(counts, sums, total);
-  int over = (int)(before >> 32), equal = (int)(before & 0xFFFFFFFFu);
-  for (int i = from; i < to; ++i) {
-    const uint32_t k = keys_s[i];
-    if (k > prefix || (k == prefix && equal < want)) out[p.lead + over + min(equal, want)] = p.lead + i;
-    over += k > prefix;
-    equal += k == prefix;
+  if (lane == 0) sums[warp] = (unsigned long long)over << 32 | (uint32_t)equal;
+  __syncthreads();
+  over = equal = 0;
+#pragma unroll
+  for (int w = 0; w < kSelectThreads / 32; ++w)
+    if (w < warp) {
+      over += (int)(sums[w] >> 32);
+      equal += (int)(uint32_t)sums[w];
+    }
+  const unsigned below = (1u << lane) - 1;
+#pragma unroll 4
+  for (int i0 = from; i0 < to; i0 += 32) {
+    const uint32_t k = i0 + lane < to ? keys_s[i0 + lane] : 0;
+    const bool is_over = i0 + lane < to && k > prefix, is_equal = i0 + lane < to && k == prefix;
+    const unsigned o = __ballot_sync(0xffffffffu, is_over), e = __ballot_sync(0xffffffffu, is_equal);
+    const int my_over = over + __popc(o & below), my_equal = equal + __popc(e & below);
+    if (is_over || (is_equal && my_equal < want)) out[p.lead + my_over + min(my_equal, want)] = p.lead + i0 + lane;
+    over += __popc(o);
+    equal += __popc(e);
   }
 }
 
@@ -386,7 +407,7 @@ template <int D, int NQ>
 void launch_scores(SelectParams p, cudaStream_t s) {
   const long long tiles = span_tiles(p.rows, p.rows.max_q_len, 8 * NQ, p.rows.search) * p.rows.hkv;
   // Pieces of the text for two rounds of CTAs, so that long texts do not hold their SMs alone in the end (64 decode rows of 4000 to 32,000 tokens, 8 key heads of
-  // 128: 48 us with half as many, 34, 37 with twice, 42 with four times as many), a step of each warp at least.
+  // 128, the scores' kernel in one run: 48 us with half as many, 34 so, 37 with twice, 42 with four times as many), a step of each warp at least.
   const long long steps = (std::max(p.stride - p.lead - p.tail, 1) + 4 * kScoreBlocks - 1) / (4 * kScoreBlocks);
   p.pieces = (int)std::max<long long>(1, std::min<long long>(16LL * sm_count() / tiles, steps));
   if (tiles * p.pieces > INT_MAX) throw std::runtime_error("select_blocks: too many query rows");
