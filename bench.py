@@ -147,7 +147,7 @@ def main() -> None:
     ap.add_argument("--batch", type=int, default=None)
     ap.add_argument("--prompt-len", type=int, default=None)
     ap.add_argument("--weight-format", default=None)
-    ap.add_argument("--kv-cache-type", default="bf16", choices=["bf16", "fp8_e4m3"],
+    ap.add_argument("--kv-cache-type", default="bf16", choices=["bf16", "fp8_e4m3", "int4"],
                     help="element type of the paged KV pool (the headline configuration uses bf16)")
     ap.add_argument("--backend", default=os.environ.get("FLLM_TP_BACKEND", "auto"),
                     help="tensor-parallel collectives: auto | fused | nccl")
