@@ -527,9 +527,11 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const PageRows page_rows{p, p.block_tables + (size_t)seq * p.max_blocks, kvh, range.head, range.lo - range.head, range.count,
                            (int)(p.num_blocks * p.hkv * p.block_pages * kPage)};
 
-  // The block was launched with 168 registers a thread (e4m3 and 4 bits: 128): 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128.
+  // The block was launched with 168 registers a thread (e4m3 and 4 bits: 128): 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128,
+  // or 256 x 184 + 256 x 72 (4 bits: 490 us where 64 for those that widen took 534, 2 x 2048 rows behind 2500 and 6143 tokens).
   if (warp >= 8) {
-    if constexpr (KV != kBf16) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (KV4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else if constexpr (KV8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     bool bad = false;
     if (q_too) {
@@ -876,7 +878,8 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     }
     if (bad && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
   } else {
-    if constexpr (KV != kBf16) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if constexpr (KV4) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    else if constexpr (KV8) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     q_loaded();
