@@ -19,7 +19,7 @@
 // query and 8 key heads of 128: 1097 TFLOP/s, e4m3 1007; under a window of 1024 with 64 first tokens 735, of the products that the window leaves. (CTAs
 // that stay and take item after item hid the way in, but missed the instruction cache 7000 times an SM for 2800: 146 us for 115 at that
 // window then; 126 for 197 with 16 trees of equal lengths.) Over a 4-bit cache 2 x 2048 rows behind 2500 and 6143 tokens take
-// 527 us, 680 TFLOP/s (bf16 323, e4m3 395): widening a tile of K and one of V takes three warps each about as long as the groups' softmax, and they share its
+// 477 us, 752 TFLOP/s (bf16 323, e4m3 395): widening a tile of K and one of V takes three warps each about as long as the groups' softmax, and they share its
 // SM's issue slots.
 //
 // What a row sees of a tile is four words of bits, from its bounds and its mask; tiles that all rows of a warp see whole have code

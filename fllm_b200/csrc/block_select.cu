@@ -69,12 +69,10 @@ __device__ __forceinline__ void load_channels(const uint8_t* row, int lane, floa
     }
   } else {
     const Kv4Scale s = kv4_scale_of(*reinterpret_cast<const uint32_t*>(row + D / 2));
+    using Codes = std::conditional_t<CH == 2, uint8_t, std::conditional_t<CH == 4, uint16_t, uint32_t>>;
+    const uint32_t codes = reinterpret_cast<const Codes*>(row)[lane];
 #pragma unroll
-    for (int i = 0; i < CH / 2; ++i) {
-      const uint32_t c = row[lane * (CH / 2) + i];
-      v[2 * i] = kv4_value(c & 15, s);
-      v[2 * i + 1] = kv4_value(c >> 4, s);
-    }
+    for (int i = 0; i < CH; ++i) v[i] = kv4_value(codes >> 4 * i & 15, s);
   }
 }
 
@@ -98,7 +96,7 @@ __global__ void __launch_bounds__(128) kv_bounds_kernel(const __grid_constant__ 
   float hi[CH], lo[CH], odd = 0.f;
 #pragma unroll
   for (int i = 0; i < CH; ++i) { hi[i] = -INFINITY; lo[i] = INFINITY; }
-#pragma unroll 8
+#pragma unroll 16
   for (int r = 0; r < p.block_size; ++r) {
     float v[CH];
     load_channels<D, KIND>(src + (size_t)r * RB, lane, v);
