@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(128, kv4_resident<D, NB>()) kv4_rows_kernel(co
         }
       }
     }
-    float top[NB][2], steepest = fmaxf(vs[0][0].step, vs[0][1].step);      // largest scores and steps of a lane
+    float top[NB][2], steepest = fmaxf(fmaxf(0.f, vs[0][0].step), vs[0][1].step);      // largest scores and steps of a lane (a NaN is none)
 #pragma unroll
     for (int h = 1; h < kPages; ++h) steepest = fmaxf(fmaxf(steepest, vs[h][0].step), vs[h][1].step);
 #pragma unroll

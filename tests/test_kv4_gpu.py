@@ -223,6 +223,24 @@ def test_values_that_are_not_finite(ops, T):
         so.check(y[~sees], o[~sees], bound[~sees])
 
 
+@pytest.mark.parametrize("hq,nodes", [(2, 60), (2, 14), (8, 200), (32, 200)])
+def test_a_branch_of_values_that_are_not_finite(ops, hq, nodes):
+    """Two chains in turn behind one root: every value of the first is NaN, and the rows of the second are as if it were not there, whatever lanes hold of it."""
+    par = [-1] + [max(0, i - 2) for i in range(1, nodes)]
+    c = ko.setup([nodes], [201], hq, 2, 128, words=4, trees=[par], seed=3)
+    row = torch.full((2, 128), float("nan"), device="cuda")
+    for node in range(1, nodes, 2):                       # at even places of the text
+        tok = 201 + node
+        c.v[int(c.tables[0, tok // 16]), :, tok % 16] = kv4_encode(row)
+        c.values[0][tok] = 0.0
+    y = ops.attention_tree(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.masks, c.base, hq, 2, 128, 128 ** -0.5, meta=c.meta)
+    o, bound = ko.want(c, 128 ** -0.5, 0, 0)
+    second = torch.arange(nodes, device="cuda") % 2 == 0
+    assert torch.isnan(y[~second]).all()
+    so.check(y[second], o[second], bound[second])
+    assert ops.check_status() == 0
+
+
 @pytest.mark.parametrize("k_scale,v_scale", [(1e-20, 1.0), (1.0, 1e-30), (1.0, 1e30), (50.0, 1e4), (1.0, 1e37)])
 def test_magnitudes(ops, k_scale, v_scale):
     """Steps of any size: of a cache's tokens alike."""
