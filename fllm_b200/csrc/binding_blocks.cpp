@@ -5,6 +5,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
+
 #include "fllm_ops.h"
 
 namespace {
@@ -115,7 +117,7 @@ void kv_bounds(const Tensor& k_cache, Tensor bounds, const Tensor& slots, const 
 // -> (blocks [rows, hkv, count], kernels launched)
 std::tuple<Tensor, int64_t> select_blocks(const Tensor& q, const Tensor& bounds, const Tensor& block_tables, const Tensor& q_starts, const Tensor& kv_lens, int64_t num_seqs,
                                           int64_t max_q_len, int64_t max_kv_len, int64_t hq, int64_t hkv, int64_t head_dim, int64_t block_size, int64_t count,
-                                          int64_t lead, int64_t tail, const optional<Tensor>& status) {
+                                          int64_t lead, int64_t tail, const optional<Tensor>& status, int64_t scores_bytes) {
   TORCH_CHECK(hq > 0 && hkv > 0 && hq % hkv == 0 && hq <= 65536, "select_blocks: query heads must be a multiple of the key heads");
   TORCH_CHECK(check_bounds(bounds, hkv) == head_dim, "select_blocks: bounds of another head_dim");
   TORCH_CHECK(q.is_cuda() && q.device() == bounds.device() && q.scalar_type() == at::kBFloat16 && q.dim() == 2 && q.size(1) == hq * head_dim &&
@@ -152,12 +154,20 @@ std::tuple<Tensor, int64_t> select_blocks(const Tensor& q, const Tensor& bounds,
   if (q.size(0) == 0) return {out, 0};
   if (num_seqs == 0) return {out.fill_(-1), 0};
   p.out = out.data_ptr<int>();
-  Tensor scores;                              // of this call alone: two streams or two captured graphs do not share them
+  // Scores are of this call alone: two streams or two captured graphs do not share them. Rows of long prompts beside long texts take their turns in them.
+  const int64_t rows = p.stride > p.count ? std::min<int64_t>(q.size(0), std::max<int64_t>(64, scores_bytes / (4 * hkv * p.stride))) : q.size(0);
+  Tensor scores;
   if (p.stride > p.count) {
-    scores = at::empty({q.size(0) * hkv * p.stride}, q.options().dtype(at::kFloat));
+    scores = at::empty({rows * hkv * p.stride}, q.options().dtype(at::kFloat));
     p.scores = scores.data_ptr<float>();
   }
-  return {out, fllm::select_blocks(p, cur_stream())};
+  int64_t n = 0;
+  for (int64_t from = 0; from < q.size(0); from += rows) {
+    p.row_from = (int)from;
+    p.row_to = (int)std::min<int64_t>(from + rows, q.size(0));
+    n += fllm::select_blocks(p, cur_stream());
+  }
+  return {out, n};
 }
 }  // namespace
 
@@ -166,5 +176,5 @@ TORCH_LIBRARY_FRAGMENT(fllm_b200, m) {
   m.def("kv4_read(Tensor cache, Tensor slots, Tensor? status=None) -> Tensor", &kv4_read);
   m.def("kv_bounds(Tensor k_cache, Tensor(a!) bounds, Tensor slots, Tensor? status=None) -> ()", &kv_bounds);
   m.def("select_blocks(Tensor q, Tensor bounds, Tensor block_tables, Tensor q_starts, Tensor kv_lens, int num_seqs, int max_q_len, int max_kv_len, int hq, int hkv, "
-        "int head_dim, int block_size, int count, int lead, int tail, Tensor? status=None) -> (Tensor, int)", &select_blocks);
+        "int head_dim, int block_size, int count, int lead, int tail, Tensor? status=None, int scores_bytes=268435456) -> (Tensor, int)", &select_blocks);
 }

@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(128) block_score_kernel(const __grid_constant_
   const int row0 = tile * kTileRows;
   if (row0 >= qn) return;
   const int n_rows = min(kTileRows, qn - row0);
+  if (q0 + row0 >= p.row_to || q0 + row0 + n_rows <= p.row_from) return;
   // blocks that the tile's last row chooses among
   const int last = max(kv_len - qn + row0 + n_rows, 0);       // its tokens
   const int most = (last + p.block_size - 1) / p.block_size;
@@ -245,7 +246,8 @@ __global__ void __launch_bounds__(128) block_score_kernel(const __grid_constant_
       for (int x = 0; x < 4; ++x) {
         const int r = 8 * n + 2 * t + (x & 1), b = b0 + g + 8 * (x >> 1), e = x >> 1 ? e1 : e0;
         const float score = e == kNotFinite ? INFINITY : e == -128 ? -INFINITY : (float)c[x] * pow2(e);
-        if (r < n_rows && b < stop) p.scores[((size_t)(q0 + row0 + r - p.row_from) * s.hkv + kvh) * p.stride + b] = score;
+        const int at = q0 + row0 + r;
+        if (r < n_rows && b < stop && at >= p.row_from && at < p.row_to) p.scores[((size_t)(at - p.row_from) * s.hkv + kvh) * p.stride + b] = score;
       }
     }
   }
@@ -438,7 +440,7 @@ int select_blocks(SelectParams p, cudaStream_t s) {
     }
     ++n;
   }
-  launch_pdl(block_choose_kernel, dim3((unsigned)((long long)p.rows.tokens * p.rows.hkv)), dim3(kSelectThreads), (size_t)(p.stride > p.count ? p.stride * 4 : 0), s, p);
+  launch_pdl(block_choose_kernel, dim3((unsigned)((long long)(p.row_to - p.row_from) * p.rows.hkv)), dim3(kSelectThreads), (size_t)(p.stride > p.count ? p.stride * 4 : 0), s, p);
   cuda_check(cudaGetLastError(), "select_blocks launch");
   return n + 1;
 }

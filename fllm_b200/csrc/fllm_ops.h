@@ -391,9 +391,9 @@ struct SelectParams {
   const int8_t* bounds;
   int group, block_size, count, lead, tail;
   int stride;                  // blocks of the longest text, at most
-  float* scores;               // [rows][hkv][stride]
+  float* scores;               // [row_to - row_from][hkv][stride]
   int* out;                    // [rows][hkv][count]
-  int row_from;
+  int row_from, row_to;        // the rows that are chosen for
   int pieces;                  // set by the launcher
 };
 int select_blocks(SelectParams p, cudaStream_t s);     // kernels launched

@@ -95,6 +95,17 @@ def test_choices_of_prompt_rows(ops, hq, hkv, D):
     assert ops.check_status() == 0
 
 
+def test_rows_that_take_turns_in_the_scores_memory(ops):
+    """Room for 64 rows at a time: the choices are the same, tiles that lie in two turns among them."""
+    c = so.setup([150, 1, 41], [700, 900, 30], 8, 2, 128, seed=6)
+    b = _bounds(c)
+    c.tables[c.tables < 0] = 0
+    m = c.meta
+    few, n = ops.k.select_blocks(c.q, b, c.tables, m.q_starts, m.seq_lens, m.num_seqs, m.max_q_len, m.max_kv_len, 8, 2, 128, 16, 7, 1, 2, ops.status, 1)
+    assert n == 6 and torch.equal(few, _choose(ops, c, b, 16, 7)) and torch.equal(few.cpu(), _choices(c, b, 16, 7, 1, 2))
+    assert ops.check_status() == 0
+
+
 def test_equal_scores_go_to_the_lower_block(ops):
     """Blocks with the same keys, queries of zeros: every score is met many times."""
     c = so.setup([1, 3], [3000, 1000], 8, 2, 128, seed=1)
