@@ -909,7 +909,8 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         const int t = n >> shift;
         if (!mbar_wait(&v_unit[t & 1], (t >> 1) & 1, abort_flag)) { ok = false; break; }
         const int up = k_up[t & 3], now = v_up[t & 3];
-        factor = row_factor * pow2_of(-(up >> 1)) * pow2_of((up >> 1) - up);
+        // Not 0, nor infinite, as factors of rows are not (span_factor): a score of 0 in an unseen place beside one, or a 0 beside the other, would be a NaN.
+        factor = fminf(fmaxf(row_factor * pow2_of(-(up >> 1)) * pow2_of((up >> 1) - up), FLT_MIN), FLT_MAX);
         if (p.softcap <= 0.f) scale = factor;
         if (k > 0 && now != up_v) shrink = pow2_of(max(now - up_v, -126));
         up_v = now;
@@ -917,7 +918,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       const bool whole = tok0 + kTile <= w_base && (tok0 >= w_beg || tok0 + kTile <= p.first);
       uint4 vis = make_uint4(0, 0, 0, 0);
       if (!whole) vis = row_bits(p, q0, qn, kv_len, gap, qi, tok0);
-      if (p.softcap > 0.f) cap_scores(t_s, factor / (p.softcap * kLog2e));
+      if (p.softcap > 0.f) cap_scores(t_s, fminf(factor / (p.softcap * kLog2e), FLT_MAX));
       softmax_tile<D, KV != kBf16>(t_s, t_o, whole, vis, scale, k > 0, &p_half[group], m_used, l, shrink);
       tc_fence_before_sync();
       __syncwarp();
