@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(128, kv4_resident<D, NB>()) kv4_rows_kernel(co
     *reinterpret_cast<uint4*>(qtile + r * S::kQPitch + c * 16) =
         make_uint4(pack_16<true>(x[0], x[4]), pack_16<true>(x[1] * 0.0625f, x[5] * 0.0625f), pack_16<true>(x[2], x[6]), pack_16<true>(x[3] * 0.0625f, x[7] * 0.0625f));
     if (c == 0) {
-      factors[r] = span_factor(p.scale_log2, up) * 16777216.f;           // products are with c 2^-24
+      factors[r] = fminf(span_factor(p.scale_log2, up) * 16777216.f, FLT_MAX);      // products are with c 2^-24; an infinity would make a NaN of a score of 0
       qsums[r] = sum * (1.f / 16777216.f);
     }
   }

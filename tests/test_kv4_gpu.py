@@ -360,3 +360,16 @@ def test_refusals(ops):
             bad()
     with pytest.raises(ValueError):
         kv4_width(96)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("hq", [2, 8, 32])
+def test_queries_of_the_largest_size_beside_keys_of_zero(ops, D, hq):
+    """Few rows: scores are 0 where the keys are, whatever the queries' size."""
+    c = ko.setup([1, 3], [200, 33], hq, 2, D, seed=D)
+    c.q = (c.q.float() * 2.0 ** 122).bfloat16()
+    c.k.zero_()
+    c.keys = [torch.zeros_like(k) for k in c.keys]
+    o, bound = so.want(c, D ** -0.5, 0, 0)
+    so.check(_attend(ops, c), o, bound + ko.slack(c))
+    assert ops.check_status() == 0
