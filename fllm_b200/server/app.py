@@ -13,6 +13,7 @@ from __future__ import annotations
 import asyncio
 import contextlib
 import json
+import math
 import queue
 import threading
 import time
@@ -637,9 +638,10 @@ def create_app(engine, tokenizer, model_name: str = "fllm-b200", api_key: Option
         import base64
         kvd = obj["kv"]
         raw = torch.frombuffer(bytearray(base64.b64decode(kvd["data"])), dtype=torch.uint8)
-        dt = engine.kv.store.dtype if kvd["elem"] == engine.kv.store.element_size() else None
-        if dt is None:
-            raise HTTPException(400, "KV element size does not match this engine")
+        # what the exporting engine's cache holds; whether this engine's takes it (itself, or converted) is for import_request to say
+        dt = {str(t): t for t in (torch.bfloat16, torch.float32, torch.float8_e4m3fn, torch.uint8)}.get(obj.get("kv_dtype"))
+        if dt is None or kvd["elem"] != dt.itemsize or raw.numel() != math.prod(kvd["shape"]) * dt.itemsize:
+            raise HTTPException(400, "KV of an unknown kind, or not of its shape")
         blob = dict(obj)
         blob["kv"] = raw.view(dt).view(*kvd["shape"])
         return blob

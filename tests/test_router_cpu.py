@@ -6,7 +6,7 @@ import pytest
 from fastapi.testclient import TestClient
 
 from fllm_b200.config import EngineConfig, preset
-from fllm_b200.runtime import LLMEngine
+from fllm_b200.runtime import LLMEngine, SamplingParams
 from fllm_b200.server.app import create_app
 from fllm_b200.server.router import create_router
 from fllm_b200.tokenizer import ByteTokenizer
@@ -108,3 +108,33 @@ def test_bench_serve_load_generator_against_an_in_process_server(stack):
     rep = asyncio.run(go())
     assert rep["errors"] == 0 and rep["requests"] == 6
     assert rep["output_tok_per_s"] > 0 and rep["ttft_ms"]["p50"] is not None and rep["e2e_ms"]["p99"] >= rep["ttft_ms"]["p50"]
+
+
+def test_servers_hand_over_between_kinds_of_caches():
+    """A prompt's blocks travel from a server with a bf16 cache to one with a 4-bit cache and back, as between their engines; kinds that do not take each other's,
+    kinds that are none and contents that are not of their shape are refused."""
+    cfg = preset("qwen3-tiny")
+    cfg.vocab_size = 512
+    mk = lambda kind: LLMEngine(cfg, EngineConfig(max_num_seqs=4, max_num_batched_tokens=64, max_model_len=256, num_kv_blocks=64, kv_cache_dtype=kind), device="cpu",
+                                eos_token_id=257, seed=0)
+    body = {"prompt": "disaggregate this prompt please", "max_tokens": 8, "temperature": 0}
+
+    def direct(blob, kind):
+        eng = mk(kind)
+        rid, toks = eng.import_request(blob), list(blob["output"])
+        while eng.has_unfinished():
+            toks += [t for ev in eng.step() if ev.request_id == rid for t in ev.token_ids]
+        return toks
+    serve = lambda kind: TestClient(create_app(mk(kind), ByteTokenizer(512), "tiny"))
+    for src, dst in (("bf16", "int4"), ("int4", "bf16"), ("int4", "int4")):
+        with serve(src) as a, serve(dst) as b:               # (of no history: blocks that were handed over are hits for the next prompt like it)
+            blob = a.post("/admin/disagg/export", json=body).json()
+            done = b.post("/admin/disagg/import", json=blob)
+            assert done.status_code == 200, done.text
+            assert done.json()["choices"][0]["token_ids"] == direct(mk(src).prefill_only(blob["prompt"], SamplingParams(**blob["params"]))[0], dst)
+    with serve("bf16") as a, serve("int4") as b, serve("fp8_e4m3") as c:
+        blob = a.post("/admin/disagg/export", json=body).json()
+        assert c.post("/admin/disagg/import", json=blob).status_code == 400
+        for bad in (dict(blob, kv_dtype="torch.int3"), {x: y for x, y in blob.items() if x != "kv_dtype"}, dict(blob, kv_dtype="torch.uint8"),
+                    dict(blob, kv=dict(blob["kv"], shape=blob["kv"]["shape"][:-1]))):
+            assert b.post("/admin/disagg/import", json=bad).status_code == 400
