@@ -326,6 +326,8 @@ class LLMEngine:
         if kv.dim() != 6 or tuple(kv.shape[:2]) != tuple(want[:2]) or tuple(kv.shape[3:last]) != tuple(want[3:last]) or \
                 (converts and kv.shape[5] != (self.kv.head_dim if self.kv.four_bit else kv4_width(self.kv.head_dim))):
             raise ValueError(f"KV shape {tuple(kv.shape)} does not fit this engine's pool {tuple(want)}")
+        if kv.shape[2] != len(blob["live_blocks"]):
+            raise ValueError(f"KV of {kv.shape[2]} blocks for {len(blob['live_blocks'])} that are named")
         params = SamplingParams(**blob["params"])
         params.validate(self.model_cfg.vocab_size)
         n = int(blob["num_computed"])

@@ -213,3 +213,19 @@ def test_command_line_flags():
     eng = build_engine(args)
     eng = eng[0] if isinstance(eng, tuple) else eng
     assert eng.kv.sparse == (6, 2, 1) and eng.kv.four_bit and eng.kv.bounds.shape[-1] == bounds_width(eng.model_cfg.head_dim)
+
+
+def test_blocks_that_are_handed_over_are_as_many_as_are_named():
+    """Fewer or more blocks than the request names, of the pool's kind or of another: refused, and nothing stays allocated."""
+    cfg = preset("qwen3-tiny")
+    w = init_random_weights(cfg, "cpu")
+    p = _prompts(cfg.vocab_size, (50,))[0]
+    for src in ("bf16", "int4"):
+        blob = _engine(w, cfg, kv_cache_dtype=src).prefill_only(p, SamplingParams(max_tokens=4))[0]
+        for dst in ("bf16", "int4"):
+            eng = _engine(w, cfg, kv_cache_dtype=dst)
+            free = eng.blocks.num_free()
+            for kv in (blob["kv"][:, :, :1], blob["kv"][:, :, [0, 1, 2, 3, 3]]):
+                with pytest.raises(ValueError, match="blocks"):
+                    eng.import_request(dict(blob, kv=kv))
+                assert eng.blocks.num_free() == free and not eng.requests
