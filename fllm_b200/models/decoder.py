@@ -104,7 +104,8 @@ class KVCache:
         (encoded) or the other way round (what the codes stand for, rounded to bf16)."""
         kv = kv.to(self.store.device)
         if kv.dtype == self.store.dtype and kv.shape[3:] == self.store.shape[3:]:
-            self.store.index_copy_(2, blocks, kv)
+            store, kv = (x.view(torch.uint8) if x.element_size() == 1 else x for x in (self.store, kv))      # (index_copy_ knows no e4m3)
+            store.index_copy_(2, blocks, kv)
         elif tuple(kv.shape[3:5]) == tuple(self.store.shape[3:5]) and {kv.dtype, self.store.dtype} == {torch.bfloat16, torch.uint8}:
             n, heads = kv.shape[2], kv.shape[3]
             slots = torch.arange(n * self.block_size, dtype=torch.int32, device=kv.device)

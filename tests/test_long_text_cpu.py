@@ -229,3 +229,20 @@ def test_blocks_that_are_handed_over_are_as_many_as_are_named():
                 with pytest.raises(ValueError, match="blocks"):
                     eng.import_request(dict(blob, kv=kv))
                 assert eng.blocks.num_free() == free and not eng.requests
+
+
+def test_e4m3_blocks_come_back():
+    """Blocks of an e4m3 cache are handed over, and swapped, like those of other kinds."""
+    cfg = preset("qwen3-tiny")
+    w = init_random_weights(cfg, "cpu")
+    mk = lambda **kw: _engine(w, cfg, kv_cache_dtype="fp8_e4m3", max_model_len=128, enable_prefix_caching=False, **kw)
+    p = _prompts(cfg.vocab_size, (40, 44, 48, 52))
+    sp = SamplingParams(max_tokens=12)
+    blob = mk().prefill_only(p[0], sp)[0]
+    eng = mk()
+    rid, toks = eng.import_request(blob), list(blob["output"])
+    while eng.has_unfinished():
+        toks += [t for ev in eng.step() if ev.request_id == rid for t in ev.token_ids]
+    assert toks == mk().generate([p[0]], sp)[0]
+    tight = mk(num_kv_blocks=13, watermark=0.0, preemption="swap", swap_space_gb=0.25)
+    assert tight.generate(p, sp) == mk().generate(p, sp) and tight.scheduler.swapper.stats["swapped_in"] > 0

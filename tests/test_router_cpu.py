@@ -126,7 +126,7 @@ def test_servers_hand_over_between_kinds_of_caches():
             toks += [t for ev in eng.step() if ev.request_id == rid for t in ev.token_ids]
         return toks
     serve = lambda kind: TestClient(create_app(mk(kind), ByteTokenizer(512), "tiny"))
-    for src, dst in (("bf16", "int4"), ("int4", "bf16"), ("int4", "int4")):
+    for src, dst in (("bf16", "int4"), ("int4", "bf16"), ("int4", "int4"), ("fp8_e4m3", "fp8_e4m3")):
         with serve(src) as a, serve(dst) as b:               # (of no history: blocks that were handed over are hits for the next prompt like it)
             blob = a.post("/admin/disagg/export", json=body).json()
             done = b.post("/admin/disagg/import", json=blob)
