@@ -1076,7 +1076,8 @@ class LLMEngine:
             if blob is None:
                 return False
             st[:, :, block].copy_(blob.view(st.dtype).view(st[:, :, block].shape).to(st.device))
-            self.kv.find_bounds(torch.tensor([block], device=st.device), self.ops)
+            if self.kv.bounds is not None:
+                self.kv.find_bounds(torch.tensor([block], device=st.device), self.ops)
             return True
         self.blocks.on_evict, self.blocks.tier_has, self.blocks.tier_restore = evict, self.kv_tier.has, restore
 

@@ -246,3 +246,19 @@ def test_e4m3_blocks_come_back():
     assert toks == mk().generate([p[0]], sp)[0]
     tight = mk(num_kv_blocks=13, watermark=0.0, preemption="swap", swap_space_gb=0.25)
     assert tight.generate(p, sp) == mk().generate(p, sp) and tight.scheduler.swapper.stats["swapped_in"] > 0
+
+
+def test_the_tiers_bring_blocks_back_without_more_where_no_bounds_are_kept(monkeypatch):
+    """No tensor is made for bounds that an engine does not have."""
+    cfg = preset("qwen3-tiny")
+    w = init_random_weights(cfg, "cpu")
+    p, sp = _prompts(cfg.vocab_size, (150, 100, 180)), SamplingParams(max_tokens=4)
+    looked = []
+    monkeypatch.setattr(KVCache, "find_bounds", lambda self, blocks, ops: looked.append(len(blocks)))
+    for sparse in (0, 4):
+        eng = _engine(w, cfg, sparse_blocks=sparse, num_kv_blocks=16, watermark=0.0, kv_tier_host_gb=0.01)
+        for _ in range(2):
+            for x in p:
+                eng.generate([x], sp)
+        assert eng.blocks.stats["tier_restored"] > 0
+        assert len(looked) == (eng.blocks.stats["tier_restored"] if sparse else 0)
