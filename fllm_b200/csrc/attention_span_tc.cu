@@ -12,7 +12,7 @@
 //   warps 0 - 7   softmax        warp 9   issuer
 //   bf16 cache    warps 8, 10 ask for K by TMA, warp 11 for V; it also looks through V where not every row sees the whole tile
 //   e4m3 cache    K is an operand as it is, with queries in two e4m3 pieces; V travels as f16: warp 8 asks for both, warps 10 - 15 widen V
-//   4-bit cache   warps 10 - 15 widen K and V (kv4.cuh) to f16, which warp 8 asks for tile by tile; queries are f16
+//   4-bit cache   warps 10 - 15 widen K and V (kv4.cuh) to f16, which warp 8 asks for tile by tile, in a unit of the tile or of each row; queries are f16
 //
 // What bounds it (times from captured graphs): two tiles of 128 x 128 scores take the softmax groups some 3200 clocks, the tensor pipe 2048 at heads of 128; and a CTA's way in (lengths,
 // table, queries, keys, first products: 9000 clocks) and out (4000), which nothing on its SM runs under. 2 x 2048 rows behind 4096 tokens without a window, 32
@@ -52,7 +52,13 @@ constexpr int kRawTokens = 64;             // of a piece of an e4m3 tile
 constexpr int kKv4Slots = 3;               // of tiles of 4-bit rows
 constexpr int kKv4Team = 3;                // warps that widen K, and V
 constexpr int kKv4Top = -6;                // their largest magnitude is below 2 to this as f16 (kv4_widen_f16)
+// A tile of 4-bit rows is widened in one unit (a power of two) where the largest magnitude of every row is 2^-13 or more in it: its values are then off by 2^-11
+// of that at most. In other tiles each row is lifted by a power of two of its own, which its scores, in fp32, or its weights give back: a row keeps its bits
+// beside rows of any size, be they seen or not. (Weights are below 2^15 and fall by the lift before they go to the product: 2^-25 of a unit in which the largest
+// is 2^6 or more, so an output loses 2^-28 of the largest value so far for a token at most.)
+constexpr int kKv4Even = 127 - 13, kKv4MostLift = 20;
 constexpr int kTcFlags = 400;              // bytes of barriers and flags
+constexpr int kAtVReady = 12, kAtPHalf = 16, kAtFlags = 38;      // of the barriers, in that order: 2, 2, and what follows them
 
 // Shared memory: two tiles of Q, two stages of K and of V, 16-bit values in rows of 128 bytes. e4m3: Q in two e4m3 pieces, four stages of K as it
 // is, V in 16 bits behind four slots of raw halves of tiles (eight where there is one tile of Q). 4 bits: three slots of raw tiles of K or V.
@@ -62,7 +68,8 @@ struct TcSmem {
   static constexpr int kStages = KV == kE4m3 ? 4 : 2, kK = KV == kE4m3 ? kTile * D : kT;      // of K
   static constexpr int kRaw = KV == kE4m3 ? kRawTokens * D : KV == kKv4 ? kTile * kKv4Row<D> : 0;
   static constexpr int kTiles = 6 * kT + (KV == kKv4 ? kKv4Slots : 4) * kRaw;
-  static constexpr int kTotal = kTiles + kTcFlags + kTcRows * 4 + 1024;
+  static constexpr int kLifts = KV == kKv4 ? 2 * 4 * kTile : 0;      // of the rows of K, then of V, by tile
+  static constexpr int kTotal = kTiles + kTcFlags + kTcRows * 4 + kLifts + 1024;
 };
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -149,8 +156,95 @@ __device__ __noinline__ void cap_scores(uint32_t t_s, float cap_in) {
   tmem_st_wait();
 }
 
+__device__ __forceinline__ int4 lds_int4(const volatile int* at) {
+  int4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem_u32(const_cast<const int*>(at))) : "memory");
+  return v;
+}
+// Exponent field of a 4-bit row's largest magnitude, and how far the row is lifted beside a tile's unit of 2^up.
+__device__ __forceinline__ int kv4_top_field(const Kv4Scale& k) {
+  return (int)(__float_as_uint(fmaxf(fabsf(k.low), fabsf(fmaf(15.f, k.step, k.low)))) >> 23);
+}
+__device__ __forceinline__ int kv4_lift(int field, int up) { return min(max(126 + kKv4Top - field - up, 0), kKv4MostLift); }
+__device__ __forceinline__ float kv4_lowered(uint32_t lifts, int byte) { return pow2_of(-(int)(lifts >> 8 * byte & 0xFF)); }
+
+// A tile of rows that are lifted, widened (kv4_widen_f16) by kKv4Team warps, `at` of their lanes this one. Values that nobody sees, of places outside [beg, end) and
+// behind `first`, are 0, and rows of values that read as NaN where `odd_met` is to know of them.
+template <int D>
+__device__ __noinline__ void widen_lifted(const uint8_t* src, uint8_t* to, int up, int at, int line_of_page, int line_of_half, bool is_v, int beg, int end, int first,
+                                          int* odd_met, uint8_t* lifts) {
+  constexpr int kWords = D / 8;
+#pragma unroll 1
+  for (int i = at; i < kTile * kWords; i += 32 * kKv4Team) {
+    const int tok = i / kWords, c = i % kWords;
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(src + tok * kKv4Row<D> + c * 4);
+    const Kv4Scale k = kv4_scale_of(*reinterpret_cast<const uint32_t*>(src + tok * kKv4Row<D> + D / 2));
+    const bool there = tok < end && (tok >= beg || tok < first), nan = !(fabsf(k.step) < INFINITY);
+    const int lift = kv4_lift(kv4_top_field(k), up);
+    if (c == 0) lifts[tok] = (uint8_t)lift;
+    uint32_t even = 0, odd = 0, low2 = 0;
+    if (!is_v || (there && !(odd_met && nan))) {
+      const int to_unit = up + lift;
+      const float f1 = pow2_of(to_unit >> 1), f2 = pow2_of(to_unit - (to_unit >> 1)), step = k.step * f1 * f2, low = k.low * f1 * f2;
+      even = pack_16<true>(step * 16777216.f, step * 16777216.f);
+      odd = pack_16<true>(step * 1048576.f, step * 1048576.f);
+      low2 = pack_16<true>(low, low);
+    }
+    if (is_v && odd_met && there && nan) *reinterpret_cast<volatile int*>(odd_met) = 1;
+    *reinterpret_cast<uint4*>(to + (tok >> 4) * line_of_page + (tok & 15) * 128 + (c >> 3) * line_of_half + (((c & 7) ^ (tok & 7)) << 4)) =
+        kv4_widen_f16(codes, even, odd, low2);
+  }
+}
+
+// Scores of a tile whose keys were lifted (`lifts`), or under a soft-cap (`cap_in`), in place.
+__device__ __noinline__ void change_scores(uint32_t t_s, const uint8_t* lifts, float cap_in) {
+#pragma unroll 1
+  for (int c = 0; c < 8; ++c) {
+    uint32_t s[16];
+    tmem_ld_32x16(t_s + 16 * c, s);
+    tmem_ld_wait();
+    if (lifts) {
+      const uint4 w = *reinterpret_cast<const uint4*>(lifts + 16 * c);
+      const uint32_t of[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * kv4_lowered(of[i >> 2], i & 3));
+    }
+    if (cap_in > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = __float_as_uint(tanhf(__uint_as_float(s[i]) * cap_in));
+    }
+    tmem_st_32x16(t_s + 16 * c, s);
+  }
+  tmem_st_wait();
+}
+// Weights of a tile whose values were lifted, in place (two to a word), and handed over, when the values are there, which write down by how much.
+template <int D>
+__device__ __noinline__ void lower_weights(uint32_t t_p, uint8_t* smem, int t, int group) {
+  using S = TcSmem<D, kKv4>;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kTiles);
+  mbar_wait(bars + kAtVReady + (t & 1), (t >> 1) & 1, reinterpret_cast<volatile int*>(bars + kAtFlags) + 1);
+  const uint8_t* lifts = smem + S::kTiles + kTcFlags + kTcRows * 4 + (4 + (t & 3)) * kTile;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t w[16];
+    tmem_ld_32x16(t_p + 16 * c, w);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t of = *reinterpret_cast<const uint16_t*>(lifts + 32 * c + 2 * i);
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      w[i] = pack_16<true>(x.x * kv4_lowered(of, 0), x.y * kv4_lowered(of, 1));
+    }
+    tmem_st_32x16(t_p + 16 * c, w);
+  }
+  tmem_st_wait();
+  tc_fence_before_sync();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bars + kAtPHalf + group);
+}
+
 // A row's softmax over one tile of 128 tokens: scores in registers, weights as 16-bit values over the scores' first columns, the first 64 of them
-// handed over before the others are computed; O of the warp is rescaled when a row's maximum has moved by more than 2^8, or its unit by `shrink`. Scores that the row
+// handed over (p_half) before the others are computed; O of the warp is rescaled when a row's maximum has moved by more than 2^8, or its unit by `shrink`. Scores that the row
 // does not see become -inf first, 32 columns at a time where some row of the warp does not see them all.
 template <int D, bool F16>
 __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, bool whole, const uint4& visible, float scale, bool have_o, uint64_t* p_half,
@@ -443,17 +537,20 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kTiles);
   constexpr int KS = S::kStages;
   uint64_t *k_full = bars, *k_empty = bars + 4;                                               // [KS] by stage
-  uint64_t *v_full = bars + 8, *v_empty = bars + 10, *v_ready = bars + 12;                    // [2] by stage; ready: looked through, or widened
-  uint64_t *s_full = bars + 14, *p_half = bars + 16, *p_ready = bars + 18;                    // [2] by softmax group
+  uint64_t *v_full = bars + 8, *v_empty = bars + 10, *v_ready = bars + kAtVReady;                    // [2] by stage; ready: looked through, or widened
+  uint64_t *s_full = bars + 14, *p_half = bars + kAtPHalf, *p_ready = bars + 18;                    // [2] by softmax group
   uint64_t *o_done = bars + 20, *q_full = bars + 21;
   uint64_t *raw_full = bars + 22, *raw_empty = bars + 30;                                     // [8] by slot
-  uint64_t* v_unit = raw_full + 4;         // [2] by stage of V: a 4-bit cache has three raw slots, and units that softmax has to know
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
+  // A 4-bit cache has three raw slots, and units that softmax has to know, by stage of V [2]; and a barrier that nobody waits for
+  uint64_t *v_unit = raw_full + 4, *nobody = raw_full + 7;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kAtFlags);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* odd_met = reinterpret_cast<int*>(tmem_slot + 2);     // values were taken out of tiles of V
-  volatile int *k_up = odd_met + 1, *v_up = k_up + 4;       // [4] by tile: keys and values of a 4-bit cache are times 2 to this
+  // [4] by tile of a 4-bit cache: keys and values are times 2 to x and y, rows are lifted where z and w are not 0
+  volatile int* units = reinterpret_cast<volatile int*>(bars + 40);
   float* factors = reinterpret_cast<float*>(smem + S::kTiles + kTcFlags);
-  static_assert(38 * 8 + 11 * 4 <= kTcFlags && kTcFlags % 16 == 0, "barriers and flags");
+  uint8_t *k_lifts = smem + S::kTiles + kTcFlags + kTcRows * 4, *v_lifts = k_lifts + 4 * kTile;      // [4][kTile]
+  static_assert(40 * 8 + 16 * 4 <= kTcFlags && kTcFlags % 16 == 0, "barriers and flags");
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -528,9 +625,9 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
                            (int)(p.num_blocks * p.hkv * p.block_pages * kPage)};
 
   // The block was launched with 168 registers a thread (e4m3 and 4 bits: 128): 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128,
-  // or 256 x 184 + 256 x 72 (4 bits: 490 us where 64 for those that widen took 534, 2 x 2048 rows behind 2500 and 6143 tokens).
+  // or 256 x 176 + 256 x 80 (4 bits, 2 x 2048 rows behind 2500 and 6143 tokens: 512 us; with 64, 72 and 88 for those that widen 576, 534 and 526).
   if (warp >= 8) {
-    if constexpr (KV4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (KV4) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     else if constexpr (KV8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     bool bad = false;
@@ -660,27 +757,33 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         const uint8_t* src = smem + 6 * TB + slot * S::kRaw;
         auto seen = [&](int tok) { return tok < any_end && (tok >= any_beg || tok < p.first); };
         // The largest magnitude of the tile that some row sees, by every warp for itself, a lane to four rows. It goes below 2^kKv4Top; that of values, whose
-        // sums go over all tiles, only where it is above that of those before, with room for four times as much.
-        uint32_t most = 0;
+        // sums go over all tiles, only where it is above that of those before, with room for four times as much. (By warp 8 for all of them, in turn with its
+        // copies: 670 us for the 2 x 2048 rows.)
+        uint32_t ends = 0;                             // the largest field, and 255 less the least (rows of zeros, and of values that are no numbers, aside)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const Kv4Scale k = kv4_scale_of(*reinterpret_cast<const uint32_t*>(src + (32 * i + lane) * kKv4Row<D> + D / 2));
-          const uint32_t field = __float_as_uint(fmaxf(fabsf(k.low), fabsf(fmaf(15.f, k.step, k.low)))) >> 23;
-          if ((!look || seen(tile0 + 32 * i + lane)) && field < 255) most = max(most, field);
+          const uint32_t field = kv4_top_field(kv4_scale_of(*reinterpret_cast<const uint32_t*>(src + (32 * i + lane) * kKv4Row<D> + D / 2)));
+          if ((!look || seen(tile0 + 32 * i + lane)) && field - 1 < 254) ends = __vmaxu2(ends, 0x00FF0000u - 0xFFFFu * field);
         }
-        most = __reduce_max_sync(0xffffffffu, most);
+        const uint32_t most = __reduce_max_sync(0xffffffffu, ends & 0xFFFFu);
         int up = 126 + kKv4Top - (int)most;
         if (is_v) up = up_v = up < up_v ? up - 2 : up_v;
         up = min(up, 120);
+        const bool lifted = __any_sync(0xffffffffu, 255 - (int)(ends >> 16) + up < kKv4Even);
         const float f1 = pow2_of(up >> 1), f2 = pow2_of(up - (up >> 1));
         if (it >= 2 && !mbar_wait_warp(is_v ? &v_empty[b] : &k_empty[b], ((it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
         if (part == 0 && lane == 0) {
-          (is_v ? v_up : k_up)[it & 3] = up;
+          units[4 * (it & 3) + is_v] = up;
+          units[4 * (it & 3) + 2 + is_v] = lifted;
           if (is_v) mbar_arrive(&v_unit[b]);
         }
         uint8_t* const to = is_v ? sv + b * TB : sk + b * TB;
         // of row tok: V: [page][half][16][64]
         const int line_of_page = is_v ? (D / 64) * 2048 : 16 * 128, line_of_half = is_v ? 2048 : kHalf;
+        if (lifted) {
+          widen_lifted<D>(src, to, up, part * 32 + lane, line_of_page, line_of_half, is_v, look ? any_beg - tile0 : 0, look ? any_end - tile0 : kTile, p.first - tile0,
+                          look ? odd_met : nullptr, (is_v ? v_lifts : k_lifts) + (it & 3) * kTile);
+        } else
 #pragma unroll
         for (int u0 = 0; u0 < kMost; u0 += kBatch) {
           uint32_t even = 0, odd = 0, low2 = 0;        // of a row of values that reads as NaN, or that nobody sees: 0
@@ -878,7 +981,7 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     }
     if (bad && p.status) atomicCAS(p.status, FLLM_OK, FLLM_ERR_BAD_ARGS);
   } else {
-    if constexpr (KV4) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    if constexpr (KV4) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     else if constexpr (KV8) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
@@ -905,10 +1008,12 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       if (!mbar_wait(&s_full[group], k & 1, abort_flag)) { ok = false; break; }
       tc_fence_after_sync();
       float shrink = 1.f;
+      const int t = n >> shift;
+      int4 unit = make_int4(0, 0, 0, 0);
       if constexpr (KV4) {
-        const int t = n >> shift;
         if (!mbar_wait(&v_unit[t & 1], (t >> 1) & 1, abort_flag)) { ok = false; break; }
-        const int up = k_up[t & 3], now = v_up[t & 3];
+        unit = lds_int4(units + 4 * (t & 3));
+        const int up = unit.x, now = unit.y;
         // Not 0, nor infinite, as factors of rows are not (span_factor): a score of 0 in an unseen place beside one, or a 0 beside the other, would be a NaN.
         factor = fminf(fmaxf(row_factor * pow2_of(-(up >> 1)) * pow2_of((up >> 1) - up), FLT_MIN), FLT_MAX);
         if (p.softcap <= 0.f) scale = factor;
@@ -918,8 +1023,16 @@ span_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       const bool whole = tok0 + kTile <= w_base && (tok0 >= w_beg || tok0 + kTile <= p.first);
       uint4 vis = make_uint4(0, 0, 0, 0);
       if (!whole) vis = row_bits(p, q0, qn, kv_len, gap, qi, tok0);
-      if (p.softcap > 0.f) cap_scores(t_s, fminf(factor / (p.softcap * kLog2e), FLT_MAX));
-      softmax_tile<D, KV != kBf16>(t_s, t_o, whole, vis, scale, k > 0, &p_half[group], m_used, l, shrink);
+      if constexpr (KV4) {
+        if (unit.z || p.softcap > 0.f)
+          change_scores(t_s, unit.z ? k_lifts + (t & 3) * kTile : nullptr, p.softcap > 0.f ? fminf(factor / (p.softcap * kLog2e), FLT_MAX) : 0.f);
+      } else {
+        if (p.softcap > 0.f) cap_scores(t_s, factor / (p.softcap * kLog2e));
+      }
+      softmax_tile<D, KV != kBf16>(t_s, t_o, whole, vis, scale, k > 0, unit.w ? nobody : &p_half[group], m_used, l, shrink);
+      if constexpr (KV4) {
+        if (unit.w) lower_weights<D>(t_s, smem, t, group);
+      }
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[group]);

@@ -101,3 +101,67 @@ def test_scores_of_zero(ops, D, rows, ctx, kind, sink):
     s = torch.linspace(-3, 3, HQ, device="cuda") if sink else None
     so.check(_attend(ops, c, s), *_want(c, sinks=s))
     assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,ctx", SHAPES)
+@pytest.mark.parametrize("kind,cap", [("values", 0.0), ("keys", 0.0), ("both", 0.0), ("both", 30.0), ("first", 0.0), ("growing", 0.0), ("shrinking", 0.0), ("ratio", 0.0)])
+def test_tokens_of_different_sizes(ops, D, rows, ctx, kind, cap):
+    """A few very large tokens without weight, before and behind other rows' ends; values that grow or shrink from tile to tile; sizes that change from token to
+    token: every token keeps its bits."""
+    g = torch.Generator(device="cuda").manual_seed(D + rows)
+    n = rows + ctx
+    tok = torch.arange(n, device="cuda")
+    q = 1.5 * torch.randn(rows, HQ, D, generator=g, device="cuda") + 1.0
+    k_exp, v_exp = torch.full((n,), -1.0, device="cuda"), torch.full((n,), -2.0, device="cuda")
+    large = (tok == 3) if kind == "first" else (tok % 150 == 77) | (tok == ctx + rows // 2)
+    ignored = None
+    low = torch.full((n,), float("nan"), device="cuda")
+    if kind in ("values", "keys", "both", "first"):
+        ignored = large
+        low[large] = -2.0 ** 17 if kind in ("keys", "both") else -8.0
+        if kind != "keys":
+            v_exp[large] = 12.0
+    elif kind == "ratio":
+        k_exp -= torch.randint(0, 10, (n,), generator=g, device="cuda") * 2
+        v_exp -= torch.randint(0, 12, (n,), generator=g, device="cuda") * 2
+    else:
+        v_exp += (tok // 128 if kind == "growing" else -(tok // 128)) * (3.0 if n < 2000 else 0.5) // 1
+    c = _case(rows, ctx, D, _rows(g, n, D, k_exp, low), _rows(g, n, D, v_exp), q)
+    so.check(_attend(ops, c, cap=cap), *_want(c, ignored, cap=cap))
+    assert ops.check_status() == 0
+
+
+def test_a_tree_with_large_nodes(ops):
+    """Nodes of large values that their descendants do not weigh, beside branches that do not see them."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    nodes, ctx, D, hq = 200, 313, 128, 32
+    n = nodes + ctx
+    large = torch.zeros(n, dtype=torch.bool, device="cuda")
+    large[[40, ctx + 20, ctx + 77]] = True
+    low = torch.where(large, -2.0 ** 17, float("nan"))
+    q = 1.5 * torch.randn(nodes, hq, D, generator=g, device="cuda") + 1.0
+    c = _case(nodes, ctx, D, _rows(g, n, D, -1, low), _rows(g, n, D, torch.where(large, 12.0, -2.0)), q, hq, so.grow(nodes, 3))
+    so.check(_attend(ops, c), *_want(c, large))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("rows,ctx", SHAPES)
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("sizes", [False, True])
+def test_a_row_that_is_not_finite(ops, rows, ctx, which, sizes):
+    """NaN in the rows that see it and nowhere else, with other tokens of the tile of other sizes or not."""
+    D = 128
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    n, bad = rows + ctx, ctx + rows // 3
+    exp = -2.0 - (torch.randint(0, 6, (n,), generator=g, device="cuda") * 4 if sizes else torch.zeros(n, device="cuda"))
+    k, v = _rows(g, n, D, exp), _rows(g, n, D, exp)
+    c = _case(rows, ctx, D, k, v)
+    row = (k if which == "k" else v)[bad:bad + 1].clone()
+    row[..., D // 2:D // 2 + 2] = torch.tensor([float("nan")], device="cuda").bfloat16().view(torch.uint8)
+    getattr(c, which)[int(c.tables[0, bad // 16]), :, bad % 16] = row[0]
+    y = _attend(ops, c)
+    sees = torch.arange(rows, device="cuda") >= bad - ctx
+    assert torch.isnan(y[sees]).all()
+    o, bound = _want(c)
+    so.check(y[~sees], o[~sees], bound[~sees])
