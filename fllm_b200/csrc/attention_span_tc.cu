@@ -55,7 +55,8 @@ constexpr int kKv4Top = -6;                // their largest magnitude is below 2
 // A tile of 4-bit rows is widened in one unit (a power of two) where the largest magnitude of every row is 2^-13 or more in it: its values are then off by 2^-11
 // of that at most. In other tiles each row is lifted by a power of two of its own, which its scores, in fp32, or its weights give back: a row keeps its bits
 // beside rows of any size, be they seen or not. (Weights are below 2^15 and fall by the lift before they go to the product: 2^-25 of a unit in which the largest
-// is 2^6 or more, so an output loses 2^-28 of the largest value so far for a token at most.)
+// is 2^6 or more, so an output loses 2^-28 of the largest value so far for a token at most.) A text whose tiles are all such takes longer: 2 x 2048 rows behind
+// 2500 and 6143 tokens 1030 us, 800 with only its keys so (513 with neither).
 constexpr int kKv4Even = 127 - 13, kKv4MostLift = 20;
 constexpr int kTcFlags = 400;              // bytes of barriers and flags
 constexpr int kAtVReady = 12, kAtPHalf = 16, kAtFlags = 38;      // of the barriers, in that order: 2, 2, and what follows them
@@ -173,15 +174,18 @@ __device__ __forceinline__ float kv4_lowered(uint32_t lifts, int byte) { return 
 template <int D>
 __device__ __noinline__ void widen_lifted(const uint8_t* src, uint8_t* to, int up, int at, int line_of_page, int line_of_half, bool is_v, int beg, int end, int first,
                                           int* odd_met, uint8_t* lifts) {
-  constexpr int kWords = D / 8;
+  constexpr int kEach = 4, kPieces = D / 8 / kEach;      // words of a row that a lane takes
 #pragma unroll 1
-  for (int i = at; i < kTile * kWords; i += 32 * kKv4Team) {
-    const int tok = i / kWords, c = i % kWords;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(src + tok * kKv4Row<D> + c * 4);
-    const Kv4Scale k = kv4_scale_of(*reinterpret_cast<const uint32_t*>(src + tok * kKv4Row<D> + D / 2));
+  for (int i = at; i < kTile * kPieces; i += 32 * kKv4Team) {
+    const int tok = i / kPieces, c0 = i % kPieces * kEach;
+    const uint8_t* row = src + tok * kKv4Row<D>;
+    uint32_t codes[kEach];
+#pragma unroll
+    for (int w = 0; w < kEach; ++w) codes[w] = *reinterpret_cast<const uint32_t*>(row + (c0 + w) * 4);
+    const Kv4Scale k = kv4_scale_of(*reinterpret_cast<const uint32_t*>(row + D / 2));
     const bool there = tok < end && (tok >= beg || tok < first), nan = !(fabsf(k.step) < INFINITY);
     const int lift = kv4_lift(kv4_top_field(k), up);
-    if (c == 0) lifts[tok] = (uint8_t)lift;
+    if (c0 == 0) lifts[tok] = (uint8_t)lift;
     uint32_t even = 0, odd = 0, low2 = 0;
     if (!is_v || (there && !(odd_met && nan))) {
       const int to_unit = up + lift;
@@ -191,8 +195,12 @@ __device__ __noinline__ void widen_lifted(const uint8_t* src, uint8_t* to, int u
       low2 = pack_16<true>(low, low);
     }
     if (is_v && odd_met && there && nan) *reinterpret_cast<volatile int*>(odd_met) = 1;
-    *reinterpret_cast<uint4*>(to + (tok >> 4) * line_of_page + (tok & 15) * 128 + (c >> 3) * line_of_half + (((c & 7) ^ (tok & 7)) << 4)) =
-        kv4_widen_f16(codes, even, odd, low2);
+    uint8_t* line = to + (tok >> 4) * line_of_page + (tok & 15) * 128;
+#pragma unroll
+    for (int w = 0; w < kEach; ++w) {
+      const int c = c0 + w;
+      *reinterpret_cast<uint4*>(line + (c >> 3) * line_of_half + (((c & 7) ^ (tok & 7)) << 4)) = kv4_widen_f16(codes[w], even, odd, low2);
+    }
   }
 }
 
