@@ -16,6 +16,7 @@ import torch
 from .kv4 import cache_values
 
 BOUNDS_TAIL = 16
+MOST_BLOCKS = 48 * 1024        # of a text that the kernel chooses from
 NOT_FINITE = 127
 
 

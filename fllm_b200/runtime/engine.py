@@ -28,6 +28,7 @@ from ..config import EngineConfig, ModelConfig, ParallelConfig
 from ..models.decoder import Decoder, KVCache, StepBatch
 from ..models.weights import DecoderWeights, init_random_weights, make_shard_spec
 from ..ops import get_ops
+from ..ops.blocks import MOST_BLOCKS
 from ..ops.kv4 import kv4_width
 from .block_manager import BlockManager
 from .request import Request, RequestStatus, SamplingParams, TokenEvent
@@ -225,6 +226,8 @@ class LLMEngine:
                 raise ValueError(f"{what} needs blocks of a multiple of 16 tokens and a model in bf16")
         if c.sparse_blocks and (c.sparse_tail < 1 or c.sparse_lead < 0 or c.sparse_blocks < c.sparse_lead + c.sparse_tail):
             raise ValueError("sparse_blocks must have room for the first and the last blocks, one of the last at least")
+        if c.sparse_blocks and native and max(c.sparse_blocks, -(-c.max_model_len // c.block_size)) > MOST_BLOCKS:
+            raise ValueError(f"attention over selected blocks has texts of at most {MOST_BLOCKS} blocks: max_model_len is too large for this block_size")
 
     # ------------------------------------------------------------------ sizing
     def _state_rows(self) -> int:

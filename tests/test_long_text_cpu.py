@@ -262,3 +262,19 @@ def test_the_tiers_bring_blocks_back_without_more_where_no_bounds_are_kept(monke
                 eng.generate([x], sp)
         assert eng.blocks.stats["tier_restored"] > 0
         assert len(looked) == (eng.blocks.stats["tier_restored"] if sparse else 0)
+
+
+def test_texts_of_too_many_blocks_are_refused_before_any_step():
+    """The kernel that chooses blocks holds the scores of MOST_BLOCKS of them; the PyTorch operators have no such limit."""
+    from types import SimpleNamespace
+
+    from fllm_b200.ops.blocks import MOST_BLOCKS
+    cfg = preset("qwen3-tiny")
+    check = lambda ops, **kw: LLMEngine._check_cache_kind(SimpleNamespace(cfg=EngineConfig(sparse_blocks=8, **kw), model_cfg=cfg, ops=ops))
+    native, plain = SimpleNamespace(k=None), SimpleNamespace()
+    check(native, max_model_len=16 * MOST_BLOCKS)
+    check(native, max_model_len=32 * MOST_BLOCKS, block_size=32)
+    check(plain, max_model_len=16 * MOST_BLOCKS + 1)
+    for bad in (dict(max_model_len=16 * MOST_BLOCKS + 1), dict(max_model_len=64 * MOST_BLOCKS, block_size=32)):
+        with pytest.raises(ValueError, match="blocks"):
+            check(native, **bad)
