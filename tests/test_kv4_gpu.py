@@ -373,3 +373,36 @@ def test_queries_of_the_largest_size_beside_keys_of_zero(ops, D, hq):
     o, bound = so.want(c, D ** -0.5, 0, 0)
     so.check(_attend(ops, c), o, bound + ko.slack(c))
     assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T", [3, 400])
+def test_codes_beside_ties(ops, D, T):
+    """Values at the middle between two codes, and one bf16 number next to it: rows written with a rotation by nothing, and without one, are the statement's."""
+    g = torch.Generator(device="cuda").manual_seed(D + T)
+    hq, hkv = 4, 2
+    n = T * hkv
+    size = torch.exp2(torch.randint(-120, 110, (n, 1), generator=g, device="cuda").float())
+    lo = (size * torch.randn(n, 1, generator=g, device="cuda")).bfloat16().float()
+    hi = (lo + size * (0.01 + torch.rand(n, 1, generator=g, device="cuda"))).bfloat16().float()
+    ends = torch.cat([lo, hi, lo.expand(n, D - 2)], 1)
+    step = kv4_encode(ends)[:, D // 2:D // 2 + 2].contiguous().view(torch.bfloat16).float()
+    x = (lo + step * (torch.randint(0, 15, (n, D), generator=g, device="cuda") + 0.5)).bfloat16()
+    x = (x.view(torch.int16) + torch.randint(-1, 2, (n, D), generator=g, device="cuda").to(torch.int16)).view(torch.bfloat16)
+    x = torch.minimum(torch.maximum(torch.nan_to_num(x.float()), lo), hi)
+    x[:, :2] = ends[:, :2]
+    x = x.bfloat16()
+    rows = kv4_encode(x).view(T, hkv, -1)
+    blocks = T // 16 + 2
+    slots = torch.randperm(blocks * 16, generator=g, device="cuda")[:T].int()
+    flat = x.view(T, hkv * D)
+    inv = 10000.0 ** (-torch.arange(0, D, 2, device="cuda").float() / D)
+    for how in ("rows", "rotated"):
+        kc, vc = _caches(blocks, hkv, 16, D)
+        if how == "rows":
+            ops.kv4_write(flat, flat, slots, kc, vc)
+        else:
+            qkv = torch.cat([torch.zeros(T, hq * D, device="cuda").bfloat16(), flat, flat], 1)
+            ops.rope_kv_write(qkv, torch.zeros(T, dtype=torch.int32, device="cuda"), slots, inv, None, None, kc, vc, hq, hkv, D, D, 0, 1e-6)
+        at = slots.long()
+        assert torch.equal(kc[at // 16, :, at % 16], rows) and torch.equal(vc[at // 16, :, at % 16], rows), how
