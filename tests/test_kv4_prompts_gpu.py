@@ -34,7 +34,7 @@ def _rows(g, n, D, exp, low=None):
     return torch.cat([codes, tail], -1)
 
 
-def _case(rows, ctx, D, k, v, q=None, hq=HQ, trees=None):
+def _case(rows, ctx, D, k, v, q=None, hq=HQ, trees=None, span=None):
     """A sequence whose tokens' rows are k and v."""
     c = so.setup([rows], [ctx], hq, HKV, D, seed=rows + D, words=4 if trees else 0, trees=trees and [trees])
     tok = torch.arange(rows + ctx, device="cuda")
@@ -45,16 +45,16 @@ def _case(rows, ctx, D, k, v, q=None, hq=HQ, trees=None):
     c.keys, c.values = [kv4_decode(k)], [kv4_decode(v)]
     if q is not None:
         c.q = q.bfloat16().view(rows, hq * D)
-    tiles = -(-rows * (hq // HKV) // 16) * HKV * -(-(rows + ctx) // 16)
+    tiles = -(-rows * (hq // HKV) // 16) * HKV * -(-(span or rows + ctx) // 16)
     assert tiles > 28 * torch.cuda.get_device_properties(0).multi_processor_count, "too little for the tensor-memory kernel"
     return c
 
 
-def _want(c, ignored=None, sinks=None, cap=0.0):
+def _want(c, ignored=None, sinks=None, cap=0.0, window=0, first=0):
     """(outputs, bounds); `ignored`: tokens whose weights are nothing beside the others (below e^-30 2^20 of them)."""
     n, N, D, scale = c.rows[0], c.lens[0], c.D, c.D ** -0.5
     q, k, v = c.q.view(n, c.hq, D), c.keys[0], c.values[0]
-    seen = so.seen_rows(c.ctx[0], n, 0, 0, c.trees[0] if c.trees else None).cuda()
+    seen = so.seen_rows(c.ctx[0], n, window, first, c.trees[0] if c.trees else None).cuda()
     size = v.double().abs().amax((1, 2))
     last = (c.ctx[0] + torch.arange(n, device="cuda") + 256).clamp(max=N - 1) if c.trees is None else torch.full((n,), N - 1, device="cuda")
     most = size.cummax(0)[0][last]
@@ -68,10 +68,10 @@ def _want(c, ignored=None, sinks=None, cap=0.0):
     return o.reshape(n, -1), (bound + extra[..., None] + 1e-7).reshape(n, -1)
 
 
-def _attend(ops, c, sinks=None, cap=0.0):
+def _attend(ops, c, sinks=None, cap=0.0, window=0, first=0):
     if c.trees:
-        return ops.attention_tree(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.masks, c.base, c.hq, HKV, c.D, c.D ** -0.5, 0, sinks, cap, meta=c.meta)
-    return ops.attention(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.hq, HKV, c.D, c.D ** -0.5, 0, sinks, cap, meta=c.meta)
+        return ops.attention_tree(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.masks, c.base, c.hq, HKV, c.D, c.D ** -0.5, window, sinks, cap, meta=c.meta, first=first)
+    return ops.attention(c.q, c.k, c.v, c.tables, c.row_seq, c.positions, c.hq, HKV, c.D, c.D ** -0.5, window, sinks, cap, meta=c.meta, first=first)
 
 
 @pytest.mark.parametrize("D", [64, 128])
@@ -129,6 +129,24 @@ def test_tokens_of_different_sizes(ops, D, rows, ctx, kind, cap):
         v_exp += (tok // 128 if kind == "growing" else -(tok // 128)) * (3.0 if n < 2000 else 0.5) // 1
     c = _case(rows, ctx, D, _rows(g, n, D, k_exp, low), _rows(g, n, D, v_exp), q)
     so.check(_attend(ops, c, cap=cap), *_want(c, ignored, cap=cap))
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,first", [(300, 20), (200, 130), (77, 1)])
+def test_windows_with_first_tokens_of_other_sizes(ops, D, window, first):
+    """First tokens and tokens of the window that are much larger, or much smaller, than the others of their tile."""
+    g = torch.Generator(device="cuda").manual_seed(D + window)
+    rows, ctx = 1500, 611
+    n = rows + ctx
+    tok = torch.arange(n, device="cuda")
+    large = (tok == 0) | (tok % 190 == 100)
+    low = torch.where(large, -2.0 ** 15, float("nan"))
+    k = _rows(g, n, D, torch.where(tok % 7 == 3, -9.0, -1.0), low)
+    v = _rows(g, n, D, torch.where(large, 12.0, torch.where(tok % 5 == 1, -13.0, -2.0)))
+    q = 1.5 * torch.randn(rows, 64, D, generator=g, device="cuda") + 1.0
+    c = _case(rows, ctx, D, k, v, q, 64, span=min(rows + ctx, window + first + rows))
+    so.check(_attend(ops, c, window=window, first=first), *_want(c, large, window=window, first=first))
     assert ops.check_status() == 0
 
 
