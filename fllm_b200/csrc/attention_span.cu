@@ -633,7 +633,8 @@ SpanPlan attention_span_plan(const SpanParams& p) {
     rows.rows_to = tc ? kSpanRows : INT_MAX;
     const long long ctas = span_rows_ctas(rows);
     const long long pages = (span + kPage - 1) / kPage;
-    // As many splits as leave all CTAs on the SMs at once, a page for each of a CTA's warps at least: a CTA's way in and out is some 5 us (64 sequences
+    // As many splits as leave all CTAs on the SMs at once, four pages at least, one for each of a CTA's warps (over a 4-bit cache a warp takes up to four at a
+    // time: in pieces of fewer than 16 some warps have none): a CTA's way in and out is some 5 us (64 sequences
     // under a window of 4096, 8 key heads of 128: 170 us whole, 182 in two, 202 in four; 16 under one of 1024: 24, 17, 24). Up to eight are a
     // cluster and join in it; more, where few sequences are long, leave their rows to a kernel behind.
     const int resident = p.kv4 ? attention_kv4_resident(rows) : p.head_dim == 256 ? 1 : p.head_dim == 64 ? rows_resident<64, false>() : p.kv_fp8 ? rows_resident<128, true>() : rows_resident<128, false>();

@@ -19,8 +19,9 @@
 // query and 8 key heads of 128: 1097 TFLOP/s, e4m3 1007; under a window of 1024 with 64 first tokens 735, of the products that the window leaves. (CTAs
 // that stay and take item after item hid the way in, but missed the instruction cache 7000 times an SM for 2800: 146 us for 115 at that
 // window then; 126 for 197 with 16 trees of equal lengths.) Over a 4-bit cache 2 x 2048 rows behind 2500 and 6143 tokens take
-// 477 us, 752 TFLOP/s (bf16 323, e4m3 395): widening a tile of K and one of V takes three warps each about as long as the groups' softmax, and they share its
-// SM's issue slots.
+// 515 us, 697 TFLOP/s (bf16 327, e4m3 395): widening a tile of K and one of V takes three warps each about as long as the groups' softmax, they share its
+// SM's issue slots, and every one of the 32 CTAs of a key head widens the same tiles. (471 us without rows of their own units, whose code, not taken there,
+// costs a third more misses of the instruction cache, and a look at the smallest row in front of each tile.)
 //
 // What a row sees of a tile is four words of bits, from its bounds and its mask; tiles that all rows of a warp see whole have code
 // without them. Values of places that some row does not see may be infinite or NaN: they are taken out of the tile there, and rows that
@@ -56,7 +57,7 @@ constexpr int kKv4Top = -6;                // their largest magnitude is below 2
 // of that at most. In other tiles each row is lifted by a power of two of its own, which its scores, in fp32, or its weights give back: a row keeps its bits
 // beside rows of any size, be they seen or not. (Weights are below 2^15 and fall by the lift before they go to the product: 2^-25 of a unit in which the largest
 // is 2^6 or more, so an output loses 2^-28 of the largest value so far for a token at most.) A text whose tiles are all such takes longer: 2 x 2048 rows behind
-// 2500 and 6143 tokens 1030 us, 800 with only its keys so (513 with neither).
+// 2500 and 6143 tokens 1026 us, 795 with only its keys so, 827 with its values (515 with neither).
 constexpr int kKv4Even = 127 - 13, kKv4MostLift = 20;
 constexpr int kTcFlags = 400;              // bytes of barriers and flags
 constexpr int kAtVReady = 12, kAtPHalf = 16, kAtFlags = 38;      // of the barriers, in that order: 2, 2, and what follows them

@@ -1,8 +1,8 @@
 // Rows written to a cache held in 4 bits (kv4.cuh), and read back. D / 8 lanes share a row, eight values of 16 bytes each; rows next to each other go to the same
 // head, whose rows of a block lie one behind the other.
 //
-// 8192 rows of 8 heads of 128, keys and values (34 MB read, 9 MB written): 25 us, 1.8 TB/s, what the codes cost to compute (34 with a division for each value and
-// for every place, of which the quotient's nearest integer now comes from a product and an exact remainder); read back (4.5 MB, 34 MB as fp32): 12 us, 3.3 TB/s.
+// 8192 rows of 8 heads of 128, keys and values (34 MB read, 9 MB written): 22 us, 1.9 TB/s, what the codes cost to compute (34 with a division for each value and
+// for every place, of which the quotient's nearest integer now comes from a product and an exact remainder); read back (4.5 MB, 34 MB as fp32): 9 us, 4.2 TB/s.
 // One row: 1 to 2 us, the launch.
 #include <stdexcept>
 

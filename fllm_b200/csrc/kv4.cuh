@@ -3,8 +3,8 @@
 //
 //   z = min x,  s = (max x - z) / 15 rounded up to bf16,  c = (x - z) / s rounded to nearest (ties to even)
 //
-// so the largest value is within reach of code 15 and no value is further than s / 2 from what its code stands for. (The quotient is that of exact
-// operands: a tie is seen as one.) A row whose values are all alike has s = 0 and is exact. One with an infinity or a NaN, or whose range fp32 does not
+// so the largest value is within reach of code 15 and no value is further than s / 2 from what its code stands for. (x - z is what fp32 makes of it.
+// kv4_code rounds its quotient by s, kv4_code_by, of kv4_write, a product that it mends by what is left of x - z; both see a tie as one and write the same bytes.) A row whose values are all alike has s = 0 and is exact. One with an infinity or a NaN, or whose range fp32 does not
 // hold, has s = NaN: all of it reads as NaN.
 #pragma once
 #include <cuda_bf16.h>
